@@ -505,6 +505,14 @@ int sx_win_decode_ok(int H, int G, int d, int dv);
 int sx_win_decode(const SxWinAttnArgs* args, cudaStream_t stream);        // decoding on tensor cores (bf16)
 int sx_win_merge(const SxWinAttnArgs* args, cudaStream_t stream);         // key slices -> y
 
+// ------------------------------------------------------------------ L2 activations in 8 bits (act8.cu)
+// dtype: 0 bf16, 1 fp16, 2 fp32. Per 32 values of a row a power of two and signed codes: codes [rows, 32 nb], exps [rows, nb], nb = ceil(width / 32).
+int sx_pack8(const void* x, void* codes, void* exps, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
+int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
+// gu [rows, 2 width] (gate | up, pitch ld) -> h [rows, width], gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb]; and back with dh.
+int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t stream);
+int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ unloadable library is an error: there is no silent fallback to PyTorch kernels f
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 
@@ -204,6 +205,15 @@ def available() -> bool:
 def stream() -> c_void_p:
     """Current stream of the current device, without a Stream object around it (0.4 us instead of 3)."""
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which t's device is the current one, so that ``stream()`` and new tensors are that device's (nothing to do, 0.3 us, where it is already)."""
+    i = t.device.index
+    return _here if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
 def ptr(t) -> c_void_p:

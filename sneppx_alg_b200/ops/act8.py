@@ -1,0 +1,207 @@
+"""Activations held in 8 bits between forward and backward.
+
+``pack_8bit`` / ``unpack_8bit`` hold any floating tensor as one exponent byte and 32 signed codes for each 32 values of its last dimension
+(33 bytes for 32 values); ``glu_8bit`` is the gated activation that keeps its input so; ``checkpoint_8bit`` recomputes a function in backward from
+arguments that were held so. CUDA tensors in bf16, fp16 and fp32 take the kernels (csrc/act8.cu); ``*_reference`` states the same in PyTorch and
+serves CPU tensors. The reference recomputes layers from inputs kept in full (grad_checkpoint.py, kernel/autodiff/tape.c:80-87).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import c_int, c_ll, ptr, stream
+from .functional import GLU_ACT
+
+BLOCK = 32
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _native(x) -> bool:
+    if not x.is_cuda:
+        return False
+    if x.dtype not in _TYPES:
+        raise TypeError(f"8-bit activations: {x.dtype} is not one of bfloat16, float16, float32")
+    return _lib.available()
+
+
+class Packed8bit:
+    """What ``pack_8bit`` returns: ``codes`` int8 [rows, 32 * ceil(width / 32)], ``exponents`` uint8 [rows, ceil(width / 32)] with the value
+    code * 2^(exponent - 127) (255: the block held an infinity or a NaN and is restored as NaN), ``shape`` and ``dtype`` of the tensor."""
+
+    __slots__ = ("codes", "exponents", "shape", "dtype")
+
+    def __init__(self, codes, exponents, shape, dtype):
+        self.codes, self.exponents, self.shape, self.dtype = codes, exponents, shape, dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exponents.numel()
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _rows(x):
+    """x as [rows, width] whose rows are contiguous (a view where x allows one)."""
+    w = x.shape[-1] if x.dim() else 1
+    x2 = x.reshape(-1, w) if x.numel() else x.reshape(0, w)
+    return x2 if x2.numel() == 0 or (x2.stride(1) == 1 or w == 1) and (x2.shape[0] == 1 or x2.stride(0) >= w) else x2.contiguous()
+
+
+def pack_8bit_reference(x2):
+    """[rows, width] -> (codes, exponents)."""
+    rows, w = x2.shape
+    nb = -(-w // BLOCK)
+    b = torch.zeros(rows, nb * BLOCK, dtype=torch.float32, device=x2.device)
+    b[:, :w] = x2.float()
+    b = b.view(rows, nb, BLOCK)
+    top = b.abs().amax(-1) if nb else b.new_zeros(rows, 0)
+    finite = torch.isfinite(top)
+    m, e = torch.frexp(torch.where(finite, top, 1.0))                        # top = m 2^e with m in [1/2, 1)
+    e = torch.where(top > 0, e - 7 + (m >= 127.5 / 128).int(), -126).clamp(min=-126)
+    codes = torch.where(finite[..., None], torch.round(torch.ldexp(b, -e[..., None])), 0.0)
+    return codes.to(torch.int8).view(rows, nb * BLOCK), torch.where(finite, e + 127, 255).to(torch.uint8)
+
+
+def unpack_8bit_reference(codes, exponents, width, dtype):
+    rows, nb = exponents.shape
+    step = torch.ldexp(torch.ones(rows, nb, device=codes.device), exponents.int() - 127)
+    step = torch.where(exponents == 255, torch.nan, step)
+    return (codes.view(rows, nb, BLOCK).float() * step[..., None]).view(rows, nb * BLOCK)[:, :width].to(dtype)
+
+
+def pack_8bit(x) -> Packed8bit:
+    """x (any shape, blocks along its last dimension; float types) in 8 bits. Not differentiable: what backward reads."""
+    if not x.is_floating_point():
+        raise TypeError(f"pack_8bit: {x.dtype} is not a floating type")
+    x2 = _rows(x.detach())
+    rows, w = x2.shape
+    nb = -(-w // BLOCK)
+    if not _native(x):
+        return Packed8bit(*pack_8bit_reference(x2), x.shape, x.dtype)
+    with _lib.on_device(x):
+        codes = torch.empty(rows, nb * BLOCK, dtype=torch.int8, device=x.device)
+        exps = torch.empty(rows, nb, dtype=torch.uint8, device=x.device)
+        _lib.call("sx_pack8", ptr(x2), ptr(codes), ptr(exps), c_ll(rows), c_int(w), c_ll(x2.stride(0)), c_int(_TYPES[x.dtype]), stream())
+    return Packed8bit(codes, exps, x.shape, x.dtype)
+
+
+def unpack_8bit(p: Packed8bit, dtype=None):
+    """The tensor that ``p`` stands for, in its own type or in ``dtype``."""
+    dtype = dtype or p.dtype
+    w = p.shape[-1] if len(p.shape) else 1
+    rows, nb = p.exponents.shape
+    if tuple(p.codes.shape) != (rows, nb * BLOCK) or nb != -(-w // BLOCK) or rows * w != p.shape.numel() or p.codes.dtype != torch.int8 \
+            or p.exponents.dtype != torch.uint8 or p.codes.device != p.exponents.device:
+        raise ValueError(f"unpack_8bit: codes {tuple(p.codes.shape)} and exponents {tuple(p.exponents.shape)} do not hold {tuple(p.shape)}")
+    if not (p.codes.is_cuda and _lib.available()):
+        return unpack_8bit_reference(p.codes, p.exponents, w, dtype).view(p.shape)
+    if dtype not in _TYPES:
+        raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
+    with _lib.on_device(p.codes):
+        x = torch.empty(p.shape, dtype=dtype, device=p.codes.device)
+        codes, exps = p.codes.contiguous(), p.exponents.contiguous()
+        _lib.call("sx_unpack8", ptr(codes), ptr(exps), ptr(x), c_ll(rows), c_int(w), c_ll(w), c_int(_TYPES[dtype]), stream())
+    return x
+
+
+# ----------------------------------------------------------------------------- gated activation
+def _gate(g, act):
+    """Value and derivative of the gate's function, in 32 bits."""
+    if act == 0:
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if act == 1:
+        k0, k1 = 0.7978845608028654, 0.044715
+        t = torch.tanh(k0 * (g + k1 * g ** 3))
+        return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * k0 * (1 + 3 * k1 * g * g)
+    return torch.relu(g), (g > 0).to(g.dtype)
+
+
+def glu_8bit_backward_reference(dh, gate, up, act):
+    """(rows of dgate | dup) from restored gate and up."""
+    a, da = _gate(gate.float(), act)
+    d = dh.float()
+    return torch.cat([d * up.float() * da, d * a], -1).to(dh.dtype)
+
+
+class _Glu8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gu, act):
+        f = gu.shape[-1] // 2
+        g2 = _rows(gu)
+        rows, nb = g2.shape[0], -(-f // BLOCK)
+        ctx.meta = act, gu.shape
+        if not _native(gu):
+            gate, up = g2[:, :f], g2[:, f:]
+            parts = [pack_8bit_reference(t) for t in (gate, up)]
+            ctx.save_for_backward(torch.cat([c for c, _ in parts], 1), torch.cat([e for _, e in parts], 1))
+            return (_gate(gate.float(), act)[0] * up.float()).to(gu.dtype).view(*gu.shape[:-1], f)
+        with _lib.on_device(gu):
+            h = torch.empty(*gu.shape[:-1], f, dtype=gu.dtype, device=gu.device)
+            codes = torch.empty(rows, 2 * nb * BLOCK, dtype=torch.int8, device=gu.device)
+            exps = torch.empty(rows, 2 * nb, dtype=torch.uint8, device=gu.device)
+            _lib.call("sx_glu8_fwd", ptr(g2), ptr(h), ptr(codes), ptr(exps), c_ll(rows), c_int(f), c_ll(g2.stride(0)), c_int(act),
+                      c_int(_TYPES[gu.dtype]), stream())
+        ctx.save_for_backward(codes, exps)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        codes, exps = ctx.saved_tensors
+        act, shape = ctx.meta
+        f, rows = shape[-1] // 2, codes.shape[0]
+        nb = exps.shape[1] // 2
+        if not _native(dh):
+            gate, up = (unpack_8bit_reference(c, e, f, torch.float32) for c, e in zip(codes.chunk(2, 1), exps.chunk(2, 1)))
+            return glu_8bit_backward_reference(dh.reshape(rows, f), gate, up, act).view(shape), None
+        with _lib.on_device(dh):
+            dh = dh.contiguous()
+            dgu = torch.empty(shape, dtype=dh.dtype, device=dh.device)
+            _lib.call("sx_glu8_bwd", ptr(dh), ptr(codes), ptr(exps), ptr(dgu), c_ll(rows), c_int(f), c_int(act), c_int(_TYPES[dh.dtype]), stream())
+        return dgu, None
+
+
+def glu_8bit(gu, act="silu"):
+    """act(gate) * up with gu = [..., 2F] laid out (gate | up), as ``glu``; what backward needs of gu is held in 8 bits (2.06 bytes instead of
+    4 for a gate and an up value of 16 bits), so the gradient is that of the restored gate and up. The result is computed from gu itself."""
+    if act not in GLU_ACT:
+        raise ValueError(f"glu_8bit: act {act!r} is not one of {sorted(GLU_ACT)}")
+    if gu.dim() == 0 or gu.shape[-1] % 2:
+        raise ValueError(f"glu_8bit: the last dimension of {tuple(gu.shape)} does not split into gate and up")
+    if not gu.is_floating_point():
+        raise TypeError(f"glu_8bit: {gu.dtype} is not a floating type")
+    if not (torch.is_grad_enabled() and gu.requires_grad):      # nothing is kept
+        from .functional import glu
+        if gu.is_cuda and gu.dtype == torch.bfloat16:
+            return glu(gu, act)
+    return _Glu8Fn.apply(gu, GLU_ACT[act])
+
+
+# ----------------------------------------------------------------------------- recomputation
+def checkpoint_8bit(fn, *args):
+    """``fn(*args)``, whose inner activations are recomputed in backward from arguments that are held in 8 bits: of ``args``, the floating CUDA / CPU
+    tensors that autograd reaches (those that require a gradient and are no leaves) are packed, the others are kept as they are. The first pass runs
+    on the arguments themselves; gradients are those of ``fn`` at the restored ones. Random state and autocast are as in torch.utils.checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+
+    held, kept = list(args), list(args)
+    if not torch.is_grad_enabled():
+        return fn(*args)
+    for i, a in enumerate(args):
+        if torch.is_tensor(a) and a.is_floating_point() and a.requires_grad and not a.is_leaf and (a.dtype in _TYPES):
+            kept[i] = pack_8bit(a)
+
+    def run():
+        if held:                       # forward
+            now = list(held)
+            held.clear()
+        else:                          # backward
+            now = [unpack_8bit(a).requires_grad_() if isinstance(a, Packed8bit) else a for a in kept]
+        return fn(*now)
+
+    return checkpoint(run, use_reentrant=False)

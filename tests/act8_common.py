@@ -1,0 +1,55 @@
+"""Definition of activations in 8 bits in 64-bit arithmetic, written apart from the operators."""
+import math
+
+import torch
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def held(x):
+    """[rows, width] of any float type -> what 8 bits hold of it, fp64. Row by row, block by block: the smallest e >= -126 with
+    round(amax / 2^e) <= 127, values round(x / 2^e) 2^e with ties to even; a block with an infinity or a NaN is NaN."""
+    out = torch.empty(x.shape, dtype=torch.float64)
+    x = x.double().cpu()
+    for i in range(0, x.shape[1], 32):
+        b = x[:, i:i + 32]
+        top = b.abs().amax(1)
+        e = torch.full_like(top, -126.0)
+        for r, t in enumerate(top.tolist()):
+            if math.isfinite(t) and t > 0:
+                n = math.frexp(t)[1] - 8                     # t < 2^(n + 8): at least 128 steps of 2^n or fewer
+                while round(t / 2.0 ** n) > 127:             # Python rounds ties to even
+                    n += 1
+                e[r] = max(n, -126)
+        step = torch.exp2(e)[:, None]
+        out[:, i:i + 32] = torch.where(torch.isfinite(top)[:, None], torch.round(b / step) * step, torch.nan)
+    return out
+
+
+def gate(g, act):
+    """Value and derivative of the gate's function in 64 bits."""
+    if act == "silu":
+        s = 1 / (1 + torch.exp(-g))
+        return g * s, s + g * s * (1 - s)
+    if act == "relu":
+        return g.clamp(min=0), (g > 0).double()
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (g + 0.044715 * g ** 3))
+    return g * (1 + t) / 2, (1 + t) / 2 + g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g) / 2
+
+
+def inputs(rows, width, dtype, seed, edge=True, device="cpu"):
+    """Columns of different size, and rows of the values where rounding turns: zeros, ties, the border of the exponent, tiny and huge ones."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g) * torch.exp(2 * torch.randn(width, generator=g))
+    if edge and rows >= 8:
+        x[0] = 0
+        x[1] = 127.5 * 2.0 ** -3                             # rounds to 128: the next exponent
+        x[2, ::2] = 1.0
+        x[2, 1::2] = 0.5                                     # halves of the maximum: 64 and 32 steps of it
+        x[3] = torch.arange(width) % 255 - 127.0
+        x[4] = (torch.arange(width) % 255 - 127.0) / 2 + 0.25
+        x[5] *= 2.0 ** -110
+        x[6, width // 2] = 60000.0
+        x[7] = -1.9921875
+    return x.to(TYPES[dtype]).to(device)

@@ -1,0 +1,117 @@
+"""Activations in 8 bits on the GPU against the definition in 64 bits."""
+import pytest
+import torch
+
+from act8_common import TYPES, gate, held, inputs
+from sneppx_alg_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [(9, 1), (8, 31), (8, 32), (11, 33), (8, 500), (77, 512), (1, 4096), (300, 1000), (8, 4104), (13, 5001)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,width", SIZES)
+def test_pack_and_unpack(rows, width, dtype):
+    x = inputs(rows, width, dtype, 1)
+    p, ref = ops.pack_8bit(x.cuda()), ops.pack_8bit(x)
+    assert torch.equal(p.codes.cpu(), ref.codes) and torch.equal(p.exponents.cpu(), ref.exponents)
+    want = held(x)
+    assert torch.equal(ops.unpack_8bit(p, torch.float32).double().cpu(), want)
+    assert torch.equal(ops.unpack_8bit(p).cpu(), want.to(x.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_strided_rows_odd_bases_and_overflows(dtype):
+    big = inputs(64, 320, dtype, 2).cuda()
+    for x in (big[:, 7:207], big[::3, 8:264], big[:, 16:], big.t(), big[5], big[:, :1], big.view(4, 16, 320)[:, 3:9]):
+        assert torch.equal(ops.unpack_8bit(ops.pack_8bit(x)), ops.unpack_8bit(ops.pack_8bit(x.contiguous())))
+        assert torch.equal(ops.unpack_8bit(ops.pack_8bit(x)).cpu(), ops.unpack_8bit(ops.pack_8bit(x.cpu())))
+    big[3, 40], big[4, 0], big[5, 319] = float("inf"), float("nan"), -float("inf")
+    y = ops.unpack_8bit(ops.pack_8bit(big))
+    bad = torch.zeros_like(big, dtype=torch.bool)
+    bad[3, 32:64], bad[4, :32], bad[5, 288:] = True, True, True
+    assert torch.equal(torch.isnan(y), bad)
+    for shape in ((0, 7), (3, 0), ()):
+        z = torch.ones(shape, dtype=TYPES[dtype], device="cuda")
+        assert torch.equal(ops.unpack_8bit(ops.pack_8bit(z)), z)
+
+
+def test_refusals():
+    with pytest.raises(TypeError):
+        ops.pack_8bit(torch.zeros(4, 64, dtype=torch.float64, device="cuda"))
+    p = ops.pack_8bit(torch.zeros(4, 64, device="cuda"))
+    with pytest.raises(TypeError):
+        ops.unpack_8bit(p, torch.float64)
+    with pytest.raises(ValueError):
+        ops.unpack_8bit(ops.Packed8bit(p.codes, p.exponents[:, :1], p.shape, p.dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows,f", [(1, 8), (9, 31), (8, 32), (77, 1000), (150, 1024), (5, 2503), (2, 16384)])
+def test_glu(rows, f, act, dtype):
+    half = torch.finfo(TYPES[dtype]).eps / 2
+    gu = inputs(rows, 2 * f, dtype, 3, edge=False).clamp(-8, 8)
+    dh = inputs(rows, f, dtype, 4, edge=False).clamp(-30, 30)
+    x = gu.cuda().requires_grad_()
+    h = ops.glu_8bit(x, act)
+    h.backward(dh.cuda())
+    g, u = gu[:, :f].double(), gu[:, f:].double()
+    # a rounding of half a step, and before it functions in 32 bits: absolute errors of a few 2^-24 (1 + |g|^3); 2^-25: the smallest step of fp16
+    want = gate(g, act)[0] * u
+    assert ((h.double().cpu() - want).abs() <= half * want.abs() + 1e-6 * (1 + g.abs() ** 3) * u.abs() + 2.0 ** -25).all()
+    g, u, d = held(gu[:, :f]), held(gu[:, f:]), dh.double()
+    a, da = gate(g, act)
+    want = torch.cat([d * u * da, d * a], 1)
+    slack = 1e-6 * torch.cat([(1 + g.abs() ** 3) * (d * u).abs(), (1 + g.abs() ** 3) * d.abs()], 1)
+    assert ((x.grad.double().cpu() - want).abs() <= half * want.abs() + slack + 2.0 ** -25).all()
+
+
+def test_glu_strided_input_and_no_gradient():
+    big = inputs(40, 300, "bf16", 5, edge=False).cuda()
+    x = big[:, 20:276].detach().requires_grad_()
+    h = ops.glu_8bit(x)
+    y = big[:, 20:276].contiguous().requires_grad_()
+    k = ops.glu_8bit(y)
+    assert torch.equal(h, k)
+    d = torch.randn_like(h)
+    gx, = torch.autograd.grad(h, x, d.t().contiguous().t())       # an incoming gradient laid out the other way
+    gy, = torch.autograd.grad(k, y, d)
+    assert torch.equal(gx, gy)
+    with torch.no_grad():
+        assert torch.equal(ops.glu_8bit(y), ops.glu(y))
+    e = torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    ops.glu_8bit(e).sum().backward()
+    assert e.grad.shape == (0, 64)
+
+
+def test_other_stream_and_captured_graph():
+    x = inputs(64, 1024, "bf16", 6).cuda()
+    want = ops.unpack_8bit(ops.pack_8bit(x))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = ops.unpack_8bit(ops.pack_8bit(x))
+    s.synchronize()
+    assert torch.equal(y, want)
+    graph, z = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        out = ops.unpack_8bit(ops.pack_8bit(z))
+    for k in (1.0, -3.0):
+        z.copy_(x * k)
+        graph.replay()
+        assert torch.equal(out, ops.unpack_8bit(ops.pack_8bit(z)))
+
+
+def test_checkpoint_of_a_block():
+    torch.manual_seed(0)
+    w = torch.randn(256, 256, device="cuda", dtype=torch.bfloat16).mul_(0.06).requires_grad_()
+    a = torch.randn(100, 256, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    x = a * 1
+    y = ops.checkpoint_8bit(lambda t: ops.glu(ops.linear(t, w).repeat(1, 2)), x)
+    assert torch.equal(y, ops.glu(ops.linear(x, w).repeat(1, 2)))
+    y.float().sum().backward()
+    b = ops.unpack_8bit(ops.pack_8bit(a.detach())).requires_grad_()
+    ga, gw = torch.autograd.grad(ops.glu(ops.linear(b, w).repeat(1, 2)).float().sum(), (b, w))
+    assert torch.equal(a.grad, ga) and torch.equal(w.grad, gw)
