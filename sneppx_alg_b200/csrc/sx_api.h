@@ -513,6 +513,17 @@ int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int
 int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t stream);
 int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype, cudaStream_t stream);
 
+// ------------------------------------------------------------------ L3 embedding (embed.cu)
+// ids int64 (ids_wide) or int32 [tokens]; w [V, d] (pitch ldw), y [tokens, d]; dtype 0 bf16, 1 fp16, 2 fp32. An id outside [0, V): a row of zeros and
+// ST_BAD_ARGUMENT in the status word.
+int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long long ldw, void* y, long long tokens, int d, long long V, float scale, int dtype,
+                 int* status, cudaStream_t stream);
+// grad [V, d] (pitch ldg; dtype or fp32) = scale * sums of dy [tokens, d] by word, or += with `add` (rows of other words are not touched).
+// Tokens of the word `padding` (-1: none) give nothing. work: sx_embed_bwd_workspace bytes, 16-byte aligned.
+long long sx_embed_bwd_workspace(long long tokens, long long V, int d, int add);
+int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long long ldg, long long tokens, int d, long long V, long long padding,
+                 float scale, int add, int dtype, int grad_dtype, void* work, long long work_bytes, int* status, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

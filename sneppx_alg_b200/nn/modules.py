@@ -14,6 +14,7 @@ import torch.nn as tnn
 import torch.nn.functional as F
 
 from ..ops import functional as ops
+from ..ops.embed import embedding
 
 
 class Module(tnn.Module):
@@ -52,7 +53,7 @@ class Embedding(Module):
         tnn.init.normal_(self.weight, std=init_std)
 
     def forward(self, indices):
-        return F.embedding(indices, self.weight)
+        return embedding(indices, self.weight)
 
 
 class Dropout(tnn.Dropout, Module):

@@ -7,3 +7,4 @@ from . import aux  # noqa: F401
 from .aux import arc_step, block_top2, dequant_int8, dropout, quant_int8, rng_fill, weighted_average  # noqa: F401
 from . import act8  # noqa: F401
 from .act8 import Packed8bit, checkpoint_8bit, glu_8bit, pack_8bit, unpack_8bit  # noqa: F401
+from .embed import embedding, embedding_backward_  # noqa: F401

@@ -1,0 +1,100 @@
+"""Embedding lookup with scaling, and its gradient by sorted tokens (csrc/embed.cu). CUDA tables in bf16, fp16 and fp32 take the kernels;
+``embedding_reference`` states the same in PyTorch and serves CPU tensors. The reference looks rows up and scatters their gradients in its Python
+module (interface_bindings/nn.py, ``Embedding``)."""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import debug as _dbg
+from ._lib import c_float, c_int, c_ll, ptr, stream
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def embedding_reference(ids, table, scale=1.0, padding_idx=None):
+    y = F.embedding(ids, table, padding_idx)
+    return y if scale == 1.0 else (y.float() * scale).to(y.dtype) if y.dtype != torch.float64 else y * scale
+
+
+def _lookup(ids, table, scale):
+    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    ids = ids.contiguous()
+    V, d = table.shape
+    with _lib.on_device(table):
+        y = torch.empty(*ids.shape, d, dtype=table.dtype, device=table.device)
+        _lib.call("sx_embed_fwd", ptr(ids), c_int(ids.dtype == torch.int64), ptr(table), c_ll(table.stride(0)), ptr(y), c_ll(ids.numel()), c_int(d),
+                  c_ll(V), c_float(scale), c_int(_TYPES[table.dtype]), ptr(_lib.status_word(table.device)), stream())
+    return y
+
+
+def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
+    """grad [V, d] = scale * (sums of the rows of dy [.., d] by their word), or, with ``add``, grad += that (rows of other words are not touched
+    then). Sums are in 32 bits and in the order of the tokens, so they are the same each time. grad has dy's type or is fp32."""
+    V, d = grad.shape
+    if dy.dtype not in _TYPES or grad.dtype not in (dy.dtype, torch.float32) or grad.stride(1) != 1 or (V > 1 and grad.stride(0) < d):
+        raise ValueError(f"embedding_backward_: gradients {dy.dtype} into {grad.dtype} with strides {grad.stride()}")
+    if dy.shape != (*ids.shape, d):
+        raise ValueError(f"embedding_backward_: gradients of shape {tuple(dy.shape)} for ids {tuple(ids.shape)} and rows of {d}")
+    ids, dy = ids.contiguous(), dy.contiguous()
+    n = ids.numel()
+    with _lib.on_device(grad):
+        fn = _lib.lib().sx_embed_bwd_workspace
+        fn.restype = c_ll
+        size = fn(c_ll(n), c_ll(V), c_int(d), c_int(add))
+        work = torch.empty(size, dtype=torch.uint8, device=grad.device)
+        _lib.call("sx_embed_bwd", ptr(ids), c_int(ids.dtype == torch.int64), ptr(dy), ptr(grad), c_ll(grad.stride(0)), c_ll(n), c_int(d), c_ll(V),
+                  c_ll(-1 if padding_idx is None else padding_idx), c_float(scale), c_int(add), c_int(_TYPES[dy.dtype]), c_int(_TYPES[grad.dtype]),
+                  ptr(work), c_ll(size), ptr(_lib.status_word(grad.device)), stream())
+    return grad
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.table, ctx.meta = table, (scale, padding_idx)
+        return _lookup(ids, table, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        table, (scale, padding_idx) = ctx.table, ctx.meta
+        mg = getattr(table, "main_grad", None)
+        if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:
+            embedding_backward_(mg, ids, dy, scale, padding_idx, add=getattr(table, "_main_grad_written", False))
+            table._main_grad_written = True
+            return None, None, None, None
+        return None, embedding_backward_(torch.empty(table.shape, dtype=dy.dtype, device=dy.device), ids, dy, scale, padding_idx), None, None
+
+
+def embedding(ids, table, scale=1.0, padding_idx=None):
+    """scale * table[ids]: table [V, d], ids any shape of integers -> [*ids.shape, d] in the table's type.
+
+    The gradient of the table is dense; where the table carries ``main_grad`` (a view into a flat gradient buffer, of its type or fp32) it is written
+    there, or added to what is there already (a tied output projection's), and ``.grad`` stays empty. ``padding_idx`` (negative counts from the
+    end): tokens of this word give no gradient. On the GPU an id outside [0, V) gives a row of zeros and sets the status word
+    (``check_status`` raises); on the CPU it raises at once."""
+    if table.dim() != 2:
+        raise ValueError(f"embedding: table of shape {tuple(table.shape)} is no matrix")
+    if ids.dtype not in (torch.int64, torch.int32):
+        if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+            raise TypeError(f"embedding: ids of {ids.dtype}")
+        ids = ids.long()
+    if ids.device != table.device:
+        raise ValueError(f"embedding: ids on {ids.device}, table on {table.device}")
+    if padding_idx is not None:
+        if not -table.shape[0] <= padding_idx < table.shape[0]:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {table.shape[0]} rows")
+        padding_idx %= table.shape[0]
+    if not (table.is_cuda and table.dtype in _TYPES and table.shape[0] > 0 and _lib.available()):
+        return embedding_reference(ids, table, scale, padding_idx)
+    if _dbg.ENABLED:
+        _dbg.check_indices(ids, 0, table.shape[0], _dbg.SITE_USER)
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
+    return _lookup(ids, table, scale)

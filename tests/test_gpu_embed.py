@@ -1,0 +1,195 @@
+"""Embedding lookup and its gradient on the GPU against sums in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from sneppx_alg_b200 import ops
+from sneppx_alg_b200.ops._lib import KernelTimeout
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _ids(n, V, law, seed):
+    g = torch.Generator().manual_seed(seed)
+    if law == "one":
+        return torch.full((n,), V // 2)
+    if law == "few":
+        return torch.randint(0, min(V, 3), (n,), generator=g) * max(1, (V - 1) // 3)
+    if law == "skew":
+        return (V * torch.rand(n, generator=g) ** 6).long().clamp(max=V - 1)
+    return torch.randint(0, V, (n,), generator=g)
+
+
+def _sums(ids, dy, V, scale, padding=None):
+    """64-bit sums by word, and the sums of magnitudes that bound their rounding."""
+    keep = ids != padding if padding is not None else torch.ones_like(ids, dtype=torch.bool)
+    out, mag = (torch.zeros(V, dy.shape[-1], dtype=torch.float64, device=dy.device) for _ in range(2))
+    d = dy[keep].double() * scale
+    return out.index_add_(0, ids[keep], d), mag.index_add_(0, ids[keep], d.abs())
+
+
+def _close(got, want, mag, dtype, n):
+    """One rounding to the gradient's type; before it a sum of up to n terms in 32 bits and a product: n + 2 roundings of at most 2^-24 of the magnitudes
+    (2^-25: the smallest step of fp16)."""
+    assert ((got.double() - want).abs() <= _half(dtype) * want.abs() + (n + 2) * 2.0 ** -24 * mag + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,V,d", [(1, 1, 1), (1, 500, 8), (77, 300, 33), (64, 32000, 512), (513, 1000, 4096), (300, 70, 5003)])
+@pytest.mark.parametrize("scale", [1.0, 22.5])
+def test_lookup(n, V, d, scale, dtype):
+    torch.manual_seed(0)
+    w = torch.randn(V, d, device="cuda").to(TYPES[dtype])
+    for ids in (_ids(n, V, "any", 1).cuda(), _ids(n, V, "one", 1).cuda().int()):
+        y = ops.embedding(ids, w, scale)
+        # the product in 32 bits is exact for 16-bit tables up to its one rounding
+        want = w[ids.long()] if scale == 1.0 else (w[ids.long()].float() * scale).to(w.dtype)
+        assert torch.equal(y, want)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("law", ["any", "one", "few", "skew"])
+@pytest.mark.parametrize("n,V,d", [(1, 1, 8), (2, 3, 1), (77, 300, 33), (500, 70, 1000), (4096, 5000, 256), (4097, 128256, 64), (9001, 300001, 40)])
+def test_gradient(n, V, d, law, dtype):
+    torch.manual_seed(0)
+    t = TYPES[dtype]
+    w = torch.randn(V, d, device="cuda").to(t).requires_grad_()
+    ids = _ids(n, V, law, 2).cuda()
+    dy = torch.randn(n, d, device="cuda").to(t)
+    most = int(torch.bincount(ids).max())
+    (g,) = torch.autograd.grad(ops.embedding(ids, w, 1.5), w, dy)
+    want, mag = _sums(ids, dy, V, 1.5)
+    assert g.dtype == t and g.shape == w.shape
+    _close(g, want, mag, t, most)
+    assert not g[torch.bincount(ids, minlength=V) == 0].any()
+    (h,) = torch.autograd.grad(ops.embedding(ids, w, 1.5), w, dy)
+    assert torch.equal(g, h)                                       # the same bits each time
+    pad = int(ids[0])
+    (g,) = torch.autograd.grad(ops.embedding(ids, w, 1.5, padding_idx=pad), w, dy)
+    want, mag = _sums(ids, dy, V, 1.5, pad)
+    _close(g, want, mag, t, most)
+    assert not g[pad].any()
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype,into", [("bf16", "fp32"), ("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
+@pytest.mark.parametrize("n,V,d", [(77, 300, 33), (3000, 500, 256), (40000, 2000, 128)])
+def test_main_grad_is_written_and_added_to(n, V, d, dtype, into):
+    torch.manual_seed(0)
+    t = TYPES[dtype]
+    w = torch.randn(V, d, device="cuda").to(t).requires_grad_()
+    buf = torch.full((V, d), math.nan, device="cuda", dtype=TYPES[into])
+    w.main_grad, w._main_grad_written = buf, False
+    ids = _ids(n, V, "skew", 3).cuda()
+    dy = torch.randn(n, d, device="cuda").to(t)
+    most = int(torch.bincount(ids).max())
+    ops.embedding(ids, w).backward(dy)
+    assert w.grad is None and w._main_grad_written
+    want, mag = _sums(ids, dy, V, 1.0)
+    _close(buf, want, mag, TYPES[into], most)                       # NaN was there: every element has been written
+    start = torch.randn(V, d, device="cuda").to(TYPES[into])
+    buf.copy_(start)
+    ops.embedding(ids, w, padding_idx=1).backward(dy)
+    want, mag = _sums(ids, dy, V, 1.0, 1)
+    _close(buf, want + start.double(), mag + start.double().abs(), TYPES[into], most + 1)
+    alone = torch.bincount(ids, minlength=V) == 0
+    alone[1] = True
+    assert torch.equal(buf[alone], start[alone])                    # rows of other words are left as they are
+
+
+def test_layouts_shapes_and_empty_batches():
+    torch.manual_seed(0)
+    big = torch.randn(200, 300, device="cuda")
+    ids = torch.randint(0, 200, (3, 7, 5), device="cuda")
+    for w in (big[:, 8:264], big[:, 3:260], big[:, ::2], torch.randn(64, 200, device="cuda").t()):
+        w = w.detach().requires_grad_()
+        y = ops.embedding(ids, w, 2.0)
+        assert torch.equal(y, w[ids] * 2)
+        dy = torch.randn(7, 5, 3, w.shape[1], device="cuda").permute(2, 0, 1, 3)      # not contiguous
+        (g,) = torch.autograd.grad(y, w, dy)
+        want, mag = _sums(ids.reshape(-1), dy.reshape(-1, w.shape[1]), 200, 2.0)
+        _close(g, want, mag, torch.float32, 105)
+    w = big.detach().requires_grad_()
+    t = torch.randint(0, 200, (8, 6), device="cuda", dtype=torch.int32).t()
+    assert torch.equal(ops.embedding(t, w), w[t.long()])
+    assert torch.equal(ops.embedding(t.to(torch.uint8), w), w[t.long()])
+    e = ops.embedding(torch.zeros(0, 4, dtype=torch.int64, device="cuda"), w)
+    assert e.shape == (0, 4, 300)
+    (g,) = torch.autograd.grad(e, w, torch.zeros_like(e))
+    assert g.shape == w.shape and not g.any()
+    assert ops.embedding(torch.tensor(3, device="cuda"), w).shape == (300,)
+
+
+def test_ids_out_of_range():
+    w = torch.randn(50, 64, device="cuda", requires_grad=True)
+    ids = torch.tensor([3, -1, 50, 3, 2 ** 40, 49, -2 ** 35], device="cuda")
+    ok = torch.tensor([1, 0, 0, 1, 0, 1, 0], device="cuda", dtype=torch.bool)
+    y = ops.embedding(ids, w)
+    with pytest.raises(KernelTimeout):
+        ops.check_status()
+    assert torch.equal(y[ok], w[ids[ok]]) and not y[~ok].any()
+    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    with pytest.raises(KernelTimeout):
+        ops.check_status()
+    want = torch.zeros(50, 64, device="cuda")
+    want[3], want[49] = 2, 1
+    assert torch.equal(g, want)
+    ops.check_status()
+
+
+def test_refusals():
+    w = torch.randn(50, 64, device="cuda")
+    with pytest.raises(ValueError):
+        ops.embedding(torch.tensor([1]), w)
+    with pytest.raises(ValueError):
+        ops.embedding_backward_(torch.zeros(50, 64, device="cuda", dtype=torch.bfloat16), torch.tensor([1], device="cuda"), torch.zeros(1, 64, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.embedding_backward_(torch.zeros(50, 64, device="cuda"), torch.tensor([1], device="cuda"), torch.zeros(2, 64, device="cuda"))
+
+
+def test_other_stream_and_captured_graph():
+    torch.manual_seed(0)
+    w = torch.randn(1000, 256, device="cuda")
+    ids = torch.randint(0, 1000, (600,), device="cuda")
+    dy = torch.randn(600, 256, device="cuda")
+    want = ops.embedding_backward_(torch.empty_like(w), ids, dy)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.embedding_backward_(torch.empty_like(w), ids, dy)
+    s.synchronize()
+    assert torch.equal(got, want)
+    # two graphs, replayed in turn: each has its own scratch
+    outs, graphs = [torch.empty_like(w) for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    i2 = ids.clone()
+    for o, gr in zip(outs, graphs):
+        with torch.cuda.graph(gr):
+            ops.embedding_backward_(o, i2, dy)
+    for k in range(3):
+        i2.copy_((ids + 17 * k) % 1000)
+        for gr in graphs:
+            gr.replay()
+        want = ops.embedding_backward_(torch.empty_like(w), i2, dy)
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_embedding_layer_in_a_model():
+    """The layer's gradient is what autograd of the plain lookup gives, up to the rounding of the sums."""
+    from sneppx_alg_b200.nn import Embedding
+    torch.manual_seed(0)
+    e = Embedding(300, 128, dtype=torch.bfloat16, device="cuda")
+    ids = torch.randint(0, 300, (4, 200), device="cuda")
+    dy = torch.randn(4, 200, 128, device="cuda").to(torch.bfloat16)
+    y = e(ids)
+    y.backward(dy)
+    want, mag = _sums(ids.reshape(-1), dy.reshape(-1, 128), 300, 1.0)
+    assert torch.equal(y, e.weight[ids])
+    _close(e.weight.grad, want, mag, torch.bfloat16, 800)
