@@ -8,3 +8,4 @@ from .aux import arc_step, block_top2, dequant_int8, dropout, quant_int8, rng_fi
 from . import act8  # noqa: F401
 from .act8 import Packed8bit, checkpoint_8bit, glu_8bit, pack_8bit, unpack_8bit  # noqa: F401
 from .embed import embedding, embedding_backward_  # noqa: F401
+from .token_loss import linear_token_loss  # noqa: F401

@@ -1,0 +1,213 @@
+"""Per-token vocabulary loss on the GPU against the definition in 64 bits.
+
+Bounds. A logit is a sum of d products of bf16 numbers, exact in 32 bits, whose additions lose at most 2^-23 of the magnitudes' sum S each (the tensor cores
+cut rather than round): ez = d 2^-23 S. The soft cap adds 2^-21 of the cap (exponential and quotient). lse then has ez, a relative error of the sum of
+exponentials (each a few 2^-23, at most 300 additions one after another: 300 x 2^-24 < 2e-5) and its rounding; nll the target's ez more. dz has a
+relative error of ez + elsa from its exponential and half a step of bf16, 2^-8; dh and dw add up its errors times the other factor, one rounding of
+2^-24 for each addition, and half a step of their own.
+"""
+import math
+
+import pytest
+import torch
+
+from sneppx_alg_b200 import ops
+from sneppx_alg_b200.ops._lib import KernelTimeout
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(T, V, d, seed, sure=6.0, ignored=0.1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn(V, d, generator=g, device="cuda") / math.sqrt(d)).to(torch.bfloat16)
+    t = torch.randint(0, V, (T,), generator=g, device="cuda")
+    h = (torch.randn(T, d, generator=g, device="cuda") + sure * torch.rand(T, 1, generator=g, device="cuda") * w[t].float()).to(torch.bfloat16)
+    gn, gz = torch.randn(T, generator=g, device="cuda"), 0.1 * torch.randn(T, generator=g, device="cuda")
+    return h, w, torch.where(torch.rand(T, generator=g, device="cuda") < ignored, -100, t), gn, gz
+
+
+def _want(h, w, t, gn, gz, cap):
+    """64-bit results, and what bounds their errors."""
+    h, w = h.double(), w.double()
+    T, d = h.shape
+    raw = h @ w.t()
+    z = cap * torch.tanh(raw / cap) if cap else raw
+    lse = torch.logsumexp(z, 1)
+    ok = t >= 0
+    at = t.clamp(min=0)[:, None]
+    nll = torch.where(ok, lse - z.gather(1, at).squeeze(1), 0.0)
+    ez = d * 2.0 ** -23 * (h.abs() @ w.abs().t()).amax(1) + 2.0 ** -21 * cap
+    el = ez + 2e-5 + 2.0 ** -23 * lse.abs()
+    p = torch.exp(z - lse[:, None])
+    a, b = (gn.double() * ok + gz.double())[:, None], (gn.double() * ok)[:, None]
+    slope = 1 - (z / cap) ** 2 if cap else torch.ones_like(z)
+    hot = torch.zeros_like(z).scatter_(1, at, 1.0)
+    dz = (a * p - b * hot) * slope
+    # errors of the exponential and of the slope (2 |z / cap| ez / cap), then the rounding to bf16
+    mag = a.abs() * p + b.abs() * hot
+    edz = mag * ((ez + el)[:, None] * 1.5 + 2.0 ** -21 + (4 * ez[:, None] / cap + 2.0 ** -20 if cap else 0.0)) + 2.0 ** -8 * dz.abs()
+    out = dict(nll=nll, lse=lse, dh=dz @ w, dw=dz.t() @ h)
+    tol = dict(nll=el + ez + 2.0 ** -23 * nll.abs(), lse=el,
+               dh=edz @ w.abs() + w.shape[0] * 2.0 ** -23 * (dz.abs() @ w.abs()) + 2.0 ** -8 * out["dh"].abs(),
+               dw=edz.t() @ h.abs() + T * 2.0 ** -23 * (dz.abs().t() @ h.abs()) + 2.0 ** -8 * out["dw"].abs())
+    return out, tol
+
+
+def _check(got, want, tol):
+    for k, v in got.items():
+        assert torch.isfinite(v).all() and v.shape == want[k].shape
+        off = (v.double() - want[k]).abs()
+        assert (off <= tol[k] + 1e-30).all(), (k, float((off - tol[k]).max()), float(off.max()))
+
+
+def _run(h, w, t, gn, gz, cap, piece=0):
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+    nll, lse = ops.linear_token_loss(h, w, t, softcap=cap, piece=piece)
+    dh, dw = torch.autograd.grad((nll, lse), (h, w), (gn, gz))
+    ops.check_status()
+    return dict(nll=nll.detach(), lse=lse.detach(), dh=dh, dw=dw)
+
+
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+@pytest.mark.parametrize("T,V,d", [(1, 1, 8), (1, 300, 64), (3, 256, 72), (77, 1000, 256), (128, 257, 64), (129, 128, 640), (255, 4099, 128), (256, 512, 64),
+                                   (257, 777, 192), (300, 33, 1024), (1000, 5000, 96), (520, 3001, 100), (33, 700, 7)])
+def test_values_and_gradients(T, V, d, cap):
+    x = _inputs(T, V, d, 1)
+    got = _run(*x, cap)
+    want, tol = _want(*x, cap)
+    _check(got, want, tol)
+    assert torch.equal(got["nll"][x[2] < 0], torch.zeros_like(got["nll"][x[2] < 0]))
+    again = _run(*x, cap)
+    assert all(torch.equal(got[k], again[k]) for k in got)          # the same bits each time
+
+
+@pytest.mark.parametrize("piece", [1, 256, 512, 700, 4096])
+def test_pieces_of_the_vocabulary(piece):
+    x = _inputs(100, 2003, 128, 2)
+    want, tol = _want(*x, 0.0)
+    got = _run(*x, 0.0, piece)
+    # the sums of dh over pieces are held in 32 bits: a rounding for each
+    tol["dh"] = tol["dh"] + 8 * 2.0 ** -24 * want["dh"].abs().amax()
+    _check(got, want, tol)
+
+
+@pytest.mark.parametrize("T,V", [(700, 1300), (64, 20000)])
+def test_which_gradients_are_asked_for(T, V):
+    h, w, t, gn, gz = _inputs(T, V, 128, 3)
+    full = _run(h, w, t, gn, gz, 0.0)
+    hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+    nll, _ = ops.linear_token_loss(hg, w, t)
+    assert torch.equal(nll, full["nll"])
+    want, tol = _want(h, w, t, gn, torch.zeros_like(gz), 0.0)
+    dh, = torch.autograd.grad(nll, hg, gn)
+    _check(dict(dh=dh), want, tol)
+    nll, _ = ops.linear_token_loss(h, wg, t)
+    dw, = torch.autograd.grad(nll, wg, gn)
+    _check(dict(dw=dw), want, tol)
+    _, lse = ops.linear_token_loss(hg, wg, t)
+    want, tol = _want(h, w, t, torch.zeros_like(gn), gz, 0.0)
+    dh, dw = torch.autograd.grad(lse, (hg, wg), gz)
+    _check(dict(dh=dh, dw=dw), want, tol)
+    nll, lse = ops.linear_token_loss(h, w, t)
+    assert not nll.requires_grad and not lse.requires_grad
+
+
+@pytest.mark.parametrize("into", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [640, 1001])
+def test_main_grad_is_written_and_added_to(V, into):
+    h, w, t, gn, gz = _inputs(200, V, 128, 4)
+    want, tol = _want(h, w, t, gn, gz, 0.0)
+    w = w.detach().requires_grad_()
+    w.main_grad, w._main_grad_written = torch.full((V, 128), math.nan, device="cuda", dtype=into), False
+    half = torch.finfo(into).eps / 2
+    for k in (1, 2):
+        nll, lse = ops.linear_token_loss(h, w, t, piece=256)
+        torch.autograd.backward((nll, lse), (gn, gz))
+        assert w.grad is None and w._main_grad_written
+        off = (w.main_grad.double() - k * want["dw"]).abs()
+        assert (off <= k * tol["dw"] + 2 * half * k * want["dw"].abs()).all()
+
+
+def test_layouts():
+    """Rows of a wider tensor, an odd base address, a transposed weight, a batch of sequences with shifted targets."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    big = torch.randn(4, 60, 200, generator=g, device="cuda").to(torch.bfloat16)
+    wide = (torch.randn(900, 300, generator=g, device="cuda") / 12).to(torch.bfloat16)
+    ids = torch.randint(0, 900, (4, 61), generator=g, device="cuda")
+    t = ids[:, 1:]                                           # not contiguous
+    for h, w in ((big[..., 8:136], wide[:, 16:144]), (big[..., 3:131], wide[:, 5:133]), (big[:, :, :128], wide[:, :128].t().contiguous().t()),
+                 (big[:, 1:, :128], wide[:, 100:228])):
+        tt = t[:, :h.shape[1]]
+        nll, lse = ops.linear_token_loss(h, w, tt)
+        T = tt.numel()
+        want, tol = _want(h.reshape(T, 128), w, tt.reshape(T), torch.ones(T, device="cuda"), torch.zeros(T, device="cuda"), 0.0)
+        assert nll.shape == tt.shape
+        _check(dict(nll=nll.reshape(-1), lse=lse.reshape(-1)), want, tol)
+        hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+        dh, dw = torch.autograd.grad(ops.linear_token_loss(hg, wg, tt)[0].sum(), (hg, wg))
+        _check(dict(dh=dh.reshape(T, 128), dw=dw), want, tol)
+    ops.check_status()
+
+
+def test_everything_ignored_and_empty():
+    h, w, _, gn, gz = _inputs(90, 500, 64, 6)
+    t = torch.full((90,), -100, device="cuda")
+    got = _run(h, w, t, gn, torch.zeros_like(gz), 0.0)
+    assert not got["nll"].any() and not got["dh"].any() and not got["dw"].any()
+    hg, wg = h[:0].detach().requires_grad_(), w.detach().requires_grad_()
+    nll, lse = ops.linear_token_loss(hg, wg, t[:0])
+    (nll.sum() + lse.sum()).backward()
+    assert hg.grad.shape == (0, 64) and not wg.grad.any()
+
+
+def test_targets_out_of_range_count_as_ignored_and_are_reported():
+    h, w, t, gn, gz = _inputs(40, 500, 64, 7, ignored=0.0)
+    bad = t.clone()
+    bad[3], bad[4], bad[5] = 500, -1, 2 ** 40
+    hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+    nll, lse = ops.linear_token_loss(hg, wg, bad)
+    with pytest.raises(KernelTimeout):
+        ops.check_status()
+    dh, dw = torch.autograd.grad((nll, lse), (hg, wg), (gn, gz))
+    t[3:6] = -100
+    good = _run(h, w, t, gn, gz, 0.0)
+    assert torch.equal(nll, good["nll"]) and torch.equal(lse, good["lse"]) and torch.equal(dh, good["dh"]) and torch.equal(dw, good["dw"])
+    # a border value of ignore_index
+    nll, _ = ops.linear_token_loss(h, w, torch.where(t < 0, 0, t), ignore_index=0)
+    ops.check_status()
+    assert not nll[(t <= 0)].any()
+
+
+def test_large_logits_and_infinities():
+    h, w, t, _, _ = _inputs(50, 400, 64, 8)
+    h = h * 300                                             # logits up to some thousands: exponentials of differences only
+    nll, lse = ops.linear_token_loss(h, w, t)
+    want, tol = _want(h, w, t, torch.zeros(50, device="cuda"), torch.zeros(50, device="cuda"), 0.0)
+    _check(dict(nll=nll, lse=lse), want, tol)
+    h[7, 3] = float("nan")
+    nll2, lse2 = ops.linear_token_loss(h, w, t)
+    rest = torch.arange(50, device="cuda") != 7
+    assert torch.isnan(lse2[7]) and torch.equal(lse2[rest], lse[rest]) and torch.equal(nll2[rest], nll[rest])
+    ops.check_status()
+
+
+def test_other_stream_and_captured_graph():
+    h, w, t, gn, gz = _inputs(200, 3000, 128, 9)
+    want = ops.linear_token_loss(h, w, t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.linear_token_loss(h, w, t)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs, x = [torch.cuda.CUDAGraph() for _ in range(2)], [], h.clone()
+    for gr in graphs:
+        with torch.cuda.graph(gr):
+            outs.append(ops.linear_token_loss(x, w, t))
+    for k in (1.0, 0.5):
+        x.copy_(h * k)
+        for gr in graphs:
+            gr.replay()
+        want = ops.linear_token_loss(x, w, t)
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+    ops.check_status()
