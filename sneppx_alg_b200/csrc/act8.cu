@@ -8,8 +8,10 @@
 // 33 bytes for 32 values. A power of two for 32 values costs what a 32-bit scale for 128 costs and is as near on normal values
 // (the block's maximum is smaller by what the step is rounded up), nearer where single values stand out.
 //
-// All kernels are bound by memory: a thread takes 8 neighbouring values (16 bytes of a 16-bit type), four threads a block.
-// Sums and functions are in 32 bits; this file is compiled without fast math, so that 32-bit inputs keep their small values.
+// All kernels are bound by memory: a thread takes 16 neighbouring values, two threads a block, so that 32 to 64 bytes a thread are on their way.
+// Rounding is an addition of 1.5 * 2^23 (the sum's low byte is the code), restoring a byte placed in the mantissa of 2^23: the conversion
+// instructions run at an eighth of the rate. Sums and functions are in 32 bits; this file is compiled without fast math, so that 32-bit inputs keep
+// their small values.
 #include <cuda_fp16.h>
 #include "common.cuh"
 #include "sx_api.h"
@@ -30,108 +32,140 @@ template <> struct Act8<float> {
   static __device__ __forceinline__ float out(float v) { return v; }
 };
 
-// 8 values from column c of a row of `width`: whole 16-byte loads where VEC (width, pitch and base are multiples of 8 values then), else one by one.
-template <bool VEC, typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int width, float (&f)[8]) {
-  if (VEC) {
-    union { uint4 q[sizeof(T) / 2]; T t[8]; } v;
+constexpr int PER = 16;      // values of a thread
+
+// How rows are read and written: 32-byte accesses where base, pitch and width are whole multiples of a thread's values (16 of them: WIDE), 16-byte ones
+// where they are multiples of 8 (PAIR), else one value at a time.
+enum { SINGLE = 0, PAIR = 1, WIDE = 2 };
+
+__device__ __forceinline__ void ld32(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+template <typename T> union Row16 {
+  uint32_t w[sizeof(T) / 2][8];
+  uint4 q[sizeof(T)];
+  T t[PER];
+};
+template <int MODE, typename T>
+__device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>& v) {
+  if (MODE == WIDE) {
     if (c < width) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v.q[i] = reinterpret_cast<const uint4*>(row + c)[i];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = Act8<T>::in(v.t[j]);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) ld32(row + c + i * (32 / (int)sizeof(T)), v.w[i]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
+      for (int i = 0; i < (int)sizeof(T); ++i) v.q[i] = make_uint4(0, 0, 0, 0);
     }
+  } else if (MODE == PAIR) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i)
+      v.q[i] = c + i * (16 / (int)sizeof(T)) < width ? *reinterpret_cast<const uint4*>(row + c + i * (16 / (int)sizeof(T))) : make_uint4(0, 0, 0, 0);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j < width ? Act8<T>::in(row[c + j]) : 0.f;
+    for (int j = 0; j < PER; ++j) v.t[j] = c + j < width ? row[c + j] : Act8<T>::out(0.f);
   }
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void store8(T* row, int c, int width, const float (&f)[8]) {
-  if (VEC) {
+template <int MODE, typename T>
+__device__ __forceinline__ void store16(T* row, int c, int width, const float (&f)[PER]) {
+  Row16<T> v;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) v.t[j] = Act8<T>::out(f[j]);
+  if (MODE == WIDE) {
     if (c < width) {
-      union { uint4 q[sizeof(T) / 2]; T t[8]; } v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v.t[j] = Act8<T>::out(f[j]);
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = v.q[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) st32(row + c + i * (32 / (int)sizeof(T)), v.w[i]);
     }
+  } else if (MODE == PAIR) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i)
+      if (c + i * (16 / (int)sizeof(T)) < width) *reinterpret_cast<uint4*>(row + c + i * (16 / (int)sizeof(T))) = v.q[i];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < width) row[c + j] = Act8<T>::out(f[j]);
+    for (int j = 0; j < PER; ++j)
+      if (c + j < width) row[c + j] = v.t[j];
   }
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Row16<T>& v, float (&f)[PER]) {
+#pragma unroll
+  for (int j = 0; j < PER; ++j) f[j] = Act8<T>::in(v.t[j]);
 }
 
-// Codes and exponent byte of a block whose four threads hold 8 values each; all four are there and get the byte.
-__device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t& byte) {
+// Codes and exponent byte of a block whose two threads hold 16 values each; both are there and get the byte.
+__device__ __forceinline__ uint4 encode16(const float (&f)[PER], uint32_t& byte) {
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-  const uint32_t four = 0xfu << (threadIdx.y * blockDim.x + threadIdx.x & 28u);
-  top = max(top, __shfl_xor_sync(four, top, 1));
-  top = max(top, __shfl_xor_sync(four, top, 2));
-  const bool finite = top < 0x7f800000u;
-  byte = finite ? max((int)((top + 0x10000u) >> 23) - 6, 1) : 255u;
-  const float inv = finite ? __uint_as_float((254u - byte) << 23) : 0.f;
-  uint32_t k[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) k[j] = finite ? (uint32_t)__float2int_rn(f[j] * inv) : 0u;
-  uint2 r;
-  r.x = __byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410);
-  r.y = __byte_perm(__byte_perm(k[4], k[5], 0x0040), __byte_perm(k[6], k[7], 0x0040), 0x5410);
-  return r;
-}
-__device__ __forceinline__ void decode8(uint2 r, uint32_t byte, float (&f)[8]) {
-  const float step = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f[j] = (float)(signed char)(r.x >> (8 * j)) * step;
-    f[4 + j] = (float)(signed char)(r.y >> (8 * j)) * step;
+  for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(3u << ((threadIdx.y * blockDim.x + threadIdx.x) & 30u), top, 1));
+  if (top >= 0x7f800000u) {
+    byte = 255u;
+    return make_uint4(0, 0, 0, 0);
   }
+  byte = max((int)((top + 0x10000u) >> 23) - 6, 1);
+  const float inv = __uint_as_float((254u - byte) << 23);
+  uint32_t k[PER], r[4];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) k[j] = __float_as_uint(fmaf(f[j], inv, 12582912.f));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040), __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410);
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ void decode16(const uint4& k, uint32_t byte, float (&f)[PER]) {
+  const float step = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+  const uint32_t r[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
+#pragma unroll
+  for (int j = 0; j < PER; ++j) f[j] = (__uint_as_float(__byte_perm(r[j / 4], 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f) * step;
 }
 
 // x [rows, width] (pitch ld) -> codes [rows, 32 nb], exps [rows, nb], nb = ceil(width / 32); codes behind the row are 0.
-template <bool VEC, typename T>
+template <int MODE, typename T>
 __global__ void pack8_kernel(const T* __restrict__ x, signed char* __restrict__ codes, unsigned char* __restrict__ exps, unsigned rows, int width,
                              long long ld, int nb) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece >= nb * 4) return;     // pieces come by four, as the block's size does
-  float f[8];
-  load8<VEC>(x + row * ld, piece * 8, width, f);
+  if (row >= rows || piece >= nb * 2) return;     // pieces come by two, as the block's size does
+  Row16<T> v;
+  load16<MODE>(x + row * ld, piece * PER, width, v);
+  float f[PER];
+  widen(v, f);
   uint32_t byte;
-  const uint2 k = encode8(f, byte);
-  reinterpret_cast<uint2*>(codes)[(long long)row * (nb * 4) + piece] = k;
-  if ((piece & 3) == 0) exps[(long long)row * nb + (piece >> 2)] = (unsigned char)byte;
+  reinterpret_cast<uint4*>(codes)[(long long)row * (nb * 2) + piece] = encode16(f, byte);
+  if ((piece & 1) == 0) exps[(long long)row * nb + (piece >> 1)] = (unsigned char)byte;
 }
-template <bool VEC, typename T>
+template <int MODE, typename T>
 __global__ void unpack8_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ exps, T* __restrict__ x, unsigned rows, int width,
                                long long ld, int nb) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece * 8 >= width) return;
-  float f[8];
-  decode8(reinterpret_cast<const uint2*>(codes)[(long long)row * (nb * 4) + piece], exps[(long long)row * nb + (piece >> 2)], f);
-  store8<VEC>(x + row * ld, piece * 8, width, f);
+  if (row >= rows || piece * PER >= width) return;
+  float f[PER];
+  decode16(reinterpret_cast<const uint4*>(codes)[(long long)row * (nb * 2) + piece], exps[(long long)row * nb + (piece >> 1)], f);
+  store16<MODE>(x + row * ld, piece * PER, width, f);
 }
 
-// Value and derivative of the gate's function: 0 silu, 1 gelu by tanh, 2 relu. 16-bit results need 2^-9 of it: the approximate exponential and
-// quotient (a few 2^-22) do; 32-bit ones take the exact functions.
+// Value and derivative of the gate's function: 0 silu, 1 gelu by tanh, 2 relu. Both smooth ones by a logistic function s: gelu's (1 + tanh y) / 2 is
+// s(2 y), which loses nothing for negative g. 16-bit results need 2^-9 of it: the approximate exponential and quotient (a few 2^-22) do; 32-bit ones
+// take the exact functions.
+template <bool FAST>
+__device__ __forceinline__ float logistic(float x) { return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x)); }
 template <bool FAST>
 __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
   if (act == 0) {
-    const float s = FAST ? __fdividef(1.f, 1.f + __expf(-g)) : 1.f / (1.f + expf(-g));
-    a = FAST ? g * s : g / (1.f + expf(-g));
-    da = s * (1.f + g * (1.f - s));
+    const float s = logistic<FAST>(g);
+    a = g * s;
+    da = fmaf(a, 1.f - s, s);
   } else if (act == 1) {
     const float k0 = 0.7978845608028654f, k1 = 0.044715f;
-    const float th = tanhf(k0 * (g + k1 * g * g * g));
-    a = 0.5f * g * (1.f + th);
-    da = 0.5f * (1.f + th) + 0.5f * g * (1.f - th * th) * k0 * (1.f + 3.f * k1 * g * g);
+    const float s = logistic<FAST>(2.f * k0 * g * fmaf(k1 * g, g, 1.f));
+    a = g * s;
+    da = fmaf(2.f * a * (1.f - s), k0 * fmaf(3.f * k1 * g, g, 1.f), s);
   } else {
     a = fmaxf(g, 0.f);
     da = g > 0.f ? 1.f : 0.f;
@@ -139,59 +173,68 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
 }
 
 // gu [rows, 2 width] (gate | up): h = act(gate) * up, and gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb].
-template <bool VEC, typename T>
+template <int MODE, typename T>
 __global__ void glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps,
                                 unsigned rows, int width, long long ld, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece >= nb * 4) return;
-  float g[8], u[8];
-  load8<VEC>(gu + row * ld, piece * 8, width, g);
-  load8<VEC>(gu + row * ld + width, piece * 8, width, u);
+  if (row >= rows || piece >= nb * 2) return;
+  Row16<T> gv, uv;
+  load16<MODE>(gu + row * ld, piece * PER, width, gv);
+  load16<MODE>(gu + row * ld + width, piece * PER, width, uv);
+  float g[PER], u[PER];
+  widen(gv, g);
+  widen(uv, u);
   uint32_t gb, ub;
-  const uint2 gk = encode8(g, gb), uk = encode8(u, ub);
-  uint2* kr = reinterpret_cast<uint2*>(codes) + (long long)row * (nb * 8);
-  kr[piece] = gk;
-  kr[nb * 4 + piece] = uk;
-  if ((piece & 3) == 0) {
+  uint4* kr = reinterpret_cast<uint4*>(codes) + (long long)row * (nb * 4);
+  kr[piece] = encode16(g, gb);
+  kr[nb * 2 + piece] = encode16(u, ub);
+  if ((piece & 1) == 0) {
     unsigned char* er = exps + (long long)row * (2 * nb);
-    er[piece >> 2] = (unsigned char)gb;
-    er[nb + (piece >> 2)] = (unsigned char)ub;
+    er[piece >> 1] = (unsigned char)gb;
+    er[nb + (piece >> 1)] = (unsigned char)ub;
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < PER; ++j) {
     float a, da;
     gate8<sizeof(T) == 2>(g[j], act, a, da);
     g[j] = a * u[j];
   }
-  store8<VEC>(h + (long long)row * width, piece * 8, width, g);
+  store16<MODE>(h + (long long)row * width, piece * PER, width, g);
 }
 // dgu = (dh * up * act'(gate) | dh * act(gate)) with gate and up as their 8 bits say.
-template <bool VEC, typename T>
+template <int MODE, typename T>
 __global__ void glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
                                 T* __restrict__ dgu, unsigned rows, int width, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece * 8 >= width) return;
-  float g[8], u[8], d[8], dg[8];
-  const uint2* kr = reinterpret_cast<const uint2*>(codes) + (long long)row * (nb * 8);
+  if (row >= rows || piece * PER >= width) return;
+  const uint4* kr = reinterpret_cast<const uint4*>(codes) + (long long)row * (nb * 4);
   const unsigned char* er = exps + (long long)row * (2 * nb);
-  load8<VEC>(dh + (long long)row * width, piece * 8, width, d);
-  decode8(kr[piece], er[piece >> 2], g);
-  decode8(kr[nb * 4 + piece], er[nb + (piece >> 2)], u);
+  Row16<T> dv;
+  load16<MODE>(dh + (long long)row * width, piece * PER, width, dv);
+  const uint4 gk = kr[piece], uk = kr[nb * 2 + piece];
+  float g[PER], u[PER], d[PER];
+  decode16(gk, er[piece >> 1], g);
+  decode16(uk, er[nb + (piece >> 1)], u);
+  widen(dv, d);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < PER; ++j) {
     float a, da;
     gate8<sizeof(T) == 2>(g[j], act, a, da);
-    dg[j] = d[j] * u[j] * da;
+    g[j] = d[j] * u[j] * da;
     d[j] *= a;
   }
   T* o = dgu + (long long)row * (2 * (long long)width);
-  store8<VEC>(o, piece * 8, width, dg);
-  store8<VEC>(o + width, piece * 8, width, d);
+  store16<MODE>(o, piece * PER, width, g);
+  store16<MODE>(o + width, piece * PER, width, d);
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static int row_mode(int width, long long ld, const void* p, const void* q, int size) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
+  if (width % PER == 0 && ld * size % 32 == 0 && at % 32 == 0) return WIDE;
+  return width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0 ? PAIR : SINGLE;
+}
 static bool act8_args_ok(long long rows, int width, int dtype) { return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 27) && dtype >= 0 && dtype <= 2; }
 
 // dtype 0 bf16, 1 fp16, 2 fp32
@@ -211,12 +254,12 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   dim3 grid, block;
-  token_grid(rows, nb * 4, &grid, &block);
+  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto run = [&](auto kern) { kern<<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb); };
-    if (width % 8 == 0 && ld % 8 == 0 && aligned16(x)) run(pack8_kernel<true, T>);
-    else run(pack8_kernel<false, T>);
+    const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
+    mode == WIDE ? run(pack8_kernel<WIDE, T>) : mode == PAIR ? run(pack8_kernel<PAIR, T>) : run(pack8_kernel<SINGLE, T>);
   });
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
@@ -224,12 +267,12 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   dim3 grid, block;
-  token_grid(rows, nb * 4, &grid, &block);
+  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto run = [&](auto kern) { kern<<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld, nb); };
-    if (width % 8 == 0 && ld % 8 == 0 && aligned16(x)) run(unpack8_kernel<true, T>);
-    else run(unpack8_kernel<false, T>);
+    const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
+    mode == WIDE ? run(unpack8_kernel<WIDE, T>) : mode == PAIR ? run(unpack8_kernel<PAIR, T>) : run(unpack8_kernel<SINGLE, T>);
   });
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
@@ -237,14 +280,14 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   dim3 grid, block;
-  token_grid(rows, nb * 4, &grid, &block);
+  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto run = [&](auto kern) {
       kern<<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb, act);
     };
-    if (width % 8 == 0 && ld % 8 == 0 && aligned16(gu) && aligned16(h)) run(glu8_fwd_kernel<true, T>);
-    else run(glu8_fwd_kernel<false, T>);
+    const int mode = row_mode(width, ld, gu, h, sizeof(T));
+    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>) : run(glu8_fwd_kernel<SINGLE, T>);
   });
 }
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
@@ -253,13 +296,13 @@ extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, 
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   dim3 grid, block;
-  token_grid(rows, nb * 4, &grid, &block);
+  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto run = [&](auto kern) {
       kern<<<grid, block, 0, st>>>((const T*)dh, (const signed char*)codes, (const unsigned char*)exps, (T*)dgu, (unsigned)rows, width, nb, act);
     };
-    if (width % 8 == 0 && aligned16(dh) && aligned16(dgu)) run(glu8_bwd_kernel<true, T>);
-    else run(glu8_bwd_kernel<false, T>);
+    const int mode = row_mode(width, width, dh, dgu, sizeof(T));
+    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>) : run(glu8_bwd_kernel<SINGLE, T>);
   });
 }

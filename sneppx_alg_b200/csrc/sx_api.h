@@ -527,7 +527,7 @@ int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long
 // ------------------------------------------------------------------ L4 per-token losses of a vocabulary projection (vocab_loss.cu)
 // h [T, d], w [V, d] bf16 (pitches ldh, ldw; d and pitches multiples of 8, 16-byte aligned); z = h w^T, cap tanh(z / cap) with cap > 0.
 // lse [T] = log sum exp z; nll [T] = lse - z[target], 0 for ignore_index (and for targets outside [0, V), which set ST_BAD_ARGUMENT).
-// part: scratch of 2 ceil(V / 256) T pairs of floats; zt: scratch of T floats.
+// part: scratch of ceil(V / 256) T pairs of floats; zt: scratch of T floats.
 int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                       long long ignore_index, float cap, void* part, float* zt, float* nll, float* lse, int* status, cudaStream_t stream);
 // Gradient of the logits [v0, v1) from lse and the gradients of nll and lse (either may be null): dz bf16 [rows, ld], T <= rows < T + 256, ld a multiple
@@ -535,6 +535,8 @@ int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw
 int sx_vocab_loss_grad(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                        long long ignore_index, float cap, const float* lse, const float* g_nll, const float* g_lse, void* dz, long long ld,
                        long long rows, long long v0, long long v1, int* status, cudaStream_t stream);
+// out [count] bf16 = sum of parts [n, count] fp32; count a multiple of 8.
+int sx_vocab_loss_sum(const float* parts, void* out, int n, long long count, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -4,11 +4,15 @@
 //   dz_v = ((g_nll + g_lse) e^{z_v - lse} - g_nll [v = target]) (1 - (z_v / c)^2)
 //
 // One kernel, two epilogues, on the CTA-pair GEMM (256 x 256 tiles, accumulators double-buffered in TMEM, operands by TMA):
-//   forward  each row's maximum and sum of exponentials over half a tile's columns (128) leave the SM as one pair of numbers, the target's logit by
-//            itself; a second kernel joins the pairs of a row. 8 bytes leave for 128 logits.
+//   forward  each row's maximum and sum of exponentials over a tile's columns leave the SM as one pair of numbers, the target's logit by itself; a second
+//            kernel joins the pairs of a row. 8 bytes leave for 256 logits.
 //   backward the tile is computed again and leaves as dz in bf16 (half a step, 2^-9, of each value: what the products that follow take), for one piece of the
 //            vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
-// Eight epilogue warps (four TMEM quadrants, two halves of the columns) keep the exponentials behind the products of widths from 256 on.
+// Sixteen epilogue warps (four TMEM quadrants, four groups of 64 columns): the exponentials of a tile are behind the products from widths of 256 on only
+// if four warps of each scheduler take turns.
+// The tensor cores cut what they add to an accumulator: over 4096 products a logit of 14 loses 1e-4. The forward pass, whose losses are differences of
+// logits, therefore takes the accumulator out after 1024 products and adds in registers, rounded: lse of 4088 tokens over [128256, 4096] is off by 1.4e-6
+// without that, by 3.7e-7 with it in the same time, by 2.2e-7 after 512 products, which cost 3% more. dz is rounded to bf16 anyway.
 // Takes the place of the reference's softmax / cross-entropy kernels (kernel/cuda/autodiff_cuda.cu:519-608).
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -22,16 +26,23 @@ constexpr int VL_BK = 64;
 constexpr int VL_STAGES = 6;
 constexpr int VL_A_BYTES = 128 * VL_BK * 2;
 constexpr int VL_STAGE_BYTES = 2 * VL_A_BYTES;       // this CTA's 128 rows of h and of w
-constexpr int VL_SMEM = VL_STAGES * VL_STAGE_BYTES + 1024 + 256;
-constexpr int VL_EPI_WARPS = 8;
+constexpr int VL_GROUPS = 4;                         // epilogue warps of a TMEM quadrant
+constexpr int VL_COLS = 256 / VL_GROUPS;             // columns of an epilogue warp
+constexpr int VL_EPI_WARPS = 4 * VL_GROUPS;
 constexpr int VL_THREADS = 64 + 32 * VL_EPI_WARPS;
+constexpr int VL_CHUNK = 1024 / VL_BK;               // forward: k-blocks that stay in one accumulator
+constexpr int VL_SLOTS = 4;                          // tiles whose pairs may wait to be joined (below)
+constexpr int VL_OFF_PAIRS = VL_STAGES * VL_STAGE_BYTES;
+constexpr int VL_PAIR_BYTES = VL_SLOTS * (VL_GROUPS - 1) * 128 * 8;
+constexpr int VL_OFF_BAR = VL_OFF_PAIRS + VL_PAIR_BYTES;
+constexpr int VL_SMEM = VL_OFF_BAR + 1024 + 512;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct VocabLossParams {
   CUtensorMap tmA, tmB;       // h [T, d], w [V, d]
   const long long* target;
   long long ignore_index;
-  float2* part;               // forward: [2 n_blks, T] maximum and sum
+  float2* part;               // forward: [n_blks, T] maximum and sum
   float* zt;                  // forward: [T] the target's logit
   const float* lse;           // backward
   const float* g_nll;         // backward: [T] or null
@@ -44,15 +55,50 @@ struct VocabLossParams {
   float cap, inv_cap;         // 0: none
 };
 
+// cap * tanh(z / cap) of a row's values. Up to |z / cap| = 0.6 (logits of 18 under a cap of 30) a polynomial: tanh u / u in u^2, minimax in the relative
+// error (2.5e-9, 1e-7 as evaluated). One exponential and one reciprocal less for each value, where the unit that computes them bounds the epilogue (4095 x
+// 50280 logits of width 768: backward's tiles 563 -> 291 us with this and whole-sector stores). Which form is taken is each row's own matter, so that a
+// token's loss does not depend on its neighbours.
+template <int N>
+__device__ __forceinline__ void softcap_row(float (&v)[N], float cap, float inv) {
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(v[j]));
+  if (top * inv <= 0.6f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float u = v[j] * inv, s = u * u;
+      float t = fmaf(s, -0.005852168625497215f, 0.020753628859718726f);
+      t = fmaf(s, t, -0.053768704695067476f);
+      t = fmaf(s, t, 0.13331688960047147f);
+      t = fmaf(s, t, -0.33333283257370855f);
+      v[j] *= fmaf(s, t, 1.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = softcap(v[j], cap, inv);
+  }
+}
+__device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x), at = top == -INFINITY ? 0.f : top * LOG2E;
+  return make_float2(top, a.y * exp2f(fmaf(a.x, LOG2E, -at)) + b.y * exp2f(fmaf(b.x, LOG2E, -at)));
+}
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 template <bool GRAD, bool CAP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab_loss_kernel(const __grid_constant__ VocabLossParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + VL_STAGES * VL_STAGE_BYTES);   // even CTA: both CTAs' loads complete on it
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + VL_OFF_BAR);                   // even CTA: both CTAs' loads complete on it
   uint64_t* empty_bar = full_bar + VL_STAGES;
   uint64_t* tfull_bar = empty_bar + VL_STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;                                                  // even CTA: the epilogue warps of both
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* pairs_bar = tempty_bar + 2;                                                  // [VL_SLOTS][4 quadrants]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pairs_bar + 4 * VL_SLOTS);
   volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_index();
   const int lane = threadIdx.x & 31;
@@ -68,6 +114,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
       mbar_init(&tfull_bar[i], 1);
       mbar_init(&tempty_bar[i], 2 * VL_EPI_WARPS);
     }
+    for (int i = 0; i < 4 * VL_SLOTS; ++i) mbar_init(&pairs_bar[i], VL_GROUPS - 1);
     *s_abort = 0;
     mbar_fence_init();
     tma_prefetch_desc(&p.tmA);
@@ -84,6 +131,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = p.m_blks * p.n_blks;
   const int num_kb = (p.d + VL_BK - 1) / VL_BK;
+  const int chunk = GRAD ? num_kb : VL_CHUNK;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -112,96 +160,136 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
       constexpr uint32_t idesc = umma_idesc_f16(256, 256, 1, 0, 0);
       int stage = 0;
       uint32_t phase = 0;
-      int it = 0;
+      int it = 0;               // accumulators handed over
       bool ok = true;
-      for (int t = cluster_id; t < total_tiles && ok; t += n_clusters, ++it) {
-        const int acc = it & 1;
-        if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1, s_abort, p.status, ST_TIMEOUT_MMA)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, s_abort, p.status, ST_TIMEOUT_MMA)) { ok = false; break; }
+      for (int t = cluster_id; t < total_tiles && ok; t += n_clusters) {
+        for (int k0 = 0; k0 < num_kb && ok; k0 += chunk, ++it) {
+          const int acc = it & 1, k1 = min(num_kb, k0 + chunk);
+          if (!mbar_wait(&tempty_bar[acc], ((it >> 1) & 1) ^ 1, s_abort, p.status, ST_TIMEOUT_MMA)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * VL_STAGE_BYTES), sb = sa + VL_A_BYTES;
+          const uint32_t d_tmem = tmem_base + acc * 256;
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, s_abort, p.status, ST_TIMEOUT_MMA)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + stage * VL_STAGE_BYTES), sb = sa + VL_A_BYTES;
 #pragma unroll
-          for (int k = 0; k < VL_BK / 16; ++k)
-            umma2_f16_ss(d_tmem, umma_desc_sw128(sa + k * 32, 16, 1024), umma_desc_sw128(sb + k * 32, 16, 1024), idesc, (kb | k) != 0 ? 1u : 0u);
-          umma2_commit_pair(&empty_bar[stage]);
-          if (++stage == VL_STAGES) { stage = 0; phase ^= 1; }
+            for (int k = 0; k < VL_BK / 16; ++k)
+              umma2_f16_ss(d_tmem, umma_desc_sw128(sa + k * 32, 16, 1024), umma_desc_sw128(sb + k * 32, 16, 1024), idesc, (kb != k0 || k != 0) ? 1u : 0u);
+            umma2_commit_pair(&empty_bar[stage]);
+            if (++stage == VL_STAGES) { stage = 0; phase ^= 1; }
+          }
+          if (ok) umma2_commit_pair(&tfull_bar[acc]);
         }
-        if (ok) umma2_commit_pair(&tfull_bar[acc]);
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue: a row a lane, 128 columns a warp
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    int it = 0;
-    for (int t = cluster_id; t < total_tiles; t += n_clusters, ++it) {
+    // ------------------------------------------------------------ epilogue: a row a lane, 64 columns a warp
+    const int q = warp & 3, group = (warp - 2) >> 2;
+    const uint32_t tmem_mine = tmem_base + group * VL_COLS + (static_cast<uint32_t>(q * 32) << 16);
+    float2* pairs = reinterpret_cast<float2*>(smem + VL_OFF_PAIRS);
+    int it = 0, tile = 0;
+    bool ok = true;
+    for (int t = cluster_id; t < total_tiles && ok; t += n_clusters, ++tile) {
       int b, m_blk, n_blk;
       tile_coords(t, p.m_blks, p.n_blks, b, m_blk, n_blk);
-      const int acc = it & 1;
       const int row = m_blk * 256 + (int)rank * 128 + q * 32 + lane;
-      const int first = p.v0 + n_blk * 256 + half * 128;          // this warp's first column
-      // the target as a column of this warp's 128, or far from them
+      const int first = p.v0 + n_blk * 256 + group * VL_COLS;     // this warp's first column
+      const int left = p.v1 - first;                              // columns that the vocabulary has from there on
+      // the target as a column of this warp's, or none
       int tgt = -1;
       float a = 0.f, gn = 0.f, off = 0.f;
       if (row < p.T) {
         const long long tv = p.target[row];
-        if (tv != p.ignore_index && tv >= first && tv < first + 128 && tv < p.v1) tgt = (int)(tv - first);
+        if (tv != p.ignore_index && tv >= first && tv < first + VL_COLS && tv < p.v1) tgt = (int)(tv - first);
         if (GRAD) {
           if (p.g_nll && tv != p.ignore_index && tv >= 0 && tv < p.V) gn = p.g_nll[row];
           a = gn + (p.g_lse ? p.g_lse[row] : 0.f);
           off = -p.lse[row] * LOG2E;
         }
       }
-      if (!mbar_wait_warp(&tfull_bar[acc], (it >> 1) & 1, s_abort, p.status, ST_TIMEOUT_EPILOGUE)) break;
-      tc_fence_after();
-      float mx = -INFINITY, sum = 0.f, zt = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        const int col0 = first + c * 32;
-        if (GRAD ? col0 - p.v0 >= p.ld : col0 >= p.v1) break;     // uniform across the warp
-        uint32_t r[32];
-        tmem_ld32(tmem_base + acc * 256 + half * 128 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), r);
-        tmem_ld_wait();
-        float v[32];
+      if (!GRAD) {
+        float v[VL_COLS];
+        for (int k0 = 0; k0 < num_kb; k0 += chunk, ++it) {
+          const int acc = it & 1;
+          ok = mbar_wait_warp(&tfull_bar[acc], (it >> 1) & 1, s_abort, p.status, ST_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = CAP ? softcap(__uint_as_float(r[j]), p.cap, p.inv_cap) : __uint_as_float(r[j]);
-        const int left = p.v1 - col0;                             // columns that the vocabulary has here
-        const bool mine = (tgt >> 5) == c;                        // -1 >> 5 is -1
-        if (!GRAD) {
-          if (left < 32) {
+          for (int c = 0; c < VL_COLS / 8; ++c) {            // eight at a time: with sixteen the values that stay leave the registers
+            uint32_t r[8];
+            tmem_ld8(tmem_mine + acc * 256 + c * 8, r);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= left) v[j] = -INFINITY;
+            for (int j = 0; j < 8; ++j) v[c * 8 + j] = k0 == 0 ? __uint_as_float(r[j]) : v[c * 8 + j] + __uint_as_float(r[j]);
           }
-          if (__any_sync(0xffffffffu, mine)) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_even_cta(&tempty_bar[acc]);
+        }
+        if (!ok) break;
+        if (CAP) softcap_row(v, p.cap, p.inv_cap);
+        if (left < VL_COLS) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (mine && (tgt & 31) == j) zt = v[j];
-          }
-          float top = v[0];
+          for (int j = 0; j < VL_COLS; ++j)
+            if (j >= left) v[j] = -INFINITY;
+        }
+        if (__any_sync(0xffffffffu, tgt >= 0)) {
+          float zt = 0.f;
 #pragma unroll
-          for (int j = 1; j < 31; j += 2) top = fmax3(top, v[j], v[j + 1]);
-          top = fmaxf(fmaxf(top, v[31]), mx);
-          const float at = top == -INFINITY ? 0.f : top * LOG2E;
-          sum *= exp2f(fmaf(mx, LOG2E, -at));
-          float s0 = 0.f, s1 = 0.f;
+          for (int j = 0; j < VL_COLS; ++j)
+            if (tgt == j) zt = v[j];
+          if (tgt >= 0) p.zt[row] = zt;
+        }
+        float top = fmaxf(v[0], v[1]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            s0 += exp2f(fmaf(v[j], LOG2E, -at));
-            s1 += exp2f(fmaf(v[j + 1], LOG2E, -at));
-          }
-          sum += s0 + s1;
-          mx = top;
+        for (int j = 2; j < VL_COLS; j += 2) top = fmax3(top, v[j], v[j + 1]);
+        const float at = top == -INFINITY ? 0.f : top * LOG2E;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < VL_COLS; ++j) sum[j & 3] += exp2f(fmaf(v[j], LOG2E, -at));
+        float2 pair = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        // The first warp of a quadrant joins the four. The others may be two tiles ahead of it at most: an accumulator is filled again when all
+        // sixteen have read it. Four slots, each with a barrier that they arrive on, are enough.
+        const int slot = tile % VL_SLOTS;
+        float2* mine = pairs + slot * (VL_GROUPS - 1) * 128 + q * 32 + lane;
+        if (group > 0) {
+          mine[(group - 1) * 128] = pair;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pairs_bar[slot * 4 + q]);
         } else {
-          float g[32];
+          ok = mbar_wait_warp(&pairs_bar[slot * 4 + q], (tile / VL_SLOTS) & 1, s_abort, p.status, ST_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < VL_GROUPS - 1; ++i) pair = join_pairs(pair, mine[i * 128]);
+          if (row < p.T) p.part[(long long)n_blk * p.T + row] = pair;
+        }
+      } else {
+        const int acc = it & 1;
+        ok = mbar_wait_warp(&tfull_bar[acc], (it >> 1) & 1, s_abort, p.status, ST_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+        tc_fence_after();
+        ++it;
+#pragma unroll
+        for (int c = 0; c < VL_COLS / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tmem_mine + acc * 256 + c * 32, r);
+          tmem_ld_wait();
+          if (c == VL_COLS / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_even_cta(&tempty_bar[acc]);
+          }
+          if (first - p.v0 + c * 32 >= p.ld) continue;             // uniform across the warp
+          float v[32], g[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          if (CAP) softcap_row(v, p.cap, p.inv_cap);
 #pragma unroll
           for (int j = 0; j < 32; ++j) g[j] = a * exp2f(fmaf(v[j], LOG2E, off));
-          if (__any_sync(0xffffffffu, mine)) {
+          if (__any_sync(0xffffffffu, (tgt >> 5) == c)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (mine && (tgt & 31) == j) g[j] -= gn;
+              if (tgt == c * 32 + j) g[j] -= gn;
           }
           if (CAP) {
 #pragma unroll
@@ -210,26 +298,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
               g[j] *= fmaf(-u, u, 1.f);
             }
           }
-          if (left < 32) {
+          if (left < (c + 1) * 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j >= left) g[j] = 0.f;
+              if (c * 32 + j >= left) g[j] = 0.f;
           }
           if (row < p.rows) {
-            uint4* o = reinterpret_cast<uint4*>(p.dz + (long long)row * p.ld + (col0 - p.v0));
+            __nv_bfloat16* o = p.dz + (long long)row * p.ld + (first - p.v0 + c * 32);
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              o[j / 8] = make_uint4(pack_bf16x2(g[j], g[j + 1]), pack_bf16x2(g[j + 2], g[j + 3]), pack_bf16x2(g[j + 4], g[j + 5]),
-                                    pack_bf16x2(g[j + 6], g[j + 7]));
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) w[j] = pack_bf16x2(g[h * 16 + 2 * j], g[h * 16 + 2 * j + 1]);
+              st_global_32(o + h * 16, w);
+            }
           }
         }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_even_cta(&tempty_bar[acc]);
-      if (!GRAD && row < p.T) {
-        p.part[(long long)(n_blk * 2 + half) * p.T + row] = make_float2(mx, sum);
-        if (tgt >= 0) p.zt[row] = zt;
       }
     }
   }
@@ -244,36 +328,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
   }
 }
 
-// Joins the parts of 32 rows a block, 16 threads a row. The last logarithm is taken in 64 bits: one a row.
+// Joins the pairs of eight rows a block, 64 threads a row. The last logarithm is taken in 64 bits: one a row.
 __global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
                                                               const long long* __restrict__ target, float* __restrict__ nll, float* __restrict__ lse, int T,
                                                               int V, int parts, long long ignore_index, int* status) {
-  __shared__ float2 s[16][33];
-  const int row = blockIdx.x * 32 + threadIdx.x;
-  float mx = -INFINITY, sum = 0.f;
+  __shared__ float2 s[64][8];
+  const int row = blockIdx.x * 8 + threadIdx.x;
+  float2 pair = make_float2(-INFINITY, 0.f);
   if (row < T) {
-    for (int i = threadIdx.y; i < parts; i += 16) {
-      const float2 v = part[(long long)i * T + row];
-      const float top = fmaxf(mx, v.x), at = top == -INFINITY ? 0.f : top * LOG2E;
-      sum = sum * exp2f(fmaf(mx, LOG2E, -at)) + v.y * exp2f(fmaf(v.x, LOG2E, -at));
-      mx = top;
-    }
+#pragma unroll 4
+    for (int i = threadIdx.y; i < parts; i += 64) pair = join_pairs(pair, part[(long long)i * T + row]);
   }
-  s[threadIdx.y][threadIdx.x] = make_float2(mx, sum);
-  __syncthreads();
+  s[threadIdx.y][threadIdx.x] = pair;
+  for (int n = 32; n > 0; n >>= 1) {
+    __syncthreads();
+    if (threadIdx.y < n) s[threadIdx.y][threadIdx.x] = pair = join_pairs(pair, s[threadIdx.y + n][threadIdx.x]);
+  }
   if (threadIdx.y != 0 || row >= T) return;
-  for (int i = 1; i < 16; ++i) {
-    const float2 v = s[i][threadIdx.x];
-    const float top = fmaxf(mx, v.x), at = top == -INFINITY ? 0.f : top * LOG2E;
-    sum = sum * exp2f(fmaf(mx, LOG2E, -at)) + v.y * exp2f(fmaf(v.x, LOG2E, -at));
-    mx = top;
-  }
-  const float l = (float)((double)mx + log((double)sum));
+  const float l = (float)((double)pair.x + log((double)pair.y));
   const long long t = target[row];
   const bool valid = t != ignore_index && t >= 0 && t < V;
   if (t != ignore_index && !valid && status) atomicCAS(status, 0, (int)ST_BAD_ARGUMENT);
   lse[row] = l;
   nll[row] = valid ? l - zt[row] : 0.f;
+}
+
+// dh of several sums over parts of the vocabulary (parts [n, count] fp32): their sum, rounded once. Eight values a thread; count is a multiple of 8.
+__global__ void __launch_bounds__(256) vocab_loss_sum_kernel(const float4* __restrict__ parts, uint4* __restrict__ out, int n, long long count8) {
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= count8) return;
+  float4 a = parts[2 * i], b = parts[2 * i + 1];
+  for (int k = 1; k < n; ++k) {
+    const float4 c = parts[2 * (k * count8 + i)], e = parts[2 * (k * count8 + i) + 1];
+    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+    b.x += e.x; b.y += e.y; b.z += e.z; b.w += e.w;
+  }
+  out[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
 }
 
 static int vocab_loss_map(CUtensorMap* tm, const void* ptr, int d, long long rows, long long ld) {
@@ -298,10 +388,15 @@ static int vocab_loss_setup(VocabLossParams* p, const void* h, long long ldh, co
 template <bool GRAD, bool CAP>
 static int vocab_loss_launch(VocabLossParams& p, cudaStream_t st) {
   auto kern = vocab_loss_kernel<GRAD, CAP>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, VL_SMEM) != cudaSuccess) return -10;
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static int known[64];      // multiprocessors of the devices that the kernel has been set up on
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
+  int sms = __atomic_load_n(&known[dev], __ATOMIC_ACQUIRE);
+  if (sms == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, VL_SMEM) != cudaSuccess) return -10;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 2) return -10;
+    __atomic_store_n(&known[dev], sms, __ATOMIC_RELEASE);
+  }
   const long long tiles = (long long)p.m_blks * p.n_blks;
   if (tiles > 0x7fffffffll) return -1;
   const int clusters = (int)(tiles < sms / 2 ? tiles : sms / 2);
@@ -322,7 +417,7 @@ extern "C" int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, lo
   p.m_blks = (int)((T + 255) / 256); p.n_blks = (int)((V + 255) / 256);
   rc = cap > 0.f ? vocab_loss_launch<false, true>(p, st) : vocab_loss_launch<false, false>(p, st);
   if (rc) return rc;
-  vocab_loss_join_kernel<<<(unsigned)((T + 31) / 32), dim3(32, 16), 0, st>>>(p.part, zt, target, nll, lse, (int)T, (int)V, 2 * p.n_blks, ignore_index, status);
+  vocab_loss_join_kernel<<<(unsigned)((T + 7) / 8), dim3(8, 64), 0, st>>>(p.part, zt, target, nll, lse, (int)T, (int)V, p.n_blks, ignore_index, status);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
@@ -332,10 +427,17 @@ extern "C" int sx_vocab_loss_grad(const void* h, long long ldh, const void* w, l
   VocabLossParams p = {};
   int rc = vocab_loss_setup(&p, h, ldh, w, ldw, T, V, d, cap);
   if (rc) return rc;
-  if (v0 < 0 || v1 <= v0 || v1 > V || ld % 32 || ld < v1 - v0 || ld > (1 << 30) || rows < T || rows > T + 255 || (reinterpret_cast<uintptr_t>(dz) & 15)) return -2;
+  if (v0 < 0 || v1 <= v0 || v1 > V || ld % 32 || ld < v1 - v0 || ld > (1 << 30) || rows < T || rows > T + 255 || (reinterpret_cast<uintptr_t>(dz) & 31)) return -2;
   p.target = target; p.ignore_index = ignore_index; p.status = status;
   p.lse = lse; p.g_nll = g_nll; p.g_lse = g_lse; p.dz = (__nv_bfloat16*)dz; p.ld = ld; p.rows = (int)rows;
   p.v0 = (int)v0; p.v1 = (int)v1;
   p.m_blks = (int)((rows + 255) / 256); p.n_blks = (int)((ld + 255) / 256);
   return cap > 0.f ? vocab_loss_launch<true, true>(p, st) : vocab_loss_launch<true, false>(p, st);
+}
+
+extern "C" int sx_vocab_loss_sum(const float* parts, void* out, int n, long long count, cudaStream_t st) {
+  if (count == 0) return 0;
+  if (n < 1 || count < 0 || count % 8 || ((reinterpret_cast<uintptr_t>(parts) | reinterpret_cast<uintptr_t>(out)) & 15) || count / 8 > 256ll * 0x7fffffff) return -1;
+  vocab_loss_sum_kernel<<<(unsigned)((count / 8 + 255) / 256), 256, 0, st>>>((const float4*)parts, (uint4*)out, n, count / 8);
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

@@ -211,9 +211,56 @@ _here = contextlib.nullcontext()
 
 
 def on_device(t):
-    """Context in which t's device is the current one, so that ``stream()`` and new tensors are that device's (nothing to do, 0.3 us, where it is already)."""
-    i = t.device.index
-    return _here if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
+    """Context in which the device of t (a CUDA tensor) is the current one, as launches on its streams need (nothing to do where it is already)."""
+    i = t.get_device()
+    return _here if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
+
+
+def here(t) -> int:
+    """Handle of the current stream of t's device (a CUDA tensor)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_status_ptr = {}
+
+
+def status_ptr(t) -> int:
+    """Address of the status word of t's device."""
+    i = t.get_device()
+    p = _status_ptr.get(i)
+    if p is None:
+        p = _status_ptr[i] = status_word(t.device).data_ptr()
+    return p
+
+
+_SIG = {"p": c_void_p, "i": c_int, "l": c_ll, "f": c_float}
+_entries = {}
+
+
+def entry(name: str, sig: str, result=None):
+    """The entry point ``name`` with its argument types declared once (p pointer, i int, l long long, f float), to be called with plain numbers:
+    ctypes then converts them itself, 0.1 us an argument less than objects made for each call. Without ``result`` it counts as a launch and raises
+    on an error code, as ``call`` does."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+
+        def check(rc):
+            global launch_count
+            launch_count += 1
+            if rc != 0:
+                raise RuntimeError(f"{name} failed with code {rc}")
+
+        fn.argtypes, fn.restype = [_SIG[k] for k in sig], result or check
+        _entries[name] = fn
+    return fn
+
+
+def once(backward):
+    """``once_differentiable`` for a static ``backward``, at its cost (5 us a call) only where a graph of the backward pass is being built."""
+    from torch.autograd.function import once_differentiable
+    slow = once_differentiable(backward)
+    return lambda ctx, *g: slow(ctx, *g) if torch.is_grad_enabled() else backward(ctx, *g)
 
 
 def ptr(t) -> c_void_p:

@@ -8,10 +8,8 @@ serves CPU tensors. The reference recomputes layers from inputs kept in full (gr
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import c_int, c_ll, ptr, stream
 from .functional import GLU_ACT
 
 BLOCK = 32
@@ -46,6 +44,8 @@ class Packed8bit:
 
 def _rows(x):
     """x as [rows, width] whose rows are contiguous (a view where x allows one)."""
+    if x.dim() > 1 and x.is_contiguous() and x.numel():
+        return x.view(-1, x.shape[-1])
     w = x.shape[-1] if x.dim() else 1
     x2 = x.reshape(-1, w) if x.numel() else x.reshape(0, w)
     return x2 if x2.numel() == 0 or (x2.stride(1) == 1 or w == 1) and (x2.shape[0] == 1 or x2.stride(0) >= w) else x2.contiguous()
@@ -82,10 +82,9 @@ def pack_8bit(x) -> Packed8bit:
     nb = -(-w // BLOCK)
     if not _native(x):
         return Packed8bit(*pack_8bit_reference(x2), x.shape, x.dtype)
+    codes, exps = x2.new_empty((rows, nb * BLOCK), dtype=torch.int8), x2.new_empty((rows, nb), dtype=torch.uint8)
     with _lib.on_device(x):
-        codes = torch.empty(rows, nb * BLOCK, dtype=torch.int8, device=x.device)
-        exps = torch.empty(rows, nb, dtype=torch.uint8, device=x.device)
-        _lib.call("sx_pack8", ptr(x2), ptr(codes), ptr(exps), c_ll(rows), c_int(w), c_ll(x2.stride(0)), c_int(_TYPES[x.dtype]), stream())
+        _lib.entry("sx_pack8", "ppplilip")(x2.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, w, x2.stride(0), _TYPES[x.dtype], _lib.here(x))
     return Packed8bit(codes, exps, x.shape, x.dtype)
 
 
@@ -101,10 +100,10 @@ def unpack_8bit(p: Packed8bit, dtype=None):
         return unpack_8bit_reference(p.codes, p.exponents, w, dtype).view(p.shape)
     if dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
-    with _lib.on_device(p.codes):
-        x = torch.empty(p.shape, dtype=dtype, device=p.codes.device)
-        codes, exps = p.codes.contiguous(), p.exponents.contiguous()
-        _lib.call("sx_unpack8", ptr(codes), ptr(exps), ptr(x), c_ll(rows), c_int(w), c_ll(w), c_int(_TYPES[dtype]), stream())
+    codes, exps = p.codes.contiguous(), p.exponents.contiguous()
+    x = codes.new_empty(p.shape, dtype=dtype)
+    with _lib.on_device(x):
+        _lib.entry("sx_unpack8", "ppplilip")(codes.data_ptr(), exps.data_ptr(), x.data_ptr(), rows, w, w, _TYPES[dtype], _lib.here(x))
     return x
 
 
@@ -140,29 +139,34 @@ class _Glu8Fn(torch.autograd.Function):
             parts = [pack_8bit_reference(t) for t in (gate, up)]
             ctx.save_for_backward(torch.cat([c for c, _ in parts], 1), torch.cat([e for _, e in parts], 1))
             return (_gate(gate.float(), act)[0] * up.float()).to(gu.dtype).view(*gu.shape[:-1], f)
+        h = gu.new_empty((*gu.shape[:-1], f))
+        held = gu.new_empty(rows * 2 * nb * (BLOCK + 1), dtype=torch.uint8)           # codes of gate and up for each row, then their exponents
         with _lib.on_device(gu):
-            h = torch.empty(*gu.shape[:-1], f, dtype=gu.dtype, device=gu.device)
-            codes = torch.empty(rows, 2 * nb * BLOCK, dtype=torch.int8, device=gu.device)
-            exps = torch.empty(rows, 2 * nb, dtype=torch.uint8, device=gu.device)
-            _lib.call("sx_glu8_fwd", ptr(g2), ptr(h), ptr(codes), ptr(exps), c_ll(rows), c_int(f), c_ll(g2.stride(0)), c_int(act),
-                      c_int(_TYPES[gu.dtype]), stream())
-        ctx.save_for_backward(codes, exps)
+            at = held.data_ptr()
+            _lib.entry("sx_glu8_fwd", "ppppliliip")(g2.data_ptr(), h.data_ptr(), at, at + rows * 2 * nb * BLOCK, rows, f, g2.stride(0), act,
+                                                   _TYPES[gu.dtype], _lib.here(gu))
+        ctx.save_for_backward(held)
         return h
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, dh):
-        codes, exps = ctx.saved_tensors
         act, shape = ctx.meta
-        f, rows = shape[-1] // 2, codes.shape[0]
-        nb = exps.shape[1] // 2
+        f = shape[-1] // 2
         if not _native(dh):
+            codes, exps = ctx.saved_tensors
+            rows = codes.shape[0]
             gate, up = (unpack_8bit_reference(c, e, f, torch.float32) for c, e in zip(codes.chunk(2, 1), exps.chunk(2, 1)))
             return glu_8bit_backward_reference(dh.reshape(rows, f), gate, up, act).view(shape), None
+        (held,) = ctx.saved_tensors
+        nb = -(-f // BLOCK)
+        rows = held.numel() // (2 * nb * (BLOCK + 1)) if nb else 0
+        dh = dh.contiguous()
+        dgu = dh.new_empty(shape)
         with _lib.on_device(dh):
-            dh = dh.contiguous()
-            dgu = torch.empty(shape, dtype=dh.dtype, device=dh.device)
-            _lib.call("sx_glu8_bwd", ptr(dh), ptr(codes), ptr(exps), ptr(dgu), c_ll(rows), c_int(f), c_int(act), c_int(_TYPES[dh.dtype]), stream())
+            at = held.data_ptr()
+            _lib.entry("sx_glu8_bwd", "ppppliiip")(dh.data_ptr(), at, at + rows * 2 * nb * BLOCK, dgu.data_ptr(), rows, f, act, _TYPES[dh.dtype],
+                                                  _lib.here(dh))
         return dgu, None
 
 

@@ -5,11 +5,9 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import debug as _dbg
-from ._lib import c_float, c_int, c_ll, ptr, stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -24,10 +22,10 @@ def _lookup(ids, table, scale):
         table = table.contiguous()
     ids = ids.contiguous()
     V, d = table.shape
+    y = table.new_empty((*ids.shape, d))
     with _lib.on_device(table):
-        y = torch.empty(*ids.shape, d, dtype=table.dtype, device=table.device)
-        _lib.call("sx_embed_fwd", ptr(ids), c_int(ids.dtype == torch.int64), ptr(table), c_ll(table.stride(0)), ptr(y), c_ll(ids.numel()), c_int(d),
-                  c_ll(V), c_float(scale), c_int(_TYPES[table.dtype]), ptr(_lib.status_word(table.device)), stream())
+        _lib.entry("sx_embed_fwd", "piplplilfipp")(ids.data_ptr(), ids.dtype == torch.int64, table.data_ptr(), table.stride(0), y.data_ptr(), ids.numel(),
+                                                   d, V, scale, _TYPES[table.dtype], _lib.status_ptr(table), _lib.here(table))
     return y
 
 
@@ -41,14 +39,12 @@ def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
         raise ValueError(f"embedding_backward_: gradients of shape {tuple(dy.shape)} for ids {tuple(ids.shape)} and rows of {d}")
     ids, dy = ids.contiguous(), dy.contiguous()
     n = ids.numel()
+    size = _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, add)
+    work = grad.new_empty(size, dtype=torch.uint8)
     with _lib.on_device(grad):
-        fn = _lib.lib().sx_embed_bwd_workspace
-        fn.restype = c_ll
-        size = fn(c_ll(n), c_ll(V), c_int(d), c_int(add))
-        work = torch.empty(size, dtype=torch.uint8, device=grad.device)
-        _lib.call("sx_embed_bwd", ptr(ids), c_int(ids.dtype == torch.int64), ptr(dy), ptr(grad), c_ll(grad.stride(0)), c_ll(n), c_int(d), c_ll(V),
-                  c_ll(-1 if padding_idx is None else padding_idx), c_float(scale), c_int(add), c_int(_TYPES[dy.dtype]), c_int(_TYPES[grad.dtype]),
-                  ptr(work), c_ll(size), ptr(_lib.status_word(grad.device)), stream())
+        _lib.entry("sx_embed_bwd", "pippllillfiiiplpp")(
+            ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, -1 if padding_idx is None else padding_idx,
+            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], work.data_ptr(), size, _lib.status_ptr(grad), _lib.here(grad))
     return grad
 
 
@@ -60,7 +56,7 @@ class _EmbeddingFn(torch.autograd.Function):
         return _lookup(ids, table, scale)
 
     @staticmethod
-    @once_differentiable
+    @_lib.once
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         table, (scale, padding_idx) = ctx.table, ctx.meta
@@ -81,11 +77,11 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     (``check_status`` raises); on the CPU it raises at once."""
     if table.dim() != 2:
         raise ValueError(f"embedding: table of shape {tuple(table.shape)} is no matrix")
-    if ids.dtype not in (torch.int64, torch.int32):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
             raise TypeError(f"embedding: ids of {ids.dtype}")
         ids = ids.long()
-    if ids.device != table.device:
+    if ids.get_device() != table.get_device():
         raise ValueError(f"embedding: ids on {ids.device}, table on {table.device}")
     if padding_idx is not None:
         if not -table.shape[0] <= padding_idx < table.shape[0]:
