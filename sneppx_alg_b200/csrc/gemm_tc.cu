@@ -982,7 +982,10 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
   if ((a->lda % 8) || (a->ldb % 8) || (reinterpret_cast<uintptr_t>(a->A) & 15) ||
       (reinterpret_cast<uintptr_t>(a->B) & 15))
     return -1;
-  if (a->K % 8) return -2;
+  // Tensor maps take any K (what is behind it is read as zero); callers that ask for it by flag have seen to the pitches.
+  const bool any_size = (a->flags & 2) != 0;
+  if (a->K % 8 && !any_size) return -2;
+  const int a_mn_rows = any_size && a->a_mn && (a->M + 63) / 64 * 64 <= a->lda ? (a->M + 63) / 64 * 64 : a->M;   // extent of an MN-major A
   GemmKernelParams kp;
   int BN = (a->N > 128 || a->force_bn == 256) && a->force_bn != 128 ? 256 : 128;
   if (cm && cm->mode == 2 && (cm->sub_rows % 256) != 0) BN = 128;
@@ -998,7 +1001,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     use_pair = e ? atoi(e) : 1;
   }
   if (use_pair && !cm && !a->tile_group && !a->k_ranges && a->M >= 256 && a->N >= 256 && a->force_bn == 0 &&
-      a->sm_limit == 0 && (!a->a_mn || a->M % 64 == 0) && (!a->b_mn || a->N % 64 == 0)) {
+      a->sm_limit == 0 && (!a->a_mn || a_mn_rows % 64 == 0) && (!a->b_mn || a->N % 64 == 0)) {
     const int bb2 = a->strideB != 0 && a->batch > 1;
     int dev2 = 0, sms2 = 148;
     cudaGetDevice(&dev2);
@@ -1011,7 +1014,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
       pair_bn = (e && atoi(e) == 128) ? 128 : 256;
     }
     const int bn2 = pair_bn;
-    int rc2 = make_operand_map(&kp.tmA, a->A, a->M, a->K, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, 128);
+    int rc2 = make_operand_map(&kp.tmA, a->A, a_mn_rows, a->K, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, 128);
     if (rc2) return rc2;
     rc2 = make_operand_map(&kp.tmB, a->B, a->N, a->K, a->ldb, bb2, a->batch, a->strideB, a->b_mn != 0, bn2 / 2);
     if (rc2) return rc2;
@@ -1025,7 +1028,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     const int am2 = a->a_mn != 0, bm2 = a->b_mn != 0;
     return bn2 == 256 ? launch_cfg2_any<256>(kp, am2, bm2, sms2, st) : launch_cfg2_any<128>(kp, am2, bm2, sms2, st);
   }
-  int rc = make_operand_map(&kp.tmA, a->A, a->M, Kfull, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, BM);
+  int rc = make_operand_map(&kp.tmA, a->A, a_mn_rows, Kfull, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, BM);
   if (rc) return rc;
   rc = make_operand_map(&kp.tmB, a->B, a->N, Kfull, a->ldb, b_batched, b_nbatch, a->strideB, a->b_mn != 0, BN);
   if (rc) return rc;

@@ -33,7 +33,8 @@ typedef struct SxGemmArgs {
   int sm_limit;  // cap on CTAs (0: one per SM)
   int force_bn;  // 0 auto, 128 or 256
   int flags;     // bit 0: B is not written by any kernel launched before this one on the stream (a weight at
-                 // inference time), so a kernel may start fetching it before its predecessor has finished
+                 // inference time), so a kernel may start fetching it before its predecessor has finished;
+                 // bit 1: K need not be a multiple of 8, nor M one of 64 with a_mn: lda covers whole groups of 64 then
   float act_a, act_b;
 } SxGemmArgs;
 int sx_gemm_bf16(const SxGemmArgs* args, cudaStream_t stream);
@@ -530,13 +531,20 @@ int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long
 // part: scratch of ceil(V / 256) T pairs of floats; zt: scratch of T floats.
 int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                       long long ignore_index, float cap, void* part, float* zt, float* nll, float* lse, int* status, cudaStream_t stream);
-// Gradient of the logits [v0, v1) from lse and the gradients of nll and lse (either may be null): dz bf16 [rows, ld], T <= rows < T + 256, ld a multiple
-// of 32, at least v1 - v0; rows from T on and columns from v1 on are zeros.
-int sx_vocab_loss_grad(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
-                       long long ignore_index, float cap, const float* lse, const float* g_nll, const float* g_lse, void* dz, long long ld,
-                       long long rows, long long v0, long long v1, int* status, cudaStream_t stream);
-// out [count] bf16 = sum of parts [n, count] fp32; count a multiple of 8.
-int sx_vocab_loss_sum(const float* parts, void* out, int n, long long count, cudaStream_t stream);
+// Backward: dh [T, d] bf16 and dw [V, d] (bf16, or fp32 with dw_fp32; written, or added to with dw_add), either may be null; d a multiple of 64. g_nll and
+// g_lse (either may be null): gradients of nll and lse. dz, the gradient of the logits, exists for `piece` words at a time (0: as many as fit 256 MiB).
+typedef struct SxVocabLossArgs {
+  const void* h; const void* w; long long ldh, ldw;
+  const long long* target; const float* lse; const float* g_nll; const float* g_lse;
+  void* dh; void* dw; long long lddw;
+  long long T, V, ignore_index, piece;
+  void* work; long long work_bytes;                      // sx_vocab_loss_bwd_workspace bytes, 256-byte aligned
+  int* status;
+  int d, dw_fp32, dw_add;
+  float cap;
+} SxVocabLossArgs;
+long long sx_vocab_loss_bwd_workspace(const SxVocabLossArgs* args);
+int sx_vocab_loss_bwd(const SxVocabLossArgs* args, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -421,23 +421,127 @@ extern "C" int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, lo
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
-extern "C" int sx_vocab_loss_grad(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
-                                  long long ignore_index, float cap, const float* lse, const float* g_nll, const float* g_lse, void* dz, long long ld,
-                                  long long rows, long long v0, long long v1, int* status, cudaStream_t st) {
-  VocabLossParams p = {};
-  int rc = vocab_loss_setup(&p, h, ldh, w, ldw, T, V, d, cap);
-  if (rc) return rc;
-  if (v0 < 0 || v1 <= v0 || v1 > V || ld % 32 || ld < v1 - v0 || ld > (1 << 30) || rows < T || rows > T + 255 || (reinterpret_cast<uintptr_t>(dz) & 31)) return -2;
-  p.target = target; p.ignore_index = ignore_index; p.status = status;
-  p.lse = lse; p.g_nll = g_nll; p.g_lse = g_lse; p.dz = (__nv_bfloat16*)dz; p.ld = ld; p.rows = (int)rows;
-  p.v0 = (int)v0; p.v1 = (int)v1;
-  p.m_blks = (int)((rows + 255) / 256); p.n_blks = (int)((ld + 255) / 256);
-  return cap > 0.f ? vocab_loss_launch<true, true>(p, st) : vocab_loss_launch<true, false>(p, st);
+namespace sx {
+
+// What backward does with its scratch and in which order, from the arguments alone.
+struct VocabLossPlan {
+  long long piece, ld;        // words of a piece, pitch of dz
+  int splits;                 // parts of a piece whose sums of dh are apart
+  bool sums;                  // dh goes through 32-bit sums in scratch
+  long long o_dz, o_acc, o_wpad, bytes;
+};
+constexpr int PAIRS = 74;                            // pairs of SMs
+constexpr long long PIECE_BYTES = 256ll << 20;       // of dz, where the caller does not say how wide a piece is
+// dh has T d results only, and for narrow models these are too few tiles of 256 x 256 for 74 pairs of SMs: the words are then cut once more, into parts
+// that run as one batch (4095 tokens of 768: 48 tiles; 3 x 48 fill two rounds, and 50280 words take 257 us instead of 321).
+// Below 512 tokens the sums' own traffic is what counts, as in parts of fewer than 2048 words.
+static int dh_splits(long long T, int d, long long words) {
+  const long long tiles = ((T + 255) / 256) * ((d + 255) / 256);
+  auto use = [&](int s) { return (double)(tiles * s) / (double)(PAIRS * ((tiles * s + PAIRS - 1) / PAIRS)); };
+  int best = 1;
+  for (int s = 1; s <= 8; ++s) {
+    if (s > 1 && (T < 512 || d < 256 || words / s < 2048)) break;
+    if (use(s) >= 0.9) return s;
+    if (use(s) > use(best)) best = s;
+  }
+  return best;
+}
+static VocabLossPlan vocab_loss_plan(const SxVocabLossArgs* a) {
+  VocabLossPlan p;
+  long long piece = a->piece > 0 ? a->piece : PIECE_BYTES / (2 * a->T);
+  if (a->piece <= 0 && piece < 1024) piece = 1024;
+  piece = (piece + 255) / 256 * 256;
+  if (piece > a->V) piece = a->V;
+  p.splits = a->dh ? dh_splits(a->T, a->d, piece) : 1;
+  if (piece < a->V) {                                // equal parts of every piece but the last
+    const long long unit = 256ll * p.splits;
+    piece = piece / unit > 0 ? piece / unit * unit : unit;
+    if (piece > a->V) piece = a->V;
+  }
+  p.piece = piece;
+  p.ld = (piece + 63) / 64 * 64;
+  p.sums = a->dh && (p.splits > 1 || piece < a->V);
+  long long o = 0;
+  auto take = [&](long long bytes) {
+    const long long at = o;
+    o += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.o_dz = take(2 * a->T * p.ld);
+  p.o_acc = take(p.sums ? 4ll * p.splits * a->T * a->d : 0);
+  const long long last = a->V - (a->V - 1) / piece * piece, unit = 8ll * p.splits;
+  p.o_wpad = take(p.splits > 1 && last % unit ? (last + unit - 1) / unit * unit * a->d * 2 : 0);
+  p.bytes = o;
+  return p;
+}
+static bool vocab_loss_args_ok(const SxVocabLossArgs* a) {
+  return a->T > 0 && a->T <= (1 << 30) && a->V > 0 && a->V <= (1 << 30) && a->d > 0 && a->d % 64 == 0 && a->piece >= 0;
 }
 
-extern "C" int sx_vocab_loss_sum(const float* parts, void* out, int n, long long count, cudaStream_t st) {
-  if (count == 0) return 0;
-  if (n < 1 || count < 0 || count % 8 || ((reinterpret_cast<uintptr_t>(parts) | reinterpret_cast<uintptr_t>(out)) & 15) || count / 8 > 256ll * 0x7fffffff) return -1;
-  vocab_loss_sum_kernel<<<(unsigned)((count / 8 + 255) / 256), 256, 0, st>>>((const float4*)parts, (uint4*)out, n, count / 8);
+}  // namespace sx
+
+extern "C" long long sx_vocab_loss_bwd_workspace(const SxVocabLossArgs* a) { return vocab_loss_args_ok(a) ? vocab_loss_plan(a).bytes : -1; }
+
+extern "C" int sx_vocab_loss_bwd(const SxVocabLossArgs* a, cudaStream_t st) {
+  if (!vocab_loss_args_ok(a)) return -1;
+  const VocabLossPlan plan = vocab_loss_plan(a);
+  if (a->work_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a->work) & 255)) return -3;
+  VocabLossParams p = {};
+  int rc = vocab_loss_setup(&p, a->h, a->ldh, a->w, a->ldw, a->T, a->V, a->d, a->cap);
+  if (rc) return rc;
+  uint8_t* work = (uint8_t*)a->work;
+  __nv_bfloat16* dz = (__nv_bfloat16*)(work + plan.o_dz);
+  float* acc = (float*)(work + plan.o_acc);
+  p.target = a->target; p.ignore_index = a->ignore_index; p.status = a->status;
+  p.lse = a->lse; p.g_nll = a->g_nll; p.g_lse = a->g_lse; p.dz = dz; p.rows = (int)a->T;
+  p.m_blks = (int)((a->T + 255) / 256);
+  for (long long v0 = 0; v0 < a->V; v0 += plan.piece) {
+    const long long v1 = v0 + plan.piece < a->V ? v0 + plan.piece : a->V, n = v1 - v0;
+    const bool first = v0 == 0, last = v1 == a->V;
+    p.v0 = (int)v0; p.v1 = (int)v1; p.ld = (n + 63) / 64 * 64;
+    p.n_blks = (int)((p.ld + 255) / 256);
+    rc = a->cap > 0.f ? vocab_loss_launch<true, true>(p, st) : vocab_loss_launch<true, false>(p, st);
+    if (rc) return rc;
+    const __nv_bfloat16* w = (const __nv_bfloat16*)a->w + v0 * a->ldw;
+    SxGemmArgs g = {};
+    g.alpha = 1.f; g.status = a->status; g.batch = 1; g.flags = 2; g.b_mn = 1;
+    g.A = dz; g.lda = p.ld;
+    if (a->dh) {
+      const int s = plan.splits;
+      const long long k = s > 1 ? (n + 8 * s - 1) / (8 * s) * 8 : n;
+      g.B = w; g.ldb = a->ldw;
+      if (s > 1 && k * s != n) {      // the last piece, in equal parts: its words and zeros behind them (dz is zero there too)
+        uint8_t* pad = work + plan.o_wpad;
+        if (cudaMemcpy2DAsync(pad, a->d * 2ll, w, a->ldw * 2, a->d * 2ll, n, cudaMemcpyDeviceToDevice, st) != cudaSuccess ||
+            cudaMemsetAsync(pad + n * a->d * 2, 0, (k * s - n) * a->d * 2, st) != cudaSuccess)
+          return -11;
+        g.B = pad; g.ldb = a->d;
+      }
+      g.M = (int)a->T; g.N = a->d; g.K = (int)k;
+      if (s > 1) {
+        g.batch = s; g.strideA = k; g.strideB = k * g.ldb; g.strideD = a->T * a->d;
+      }
+      g.ldd = a->d;
+      const bool out = !plan.sums || (s == 1 && last);
+      g.D = out ? a->dh : (void*)acc;
+      g.out_fp32 = !out;
+      if (!first) {
+        g.C = acc; g.ldc = a->d; g.strideC = g.strideD; g.c_fp32 = 1; g.beta = 1.f;
+      }
+      if ((rc = sx_gemm_bf16(&g, st))) return rc;
+    }
+    if (a->dw) {
+      g.a_mn = 1; g.B = a->h; g.ldb = a->ldh; g.batch = 1; g.strideA = g.strideB = g.strideC = g.strideD = 0;
+      g.M = (int)n; g.N = a->d; g.K = (int)a->T;
+      g.D = (char*)a->dw + v0 * a->lddw * (a->dw_fp32 ? 4 : 2);
+      g.ldd = a->lddw; g.out_fp32 = a->dw_fp32;
+      g.C = a->dw_add ? g.D : nullptr; g.ldc = a->lddw; g.c_fp32 = a->dw_fp32; g.beta = a->dw_add ? 1.f : 0.f;
+      if ((rc = sx_gemm_bf16(&g, st))) return rc;
+    }
+  }
+  if (a->dh && plan.splits > 1) {
+    const long long count8 = a->T * a->d / 8;
+    vocab_loss_sum_kernel<<<(unsigned)((count8 + 255) / 256), 256, 0, st>>>((const float4*)acc, (uint4*)a->dh, plan.splits, count8);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

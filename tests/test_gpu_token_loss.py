@@ -70,7 +70,8 @@ def _run(h, w, t, gn, gz, cap, piece=0):
 
 @pytest.mark.parametrize("cap", [0.0, 3.0])
 @pytest.mark.parametrize("T,V,d", [(1, 1, 8), (1, 300, 64), (3, 256, 72), (77, 1000, 256), (128, 257, 64), (129, 128, 640), (255, 4099, 128), (256, 512, 64),
-                                   (257, 777, 192), (300, 33, 1024), (1000, 5000, 96), (520, 3001, 100), (33, 700, 7)])
+                                   (257, 777, 192), (300, 33, 1024), (1000, 5000, 96), (520, 3001, 100), (33, 700, 7),
+                                   (600, 20000, 256)])
 def test_values_and_gradients(T, V, d, cap):
     x = _inputs(T, V, d, 1)
     got = _run(*x, cap)
@@ -146,6 +147,15 @@ def test_layouts():
         hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
         dh, dw = torch.autograd.grad(ops.linear_token_loss(hg, wg, tt)[0].sum(), (hg, wg))
         _check(dict(dh=dh.reshape(T, 128), dw=dw), want, tol)
+    # a single token out of wider rows with an odd pitch, a vocabulary of one word
+    one = torch.randn(3, 131, generator=g, device="cuda").to(torch.bfloat16)
+    for h, w in ((one[1:2, :128], wide[:, :128]), (one[:, :128], one[2:3, :128])):
+        t = torch.zeros(h.shape[0], dtype=torch.int64, device="cuda")
+        hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+        nll, lse = ops.linear_token_loss(hg, wg, t)
+        dh, dw = torch.autograd.grad(nll.sum(), (hg, wg))
+        want, tol = _want(h, w, t, torch.ones(len(t), device="cuda"), torch.zeros(len(t), device="cuda"), 0.0)
+        _check(dict(nll=nll, lse=lse, dh=dh, dw=dw), want, tol)
     ops.check_status()
 
 
