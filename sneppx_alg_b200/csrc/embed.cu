@@ -9,6 +9,7 @@
 // Words that do not occur are known without a table of flags that would have to be cleared: mark[v] holds the position of one token of word v, or
 // whatever was there, and only counts if that token exists and is v's.
 // Ids outside [0, V) give rows of zeros and no gradient, and ST_BAD_ARGUMENT in the status word.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>
 #include "common.cuh"
@@ -92,6 +93,8 @@ struct SortArgs {
   unsigned* counts;                 // [bins, tiles]
   unsigned* totals;                 // [bins]
   unsigned* mark;                   // [V] or null
+  unsigned* open_count;             // set to 0 for the sums that follow
+  unsigned* zero_next;              // next words whose rows may have to be zeros, or null
   int* status;
   long long V, padding;
   unsigned n, tiles;
@@ -136,7 +139,8 @@ __global__ void __launch_bounds__(TILE_THREADS) sort_count_kernel(const SortArgs
     if (i < a.n) {
       const unsigned k = sort_key(a, i);
       atomicAdd(&hist[(k >> a.shift) & mask], 1u);
-      if (a.mark && k < a.V) a.mark[k] = i;
+      if (a.mark && !a.key_in && k < a.V) a.mark[k] = i;
+      if (i == 0 && a.zero_next) *a.zero_next = 0;
     }
   }
   __syncthreads();
@@ -168,7 +172,10 @@ __global__ void __launch_bounds__(256) sort_prefix_kernel(const SortArgs a) {
     carry += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) a.totals[blockIdx.x] = carry;
+  if (threadIdx.x == 0) {
+    a.totals[blockIdx.x] = carry;
+    if (blockIdx.x == 0) *a.open_count = 0;
+  }
 }
 __global__ void __launch_bounds__(TILE_THREADS) sort_place_kernel(const SortArgs a) {
   __shared__ unsigned short cnt[TILE_WARPS][1 << DIGIT_MAX];
@@ -218,6 +225,111 @@ __global__ void __launch_bounds__(TILE_THREADS) sort_place_kernel(const SortArgs
   }
 }
 
+// The whole sort in one cluster of up to eight CTAs, which exchange counts and tokens through each other's shared memory: 1024 threads of up to eight
+// tokens each, so up to 65536 tokens. Two passes over 8192 tokens are one launch instead of six (33 us of kernels, and the host's time for them).
+// CTAs beyond the first cluster write zeros to the rows of words that do not occur meanwhile (embed_sort_zero_kernel).
+constexpr int CS_THREADS = 1024, CS_WARPS = CS_THREADS / 32, CS_MAX = 8;
+struct ClusterSort {
+  unsigned long long item[CS_THREADS * TILE_ITEMS];          // key << 32 | position
+  unsigned short cnt[CS_WARPS][1 << DIGIT_MAX];
+  unsigned hist[1 << DIGIT_MAX];
+  unsigned base[1 << DIGIT_MAX];
+  unsigned warp_total[16];
+};
+__device__ __forceinline__ void cluster_sort(ClusterSort& sm, const SortArgs& a, int passes, unsigned* key_out, unsigned* pos_out) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned ctas = cluster.num_blocks(), rank = cluster.block_rank();
+  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5, bins = 1u << a.bits, mask = bins - 1;
+  const unsigned rounds = (a.n + ctas * CS_THREADS - 1) / (ctas * CS_THREADS), per = rounds * CS_THREADS;   // tokens of a thread, of a CTA
+  const unsigned first = rank * per + w * (rounds * 32);
+  unsigned key[TILE_ITEMS], pos[TILE_ITEMS], place[TILE_ITEMS];
+  if (rank == 0 && threadIdx.x == 0) *a.open_count = 0;
+#pragma unroll
+  for (int r = 0; r < TILE_ITEMS; ++r) {
+    const unsigned i = first + r * 32 + lane;
+    const bool live = r < rounds && i < a.n;
+    key[r] = live ? sort_key(a, i) : 0;
+    pos[r] = i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * a.bits;
+    for (unsigned b = lane; b < bins; b += 32) sm.cnt[w][b] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < TILE_ITEMS; ++r) {
+      if (r >= rounds) break;
+      const bool live = first + r * 32 + lane < a.n;
+      const unsigned digit = live ? (key[r] >> shift) & mask : 0xffffffffu;
+      const unsigned same = __match_any_sync(0xffffffffu, digit);
+      const unsigned before = live ? sm.cnt[w][digit] : 0;
+      __syncwarp();
+      place[r] = before + __popc(same & ((1u << lane) - 1));
+      if (live && (same >> lane) == 1u) sm.cnt[w][digit] = (unsigned short)(place[r] + 1);
+      __syncwarp();
+    }
+    __syncthreads();
+    // a bin's counts over the CTA's warps: their prefix, and the CTA's count
+    if (threadIdx.x < bins) {
+      unsigned run = 0;
+#pragma unroll 8
+      for (int k = 0; k < CS_WARPS; ++k) {
+        const unsigned c = sm.cnt[k][threadIdx.x];
+        sm.cnt[k][threadIdx.x] = (unsigned short)run;
+        run += c;
+      }
+      sm.hist[threadIdx.x] = run;
+    }
+    cluster.sync();
+    unsigned all = 0, earlier = 0;
+    if (threadIdx.x < bins) {
+      for (unsigned c = 0; c < ctas; ++c) {
+        const unsigned v = *cluster.map_shared_rank(&sm.hist[threadIdx.x], c);
+        earlier += c < rank ? v : 0;
+        all += v;
+      }
+    }
+    unsigned s = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= (unsigned)o) s += u;
+    }
+    if (lane == 31 && w < 16) sm.warp_total[w] = s;
+    __syncthreads();
+    if (threadIdx.x < bins) {
+      unsigned before = s - all + earlier;
+      for (unsigned k = 0; k < w; ++k) before += sm.warp_total[k];
+      sm.base[threadIdx.x] = before;
+    }
+    __syncthreads();
+    const bool last = pass == passes - 1;
+#pragma unroll
+    for (int r = 0; r < TILE_ITEMS; ++r) {
+      if (r >= rounds || first + r * 32 + lane >= a.n) break;
+      const unsigned digit = (key[r] >> shift) & mask, to = sm.base[digit] + sm.cnt[w][digit] + place[r];
+      if (last) {
+        key_out[to] = key[r];
+        pos_out[to] = pos[r];
+      } else {
+        const unsigned cta = to / per;
+        *cluster.map_shared_rank(&sm.item[to - cta * per], cta) = (unsigned long long)key[r] << 32 | pos[r];
+      }
+    }
+    cluster.sync();               // all tokens are where they belong, and nobody reads this CTA's counts any more
+    if (last) return;
+#pragma unroll
+    for (int r = 0; r < TILE_ITEMS; ++r) {
+      const unsigned i = w * (rounds * 32) + r * 32 + lane;
+      if (r < rounds && rank * per + i < a.n) {
+        const unsigned long long v = sm.item[i];
+        key[r] = (unsigned)(v >> 32);
+        pos[r] = (unsigned)v;
+      }
+    }
+  }
+}
+
 // ----------------------------------------------------------------------------- sums of runs
 // Thread (x, y): eight columns, piece y of the sorted list. part [pieces, 2, d8]: partial sums of the run that a piece begins in the middle of (0) and
 // of the run that begins in it and goes on (1).
@@ -225,6 +337,15 @@ template <bool VEC, typename G>
 __device__ __forceinline__ void emb_finish(G* grad, long long ldg, unsigned word, int c, int d, const float (&acc)[8], float scale, int add) {
   G* row = grad + (long long)word * ldg;
   Emb8<G> o;
+  if (VEC && sizeof(G) == 4 && add) {
+    // nobody else writes this row in this launch: the addition at the cache has the load and addition's result, and nothing waits for it
+#pragma unroll
+    for (int j = 0; j < 8; j += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + c + j), "f"(acc[j] * scale), "f"(acc[j + 1] * scale), "f"(acc[j + 2] * scale),
+                   "f"(acc[j + 3] * scale)
+                   : "memory");
+    return;
+  }
   if (add) {
     emb_load<VEC>(row, c, d, o);
 #pragma unroll
@@ -240,102 +361,166 @@ __device__ __forceinline__ void part_store(float* part, unsigned piece, int side
   p[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   p[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
+// Keys and positions of 32 tokens are read by the lanes at once and passed round; a warp goes from run to run and asks for four rows of a run at a time.
+// Most words occur a few times only: what keeps memory busy is many warps, not long loads (eight rows of several runs in registers: 103 of them, a quarter
+// of the warps, 93 us instead of @SUM@ for 32768 tokens of 2048).
 template <bool VEC, typename T, typename G>
 __global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ dy, const unsigned* __restrict__ key, const unsigned* __restrict__ pos, G* grad,
-                                                        long long ldg, float* __restrict__ part, unsigned n, unsigned len, int d, int d8, unsigned V,
-                                                        float scale, int add) {
-  const unsigned piece = blockIdx.x * blockDim.y + threadIdx.y;
+                                                        long long ldg, float* __restrict__ part, unsigned* open_count, unsigned* __restrict__ open_piece,
+                                                        unsigned n, unsigned len, int d, int d8, unsigned V, float scale, int add) {
+  const unsigned piece = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   const unsigned i0 = piece * len;
-  if (i0 >= n || c >= d) return;
+  if (i0 >= n) return;                 // a warp's threads have one piece
   const unsigned i1 = min(n, i0 + len);
-  unsigned word = key[i0];
-  if (word >= V) return;               // V and beyond stand at the end of the list
-  bool open = i0 > 0 && key[i0 - 1] == word;
+  const unsigned before = i0 > 0 ? key[i0 - 1] : 0xffffffffu, after = i1 < n ? key[i1] : 0xffffffffu;
+  const bool mine = c < d;
+  unsigned word = 0xffffffffu;         // none yet
+  bool open = false;
   float acc[8];
+  for (unsigned base = i0; base < i1; base += 32) {
+    const unsigned kl = base + lane < i1 ? key[base + lane] : 0xffffffffu, pl = base + lane < i1 ? pos[base + lane] : 0;
+    const unsigned count = __popc(__ballot_sync(0xffffffffu, kl < V));           // V and beyond stand at the end of the list
+    unsigned prev = __shfl_up_sync(0xffffffffu, kl, 1);
+    if (lane == 0) prev = word;
+    const unsigned heads = __ballot_sync(0xffffffffu, kl != prev && kl < V);
+    for (unsigned j = 0; j < count;) {
+      if (heads >> j & 1) {            // another word
+        if (word < V && mine) {
+          if (open) part_store(part, piece, 0, d8, c, acc);
+          else emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
+        }
+        const bool none = word >= V;
+        word = __shfl_sync(0xffffffffu, kl, j);
+        open = none && word == before;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  constexpr int U = 8;
-  for (unsigned i = i0; i < i1 && word < V; i += U) {
-    unsigned k[U];
-    Emb8<T> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      k[u] = i + u < i1 ? key[i + u] : 0xffffffffu;
-      if (k[u] < V) emb_load<VEC>(dy + (long long)pos[i + u] * d, c, d, v[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= i1 || word >= V) continue;
-      if (k[u] != word) {
-        if (open) part_store(part, piece, 0, d8, c, acc);
-        else emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
-        open = false;
-        word = k[u];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
       }
-      if (word < V) {
+      const unsigned rest = heads & ~((2u << j) - 1), end = rest ? __ffs(rest) - 1 : count;
+      for (; j < end; j += 4) {
+        Emb8<T> v[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += emb_in(v[u].t[j]);
+        for (int u = 0; u < 4; ++u) {
+          const unsigned at = __shfl_sync(0xffffffffu, pl, j + u);
+          if (j + u < end && mine) emb_load<VEC>(dy + (long long)at * d, c, d, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (j + u < end) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += emb_in(v[u].t[k]);
+          }
+        }
       }
+      j = end;
     }
   }
-  if (word >= V) return;
-  if (open) part_store(part, piece, 0, d8, c, acc);
-  else if (i1 < n && key[i1] == word) part_store(part, piece, 1, d8, c, acc);
-  else emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
-}
-// Pieces whose last run begins in them and goes on: its sum over the pieces that it reaches.
-template <bool VEC, typename G>
-__global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restrict__ key, G* grad, long long ldg, const float* __restrict__ part, unsigned n,
-                                                         unsigned len, int d, int d8, unsigned V, float scale, int add) {
-  const unsigned piece = blockIdx.x * blockDim.y + threadIdx.y;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
-  const unsigned i0 = piece * len;
-  if (i0 >= n || n - i0 <= len || c >= d) return;
-  const unsigned i1 = i0 + len, word = key[i1];
-  if (word >= V || key[i1 - 1] != word || (key[i0] == word && i0 > 0 && key[i0 - 1] == word)) return;
-  float acc[8];
-  const float* p = part + ((size_t)piece * 2 + 1) * d8 + c;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = p[j];
-  for (unsigned q = piece + 1;; ++q) {
-    p = part + (size_t)q * 2 * d8 + c;
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
-    acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
-    const unsigned long long next = (unsigned long long)(q + 1) * len;
-    if (next >= n || key[next] != word) break;
+  if (word >= V || !mine) return;
+  if (open) {
+    part_store(part, piece, 0, d8, c, acc);
+  } else if (after == word) {
+    part_store(part, piece, 1, d8, c, acc);
+    if (c == 0) open_piece[atomicAdd(open_count, 1u)] = piece;       // in any order: each entry is a sum of its own
+  } else {
+    emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
   }
-  emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
 }
-// Rows of words that do not occur: 32 at a time a block, their marks read together.
+// Runs that go over several pieces: block (x, y) takes 256 columns of a run, thread y every eighth of its partial sums; the eight are added in order.
 template <bool VEC, typename G>
-__global__ void __launch_bounds__(256) embed_zero_kernel(const void* __restrict__ ids, int wide, long long padding, const unsigned* __restrict__ mark, G* grad,
-                                                         long long ldg, unsigned n, int d, unsigned V) {
-  __shared__ unsigned absent;
-  for (unsigned long long v0 = (unsigned long long)blockIdx.x * 32; v0 < V; v0 += (unsigned long long)gridDim.x * 32) {
+__global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restrict__ key, G* grad, long long ldg, const float* __restrict__ part,
+                                                         const unsigned* __restrict__ open_count, const unsigned* __restrict__ open_piece, unsigned n,
+                                                         unsigned len, int d, int d8, float scale, int add) {
+  __shared__ float s[8][32][9];
+  const unsigned lane = threadIdx.x, y = threadIdx.y, blocks = (d + 255) / 256, total = *open_count;
+  for (unsigned long long item = blockIdx.x; item < (unsigned long long)total * blocks; item += gridDim.x) {
+    const unsigned piece = open_piece[item / blocks];
+    const int c = ((int)(item % blocks) * 32 + lane) * 8;
+    const unsigned long long i1 = (unsigned long long)(piece + 1) * len;
+    const unsigned word = key[i1];
+    unsigned more = 0;                 // pieces behind it that begin with the word
+    for (bool all = true; all; ) {
+      const unsigned long long at = i1 + (unsigned long long)(more + lane) * len;
+      const unsigned b = __ballot_sync(0xffffffffu, at < n && key[at] == word);
+      all = b == 0xffffffffu;
+      more += all ? 32 : __ffs(~b) - 1;
+    }
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    if (c < d8) {
+#pragma unroll 4
+      for (unsigned q = y; q <= more; q += 8) {
+        const float4* p = reinterpret_cast<const float4*>(part + ((size_t)(piece + q) * 2 + (q == 0 ? 1 : 0)) * d8 + c);
+        const float4 a = p[0], b = p[1];
+        acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
+        acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[y][lane][j] = acc[j];
+    __syncthreads();
+    if (y == 0 && c < d) {
+      for (int k = 1; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += s[k][lane][j];
+      emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
+    }
+    __syncthreads();
+  }
+}
+// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once. Blocks take words as they get to
+// them: not all of a grid of clusters may be on the machine at once.
+template <bool VEC, typename G>
+__device__ __forceinline__ void zero_rows(unsigned (&row_of)[34], const SortArgs& a, G* grad, long long ldg, int d) {
+  const unsigned vecs = (d + 7) / 8, side = max(blockDim.x / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
+  Emb8<G> z;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
+  for (;;) {
     __syncthreads();
     if (threadIdx.x < 32) {
-      const unsigned v = (unsigned)v0 + threadIdx.x;
-      bool zero = v < V;
-      if (zero && v != padding) {
-        const unsigned m = mark[v];
-        zero = m >= n || emb_id(ids, wide, m) != v;
+      unsigned next = 0;
+      if (threadIdx.x == 0) next = atomicAdd(a.zero_next, 1u);
+      next = __shfl_sync(0xffffffffu, next, 0);
+      const unsigned long long v = (unsigned long long)next * 32 + threadIdx.x;
+      bool zero = v < (unsigned long long)a.V;
+      if (threadIdx.x == 0) row_of[33] = zero;
+      if (zero && (long long)v != a.padding) {
+        const unsigned m = a.mark[v];
+        zero = m >= a.n || emb_id(a.ids, a.wide, m) != (long long)v;
       }
       const unsigned b = __ballot_sync(0xffffffffu, zero);
-      if (threadIdx.x == 0) absent = b;
+      if (zero) row_of[__popc(b & ((1u << threadIdx.x) - 1))] = (unsigned)v;
+      if (threadIdx.x == 0) row_of[32] = __popc(b);
     }
     __syncthreads();
-    Emb8<G> z;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
-    for (unsigned b = absent; b; b &= b - 1) {
-      G* row = grad + (long long)(v0 + __ffs(b) - 1) * ldg;
-      for (int c = threadIdx.x * 8; c < d; c += 256 * 8) emb_store<VEC>(row, c, d, z);
+    const unsigned rows = row_of[32];
+    if (!row_of[33]) return;
+    if (mine < side) {
+      for (unsigned k = mine; k < rows; k += side) {
+        G* row = grad + (long long)row_of[k] * ldg;
+        for (int c = c0; c < d; c += blockDim.x * 8) emb_store<VEC>(row, c, d, z);
+      }
     }
   }
+}
+template <bool VEC, typename G>
+__global__ void __launch_bounds__(256) embed_zero_kernel(const SortArgs a, G* grad, long long ldg, int d) {
+  __shared__ unsigned rows[34];
+  zero_rows<VEC>(rows, a, grad, ldg, d);
+}
+template <bool VEC, typename G>
+__global__ void __launch_bounds__(CS_THREADS) embed_sort_zero_kernel(const SortArgs a, int passes, G* grad, long long ldg, int d) {
+  extern __shared__ uint8_t smem[];
+  if (blockIdx.x < cooperative_groups::this_cluster().num_blocks()) cluster_sort(*reinterpret_cast<ClusterSort*>(smem), a, passes, a.key_out, a.pos_out);
+  if (a.zero_next) zero_rows<VEC>(*reinterpret_cast<unsigned(*)[34]>(smem), a, grad, ldg, d);
+}
+__global__ void __launch_bounds__(256) embed_mark_kernel(const SortArgs a) {
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  if (i == 0) *a.zero_next = 0;
+  if (i >= a.n) return;
+  const long long id = emb_id(a.ids, a.wide, i);
+  if (id >= 0 && id < a.V) a.mark[id] = i;
 }
 
 static bool emb_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -354,7 +539,7 @@ static unsigned piece_len(long long n, int d) {
 struct EmbPlan {
   unsigned tiles, len, pieces;
   int passes, bits, d8;
-  long long o_key[2], o_pos[2], o_counts, o_totals, o_mark, o_part, bytes;
+  long long o_key[2], o_pos[2], o_counts, o_totals, o_mark, o_part, o_open, bytes;
 };
 static EmbPlan emb_plan(long long n, long long V, int d, int dense) {
   EmbPlan p;
@@ -379,8 +564,38 @@ static EmbPlan emb_plan(long long n, long long V, int d, int dense) {
   p.o_totals = take(4ll << p.bits);
   p.o_mark = take(dense ? 4 * V : 0);
   p.o_part = take(8ll * p.pieces * p.d8);
+  p.o_open = take(4ll * (p.pieces + 2));           // next words to be zeros, count, the pieces
   p.bytes = o;
   return p;
+}
+
+// One cluster that sorts, as wide as leaves a thread few tokens, and, where the gradient is written whole, one CTA an SM in all.
+template <bool VEC, typename G>
+static int launch_sort_zero(const SortArgs& a, int passes, G* grad, long long ldg, int d, int add, cudaStream_t st) {
+  auto kern = embed_sort_zero_kernel<VEC, G>;
+  static int known[64];        // devices that the kernel has been set up on
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
+  if (!__atomic_load_n(&known[dev], __ATOMIC_ACQUIRE)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSort)) != cudaSuccess) return -10;
+    __atomic_store_n(&known[dev], 1, __ATOMIC_RELEASE);
+  }
+  unsigned ctas = 1;
+  while (ctas < CS_MAX && a.n > ctas * CS_THREADS) ctas *= 2;
+  const long long zero = add ? 0 : (a.V + 31) / 32, room = 148 - ctas;
+  const unsigned more = (unsigned)((zero < room ? zero : room) + ctas - 1) / ctas * ctas;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas + more);
+  cfg.blockDim = dim3(CS_THREADS);
+  cfg.dynamicSmemBytes = sizeof(ClusterSort);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a, passes, grad, ldg, d) == cudaSuccess ? 0 : -11;
 }
 
 }  // namespace sx
@@ -418,19 +633,51 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
   a.ids = ids; a.wide = ids_wide; a.V = V; a.padding = padding; a.n = (unsigned)tokens; a.tiles = p.tiles; a.bits = p.bits;
   a.counts = (unsigned*)(b + p.o_counts); a.totals = (unsigned*)(b + p.o_totals); a.status = status;
   unsigned* mark = (unsigned*)(b + p.o_mark);
-  int at = 0;
-  for (int pass = 0; pass < p.passes && tokens > 0; ++pass, at ^= 1) {
-    a.mark = pass == 0 && !add ? mark : nullptr;
-    a.shift = pass * p.bits;
-    a.key_out = (unsigned*)(b + p.o_key[at]);
-    a.pos_out = (unsigned*)(b + p.o_pos[at]);
-    sort_count_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
-    sort_prefix_kernel<<<1u << p.bits, 256, 0, st>>>(a);
-    sort_place_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
-    a.key_in = a.key_out;
-    a.pos_in = a.pos_out;
+  a.zero_next = add ? nullptr : (unsigned*)(b + p.o_open);
+  a.open_count = (unsigned*)(b + p.o_open) + 1;
+  a.mark = add ? nullptr : mark;
+  const bool vec = d % 8 == 0 && ldg % 8 == 0 && emb_aligned(dy) && emb_aligned(grad);
+  auto typed = [&](auto f) {                       // f(element of dy, element of grad, whole vectors)
+    auto two = [&](auto t, auto g) { return vec ? f(t, g, std::true_type()) : f(t, g, std::false_type()); };
+    if (dtype == 2) return two(float(), float());
+    if (dtype == 1 && grad_dtype == 1) return two(__half(), __half());
+    if (dtype == 1) return two(__half(), float());
+    if (grad_dtype == 0) return two(__nv_bfloat16(), __nv_bfloat16());
+    return two(__nv_bfloat16(), float());
+  };
+  const unsigned *key, *pos;
+  int rc;
+  if (tokens <= (long long)CS_MAX * CS_THREADS * TILE_ITEMS) {
+    a.key_out = (unsigned*)(b + p.o_key[0]);
+    a.pos_out = (unsigned*)(b + p.o_pos[0]);
+    if (!add) embed_mark_kernel<<<(unsigned)((tokens + 256) / 256), 256, 0, st>>>(a);
+    rc = typed([&](auto, auto g, auto v) { return launch_sort_zero<decltype(v)::value, decltype(g)>(a, p.passes, (decltype(g)*)grad, ldg, d, add, st); });
+    if (rc) return rc;
+    key = a.key_out;
+    pos = a.pos_out;
+  } else {
+    for (int pass = 0, at = 0; pass < p.passes; ++pass, at ^= 1) {
+      a.shift = pass * p.bits;
+      a.key_out = (unsigned*)(b + p.o_key[at]);
+      a.pos_out = (unsigned*)(b + p.o_pos[at]);
+      sort_count_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
+      sort_prefix_kernel<<<1u << p.bits, 256, 0, st>>>(a);
+      sort_place_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
+      a.key_in = a.key_out;
+      a.pos_in = a.pos_out;
+    }
+    key = a.key_in;
+    pos = a.pos_in;
+    if (!add) {
+      const unsigned blocks = (unsigned)((V + 31) / 32);
+      rc = typed([&](auto, auto g, auto v) {
+        using G = decltype(g);
+        embed_zero_kernel<decltype(v)::value, G><<<blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st>>>(a, (G*)grad, ldg, d);
+        return 0;
+      });
+    }
   }
-  const unsigned *key = a.key_in, *pos = a.pos_in;
+  if (tokens == 0) return cudaGetLastError() == cudaSuccess ? 0 : -11;
   float* part = (float*)(b + p.o_part);
   const int items = p.d8 / 8;
   dim3 block, grid;
@@ -438,28 +685,19 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
   block.y = 256 / block.x;
   grid.x = (p.pieces + block.y - 1) / block.y;
   grid.y = (items + block.x - 1) / block.x;
-  auto run = [&](auto t, auto g) {
+  unsigned* open_piece = a.open_count + 1;
+  rc = typed([&](auto t, auto g, auto v) {
     using T = decltype(t);
     using G = decltype(g);
-    auto go = [&](auto vec) {
-      constexpr bool VEC = decltype(vec)::value;
-      if (!add) {
-        const unsigned blocks = (unsigned)((V + 31) / 32);
-        embed_zero_kernel<VEC, G><<<blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st>>>(ids, ids_wide, padding, mark, (G*)grad, ldg, (unsigned)tokens, d,
-                                                                                      (unsigned)V);
-      }
-      if (tokens == 0) return;
-      embed_sum_kernel<VEC, T, G><<<grid, block, 0, st>>>((const T*)dy, key, pos, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
-      if (p.pieces > 1)
-        embed_join_kernel<VEC, G><<<grid, block, 0, st>>>(key, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
-    };
-    if (d % 8 == 0 && ldg % 8 == 0 && emb_aligned(dy) && emb_aligned(grad)) go(std::true_type());
-    else go(std::false_type());
-  };
-  if (dtype == 2) run(float(), float());
-  else if (dtype == 1 && grad_dtype == 1) run(__half(), __half());
-  else if (dtype == 1) run(__half(), float());
-  else if (grad_dtype == 0) run(__nv_bfloat16(), __nv_bfloat16());
-  else run(__nv_bfloat16(), float());
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+    constexpr bool VEC = decltype(v)::value;
+    embed_sum_kernel<VEC, T, G><<<grid, block, 0, st>>>((const T*)dy, key, pos, (G*)grad, ldg, part, a.open_count, open_piece, (unsigned)tokens, p.len, d,
+                                                       p.d8, (unsigned)V, scale, add);
+    if (p.pieces > 1) {
+      const long long items = (long long)p.pieces * ((d + 255) / 256);
+      embed_join_kernel<VEC, G><<<(unsigned)(items < 148 * 8 ? items : 148 * 8), dim3(32, 8), 0, st>>>(key, (G*)grad, ldg, part, a.open_count, open_piece,
+                                                                                                    (unsigned)tokens, p.len, d, p.d8, scale, add);
+    }
+    return 0;
+  });
+  return rc ? rc : cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

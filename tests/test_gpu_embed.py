@@ -57,7 +57,8 @@ def test_lookup(n, V, d, scale, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("law", ["any", "one", "few", "skew"])
-@pytest.mark.parametrize("n,V,d", [(1, 1, 8), (2, 3, 1), (77, 300, 33), (500, 70, 1000), (4096, 5000, 256), (4097, 128256, 64), (9001, 300001, 40)])
+@pytest.mark.parametrize("n,V,d", [(1, 1, 8), (2, 3, 1), (77, 300, 33), (500, 70, 1000), (4096, 5000, 256), (4097, 128256, 64), (9001, 300001, 40),
+                                   (65536, 70000, 16), (65537, 3000, 24), (200003, 1000000, 8)])
 def test_gradient(n, V, d, law, dtype):
     torch.manual_seed(0)
     t = TYPES[dtype]
@@ -81,7 +82,7 @@ def test_gradient(n, V, d, law, dtype):
 
 
 @pytest.mark.parametrize("dtype,into", [("bf16", "fp32"), ("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")])
-@pytest.mark.parametrize("n,V,d", [(77, 300, 33), (3000, 500, 256), (40000, 2000, 128)])
+@pytest.mark.parametrize("n,V,d", [(77, 300, 33), (3000, 500, 256), (40000, 2000, 128), (100000, 2000, 16)])
 def test_main_grad_is_written_and_added_to(n, V, d, dtype, into):
     torch.manual_seed(0)
     t = TYPES[dtype]
