@@ -93,8 +93,6 @@ struct SortArgs {
   unsigned* counts;                 // [bins, tiles]
   unsigned* totals;                 // [bins]
   unsigned* mark;                   // [V] or null
-  unsigned* open_count;             // set to 0 for the sums that follow
-  unsigned* zero_next;              // next words whose rows may have to be zeros, or null
   int* status;
   long long V, padding;
   unsigned n, tiles;
@@ -140,7 +138,6 @@ __global__ void __launch_bounds__(TILE_THREADS) sort_count_kernel(const SortArgs
       const unsigned k = sort_key(a, i);
       atomicAdd(&hist[(k >> a.shift) & mask], 1u);
       if (a.mark && !a.key_in && k < a.V) a.mark[k] = i;
-      if (i == 0 && a.zero_next) *a.zero_next = 0;
     }
   }
   __syncthreads();
@@ -172,10 +169,7 @@ __global__ void __launch_bounds__(256) sort_prefix_kernel(const SortArgs a) {
     carry += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    a.totals[blockIdx.x] = carry;
-    if (blockIdx.x == 0) *a.open_count = 0;
-  }
+  if (threadIdx.x == 0) a.totals[blockIdx.x] = carry;
 }
 __global__ void __launch_bounds__(TILE_THREADS) sort_place_kernel(const SortArgs a) {
   __shared__ unsigned short cnt[TILE_WARPS][1 << DIGIT_MAX];
@@ -227,7 +221,6 @@ __global__ void __launch_bounds__(TILE_THREADS) sort_place_kernel(const SortArgs
 
 // The whole sort in one cluster of up to eight CTAs, which exchange counts and tokens through each other's shared memory: 1024 threads of up to eight
 // tokens each, so up to 65536 tokens. Two passes over 8192 tokens are one launch instead of six (33 us of kernels, and the host's time for them).
-// CTAs beyond the first cluster write zeros to the rows of words that do not occur meanwhile (embed_sort_zero_kernel).
 constexpr int CS_THREADS = 1024, CS_WARPS = CS_THREADS / 32, CS_MAX = 8;
 struct ClusterSort {
   unsigned long long item[CS_THREADS * TILE_ITEMS];          // key << 32 | position
@@ -244,13 +237,13 @@ __device__ __forceinline__ void cluster_sort(ClusterSort& sm, const SortArgs& a,
   const unsigned rounds = (a.n + ctas * CS_THREADS - 1) / (ctas * CS_THREADS), per = rounds * CS_THREADS;   // tokens of a thread, of a CTA
   const unsigned first = rank * per + w * (rounds * 32);
   unsigned key[TILE_ITEMS], pos[TILE_ITEMS], place[TILE_ITEMS];
-  if (rank == 0 && threadIdx.x == 0) *a.open_count = 0;
 #pragma unroll
   for (int r = 0; r < TILE_ITEMS; ++r) {
     const unsigned i = first + r * 32 + lane;
     const bool live = r < rounds && i < a.n;
     key[r] = live ? sort_key(a, i) : 0;
     pos[r] = i;
+    if (live && a.mark && key[r] < a.V) a.mark[key[r]] = i;
   }
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * a.bits;
@@ -366,8 +359,7 @@ __device__ __forceinline__ void part_store(float* part, unsigned piece, int side
 // of the warps, 93 us instead of @SUM@ for 32768 tokens of 2048).
 template <bool VEC, typename T, typename G>
 __global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ dy, const unsigned* __restrict__ key, const unsigned* __restrict__ pos, G* grad,
-                                                        long long ldg, float* __restrict__ part, unsigned* open_count, unsigned* __restrict__ open_piece,
-                                                        unsigned n, unsigned len, int d, int d8, unsigned V, float scale, int add) {
+                                                        long long ldg, float* __restrict__ part, unsigned n, unsigned len, int d, int d8, unsigned V, float scale, int add) {
   const unsigned piece = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   const unsigned i0 = piece * len;
@@ -420,25 +412,33 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ dy
     part_store(part, piece, 0, d8, c, acc);
   } else if (after == word) {
     part_store(part, piece, 1, d8, c, acc);
-    if (c == 0) open_piece[atomicAdd(open_count, 1u)] = piece;       // in any order: each entry is a sum of its own
   } else {
     emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
   }
 }
-// Runs that go over several pieces: block (x, y) takes 256 columns of a run, thread y every eighth of its partial sums; the eight are added in order.
+// Runs that go over several pieces. A block takes 256 columns of the runs that begin in four neighbouring pieces and go on, thread y every eighth of a run's
+// partial sums; the eight are added in order.
+constexpr int JOIN_PIECES = 4;
 template <bool VEC, typename G>
-__global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restrict__ key, G* grad, long long ldg, const float* __restrict__ part,
-                                                         const unsigned* __restrict__ open_count, const unsigned* __restrict__ open_piece, unsigned n,
-                                                         unsigned len, int d, int d8, float scale, int add) {
+__global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restrict__ key, G* grad, long long ldg, const float* __restrict__ part, unsigned n,
+                                                         unsigned len, int d, int d8, unsigned V, float scale, int add) {
   __shared__ float s[8][32][9];
-  const unsigned lane = threadIdx.x, y = threadIdx.y, blocks = (d + 255) / 256, total = *open_count;
-  for (unsigned long long item = blockIdx.x; item < (unsigned long long)total * blocks; item += gridDim.x) {
-    const unsigned piece = open_piece[item / blocks];
-    const int c = ((int)(item % blocks) * 32 + lane) * 8;
+  const unsigned lane = threadIdx.x, y = threadIdx.y, first = blockIdx.x * JOIN_PIECES;
+  const int c = (int)(blockIdx.y * 32 + lane) * 8;
+  bool begins = false;
+  if (lane < JOIN_PIECES) {
+    const unsigned long long i0 = (unsigned long long)(first + lane) * len, i1 = i0 + len;
+    if (i1 < n) {
+      const unsigned word = key[i1];
+      begins = word < V && key[i1 - 1] == word && (key[i0] != word || i0 == 0 || key[i0 - 1] != word);
+    }
+  }
+  for (unsigned left = __ballot_sync(0xffffffffu, begins); left; left &= left - 1) {
+    const unsigned piece = first + __ffs(left) - 1;
     const unsigned long long i1 = (unsigned long long)(piece + 1) * len;
     const unsigned word = key[i1];
     unsigned more = 0;                 // pieces behind it that begin with the word
-    for (bool all = true; all; ) {
+    for (bool all = true; all;) {
       const unsigned long long at = i1 + (unsigned long long)(more + lane) * len;
       const unsigned b = __ballot_sync(0xffffffffu, at < n && key[at] == word);
       all = b == 0xffffffffu;
@@ -468,59 +468,81 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restr
     __syncthreads();
   }
 }
-// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once. Blocks take words as they get to
-// them: not all of a grid of clusters may be on the machine at once.
+// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once.
 template <bool VEC, typename G>
-__device__ __forceinline__ void zero_rows(unsigned (&row_of)[34], const SortArgs& a, G* grad, long long ldg, int d) {
-  const unsigned vecs = (d + 7) / 8, side = max(blockDim.x / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
+__global__ void __launch_bounds__(256) embed_zero_kernel(const SortArgs a, G* grad, long long ldg, int d) {
+  __shared__ unsigned row_of[32], rows;
+  const unsigned vecs = (d + 7) / 8, side = max(256 / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
   Emb8<G> z;
 #pragma unroll
   for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
-  for (;;) {
+  for (unsigned long long v0 = (unsigned long long)blockIdx.x * 32; v0 < (unsigned long long)a.V; v0 += (unsigned long long)gridDim.x * 32) {
     __syncthreads();
     if (threadIdx.x < 32) {
-      unsigned next = 0;
-      if (threadIdx.x == 0) next = atomicAdd(a.zero_next, 1u);
-      next = __shfl_sync(0xffffffffu, next, 0);
-      const unsigned long long v = (unsigned long long)next * 32 + threadIdx.x;
+      const unsigned long long v = v0 + threadIdx.x;
       bool zero = v < (unsigned long long)a.V;
-      if (threadIdx.x == 0) row_of[33] = zero;
       if (zero && (long long)v != a.padding) {
         const unsigned m = a.mark[v];
         zero = m >= a.n || emb_id(a.ids, a.wide, m) != (long long)v;
       }
       const unsigned b = __ballot_sync(0xffffffffu, zero);
       if (zero) row_of[__popc(b & ((1u << threadIdx.x) - 1))] = (unsigned)v;
-      if (threadIdx.x == 0) row_of[32] = __popc(b);
+      if (threadIdx.x == 0) rows = __popc(b);
     }
     __syncthreads();
-    const unsigned rows = row_of[32];
-    if (!row_of[33]) return;
     if (mine < side) {
       for (unsigned k = mine; k < rows; k += side) {
         G* row = grad + (long long)row_of[k] * ldg;
-        for (int c = c0; c < d; c += blockDim.x * 8) emb_store<VEC>(row, c, d, z);
+        for (int c = c0; c < d; c += 256 * 8) emb_store<VEC>(row, c, d, z);
       }
     }
   }
 }
-template <bool VEC, typename G>
-__global__ void __launch_bounds__(256) embed_zero_kernel(const SortArgs a, G* grad, long long ldg, int d) {
-  __shared__ unsigned rows[34];
-  zero_rows<VEC>(rows, a, grad, ldg, d);
-}
-template <bool VEC, typename G>
-__global__ void __launch_bounds__(CS_THREADS) embed_sort_zero_kernel(const SortArgs a, int passes, G* grad, long long ldg, int d) {
+// The first cluster sorts the tokens for the gradient while the other CTAs look the rows up (y null: nothing to look up): the sort, which takes a few
+// SMs for 10 to 20 us, costs nothing behind the lookup.
+template <bool VEC, typename T>
+__global__ void __launch_bounds__(CS_THREADS) embed_sort_lookup_kernel(const SortArgs a, int passes, const T* __restrict__ w, long long ldw, T* __restrict__ y,
+                                                                       int d, float scale) {
   extern __shared__ uint8_t smem[];
-  if (blockIdx.x < cooperative_groups::this_cluster().num_blocks()) cluster_sort(*reinterpret_cast<ClusterSort*>(smem), a, passes, a.key_out, a.pos_out);
-  if (a.zero_next) zero_rows<VEC>(*reinterpret_cast<unsigned(*)[34]>(smem), a, grad, ldg, d);
-}
-__global__ void __launch_bounds__(256) embed_mark_kernel(const SortArgs a) {
-  const unsigned i = blockIdx.x * 256 + threadIdx.x;
-  if (i == 0) *a.zero_next = 0;
-  if (i >= a.n) return;
-  const long long id = emb_id(a.ids, a.wide, i);
-  if (id >= 0 && id < a.V) a.mark[id] = i;
+  const unsigned ctas = cooperative_groups::this_cluster().num_blocks();
+  if (blockIdx.x < ctas) {
+    cluster_sort(*reinterpret_cast<ClusterSort*>(smem), a, passes, a.key_out, a.pos_out);
+    return;
+  }
+  constexpr int U = 4;
+  const unsigned vecs = (d + 7) / 8, side = max(CS_THREADS / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
+  if (mine >= side) return;
+  const unsigned step = (gridDim.x - ctas) * side;
+  for (unsigned long long t0 = (blockIdx.x - ctas) * side + mine; t0 < a.n; t0 += (unsigned long long)step * U) {
+    long long id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned long long t = t0 + (unsigned long long)u * step;
+      id[u] = t < a.n ? emb_id(a.ids, a.wide, t) : -1;
+    }
+    for (int c = c0; c < d; c += CS_THREADS * 8) {
+      Emb8<T> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (id[u] >= 0 && id[u] < a.V) {
+          emb_load<VEC>(w + id[u] * ldw, c, d, v[u]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(0.f);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const unsigned long long t = t0 + (unsigned long long)u * step;
+        if (t >= a.n) break;
+        if (scale != 1.f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(emb_in(v[u].t[j]) * scale);
+        }
+        emb_store<VEC>(y + (long long)t * d, c, d, v[u]);
+      }
+    }
+  }
 }
 
 static bool emb_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -536,43 +558,45 @@ static unsigned piece_len(long long n, int d) {
   while (len < 128 && n * threads / len > want) len *= 2;
   return len;
 }
-struct EmbPlan {
-  unsigned tiles, len, pieces;
-  int passes, bits, d8;
-  long long o_key[2], o_pos[2], o_counts, o_totals, o_mark, o_part, o_open, bytes;
-};
-static EmbPlan emb_plan(long long n, long long V, int d, int dense) {
-  EmbPlan p;
-  const int bits = bits_of(V);           // keys up to V
-  p.passes = (bits + DIGIT_MAX - 1) / DIGIT_MAX;
-  p.bits = (bits + p.passes - 1) / p.passes;
-  p.tiles = (unsigned)((n + TILE - 1) / TILE);
-  p.len = piece_len(n, d);
-  p.pieces = (unsigned)((n + p.len - 1) / p.len);
-  p.d8 = (d + 7) / 8 * 8;
-  long long o = 0;
-  auto take = [&](long long bytes) {
-    const long long at = o;
-    o += (bytes + 255) / 256 * 256;
-    return at;
-  };
-  for (int i = 0; i < 2; ++i) {
-    p.o_key[i] = take(4 * n);
-    p.o_pos[i] = take(4 * n);
+constexpr long long ONE_CLUSTER = (long long)CS_MAX * CS_THREADS * TILE_ITEMS;
+static long long up256(long long bytes) { return (bytes + 255) / 256 * 256; }
+// Tokens in the order of their words: keys, positions, and the mark of every word.
+struct EmbSorted {
+  long long o_pos, o_mark, bytes;
+  int passes, bits;
+  EmbSorted(long long n, long long V) {
+    const int all = bits_of(V);            // keys up to V
+    passes = (all + DIGIT_MAX - 1) / DIGIT_MAX;
+    bits = (all + passes - 1) / passes;
+    o_pos = up256(4 * n);
+    o_mark = 2 * o_pos;
+    bytes = o_mark + up256(4 * V);
   }
-  p.o_counts = take(4ll * p.tiles << p.bits);
-  p.o_totals = take(4ll << p.bits);
-  p.o_mark = take(dense ? 4 * V : 0);
-  p.o_part = take(8ll * p.pieces * p.d8);
-  p.o_open = take(4ll * (p.pieces + 2));           // next words to be zeros, count, the pieces
-  p.bytes = o;
-  return p;
-}
+};
+// Scratch of the backward pass.
+struct EmbWork {
+  unsigned tiles, len, pieces;
+  int d8;
+  long long o_sorted, o_other, o_counts, o_totals, o_part, bytes;
+  EmbWork(long long n, long long V, int d, bool presorted) {
+    const EmbSorted s(n, V);
+    len = piece_len(n, d);
+    pieces = (unsigned)((n + len - 1) / len);
+    tiles = (unsigned)((n + TILE - 1) / TILE);
+    d8 = (d + 7) / 8 * 8;
+    o_part = 0;
+    o_sorted = up256(8ll * pieces * d8);
+    o_other = o_sorted + (presorted ? 0 : s.bytes);
+    o_counts = o_other + (presorted || n <= ONE_CLUSTER ? 0 : 2 * s.o_pos);
+    o_totals = o_counts + (presorted || n <= ONE_CLUSTER ? 0 : up256(4ll * tiles << s.bits));
+    bytes = o_totals + (presorted || n <= ONE_CLUSTER ? 0 : up256(4ll << s.bits));
+  }
+};
 
-// One cluster that sorts, as wide as leaves a thread few tokens, and, where the gradient is written whole, one CTA an SM in all.
-template <bool VEC, typename G>
-static int launch_sort_zero(const SortArgs& a, int passes, G* grad, long long ldg, int d, int add, cudaStream_t st) {
-  auto kern = embed_sort_zero_kernel<VEC, G>;
+// One cluster that sorts, as wide as leaves a thread few tokens; with rows to look up, CTAs for them on the other SMs.
+template <bool VEC, typename T>
+static int launch_sort_lookup(const SortArgs& a, int passes, const T* w, long long ldw, T* y, int d, float scale, cudaStream_t st) {
+  auto kern = embed_sort_lookup_kernel<VEC, T>;
   static int known[64];        // devices that the kernel has been set up on
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
@@ -582,8 +606,11 @@ static int launch_sort_zero(const SortArgs& a, int passes, G* grad, long long ld
   }
   unsigned ctas = 1;
   while (ctas < CS_MAX && a.n > ctas * CS_THREADS) ctas *= 2;
-  const long long zero = add ? 0 : (a.V + 31) / 32, room = 148 - ctas;
-  const unsigned more = (unsigned)((zero < room ? zero : room) + ctas - 1) / ctas * ctas;
+  unsigned more = 0;
+  if (y) {
+    const long long want = ((long long)a.n * ((d + 7) / 8) + CS_THREADS - 1) / CS_THREADS, room = 148 - ctas;
+    more = (unsigned)((want < room ? want : room) + ctas - 1) / ctas * ctas;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas + more);
   cfg.blockDim = dim3(CS_THREADS);
@@ -595,89 +622,81 @@ static int launch_sort_zero(const SortArgs& a, int passes, G* grad, long long ld
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a, passes, grad, ldg, d) == cudaSuccess ? 0 : -11;
+  return cudaLaunchKernelEx(&cfg, kern, a, passes, w, ldw, y, d, scale) == cudaSuccess ? 0 : -11;
+}
+static SortArgs sort_args(const void* ids, int wide, long long tokens, long long V, long long padding, const EmbSorted& s, uint8_t* sorted, int* status) {
+  SortArgs a = {};
+  a.ids = ids; a.wide = wide; a.V = V; a.padding = padding; a.n = (unsigned)tokens; a.bits = s.bits; a.status = status;
+  a.key_out = (unsigned*)sorted;
+  a.pos_out = (unsigned*)(sorted + s.o_pos);
+  a.mark = (unsigned*)(sorted + s.o_mark);
+  return a;
+}
+static bool emb_args_ok(long long tokens, int d, long long V, int dtype) {
+  return tokens >= 0 && tokens <= 0x7fffffffll && d >= 0 && d <= (1 << 25) && V > 0 && V <= 0x7ffffffell && dtype >= 0 && dtype <= 2;
 }
 
 }  // namespace sx
 using namespace sx;
 
+// Bytes of `sorted`, or 0: so many tokens are not sorted by the forward pass.
+extern "C" long long sx_embed_sorted_bytes(long long tokens, long long V) { return tokens > 0 && tokens <= ONE_CLUSTER ? EmbSorted(tokens, V).bytes : 0; }
+
 extern "C" int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long long ldw, void* y, long long tokens, int d, long long V, float scale, int dtype,
-                            int* status, cudaStream_t st) {
+                            long long padding, void* sorted, int* status, cudaStream_t st) {
   if (tokens == 0 || d == 0) return 0;
-  if (tokens < 0 || tokens > 0x7fffffffll || d < 0 || d > (1 << 25) || V <= 0 || dtype < 0 || dtype > 2) return -1;
-  dim3 grid, block;
-  token_grid(tokens, (d + 7) / 8, &grid, &block);
-  auto run = [&](auto t) {
+  if (!emb_args_ok(tokens, d, V, dtype) || (sorted && (tokens > ONE_CLUSTER || (reinterpret_cast<uintptr_t>(sorted) & 255)))) return -1;
+  const bool vec = d % 8 == 0 && ldw % 8 == 0 && emb_aligned(w) && emb_aligned(y);
+  auto run = [&](auto t, auto v) {
     using T = decltype(t);
-    auto go = [&](auto kern) { kern<<<grid, block, 0, st>>>(ids, ids_wide, (const T*)w, ldw, (T*)y, (unsigned)tokens, d, V, scale, status); };
-    if (d % 8 == 0 && ldw % 8 == 0 && emb_aligned(w) && emb_aligned(y)) go(embed_fwd_kernel<true, T>);
-    else go(embed_fwd_kernel<false, T>);
+    constexpr bool VEC = decltype(v)::value;
+    if (sorted) {
+      const EmbSorted s(tokens, V);
+      return launch_sort_lookup<VEC, T>(sort_args(ids, ids_wide, tokens, V, padding, s, (uint8_t*)sorted, status), s.passes, (const T*)w, ldw, (T*)y, d, scale, st);
+    }
+    dim3 grid, block;
+    token_grid(tokens, (d + 7) / 8, &grid, &block);
+    embed_fwd_kernel<VEC, T><<<grid, block, 0, st>>>(ids, ids_wide, (const T*)w, ldw, (T*)y, (unsigned)tokens, d, V, scale, status);
+    return cudaGetLastError() == cudaSuccess ? 0 : -11;
   };
-  if (dtype == 0) run(__nv_bfloat16());
-  else if (dtype == 1) run(__half());
-  else run(float());
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  auto typed = [&](auto t) { return vec ? run(t, std::true_type()) : run(t, std::false_type()); };
+  return dtype == 0 ? typed(__nv_bfloat16()) : dtype == 1 ? typed(__half()) : typed(float());
 }
 
-extern "C" long long sx_embed_bwd_workspace(long long tokens, long long V, int d, int add) { return emb_plan(tokens, V, d, !add).bytes; }
+extern "C" long long sx_embed_bwd_workspace(long long tokens, long long V, int d, int presorted) { return EmbWork(tokens, V, d, presorted != 0).bytes; }
 
 extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long long ldg, long long tokens, int d, long long V, long long padding,
-                            float scale, int add, int dtype, int grad_dtype, void* work, long long work_bytes, int* status, cudaStream_t st) {
+                            float scale, int add, int dtype, int grad_dtype, const void* sorted, void* work, long long work_bytes, int* status,
+                            cudaStream_t st) {
   if (d == 0 || (tokens == 0 && add)) return 0;
-  if (tokens < 0 || tokens > 0x7fffffffll || d < 0 || d > (1 << 25) || V <= 0 || V > 0x7ffffffell || dtype < 0 || dtype > 2) return -1;
+  if (!emb_args_ok(tokens, d, V, dtype)) return -1;
   if (grad_dtype != dtype && grad_dtype != 2) return -2;
-  const EmbPlan p = emb_plan(tokens, V, d, !add);
-  if (work_bytes < p.bytes || !emb_aligned(work)) return -3;
+  const EmbSorted s(tokens, V);
+  const EmbWork p(tokens, V, d, sorted != nullptr);
+  if (work_bytes < p.bytes || (reinterpret_cast<uintptr_t>(work) & 255)) return -3;
   uint8_t* b = (uint8_t*)work;
-  SortArgs a = {};
-  a.ids = ids; a.wide = ids_wide; a.V = V; a.padding = padding; a.n = (unsigned)tokens; a.tiles = p.tiles; a.bits = p.bits;
-  a.counts = (unsigned*)(b + p.o_counts); a.totals = (unsigned*)(b + p.o_totals); a.status = status;
-  unsigned* mark = (unsigned*)(b + p.o_mark);
-  a.zero_next = add ? nullptr : (unsigned*)(b + p.o_open);
-  a.open_count = (unsigned*)(b + p.o_open) + 1;
-  a.mark = add ? nullptr : mark;
   const bool vec = d % 8 == 0 && ldg % 8 == 0 && emb_aligned(dy) && emb_aligned(grad);
-  auto typed = [&](auto f) {                       // f(element of dy, element of grad, whole vectors)
-    auto two = [&](auto t, auto g) { return vec ? f(t, g, std::true_type()) : f(t, g, std::false_type()); };
-    if (dtype == 2) return two(float(), float());
-    if (dtype == 1 && grad_dtype == 1) return two(__half(), __half());
-    if (dtype == 1) return two(__half(), float());
-    if (grad_dtype == 0) return two(__nv_bfloat16(), __nv_bfloat16());
-    return two(__nv_bfloat16(), float());
-  };
-  const unsigned *key, *pos;
-  int rc;
-  if (tokens <= (long long)CS_MAX * CS_THREADS * TILE_ITEMS) {
-    a.key_out = (unsigned*)(b + p.o_key[0]);
-    a.pos_out = (unsigned*)(b + p.o_pos[0]);
-    if (!add) embed_mark_kernel<<<(unsigned)((tokens + 256) / 256), 256, 0, st>>>(a);
-    rc = typed([&](auto, auto g, auto v) { return launch_sort_zero<decltype(v)::value, decltype(g)>(a, p.passes, (decltype(g)*)grad, ldg, d, add, st); });
+  SortArgs a = sort_args(ids, ids_wide, tokens, V, padding, s, sorted ? (uint8_t*)sorted : b + p.o_sorted, status);
+  if (!sorted && tokens > 0 && tokens <= ONE_CLUSTER) {
+    const int rc = launch_sort_lookup<true, float>(a, s.passes, nullptr, 0, nullptr, 0, 1.f, st);
     if (rc) return rc;
-    key = a.key_out;
-    pos = a.pos_out;
-  } else {
-    for (int pass = 0, at = 0; pass < p.passes; ++pass, at ^= 1) {
-      a.shift = pass * p.bits;
-      a.key_out = (unsigned*)(b + p.o_key[at]);
-      a.pos_out = (unsigned*)(b + p.o_pos[at]);
+  } else if (!sorted && tokens > 0) {
+    a.tiles = p.tiles;
+    a.counts = (unsigned*)(b + p.o_counts);
+    a.totals = (unsigned*)(b + p.o_totals);
+    for (int pass = 0; pass < s.passes; ++pass) {
+      uint8_t* to = (s.passes - pass) % 2 ? b + p.o_sorted : b + p.o_other;        // the last pass ends in o_sorted
+      a.shift = pass * s.bits;
+      a.key_out = (unsigned*)to;
+      a.pos_out = (unsigned*)(to + s.o_pos);
       sort_count_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
-      sort_prefix_kernel<<<1u << p.bits, 256, 0, st>>>(a);
+      sort_prefix_kernel<<<1u << s.bits, 256, 0, st>>>(a);
       sort_place_kernel<<<p.tiles, TILE_THREADS, 0, st>>>(a);
       a.key_in = a.key_out;
       a.pos_in = a.pos_out;
     }
-    key = a.key_in;
-    pos = a.pos_in;
-    if (!add) {
-      const unsigned blocks = (unsigned)((V + 31) / 32);
-      rc = typed([&](auto, auto g, auto v) {
-        using G = decltype(g);
-        embed_zero_kernel<decltype(v)::value, G><<<blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st>>>(a, (G*)grad, ldg, d);
-        return 0;
-      });
-    }
   }
-  if (tokens == 0) return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  const unsigned *key = a.key_out, *pos = a.pos_out;
   float* part = (float*)(b + p.o_part);
   const int items = p.d8 / 8;
   dim3 block, grid;
@@ -685,19 +704,25 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
   block.y = 256 / block.x;
   grid.x = (p.pieces + block.y - 1) / block.y;
   grid.y = (items + block.x - 1) / block.x;
-  unsigned* open_piece = a.open_count + 1;
-  rc = typed([&](auto t, auto g, auto v) {
+  auto run = [&](auto t, auto g, auto v) {
     using T = decltype(t);
     using G = decltype(g);
     constexpr bool VEC = decltype(v)::value;
-    embed_sum_kernel<VEC, T, G><<<grid, block, 0, st>>>((const T*)dy, key, pos, (G*)grad, ldg, part, a.open_count, open_piece, (unsigned)tokens, p.len, d,
-                                                       p.d8, (unsigned)V, scale, add);
-    if (p.pieces > 1) {
-      const long long items = (long long)p.pieces * ((d + 255) / 256);
-      embed_join_kernel<VEC, G><<<(unsigned)(items < 148 * 8 ? items : 148 * 8), dim3(32, 8), 0, st>>>(key, (G*)grad, ldg, part, a.open_count, open_piece,
-                                                                                                    (unsigned)tokens, p.len, d, p.d8, scale, add);
+    if (!add) {
+      const unsigned blocks = (unsigned)((V + 31) / 32);
+      embed_zero_kernel<VEC, G><<<blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st>>>(a, (G*)grad, ldg, d);
     }
-    return 0;
-  });
-  return rc ? rc : cudaGetLastError() == cudaSuccess ? 0 : -11;
+    if (tokens == 0) return;
+    embed_sum_kernel<VEC, T, G><<<grid, block, 0, st>>>((const T*)dy, key, pos, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
+    if (p.pieces > 1)
+      embed_join_kernel<VEC, G><<<dim3((p.pieces + JOIN_PIECES - 1) / JOIN_PIECES, (d + 255) / 256), dim3(32, 8), 0, st>>>(
+          key, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
+  };
+  auto typed = [&](auto t, auto g) { vec ? run(t, g, std::true_type()) : run(t, g, std::false_type()); };
+  if (dtype == 2) typed(float(), float());
+  else if (dtype == 1 && grad_dtype == 1) typed(__half(), __half());
+  else if (dtype == 1) typed(__half(), float());
+  else if (grad_dtype == 0) typed(__nv_bfloat16(), __nv_bfloat16());
+  else typed(__nv_bfloat16(), float());
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

@@ -517,13 +517,17 @@ int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, 
 // ------------------------------------------------------------------ L3 embedding (embed.cu)
 // ids int64 (ids_wide) or int32 [tokens]; w [V, d] (pitch ldw), y [tokens, d]; dtype 0 bf16, 1 fp16, 2 fp32. An id outside [0, V): a row of zeros and
 // ST_BAD_ARGUMENT in the status word.
+// sorted (or null): sx_embed_sorted_bytes bytes, 256-byte aligned, that take the tokens in the order of their words for sx_embed_bwd. Tokens of the word
+// `padding` (-1: none) give no gradient.
+long long sx_embed_sorted_bytes(long long tokens, long long V);
 int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long long ldw, void* y, long long tokens, int d, long long V, float scale, int dtype,
-                 int* status, cudaStream_t stream);
+                 long long padding, void* sorted, int* status, cudaStream_t stream);
 // grad [V, d] (pitch ldg; dtype or fp32) = scale * sums of dy [tokens, d] by word, or += with `add` (rows of other words are not touched).
-// Tokens of the word `padding` (-1: none) give nothing. work: sx_embed_bwd_workspace bytes, 16-byte aligned.
-long long sx_embed_bwd_workspace(long long tokens, long long V, int d, int add);
+// sorted: what the forward pass left for these ids and this padding, or null. work: sx_embed_bwd_workspace bytes, 256-byte aligned.
+long long sx_embed_bwd_workspace(long long tokens, long long V, int d, int presorted);
 int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long long ldg, long long tokens, int d, long long V, long long padding,
-                 float scale, int add, int dtype, int grad_dtype, void* work, long long work_bytes, int* status, cudaStream_t stream);
+                 float scale, int add, int dtype, int grad_dtype, const void* sorted, void* work, long long work_bytes, int* status,
+                 cudaStream_t stream);
 
 // ------------------------------------------------------------------ L4 per-token losses of a vocabulary projection (vocab_loss.cu)
 // h [T, d], w [V, d] bf16 (pitches ldh, ldw; d and pitches multiples of 8, 16-byte aligned); z = h w^T, cap tanh(z / cap) with cap > 0.

@@ -17,55 +17,70 @@ def embedding_reference(ids, table, scale=1.0, padding_idx=None):
     return y if scale == 1.0 else (y.float() * scale).to(y.dtype) if y.dtype != torch.float64 else y * scale
 
 
-def _lookup(ids, table, scale):
+def _lookup(ids, table, scale, padding_idx=None, sort=False):
+    """(rows, ids as they were read, those in the order of their words or None)."""
     if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
         table = table.contiguous()
     ids = ids.contiguous()
     V, d = table.shape
+    n = ids.numel()
     y = table.new_empty((*ids.shape, d))
+    size = _lib.entry("sx_embed_sorted_bytes", "ll", _lib.c_ll)(n, V) if sort and d else 0
+    order = table.new_empty(size, dtype=torch.uint8) if size else None
     with _lib.on_device(table):
-        _lib.entry("sx_embed_fwd", "piplplilfipp")(ids.data_ptr(), ids.dtype == torch.int64, table.data_ptr(), table.stride(0), y.data_ptr(), ids.numel(),
-                                                   d, V, scale, _TYPES[table.dtype], _lib.status_ptr(table), _lib.here(table))
-    return y
+        _lib.entry("sx_embed_fwd", "piplplilfilppp")(
+            ids.data_ptr(), ids.dtype is torch.int64, table.data_ptr(), table.stride(0), y.data_ptr(), n, d, V, scale, _TYPES[table.dtype],
+            -1 if padding_idx is None else padding_idx, order.data_ptr() if size else 0, _lib.status_ptr(table), _lib.here(table))
+    return y, ids, order
 
 
 def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
     """grad [V, d] = scale * (sums of the rows of dy [.., d] by their word), or, with ``add``, grad += that (rows of other words are not touched
     then). Sums are in 32 bits and in the order of the tokens, so they are the same each time. grad has dy's type or is fp32."""
+    return _backward(grad, ids, dy, scale, padding_idx, add, None)
+
+
+def _backward(grad, ids, dy, scale, padding_idx, add, order):
     V, d = grad.shape
     if dy.dtype not in _TYPES or grad.dtype not in (dy.dtype, torch.float32) or grad.stride(1) != 1 or (V > 1 and grad.stride(0) < d):
         raise ValueError(f"embedding_backward_: gradients {dy.dtype} into {grad.dtype} with strides {grad.stride()}")
     if dy.shape != (*ids.shape, d):
         raise ValueError(f"embedding_backward_: gradients of shape {tuple(dy.shape)} for ids {tuple(ids.shape)} and rows of {d}")
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
+        raise TypeError(f"embedding_backward_: ids of {ids.dtype}")
+    if not (grad.is_cuda and grad.get_device() == dy.get_device() == ids.get_device()):
+        raise ValueError(f"embedding_backward_: tensors on {grad.device}, {dy.device} and {ids.device}")
     ids, dy = ids.contiguous(), dy.contiguous()
     n = ids.numel()
-    size = _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, add)
+    size = _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)
     with _lib.on_device(grad):
-        _lib.entry("sx_embed_bwd", "pippllillfiiiplpp")(
-            ids.data_ptr(), ids.dtype == torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, -1 if padding_idx is None else padding_idx,
-            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], work.data_ptr(), size, _lib.status_ptr(grad), _lib.here(grad))
+        _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")(
+            ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, -1 if padding_idx is None else padding_idx,
+            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], order.data_ptr() if order is not None else 0, work.data_ptr(), size,
+            _lib.status_ptr(grad), _lib.here(grad))
     return grad
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
-        ctx.save_for_backward(ids)
+        y, ids, order = _lookup(ids, table, scale, padding_idx, sort=True)
+        ctx.save_for_backward(ids, order)
         ctx.table, ctx.meta = table, (scale, padding_idx)
-        return _lookup(ids, table, scale)
+        return y
 
     @staticmethod
     @_lib.once
     def backward(ctx, dy):
-        (ids,) = ctx.saved_tensors
+        ids, order = ctx.saved_tensors
         table, (scale, padding_idx) = ctx.table, ctx.meta
         mg = getattr(table, "main_grad", None)
         if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:
-            embedding_backward_(mg, ids, dy, scale, padding_idx, add=getattr(table, "_main_grad_written", False))
+            _backward(mg, ids, dy, scale, padding_idx, getattr(table, "_main_grad_written", False), order)
             table._main_grad_written = True
             return None, None, None, None
-        return None, embedding_backward_(torch.empty(table.shape, dtype=dy.dtype, device=dy.device), ids, dy, scale, padding_idx), None, None
+        return None, _backward(dy.new_empty(table.shape), ids, dy, scale, padding_idx, False, order), None, None
 
 
 def embedding(ids, table, scale=1.0, padding_idx=None):
@@ -93,4 +108,4 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         _dbg.check_indices(ids, 0, table.shape[0], _dbg.SITE_USER)
     if torch.is_grad_enabled() and table.requires_grad:
         return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
-    return _lookup(ids, table, scale)
+    return _lookup(ids, table, scale)[0]

@@ -137,13 +137,14 @@ def test_ids_out_of_range():
     with pytest.raises(KernelTimeout):
         ops.check_status()
     assert torch.equal(y[ok], w[ids[ok]]) and not y[~ok].any()
-    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
-    with pytest.raises(KernelTimeout):
-        ops.check_status()
+    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))          # the forward pass has sorted the ids and reported them
+    ops.check_status()
     want = torch.zeros(50, 64, device="cuda")
     want[3], want[49] = 2, 1
     assert torch.equal(g, want)
-    ops.check_status()
+    assert torch.equal(ops.embedding_backward_(torch.empty_like(w), ids, torch.ones_like(y)), want)
+    with pytest.raises(KernelTimeout):
+        ops.check_status()
 
 
 def test_refusals():
