@@ -58,27 +58,51 @@ __device__ __forceinline__ long long emb_id(const void* ids, int wide, long long
   return wide ? reinterpret_cast<const long long*>(ids)[i] : (long long)reinterpret_cast<const int*>(ids)[i];
 }
 
-template <bool VEC, typename T>
+// U tokens of a thread: t0, t0 + step, ... Their ids are read together and then their rows, so that U row pieces are on their way.
+template <bool VEC, int U, typename T>
+__device__ __forceinline__ void lookup(const void* ids, int wide, const T* __restrict__ w, long long ldw, T* __restrict__ y, unsigned long long t0,
+                                       unsigned long long step, unsigned tokens, int c0, int c_step, int d, long long V, float scale, int* status) {
+  long long id[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned long long t = t0 + u * step;
+    id[u] = t < tokens ? emb_id(ids, wide, t) : 0;
+    if (id[u] < 0 || id[u] >= V) {
+      id[u] = -1;
+      if (c0 == 0 && status) atomicCAS(status, 0, EMB_BAD_ARGUMENT);
+    }
+  }
+  for (int c = c0; c < d; c += c_step) {
+    Emb8<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (id[u] >= 0) {
+        emb_load<VEC>(w + id[u] * ldw, c, d, v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(0.f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned long long t = t0 + u * step;
+      if (t >= tokens) break;
+      if (scale != 1.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(emb_in(v[u].t[j]) * scale);
+      }
+      emb_store<VEC>(y + (long long)t * d, c, d, v[u]);
+    }
+  }
+}
+// Block (pieces of a row, tokens). Four tokens a thread where that leaves eight warps for each scheduler (8192 rows of 4096: 23 us with one, 18.8 with four).
+template <bool VEC, int U, typename T>
 __global__ void embed_fwd_kernel(const void* __restrict__ ids, int wide, const T* __restrict__ w, long long ldw, T* __restrict__ y, unsigned tokens, int d,
                                  long long V, float scale, int* status) {
-  const unsigned t = blockIdx.x * blockDim.y + threadIdx.y;
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  const unsigned long long rows = (unsigned long long)gridDim.x * blockDim.y, t = blockIdx.x * (unsigned long long)blockDim.y + threadIdx.y;
   if (t >= tokens || c >= d) return;
-  const long long id = emb_id(ids, wide, t);
-  const bool ok = id >= 0 && id < V;
-  Emb8<T> v;
-  if (ok) {
-    emb_load<VEC>(w + id * ldw, c, d, v);
-    if (scale != 1.f) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v.t[j] = emb_out<T>(emb_in(v.t[j]) * scale);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v.t[j] = emb_out<T>(0.f);
-    if (c == 0 && status) atomicCAS(status, 0, EMB_BAD_ARGUMENT);
-  }
-  emb_store<VEC>(y + (long long)t * d, c, d, v);
+  lookup<VEC, U>(ids, wide, w, ldw, y, t, rows, tokens, c, d, d, V, scale, status);
 }
 
 // ----------------------------------------------------------------------------- tokens sorted by word
@@ -354,14 +378,50 @@ __device__ __forceinline__ void part_store(float* part, unsigned piece, int side
   p[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   p[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
+// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once.
+template <bool VEC, typename G>
+__device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long ldg, int d, unsigned block, unsigned blocks) {
+  __shared__ unsigned row_of[32], rows;
+  const unsigned threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const unsigned vecs = (d + 7) / 8, side = max(threads / vecs, 1u), mine = tid / vecs, c0 = (tid - mine * vecs) * 8;
+  Emb8<G> z;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
+  for (unsigned long long v0 = (unsigned long long)block * 32; v0 < (unsigned long long)a.V; v0 += (unsigned long long)blocks * 32) {
+    __syncthreads();
+    if (tid < 32) {
+      const unsigned long long v = v0 + tid;
+      bool zero = v < (unsigned long long)a.V;
+      if (zero && (long long)v != a.padding) {
+        const unsigned m = a.mark[v];
+        zero = m >= a.n || emb_id(a.ids, a.wide, m) != (long long)v;
+      }
+      const unsigned b = __ballot_sync(0xffffffffu, zero);
+      if (zero) row_of[__popc(b & ((1u << tid) - 1))] = (unsigned)v;
+      if (tid == 0) rows = __popc(b);
+    }
+    __syncthreads();
+    if (mine < side) {
+      for (unsigned k = mine; k < rows; k += side) {
+        G* row = grad + (long long)row_of[k] * ldg;
+        for (int c = c0; c < d; c += threads * 8) emb_store<VEC>(row, c, d, z);
+      }
+    }
+  }
+}
 // Keys and positions of 32 tokens are read by the lanes at once and passed round; a warp goes from run to run and asks for four rows of a run at a time.
 // Most words occur a few times only: what keeps memory busy is many warps, not long loads (eight rows of several runs in registers: 103 of them, a quarter
-// of the warps, 93 us instead of @SUM@ for 32768 tokens of 2048).
+// of the warps, 93 us instead of 67 for 32768 tokens of 2048).
 template <bool VEC, typename T, typename G>
-__global__ void __launch_bounds__(256) embed_sum_kernel(const T* __restrict__ dy, const unsigned* __restrict__ key, const unsigned* __restrict__ pos, G* grad,
-                                                        long long ldg, float* __restrict__ part, unsigned n, unsigned len, int d, int d8, unsigned V, float scale, int add) {
-  const unsigned piece = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+__global__ void __launch_bounds__(256, 5) embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part,
+                                                           unsigned len, int d, int d8, float scale, int add, unsigned blocks_x, unsigned blocks) {
+  if (blockIdx.x >= blocks) {          // the gradient is written whole: rows that have no sum, beside those that have
+    zero_rows<VEC>(a, grad, ldg, d, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  const unsigned *key = a.key_out, *pos = a.pos_out, n = a.n, V = (unsigned)a.V;
+  const unsigned by = blockIdx.x / blocks_x, piece = (blockIdx.x - by * blocks_x) * blockDim.y + threadIdx.y, lane = threadIdx.x & 31;
+  const int c = (by * blockDim.x + threadIdx.x) * 8;
   const unsigned i0 = piece * len;
   if (i0 >= n) return;                 // a warp's threads have one piece
   const unsigned i1 = min(n, i0 + len);
@@ -468,36 +528,6 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restr
     __syncthreads();
   }
 }
-// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once.
-template <bool VEC, typename G>
-__global__ void __launch_bounds__(256) embed_zero_kernel(const SortArgs a, G* grad, long long ldg, int d) {
-  __shared__ unsigned row_of[32], rows;
-  const unsigned vecs = (d + 7) / 8, side = max(256 / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
-  Emb8<G> z;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
-  for (unsigned long long v0 = (unsigned long long)blockIdx.x * 32; v0 < (unsigned long long)a.V; v0 += (unsigned long long)gridDim.x * 32) {
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const unsigned long long v = v0 + threadIdx.x;
-      bool zero = v < (unsigned long long)a.V;
-      if (zero && (long long)v != a.padding) {
-        const unsigned m = a.mark[v];
-        zero = m >= a.n || emb_id(a.ids, a.wide, m) != (long long)v;
-      }
-      const unsigned b = __ballot_sync(0xffffffffu, zero);
-      if (zero) row_of[__popc(b & ((1u << threadIdx.x) - 1))] = (unsigned)v;
-      if (threadIdx.x == 0) rows = __popc(b);
-    }
-    __syncthreads();
-    if (mine < side) {
-      for (unsigned k = mine; k < rows; k += side) {
-        G* row = grad + (long long)row_of[k] * ldg;
-        for (int c = c0; c < d; c += 256 * 8) emb_store<VEC>(row, c, d, z);
-      }
-    }
-  }
-}
 // The first cluster sorts the tokens for the gradient while the other CTAs look the rows up (y null: nothing to look up): the sort, which takes a few
 // SMs for 10 to 20 us, costs nothing behind the lookup.
 template <bool VEC, typename T>
@@ -509,40 +539,11 @@ __global__ void __launch_bounds__(CS_THREADS) embed_sort_lookup_kernel(const Sor
     cluster_sort(*reinterpret_cast<ClusterSort*>(smem), a, passes, a.key_out, a.pos_out);
     return;
   }
-  constexpr int U = 4;
   const unsigned vecs = (d + 7) / 8, side = max(CS_THREADS / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
   if (mine >= side) return;
-  const unsigned step = (gridDim.x - ctas) * side;
-  for (unsigned long long t0 = (blockIdx.x - ctas) * side + mine; t0 < a.n; t0 += (unsigned long long)step * U) {
-    long long id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned long long t = t0 + (unsigned long long)u * step;
-      id[u] = t < a.n ? emb_id(a.ids, a.wide, t) : -1;
-    }
-    for (int c = c0; c < d; c += CS_THREADS * 8) {
-      Emb8<T> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (id[u] >= 0 && id[u] < a.V) {
-          emb_load<VEC>(w + id[u] * ldw, c, d, v[u]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(0.f);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned long long t = t0 + (unsigned long long)u * step;
-        if (t >= a.n) break;
-        if (scale != 1.f) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[u].t[j] = emb_out<T>(emb_in(v[u].t[j]) * scale);
-        }
-        emb_store<VEC>(y + (long long)t * d, c, d, v[u]);
-      }
-    }
-  }
+  const unsigned long long step = (unsigned long long)(gridDim.x - ctas) * side;
+  for (unsigned long long t0 = (unsigned long long)(blockIdx.x - ctas) * side + mine; t0 < a.n; t0 += step * 4)
+    lookup<VEC, 4>(a.ids, a.wide, w, ldw, y, t0, step, a.n, c0, CS_THREADS * 8, d, a.V, scale, nullptr);       // the sort reports bad ids
 }
 
 static bool emb_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -597,22 +598,13 @@ struct EmbWork {
 template <bool VEC, typename T>
 static int launch_sort_lookup(const SortArgs& a, int passes, const T* w, long long ldw, T* y, int d, float scale, cudaStream_t st) {
   auto kern = embed_sort_lookup_kernel<VEC, T>;
-  static int known[64];        // devices that the kernel has been set up on
-  int dev = 0;
+  static int fits[64][4];      // clusters of 1, 2, 4, 8 CTAs that a device has room for at once
+  int dev = 0, size = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
-  if (!__atomic_load_n(&known[dev], __ATOMIC_ACQUIRE)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSort)) != cudaSuccess) return -10;
-    __atomic_store_n(&known[dev], 1, __ATOMIC_RELEASE);
-  }
-  unsigned ctas = 1;
-  while (ctas < CS_MAX && a.n > ctas * CS_THREADS) ctas *= 2;
-  unsigned more = 0;
-  if (y) {
-    const long long want = ((long long)a.n * ((d + 7) / 8) + CS_THREADS - 1) / CS_THREADS, room = 148 - ctas;
-    more = (unsigned)((want < room ? want : room) + ctas - 1) / ctas * ctas;
-  }
+  while (size < 3 && a.n > CS_THREADS << size) ++size;
+  const unsigned ctas = 1u << size;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas + more);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(CS_THREADS);
   cfg.dynamicSmemBytes = sizeof(ClusterSort);
   cfg.stream = st;
@@ -622,6 +614,16 @@ static int launch_sort_lookup(const SortArgs& a, int passes, const T* w, long lo
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  int room = __atomic_load_n(&fits[dev][size], __ATOMIC_ACQUIRE);
+  if (room == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ClusterSort)) != cudaSuccess) return -10;
+    if (cudaOccupancyMaxActiveClusters(&room, kern, &cfg) != cudaSuccess || room < 1) return -10;
+    __atomic_store_n(&fits[dev][size], room, __ATOMIC_RELEASE);
+  }
+  if (y) {                     // the tokens are dealt out evenly: no more clusters than run at once
+    const long long want = (((long long)a.n * ((d + 7) / 8) + CS_THREADS - 1) / CS_THREADS + ctas - 1) / ctas, most = room > 1 ? room - 1 : 1;
+    cfg.gridDim = dim3(ctas * (unsigned)(1 + (want < most ? want : most)));
+  }
   return cudaLaunchKernelEx(&cfg, kern, a, passes, w, ldw, y, d, scale) == cudaSuccess ? 0 : -11;
 }
 static SortArgs sort_args(const void* ids, int wide, long long tokens, long long V, long long padding, const EmbSorted& s, uint8_t* sorted, int* status) {
@@ -655,8 +657,14 @@ extern "C" int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long l
       return launch_sort_lookup<VEC, T>(sort_args(ids, ids_wide, tokens, V, padding, s, (uint8_t*)sorted, status), s.passes, (const T*)w, ldw, (T*)y, d, scale, st);
     }
     dim3 grid, block;
-    token_grid(tokens, (d + 7) / 8, &grid, &block);
-    embed_fwd_kernel<VEC, T><<<grid, block, 0, st>>>(ids, ids_wide, (const T*)w, ldw, (T*)y, (unsigned)tokens, d, V, scale, status);
+    const int vecs = (d + 7) / 8;
+    token_grid(tokens, vecs, &grid, &block);
+    if (tokens * vecs >= 4ll * 148 * 1024) {
+      grid.x = (grid.x + 3) / 4;
+      embed_fwd_kernel<VEC, 4, T><<<grid, block, 0, st>>>(ids, ids_wide, (const T*)w, ldw, (T*)y, (unsigned)tokens, d, V, scale, status);
+    } else {
+      embed_fwd_kernel<VEC, 1, T><<<grid, block, 0, st>>>(ids, ids_wide, (const T*)w, ldw, (T*)y, (unsigned)tokens, d, V, scale, status);
+    }
     return cudaGetLastError() == cudaSuccess ? 0 : -11;
   };
   auto typed = [&](auto t) { return vec ? run(t, std::true_type()) : run(t, std::false_type()); };
@@ -696,7 +704,7 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
       a.pos_in = a.pos_out;
     }
   }
-  const unsigned *key = a.key_out, *pos = a.pos_out;
+  const unsigned* key = a.key_out;
   float* part = (float*)(b + p.o_part);
   const int items = p.d8 / 8;
   dim3 block, grid;
@@ -708,12 +716,10 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
     using T = decltype(t);
     using G = decltype(g);
     constexpr bool VEC = decltype(v)::value;
-    if (!add) {
-      const unsigned blocks = (unsigned)((V + 31) / 32);
-      embed_zero_kernel<VEC, G><<<blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st>>>(a, (G*)grad, ldg, d);
-    }
-    if (tokens == 0) return;
-    embed_sum_kernel<VEC, T, G><<<grid, block, 0, st>>>((const T*)dy, key, pos, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
+    const unsigned sums = grid.x * grid.y;
+    const long long groups = add ? 0 : (V + 31) / 32;
+    embed_sum_kernel<VEC, T, G><<<sums + (unsigned)(groups < 148 * 8 ? groups : 148 * 8), block, 0, st>>>(
+        a, (const T*)dy, (G*)grad, ldg, part, p.len, d, p.d8, scale, add, grid.x > 0 ? grid.x : 1, sums);
     if (p.pieces > 1)
       embed_join_kernel<VEC, G><<<dim3((p.pieces + JOIN_PIECES - 1) / JOIN_PIECES, (d + 255) / 256), dim3(32, 8), 0, st>>>(
           key, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);

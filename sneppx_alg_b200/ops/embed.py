@@ -66,15 +66,15 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
         y, ids, order = _lookup(ids, table, scale, padding_idx, sort=True)
-        ctx.save_for_backward(ids, order)
-        ctx.table, ctx.meta = table, (scale, padding_idx)
+        ctx.save_for_backward(ids)
+        ctx.table, ctx.meta = table, (scale, padding_idx, order)
         return y
 
     @staticmethod
     @_lib.once
     def backward(ctx, dy):
-        ids, order = ctx.saved_tensors
-        table, (scale, padding_idx) = ctx.table, ctx.meta
+        (ids,) = ctx.saved_tensors
+        table, (scale, padding_idx, order) = ctx.table, ctx.meta
         mg = getattr(table, "main_grad", None)
         if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:
             _backward(mg, ids, dy, scale, padding_idx, getattr(table, "_main_grad_written", False), order)
