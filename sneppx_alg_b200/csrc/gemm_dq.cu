@@ -199,12 +199,6 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
       if (ab >= Cfg::NA) { ab -= Cfg::NA; aph ^= 1; }
       const uint32_t tA = tmem_base + ab * 64 + (static_cast<uint32_t>(q * 32) << 16);
       while (s >= p.stages) { s -= p.stages; sph ^= 1; }
-      // Where the ring is no multiple of the groups (fp8, 64 rows: six stages, four groups), another group takes this stage in turn: the load before
-      // this one may still be on its way (loads of a ring need not arrive in order), and the parity of this one would pass for a phase that has not
-      // begun. So the one before is waited for first.
-      if (i >= p.stages * KPS && (p.stages * KPS) % Cfg::NG != 0 &&
-          !mbar_wait_warp(&full[s], sph ^ 1, s_abort, p.status, ST_TIMEOUT_CONVERT))
-        break;
       if (!mbar_wait_warp(&full[s], sph, s_abort, p.status, ST_TIMEOUT_CONVERT)) break;
       const uint8_t* src = smem + s * STAGE_BYTES + row * 128;
       bool ok = true;
