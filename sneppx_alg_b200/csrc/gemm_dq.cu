@@ -344,8 +344,12 @@ template <int BT, bool INT4>
 static int dq_launch(DqParams& p, int sms, cudaStream_t st) {
   using Cfg = DqCfg<BT>;
   constexpr int STAGE_BYTES = DQ_W_BYTES + (INT4 ? 2 : 1) * Cfg::X_BYTES;
-  p.stages = Cfg::BUDGET / STAGE_BYTES < DQ_MAX_STAGES ? Cfg::BUDGET / STAGE_BYTES : DQ_MAX_STAGES;
-  static_assert(Cfg::BUDGET / STAGE_BYTES >= 2, "at least two stages");
+  // A stage belongs to the same groups of converters each time it is filled: the parity of a barrier says nothing to a group that has not seen the phase
+  // before (a ring's loads need not arrive in order). With six stages and four groups, fp8 at 64 rows, a group could take a stage that was still empty.
+  constexpr int KPS = INT4 ? 2 : 1, ROOM = Cfg::BUDGET / STAGE_BYTES < DQ_MAX_STAGES ? Cfg::BUDGET / STAGE_BYTES : DQ_MAX_STAGES;
+  constexpr int TURN = Cfg::NG > KPS ? Cfg::NG / KPS : 1;
+  p.stages = ROOM / TURN * TURN;
+  static_assert(ROOM / TURN * TURN >= 2, "at least two stages");
   static_assert(2 * STAGE_BYTES >= BT * DQ_BM * 4, "the partial tile lies over the stages");
   const int smem = p.stages * STAGE_BYTES + 1024 + 256;
   static int set = 0;
