@@ -80,6 +80,7 @@ struct GemmKernelParams {
   int* status;
   long long ldd, ldc, strideD, strideC;
   int M, N, K, batch;
+  int k_step;             // > 0: batch b reduces over [b k_step, (b + 1) k_step) of K; operands have no batches
   int a_batched, b_batched;
   int out_fp32, c_fp32, act;
   float alpha, beta, act_a, act_b;
@@ -101,6 +102,97 @@ struct GemmCfg {
   static constexpr int OFF_BAR = OFF_OUT + OUT_BYTES;
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 /*align slack*/ + 256 /*barriers*/;
 };
+
+// A lane's 32 columns of its row. It alone touches them, so every access is 32 bytes where the address allows (a whole sector: with 16-byte accesses each
+// sector is read and written twice), else 16 bytes, else single values; `left`: columns that the row has from here on.
+__device__ __forceinline__ void ld_sector(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ int access_of(const void* p, int left) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  return left < 32 ? 0 : (a & 31) == 0 ? 32 : (a & 15) == 0 ? 16 : 0;
+}
+__device__ __forceinline__ void add_c32(float (&v)[32], const float* c, float beta, int left) {
+  const int how = access_of(c, left);
+  if (how == 32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      uint32_t r[8];
+      ld_sector(c + j, r);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[j + k] += beta * __uint_as_float(r[k]);
+    }
+  } else if (how == 16) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 r = *reinterpret_cast<const float4*>(c + j);
+      v[j] += beta * r.x; v[j + 1] += beta * r.y; v[j + 2] += beta * r.z; v[j + 3] += beta * r.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) v[j] += beta * c[j];
+  }
+}
+__device__ __forceinline__ void add_c32(float (&v)[32], const __nv_bfloat16* c, float beta, int left) {
+  if (access_of(c, left)) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      float f[8];
+      unpack8(ld8(c + j), f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[j + k] += beta * f[k];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) v[j] += beta * __bfloat162float(c[j]);
+  }
+}
+__device__ __forceinline__ void store_d32(const float (&v)[32], float* d, int left) {
+  const int how = access_of(d, left);
+  if (how == 32) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      uint32_t r[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] = __float_as_uint(v[j + k]);
+      st_sector(d + j, r);
+    }
+  } else if (how == 16) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(d + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+    for (int j = 0; j < 32; ++j)
+      if (j < left) d[j] = v[j];
+  }
+}
+__device__ __forceinline__ void store_d32(const float (&v)[32], __nv_bfloat16* d, int left) {
+  const int how = access_of(d, left);
+  if (how) {
+    uint32_t r[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    if (how == 32) {
+      const uint32_t a[8] = {r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]}, b[8] = {r[8], r[9], r[10], r[11], r[12], r[13], r[14], r[15]};
+      st_sector(d, a);
+      st_sector(d + 16, b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(d)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    }
+  } else {
+    for (int j = 0; j < 32; ++j)
+      if (j < left) d[j] = __float2bfloat16(v[j]);
+  }
+}
 
 template <int BN, bool A_MN, bool B_MN, int COMM>
 __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_constant__ GemmKernelParams p) {
@@ -343,6 +435,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
           k0 = p.k_ranges[2 * b];
           k1 = p.k_ranges[2 * b + 1];
         }
+        if (p.k_step) {
+          k0 = b * p.k_step;
+          k1 = min(p.K, k0 + p.k_step);
+        }
         const int ab = p.a_batched ? b : 0;
         const int bb = p.b_batched ? bsel : 0;
         const int num_kb = (k1 - k0 + BK - 1) / BK;
@@ -404,6 +500,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
         if (p.k_ranges) {
           k0 = p.k_ranges[2 * b];
           k1 = p.k_ranges[2 * b + 1];
+        }
+        if (p.k_step) {
+          k0 = b * p.k_step;
+          k1 = min(p.K, k0 + p.k_step);
         }
         const int num_kb = (k1 - k0 + BK - 1) / BK;
         const int acc = it & 1;
@@ -484,17 +584,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
             if (full || col0 + j < p.N) v[j] += p.bias[col0 + j];
         }
         if (p.beta != 0.f && p.C) {
-          if (p.c_fp32) {
-            const float* cp = reinterpret_cast<const float*>(p.C) + crow + col0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (full || col0 + j < p.N) v[j] += p.beta * cp[j];
-          } else {
-            const __nv_bfloat16* cp = reinterpret_cast<const __nv_bfloat16*>(p.C) + crow + col0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (full || col0 + j < p.N) v[j] += p.beta * __bfloat162float(cp[j]);
-          }
+          if (p.c_fp32) add_c32(v, reinterpret_cast<const float*>(p.C) + crow + col0, p.beta, p.N - col0);
+          else add_c32(v, reinterpret_cast<const __nv_bfloat16*>(p.C) + crow + col0, p.beta, p.N - col0);
         }
         if (p.act == 1) {
 #pragma unroll
@@ -530,31 +621,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
             *reinterpret_cast<uint4*>(slab + (((ci ^ lane) & (BN / 8 - 1)) << 4)) = o;
           }
         } else if (p.out_fp32) {
-          float* dp = reinterpret_cast<float*>(Dptr) + drow + col0;
-          if (full && ((reinterpret_cast<uintptr_t>(dp) & 15) == 0)) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(dp + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else {
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.N) dp[j] = v[j];
-          }
+          store_d32(v, reinterpret_cast<float*>(Dptr) + drow + col0, p.N - col0);
         } else {
-          __nv_bfloat16* dp = reinterpret_cast<__nv_bfloat16*>(Dptr) + drow + col0;
-          if (full && ((reinterpret_cast<uintptr_t>(dp) & 15) == 0)) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              uint4 o;
-              o.x = pack_bf16x2(v[j], v[j + 1]);
-              o.y = pack_bf16x2(v[j + 2], v[j + 3]);
-              o.z = pack_bf16x2(v[j + 4], v[j + 5]);
-              o.w = pack_bf16x2(v[j + 6], v[j + 7]);
-              *reinterpret_cast<uint4*>(dp + j) = o;
-            }
-          } else {
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.N) dp[j] = __float2bfloat16(v[j]);
-          }
+          store_d32(v, reinterpret_cast<__nv_bfloat16*>(Dptr) + drow + col0, p.N - col0);
         }
       }
       tc_fence_before();
@@ -765,7 +834,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
         int b, m_blk, n_blk;
         tile_coords(t, p.m_blks, p.n_blks, b, m_blk, n_blk);
         const int ab = p.a_batched ? b : 0, bb = p.b_batched ? b : 0;
-        const int num_kb = (p.K + BK - 1) / BK;
+        const int k0 = p.k_step ? b * p.k_step : 0, num_kb = ((p.k_step ? min(p.K - k0, p.k_step) : p.K) + BK - 1) / BK;
         const int arow = m_blk * 256 + (int)rank * 128, brow = n_blk * BN2 + (int)rank * (BN2 / 2);
         bool ok = true;
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -774,7 +843,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
           uint8_t* sb = sa + G2_A_BYTES;
           if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * G2_STAGE_BYTES);
           const uint32_t fb = smem_u32(&full_bar[stage]) & PEER_MASK;
-          const int kc = kb * BK;
+          const int kc = k0 + kb * BK;
           if (A_MN) tma2_load_4d(sa, &p.tmA, fb, 0, kc, arow / 64, ab);
           else      tma2_load_3d(sa, &p.tmA, fb, kc, arow, ab);
           if (B_MN) tma2_load_4d(sb, &p.tmB, fb, 0, kc, brow / 64, bb);
@@ -793,7 +862,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
       int it = 0;
       bool ok = true;
       for (int t = cluster_id; t < total_tiles && ok; t += n_clusters) {
-        const int num_kb = (p.K + BK - 1) / BK;
+        const int b = t / (p.m_blks * p.n_blks);
+        const int num_kb = ((p.k_step ? min(p.K - b * p.k_step, p.k_step) : p.K) + BK - 1) / BK;
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1;
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, s_abort, p.status, ST_TIMEOUT_MMA)) break;
@@ -853,17 +923,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
             if (full || col0 + j < p.N) v[j] += p.bias[col0 + j];
         }
         if (p.beta != 0.f && p.C) {
-          if (p.c_fp32) {
-            const float* cp = reinterpret_cast<const float*>(p.C) + crow + col0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (full || col0 + j < p.N) v[j] += p.beta * cp[j];
-          } else {
-            const __nv_bfloat16* cp = reinterpret_cast<const __nv_bfloat16*>(p.C) + crow + col0;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (full || col0 + j < p.N) v[j] += p.beta * __bfloat162float(cp[j]);
-          }
+          if (p.c_fp32) add_c32(v, reinterpret_cast<const float*>(p.C) + crow + col0, p.beta, p.N - col0);
+          else add_c32(v, reinterpret_cast<const __nv_bfloat16*>(p.C) + crow + col0, p.beta, p.N - col0);
         }
         if (p.act == 1) {
 #pragma unroll
@@ -885,31 +946,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
           for (int j = 0; j < 32; ++j) v[j] = softcap(v[j], p.act_a, p.act_b);
         }
         if (p.out_fp32) {
-          float* dp = reinterpret_cast<float*>(p.D) + drow + col0;
-          if (full && ((reinterpret_cast<uintptr_t>(dp) & 15) == 0)) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(dp + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          } else {
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.N) dp[j] = v[j];
-          }
+          store_d32(v, reinterpret_cast<float*>(p.D) + drow + col0, p.N - col0);
         } else {
-          __nv_bfloat16* dp = reinterpret_cast<__nv_bfloat16*>(p.D) + drow + col0;
-          if (full && ((reinterpret_cast<uintptr_t>(dp) & 15) == 0)) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              uint4 o;
-              o.x = pack_bf16x2(v[j], v[j + 1]);
-              o.y = pack_bf16x2(v[j + 2], v[j + 3]);
-              o.z = pack_bf16x2(v[j + 4], v[j + 5]);
-              o.w = pack_bf16x2(v[j + 6], v[j + 7]);
-              *reinterpret_cast<uint4*>(dp + j) = o;
-            }
-          } else {
-            for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.N) dp[j] = __float2bfloat16(v[j]);
-          }
+          store_d32(v, reinterpret_cast<__nv_bfloat16*>(p.D) + drow + col0, p.N - col0);
         }
       }
       tc_fence_before();
@@ -989,6 +1028,9 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
   GemmKernelParams kp;
   int BN = (a->N > 128 || a->force_bn == 256) && a->force_bn != 128 ? 256 : 128;
   if (cm && cm->mode == 2 && (cm->sub_rows % 256) != 0) BN = 128;
+  if (a->k_step && (a->k_step < 0 || a->k_step % BK || a->strideA || a->strideB || a->tile_group || a->k_ranges || cm ||
+                    (long long)(a->batch - 1) * a->k_step >= a->K || (long long)a->batch * a->k_step < a->K))
+    return -3;
   const int a_batched = a->strideA != 0 && a->batch > 1;
   const int b_batched = (a->strideB != 0 && a->batch > 1) || a->tile_group != nullptr;
   const int b_nbatch = a->tile_group ? a->num_groups : a->batch;
@@ -1020,7 +1062,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     if (rc2) return rc2;
     kp.D = a->D; kp.C = a->C; kp.bias = a->bias; kp.tile_group = nullptr; kp.k_ranges = nullptr; kp.status = a->status;
     kp.ldd = a->ldd; kp.ldc = a->ldc; kp.strideD = a->strideD; kp.strideC = a->strideC;
-    kp.M = a->M; kp.N = a->N; kp.K = a->K; kp.batch = a->batch;
+    kp.M = a->M; kp.N = a->N; kp.K = a->K; kp.batch = a->batch; kp.k_step = a->k_step;
     kp.a_batched = a_batched; kp.b_batched = bb2;
     kp.out_fp32 = a->out_fp32; kp.c_fp32 = a->c_fp32; kp.act = a->act; kp.alpha = a->alpha; kp.beta = a->beta;
     kp.act_a = a->act_a; kp.act_b = a->act_b;
@@ -1046,6 +1088,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
   kp.N = a->N;
   kp.K = a->K;
   kp.batch = a->batch;
+  kp.k_step = a->k_step;
   kp.a_batched = a_batched;
   kp.b_batched = b_batched;
   kp.out_fp32 = a->out_fp32;

@@ -36,6 +36,7 @@ typedef struct SxGemmArgs {
                  // inference time), so a kernel may start fetching it before its predecessor has finished;
                  // bit 1: K need not be a multiple of 8, nor M one of 64 with a_mn: lda covers whole groups of 64 then
   float act_a, act_b;
+  int k_step;    // > 0 (a multiple of 64): one product split over K; batch b sums [b k_step, (b + 1) k_step) into D[b], operands without batches
 } SxGemmArgs;
 int sx_gemm_bf16(const SxGemmArgs* args, cudaStream_t stream);
 

@@ -428,35 +428,35 @@ struct VocabLossPlan {
   long long piece, ld;        // words of a piece, pitch of dz
   int splits;                 // parts of a piece whose sums of dh are apart
   bool sums;                  // dh goes through 32-bit sums in scratch
-  long long o_dz, o_acc, o_wpad, bytes;
+  long long o_dz, o_acc, bytes;
 };
-constexpr int PAIRS = 74;                            // pairs of SMs
 constexpr long long PIECE_BYTES = 256ll << 20;       // of dz, where the caller does not say how wide a piece is
-// dh has T d results only, and for narrow models these are too few tiles of 256 x 256 for 74 pairs of SMs: the words are then cut once more, into parts
-// that run as one batch (4095 tokens of 768: 48 tiles; 3 x 48 fill two rounds, and 50280 words take 257 us instead of 321).
-// Below 512 tokens the sums' own traffic is what counts, as in parts of fewer than 2048 words.
+// dh has T d results only, and for few tokens or narrow models these are too few tiles for the machine: the product is then split over the words into sums of
+// their own (4095 tokens of 768: 48 tiles on 74 pairs of SMs; 3 x 48 fill two rounds, and 50280 words take 255 us instead of 321; 64 tokens of 4096: 16
+// tiles on 148 SMs, 128256 words 693 us). Parts of 2048 words at least: shorter ones are bound by the sums' own traffic.
 static int dh_splits(long long T, int d, long long words) {
-  const long long tiles = ((T + 255) / 256) * ((d + 255) / 256);
-  auto use = [&](int s) { return (double)(tiles * s) / (double)(PAIRS * ((tiles * s + PAIRS - 1) / PAIRS)); };
+  const int places = T < 256 ? 148 : 74;             // the GEMM takes pairs of SMs from 256 rows on
+  const long long tiles = (T < 256 ? (T + 127) / 128 : (T + 255) / 256) * ((d + 255) / 256);
+  auto use = [&](int s) { return (double)(tiles * s) / (double)(places * ((tiles * s + places - 1) / places)); };
   int best = 1;
-  for (int s = 1; s <= 8; ++s) {
-    if (s > 1 && (T < 512 || d < 256 || words / s < 2048)) break;
+  for (int s = 1; s <= 16; ++s) {
+    if (s > 1 && words / s < 2048) break;
     if (use(s) >= 0.9) return s;
     if (use(s) > use(best)) best = s;
   }
   return best;
 }
+static long long k_part(long long words, int splits) { return ((words + splits - 1) / splits + 63) / 64 * 64; }   // at most `splits` parts
 static VocabLossPlan vocab_loss_plan(const SxVocabLossArgs* a) {
   VocabLossPlan p;
   long long piece = a->piece > 0 ? a->piece : PIECE_BYTES / (2 * a->T);
   if (a->piece <= 0 && piece < 1024) piece = 1024;
   piece = (piece + 255) / 256 * 256;
   if (piece > a->V) piece = a->V;
-  p.splits = a->dh ? dh_splits(a->T, a->d, piece) : 1;
-  if (piece < a->V) {                                // equal parts of every piece but the last
-    const long long unit = 256ll * p.splits;
-    piece = piece / unit > 0 ? piece / unit * unit : unit;
-    if (piece > a->V) piece = a->V;
+  p.splits = 1;
+  if (a->dh) {
+    const int s = dh_splits(a->T, a->d, piece);
+    p.splits = (int)((piece + k_part(piece, s) - 1) / k_part(piece, s));
   }
   p.piece = piece;
   p.ld = (piece + 63) / 64 * 64;
@@ -469,8 +469,6 @@ static VocabLossPlan vocab_loss_plan(const SxVocabLossArgs* a) {
   };
   p.o_dz = take(2 * a->T * p.ld);
   p.o_acc = take(p.sums ? 4ll * p.splits * a->T * a->d : 0);
-  const long long last = a->V - (a->V - 1) / piece * piece, unit = 8ll * p.splits;
-  p.o_wpad = take(p.splits > 1 && last % unit ? (last + unit - 1) / unit * unit * a->d * 2 : 0);
   p.bytes = o;
   return p;
 }
@@ -508,18 +506,12 @@ extern "C" int sx_vocab_loss_bwd(const SxVocabLossArgs* a, cudaStream_t st) {
     g.A = dz; g.lda = p.ld;
     if (a->dh) {
       const int s = plan.splits;
-      const long long k = s > 1 ? (n + 8 * s - 1) / (8 * s) * 8 : n;
       g.B = w; g.ldb = a->ldw;
-      if (s > 1 && k * s != n) {      // the last piece, in equal parts: its words and zeros behind them (dz is zero there too)
-        uint8_t* pad = work + plan.o_wpad;
-        if (cudaMemcpy2DAsync(pad, a->d * 2ll, w, a->ldw * 2, a->d * 2ll, n, cudaMemcpyDeviceToDevice, st) != cudaSuccess ||
-            cudaMemsetAsync(pad + n * a->d * 2, 0, (k * s - n) * a->d * 2, st) != cudaSuccess)
-          return -11;
-        g.B = pad; g.ldb = a->d;
-      }
-      g.M = (int)a->T; g.N = a->d; g.K = (int)k;
-      if (s > 1) {
-        g.batch = s; g.strideA = k; g.strideB = k * g.ldb; g.strideD = a->T * a->d;
+      g.M = (int)a->T; g.N = a->d; g.K = (int)n;
+      if (s > 1) {                    // a last piece may have fewer parts
+        g.k_step = (int)k_part(n, s);
+        g.batch = (int)((n + g.k_step - 1) / g.k_step);
+        g.strideD = a->T * a->d;
       }
       g.ldd = a->d;
       const bool out = !plan.sums || (s == 1 && last);
@@ -531,7 +523,7 @@ extern "C" int sx_vocab_loss_bwd(const SxVocabLossArgs* a, cudaStream_t st) {
       if ((rc = sx_gemm_bf16(&g, st))) return rc;
     }
     if (a->dw) {
-      g.a_mn = 1; g.B = a->h; g.ldb = a->ldh; g.batch = 1; g.strideA = g.strideB = g.strideC = g.strideD = 0;
+      g.a_mn = 1; g.B = a->h; g.ldb = a->ldh; g.batch = 1; g.k_step = 0; g.strideC = g.strideD = 0;
       g.M = (int)n; g.N = a->d; g.K = (int)a->T;
       g.D = (char*)a->dw + v0 * a->lddw * (a->dw_fp32 ? 4 : 2);
       g.ldd = a->lddw; g.out_fp32 = a->dw_fp32;

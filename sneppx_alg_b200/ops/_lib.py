@@ -27,7 +27,7 @@ class SxGemmArgs(C.Structure):
         ("tile_group", c_void_p), ("num_groups", c_int),
         ("k_ranges", c_void_p), ("k_total", c_int),
         ("status", c_void_p), ("sm_limit", c_int), ("force_bn", c_int), ("flags", c_int),
-        ("act_a", c_float), ("act_b", c_float),
+        ("act_a", c_float), ("act_b", c_float), ("k_step", c_int),
     ]
 
 
