@@ -35,8 +35,13 @@ template <> struct Act8<float> {
 constexpr int PER = 16;      // values of a thread
 
 // How rows are read and written: 32-byte accesses where base, pitch and width are whole multiples of a thread's values (16 of them: WIDE), 16-byte ones
-// where they are multiples of 8 (PAIR), else one value at a time.
+// where they are multiples of 8 (PAIR; the block's two threads take its vectors in turn, so that they fill sectors together). Else one value at a time
+// (SINGLE), and a warp then shares 512 values so that neighbouring threads touch
+// neighbouring ones: value j of a thread is 32 j behind its first, in the j-th block of the warp's (4101 columns: packed and restored in 222 us with 16
+// neighbouring values a thread, 74 so).
 enum { SINGLE = 0, PAIR = 1, WIDE = 2 };
+template <int MODE>
+__host__ __device__ __forceinline__ int threads_of(int nb) { return MODE == SINGLE ? (nb + 15) / 16 * 32 : nb * 2; }   // of a row of nb blocks
 
 __device__ __forceinline__ void ld32(const void* p, uint32_t (&r)[8]) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -53,6 +58,7 @@ template <typename T> union Row16 {
   uint4 q[sizeof(T)];
   T t[PER];
 };
+// c: 16 times the thread's place in the row
 template <int MODE, typename T>
 __device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>& v) {
   if (MODE == WIDE) {
@@ -65,11 +71,14 @@ __device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>&
     }
   } else if (MODE == PAIR) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i)
-      v.q[i] = c + i * (16 / (int)sizeof(T)) < width ? *reinterpret_cast<const uint4*>(row + c + i * (16 / (int)sizeof(T))) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < (int)sizeof(T); ++i) {
+      const int at = (c & ~31) + (2 * i + (c >> 4 & 1)) * (16 / (int)sizeof(T));
+      v.q[i] = at < width ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+    }
   } else {
+    const int first = (c & ~511) + ((c >> 4) & 31);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) v.t[j] = c + j < width ? row[c + j] : Act8<T>::out(0.f);
+    for (int j = 0; j < PER; ++j) v.t[j] = first + 32 * j < width ? row[first + 32 * j] : Act8<T>::out(0.f);
   }
 }
 template <int MODE, typename T>
@@ -84,12 +93,15 @@ __device__ __forceinline__ void store16(T* row, int c, int width, const float (&
     }
   } else if (MODE == PAIR) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i)
-      if (c + i * (16 / (int)sizeof(T)) < width) *reinterpret_cast<uint4*>(row + c + i * (16 / (int)sizeof(T))) = v.q[i];
+    for (int i = 0; i < (int)sizeof(T); ++i) {
+      const int at = (c & ~31) + (2 * i + (c >> 4 & 1)) * (16 / (int)sizeof(T));
+      if (at < width) *reinterpret_cast<uint4*>(row + at) = v.q[i];
+    }
   } else {
+    const int first = (c & ~511) + ((c >> 4) & 31);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (c + j < width) row[c + j] = v.t[j];
+      if (first + 32 * j < width) row[first + 32 * j] = v.t[j];
   }
 }
 template <typename T>
@@ -98,31 +110,85 @@ __device__ __forceinline__ void widen(const Row16<T>& v, float (&f)[PER]) {
   for (int j = 0; j < PER; ++j) f[j] = Act8<T>::in(v.t[j]);
 }
 
-// Codes and exponent byte of a block whose two threads hold 16 values each; both are there and get the byte.
-__device__ __forceinline__ uint4 encode16(const float (&f)[PER], uint32_t& byte) {
+// A block's exponent byte from the bits of its largest magnitude, and the factor that turns a value into steps (0 for a block that is not finite: its codes
+// are 0, as infinity times 0 is a NaN whose low byte would be anything).
+__device__ __forceinline__ uint32_t exponent_of(uint32_t top) { return top >= 0x7f800000u ? 255u : max((int)((top + 0x10000u) >> 23) - 6, 1); }
+__device__ __forceinline__ uint32_t code_of(float f, uint32_t byte) {
+  return byte == 255u ? 0u : __float_as_uint(fmaf(f, __uint_as_float((254u - byte) << 23), 12582912.f));
+}
+__device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23); }
+// PAIR: word j of four codes of a thread in its block, by vectors of 8 values (16-bit types) or 4.
+template <typename T>
+__device__ __forceinline__ int word_at(int j, int side) { return sizeof(T) == 2 ? (j >> 1) * 4 + side * 2 + (j & 1) : j * 2 + side; }
+// Blocks of a row of nb, from the threads of whole warps (SINGLE) or pairs that hold them: codes and exponents of the row.
+template <int MODE, typename T>
+__device__ __forceinline__ void encode16(const float (&f)[PER], int place, int nb, signed char* codes, unsigned char* exps) {
+  if (MODE == SINGLE) {
+    const int lane = place & 31, first = (place >> 5) * 16;      // the warp's first block
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (first + j >= nb) break;                                // uniform across the warp
+      const uint32_t byte = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(f[j]) & 0x7fffffffu));
+      codes[(first + j) * 32 + lane] = (signed char)code_of(f[j], byte);
+      if (lane == j) mine = byte;
+    }
+    if (lane < PER && first + lane < nb) exps[first + lane] = (unsigned char)mine;
+    return;
+  }
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
   top = max(top, __shfl_xor_sync(3u << ((threadIdx.y * blockDim.x + threadIdx.x) & 30u), top, 1));
-  if (top >= 0x7f800000u) {
-    byte = 255u;
-    return make_uint4(0, 0, 0, 0);
-  }
-  byte = max((int)((top + 0x10000u) >> 23) - 6, 1);
-  const float inv = __uint_as_float((254u - byte) << 23);
+  const uint32_t byte = exponent_of(top);
   uint32_t k[PER], r[4];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) k[j] = __float_as_uint(fmaf(f[j], inv, 12582912.f));
+  for (int j = 0; j < PER; ++j) k[j] = code_of(f[j], byte);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040), __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410);
-  return make_uint4(r[0], r[1], r[2], r[3]);
-}
-__device__ __forceinline__ void decode16(const uint4& k, uint32_t byte, float (&f)[PER]) {
-  const float step = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-  const uint32_t r[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
+  if (MODE == WIDE) {
+    reinterpret_cast<uint4*>(codes)[place] = make_uint4(r[0], r[1], r[2], r[3]);
+  } else {
+    uint32_t* at = reinterpret_cast<uint32_t*>(codes) + (place >> 1) * 8;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) f[j] = (__uint_as_float(__byte_perm(r[j / 4], 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f) * step;
+    for (int j = 0; j < 4; ++j) at[word_at<T>(j, place & 1)] = r[j];
+  }
+  if ((place & 1) == 0) exps[place >> 1] = (unsigned char)byte;
 }
+template <int MODE, typename T>
+struct Held16 {                                                  // read first, restored when the other operands are there
+  uint4 k;
+  uint32_t byte;
+  signed char c[MODE == SINGLE ? PER : 1];
+  __device__ __forceinline__ void load(int place, int nb, const signed char* codes, const unsigned char* exps) {
+    if (MODE == SINGLE) {
+      const int lane = place & 31, first = (place >> 5) * 16;
+      byte = lane < PER && first + lane < nb ? exps[first + lane] : 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) c[MODE == SINGLE ? j : 0] = first + j < nb ? codes[(first + j) * 32 + lane] : 0;
+    } else {
+      if (MODE == WIDE) {
+        k = reinterpret_cast<const uint4*>(codes)[place];
+      } else {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(codes) + (place >> 1) * 8;
+        const int side = place & 1;
+        k = make_uint4(at[word_at<T>(0, side)], at[word_at<T>(1, side)], at[word_at<T>(2, side)], at[word_at<T>(3, side)]);
+      }
+      byte = exps[place >> 1];
+    }
+  }
+  __device__ __forceinline__ void restore(float (&f)[PER]) const {
+    if (MODE == SINGLE) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) f[j] = (float)c[MODE == SINGLE ? j : 0] * step_of(__shfl_sync(0xffffffffu, byte, j));
+      return;
+    }
+    const float step = step_of(byte);
+    const uint32_t r[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) f[j] = (__uint_as_float(__byte_perm(r[j / 4], 0x4b000000u, 0x7440 | (j & 3))) - 8388736.f) * step;
+  }
+};
 
 // x [rows, width] (pitch ld) -> codes [rows, 32 nb], exps [rows, nb], nb = ceil(width / 32); codes behind the row are 0.
 template <int MODE, typename T>
@@ -130,23 +196,23 @@ __global__ void pack8_kernel(const T* __restrict__ x, signed char* __restrict__ 
                              long long ld, int nb) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece >= nb * 2) return;     // pieces come by two, as the block's size does
+  if (row >= rows || piece >= threads_of<MODE>(nb)) return;     // by twos, or by whole warps, as the block's size is
   Row16<T> v;
   load16<MODE>(x + row * ld, piece * PER, width, v);
   float f[PER];
   widen(v, f);
-  uint32_t byte;
-  reinterpret_cast<uint4*>(codes)[(long long)row * (nb * 2) + piece] = encode16(f, byte);
-  if ((piece & 1) == 0) exps[(long long)row * nb + (piece >> 1)] = (unsigned char)byte;
+  encode16<MODE, T>(f, piece, nb, codes + (long long)row * (nb * 32), exps + (long long)row * nb);
 }
 template <int MODE, typename T>
 __global__ void unpack8_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ exps, T* __restrict__ x, unsigned rows, int width,
                                long long ld, int nb) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece * PER >= width) return;
+  if (row >= rows || piece >= threads_of<MODE>(nb)) return;
   float f[PER];
-  decode16(reinterpret_cast<const uint4*>(codes)[(long long)row * (nb * 2) + piece], exps[(long long)row * nb + (piece >> 1)], f);
+  Held16<MODE, T> x8;
+  x8.load(piece, nb, codes + (long long)row * (nb * 32), exps + (long long)row * nb);
+  x8.restore(f);
   store16<MODE>(x + row * ld, piece * PER, width, f);
 }
 
@@ -178,22 +244,17 @@ __global__ void glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, sig
                                 unsigned rows, int width, long long ld, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece >= nb * 2) return;
+  if (row >= rows || piece >= threads_of<MODE>(nb)) return;
   Row16<T> gv, uv;
   load16<MODE>(gu + row * ld, piece * PER, width, gv);
   load16<MODE>(gu + row * ld + width, piece * PER, width, uv);
   float g[PER], u[PER];
   widen(gv, g);
   widen(uv, u);
-  uint32_t gb, ub;
-  uint4* kr = reinterpret_cast<uint4*>(codes) + (long long)row * (nb * 4);
-  kr[piece] = encode16(g, gb);
-  kr[nb * 2 + piece] = encode16(u, ub);
-  if ((piece & 1) == 0) {
-    unsigned char* er = exps + (long long)row * (2 * nb);
-    er[piece >> 1] = (unsigned char)gb;
-    er[nb + (piece >> 1)] = (unsigned char)ub;
-  }
+  signed char* kr = codes + (long long)row * (nb * 64);
+  unsigned char* er = exps + (long long)row * (2 * nb);
+  encode16<MODE, T>(g, piece, nb, kr, er);
+  encode16<MODE, T>(u, piece, nb, kr + nb * 32, er + nb);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     float a, da;
@@ -208,15 +269,17 @@ __global__ void glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __r
                                 T* __restrict__ dgu, unsigned rows, int width, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
-  if (row >= rows || piece * PER >= width) return;
-  const uint4* kr = reinterpret_cast<const uint4*>(codes) + (long long)row * (nb * 4);
+  if (row >= rows || piece >= threads_of<MODE>(nb)) return;
+  const signed char* kr = codes + (long long)row * (nb * 64);
   const unsigned char* er = exps + (long long)row * (2 * nb);
   Row16<T> dv;
   load16<MODE>(dh + (long long)row * width, piece * PER, width, dv);
-  const uint4 gk = kr[piece], uk = kr[nb * 2 + piece];
+  Held16<MODE, T> g8, u8;
+  g8.load(piece, nb, kr, er);
+  u8.load(piece, nb, kr + nb * 32, er + nb);
   float g[PER], u[PER], d[PER];
-  decode16(gk, er[piece >> 1], g);
-  decode16(uk, er[nb + (piece >> 1)], u);
+  g8.restore(g);
+  u8.restore(u);
   widen(dv, d);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -253,41 +316,41 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
   if (rows == 0 || width == 0) return 0;
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
-  dim3 grid, block;
-  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern) { kern<<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb); };
+    auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
-    mode == WIDE ? run(pack8_kernel<WIDE, T>) : mode == PAIR ? run(pack8_kernel<PAIR, T>) : run(pack8_kernel<SINGLE, T>);
+    dim3 grid, block;
+    token_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : run(pack8_kernel<SINGLE, T>, grid, block);
   });
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
-  dim3 grid, block;
-  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern) { kern<<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld, nb); };
+    auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
-    mode == WIDE ? run(unpack8_kernel<WIDE, T>) : mode == PAIR ? run(unpack8_kernel<PAIR, T>) : run(unpack8_kernel<SINGLE, T>);
+    dim3 grid, block;
+    token_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : run(unpack8_kernel<SINGLE, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
-  dim3 grid, block;
-  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern) {
+    auto run = [&](auto kern, dim3 grid, dim3 block) {
       kern<<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb, act);
     };
     const int mode = row_mode(width, ld, gu, h, sizeof(T));
-    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>) : run(glu8_fwd_kernel<SINGLE, T>);
+    dim3 grid, block;
+    token_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : run(glu8_fwd_kernel<SINGLE, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
@@ -295,14 +358,14 @@ extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, 
   if (rows == 0 || width == 0) return 0;
   if (!act8_args_ok(rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
-  dim3 grid, block;
-  token_grid(rows, nb * 2, &grid, &block);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern) {
+    auto run = [&](auto kern, dim3 grid, dim3 block) {
       kern<<<grid, block, 0, st>>>((const T*)dh, (const signed char*)codes, (const unsigned char*)exps, (T*)dgu, (unsigned)rows, width, nb, act);
     };
     const int mode = row_mode(width, width, dh, dgu, sizeof(T));
-    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>) : run(glu8_bwd_kernel<SINGLE, T>);
+    dim3 grid, block;
+    token_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : run(glu8_bwd_kernel<SINGLE, T>, grid, block);
   });
 }

@@ -30,16 +30,25 @@ template <> __device__ __forceinline__ __nv_bfloat16 emb_out<__nv_bfloat16>(floa
 template <> __device__ __forceinline__ __half emb_out<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float emb_out<float>(float v) { return v; }
 
-// Eight neighbouring values in 16-byte accesses (VEC) or one by one up to the row's end.
+// A thread's place c, a multiple of 8, in a row of d values. VEC (whole 16-byte accesses: d, pitch and base allow them): the values c to c + 7. Else the 32
+// threads of a warp share 256 values so that neighbours touch neighbouring ones: value j of a thread is 32 j behind its first (2049 columns: 385 us
+// with eight neighbouring values a thread, 97 so).
 template <typename T> union Emb8 { uint4 q[sizeof(T) / 2]; T t[8]; };
+template <bool VEC>
+__host__ __device__ __forceinline__ int emb_places(int d) { return VEC ? (d + 7) / 8 : (d + 255) / 256 * 32; }   // threads of a row
+template <bool VEC>
+__device__ __forceinline__ bool emb_has(int c, int d) { return VEC ? c < d : (c & ~255) < d; }
+template <bool VEC>
+__device__ __forceinline__ int emb_first(int c) { return VEC ? c : (c & ~255) + ((c >> 3) & 31); }
 template <bool VEC, typename T>
 __device__ __forceinline__ void emb_load(const T* row, int c, int d, Emb8<T>& v) {
   if (VEC) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v.q[i] = reinterpret_cast<const uint4*>(row + c)[i];
   } else {
+    const int first = emb_first<VEC>(c);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v.t[j] = c + j < d ? row[c + j] : emb_out<T>(0.f);
+    for (int j = 0; j < 8; ++j) v.t[j] = first + 32 * j < d ? row[first + 32 * j] : emb_out<T>(0.f);
   }
 }
 template <bool VEC, typename T>
@@ -48,9 +57,10 @@ __device__ __forceinline__ void emb_store(T* row, int c, int d, const Emb8<T>& v
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = v.q[i];
   } else {
+    const int first = emb_first<VEC>(c);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (c + j < d) row[c + j] = v.t[j];
+      if (first + 32 * j < d) row[first + 32 * j] = v.t[j];
   }
 }
 
@@ -72,7 +82,7 @@ __device__ __forceinline__ void lookup(const void* ids, int wide, const T* __res
       if (c0 == 0 && status) atomicCAS(status, 0, EMB_BAD_ARGUMENT);
     }
   }
-  for (int c = c0; c < d; c += c_step) {
+  for (int c = c0; emb_has<VEC>(c, d); c += c_step) {
     Emb8<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -101,8 +111,8 @@ __global__ void embed_fwd_kernel(const void* __restrict__ ids, int wide, const T
                                  long long V, float scale, int* status) {
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   const unsigned long long rows = (unsigned long long)gridDim.x * blockDim.y, t = blockIdx.x * (unsigned long long)blockDim.y + threadIdx.y;
-  if (t >= tokens || c >= d) return;
-  lookup<VEC, U>(ids, wide, w, ldw, y, t, rows, tokens, c, d, d, V, scale, status);
+  if (t >= tokens || !emb_has<VEC>(c, d)) return;
+  lookup<VEC, U>(ids, wide, w, ldw, y, t, rows, tokens, c, 1 << 28, d, V, scale, status);
 }
 
 // ----------------------------------------------------------------------------- tokens sorted by word
@@ -383,7 +393,7 @@ template <bool VEC, typename G>
 __device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long ldg, int d, unsigned block, unsigned blocks) {
   __shared__ unsigned row_of[32], rows;
   const unsigned threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
-  const unsigned vecs = (d + 7) / 8, side = max(threads / vecs, 1u), mine = tid / vecs, c0 = (tid - mine * vecs) * 8;
+  const unsigned vecs = emb_places<VEC>(d), side = max(threads / vecs, 1u), mine = tid / vecs, c0 = (tid - mine * vecs) * 8;
   Emb8<G> z;
 #pragma unroll
   for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
@@ -404,7 +414,7 @@ __device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long 
     if (mine < side) {
       for (unsigned k = mine; k < rows; k += side) {
         G* row = grad + (long long)row_of[k] * ldg;
-        for (int c = c0; c < d; c += threads * 8) emb_store<VEC>(row, c, d, z);
+        for (int c = c0; emb_has<VEC>(c, d); c += threads * 8) emb_store<VEC>(row, c, d, z);
       }
     }
   }
@@ -426,7 +436,7 @@ __global__ void __launch_bounds__(256, 5) embed_sum_kernel(const SortArgs a, con
   if (i0 >= n) return;                 // a warp's threads have one piece
   const unsigned i1 = min(n, i0 + len);
   const unsigned before = i0 > 0 ? key[i0 - 1] : 0xffffffffu, after = i1 < n ? key[i1] : 0xffffffffu;
-  const bool mine = c < d;
+  const bool mine = emb_has<VEC>(c, d);
   unsigned word = 0xffffffffu;         // none yet
   bool open = false;
   float acc[8];
@@ -507,7 +517,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restr
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    if (c < d8) {
+    if (emb_has<VEC>(c, d)) {
 #pragma unroll 4
       for (unsigned q = y; q <= more; q += 8) {
         const float4* p = reinterpret_cast<const float4*>(part + ((size_t)(piece + q) * 2 + (q == 0 ? 1 : 0)) * d8 + c);
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restr
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[y][lane][j] = acc[j];
     __syncthreads();
-    if (y == 0 && c < d) {
+    if (y == 0 && emb_has<VEC>(c, d)) {
       for (int k = 1; k < 8; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] += s[k][lane][j];
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(CS_THREADS) embed_sort_lookup_kernel(const Sor
     cluster_sort(*reinterpret_cast<ClusterSort*>(smem), a, passes, a.key_out, a.pos_out);
     return;
   }
-  const unsigned vecs = (d + 7) / 8, side = max(CS_THREADS / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
+  const unsigned vecs = emb_places<VEC>(d), side = max(CS_THREADS / vecs, 1u), mine = threadIdx.x / vecs, c0 = (threadIdx.x - mine * vecs) * 8;
   if (mine >= side) return;
   const unsigned long long step = (unsigned long long)(gridDim.x - ctas) * side;
   for (unsigned long long t0 = (unsigned long long)(blockIdx.x - ctas) * side + mine; t0 < a.n; t0 += step * 4)
@@ -584,7 +594,7 @@ struct EmbWork {
     len = piece_len(n, d);
     pieces = (unsigned)((n + len - 1) / len);
     tiles = (unsigned)((n + TILE - 1) / TILE);
-    d8 = (d + 7) / 8 * 8;
+    d8 = (d + 255) / 256 * 256;            // a partial sum's floats: places of either kind
     o_part = 0;
     o_sorted = up256(8ll * pieces * d8);
     o_other = o_sorted + (presorted ? 0 : s.bytes);
@@ -621,7 +631,7 @@ static int launch_sort_lookup(const SortArgs& a, int passes, const T* w, long lo
     __atomic_store_n(&fits[dev][size], room, __ATOMIC_RELEASE);
   }
   if (y) {                     // the tokens are dealt out evenly: no more clusters than run at once
-    const long long want = (((long long)a.n * ((d + 7) / 8) + CS_THREADS - 1) / CS_THREADS + ctas - 1) / ctas, most = room > 1 ? room - 1 : 1;
+    const long long want = (((long long)a.n * emb_places<VEC>(d) + CS_THREADS - 1) / CS_THREADS + ctas - 1) / ctas, most = room > 1 ? room - 1 : 1;
     cfg.gridDim = dim3(ctas * (unsigned)(1 + (want < most ? want : most)));
   }
   return cudaLaunchKernelEx(&cfg, kern, a, passes, w, ldw, y, d, scale) == cudaSuccess ? 0 : -11;
@@ -657,7 +667,7 @@ extern "C" int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long l
       return launch_sort_lookup<VEC, T>(sort_args(ids, ids_wide, tokens, V, padding, s, (uint8_t*)sorted, status), s.passes, (const T*)w, ldw, (T*)y, d, scale, st);
     }
     dim3 grid, block;
-    const int vecs = (d + 7) / 8;
+    const int vecs = emb_places<VEC>(d);
     token_grid(tokens, vecs, &grid, &block);
     if (tokens * vecs >= 4ll * 148 * 1024) {
       grid.x = (grid.x + 3) / 4;
@@ -706,7 +716,7 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
   }
   const unsigned* key = a.key_out;
   float* part = (float*)(b + p.o_part);
-  const int items = p.d8 / 8;
+  const int items = vec ? (d + 7) / 8 : p.d8 / 8;
   dim3 block, grid;
   block.x = items >= 128 ? 128 : (items + 31) / 32 * 32;
   block.y = 256 / block.x;
