@@ -486,54 +486,67 @@ __global__ void __launch_bounds__(256, 5) embed_sum_kernel(const SortArgs a, con
     emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
   }
 }
-// Runs that go over several pieces. A block takes 256 columns of the runs that begin in four neighbouring pieces and go on, thread y every eighth of a run's
-// partial sums; the eight are added in order.
-constexpr int JOIN_PIECES = 4;
+// Runs that go over several pieces. A block takes 256 columns of eight neighbouring pieces, a warp a piece: it adds up a run that begins there and reaches
+// up to 16 more by itself. Longer ones are the whole block's, one after another: warp y every eighth of their partial sums, the eight added in order.
+constexpr int JOIN_ALONE = 16;
+__device__ __forceinline__ void add_part(float (&acc)[8], const float* part, unsigned piece, int side, int d8, int c) {
+  const float4* p = reinterpret_cast<const float4*>(part + ((size_t)piece * 2 + side) * d8 + c);
+  const float4 a = p[0], b = p[1];
+  acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
+  acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
+}
 template <bool VEC, typename G>
 __global__ void __launch_bounds__(256) embed_join_kernel(const unsigned* __restrict__ key, G* grad, long long ldg, const float* __restrict__ part, unsigned n,
                                                          unsigned len, int d, int d8, unsigned V, float scale, int add) {
   __shared__ float s[8][32][9];
-  const unsigned lane = threadIdx.x, y = threadIdx.y, first = blockIdx.x * JOIN_PIECES;
+  __shared__ unsigned reach[8];        // pieces behind a warp's own that its run goes on into, where the block adds it up
+  const unsigned lane = threadIdx.x, y = threadIdx.y, piece = blockIdx.x * 8 + y;
   const int c = (int)(blockIdx.y * 32 + lane) * 8;
-  bool begins = false;
-  if (lane < JOIN_PIECES) {
-    const unsigned long long i0 = (unsigned long long)(first + lane) * len, i1 = i0 + len;
-    if (i1 < n) {
-      const unsigned word = key[i1];
-      begins = word < V && key[i1 - 1] == word && (key[i0] != word || i0 == 0 || key[i0 - 1] != word);
+  const bool mine = emb_has<VEC>(c, d);
+  const unsigned long long i0 = (unsigned long long)piece * len, i1 = i0 + len;
+  unsigned more = 0;
+  if (i1 < n) {
+    const unsigned word = key[i1], last = key[i1 - 1], head = key[i0], before = i0 > 0 ? key[i0 - 1] : 0xffffffffu;
+    if (word < V && last == word && (head != word || before != word)) {
+      // how many pieces behind begin with the word: 32 probes 32 pieces apart, then the 32 behind the last that has it
+      auto probe = [&](unsigned apart) {
+        const unsigned long long at = i1 + (unsigned long long)(more + lane * apart) * len;
+        const unsigned b = __ballot_sync(0xffffffffu, at < n && key[at] == word);
+        return b == 0xffffffffu ? 32 : __ffs(~b) - 1;
+      };
+      for (int found = 32; found == 32;) {
+        found = probe(32);
+        more += found > 0 ? 32 * (found - 1) : 0;
+      }
+      more += probe(1);
+    }
+    if (more > 0 && more <= JOIN_ALONE && mine) {
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      add_part(acc, part, piece, 1, d8, c);
+#pragma unroll 4
+      for (unsigned q = 1; q <= more; ++q) add_part(acc, part, piece + q, 0, d8, c);
+      emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
     }
   }
-  for (unsigned left = __ballot_sync(0xffffffffu, begins); left; left &= left - 1) {
-    const unsigned piece = first + __ffs(left) - 1;
-    const unsigned long long i1 = (unsigned long long)(piece + 1) * len;
-    const unsigned word = key[i1];
-    unsigned more = 0;                 // pieces behind it that begin with the word
-    for (bool all = true; all;) {
-      const unsigned long long at = i1 + (unsigned long long)(more + lane) * len;
-      const unsigned b = __ballot_sync(0xffffffffu, at < n && key[at] == word);
-      all = b == 0xffffffffu;
-      more += all ? 32 : __ffs(~b) - 1;
-    }
-    float acc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-    if (emb_has<VEC>(c, d)) {
-#pragma unroll 4
-      for (unsigned q = y; q <= more; q += 8) {
-        const float4* p = reinterpret_cast<const float4*>(part + ((size_t)(piece + q) * 2 + (q == 0 ? 1 : 0)) * d8 + c);
-        const float4 a = p[0], b = p[1];
-        acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
-        acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
-      }
+  if (lane == 0) reach[y] = more > JOIN_ALONE ? more : 0;
+  __syncthreads();
+  for (unsigned k = 0; k < 8; ++k) {
+    const unsigned long_more = reach[k];
+    if (long_more == 0) continue;      // the same for the whole block
+    const unsigned from = blockIdx.x * 8 + k;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (mine) {
+#pragma unroll 8
+      for (unsigned q = y; q <= long_more; q += 8) add_part(acc, part, from + q, q == 0, d8, c);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[y][lane][j] = acc[j];
     __syncthreads();
-    if (y == 0 && emb_has<VEC>(c, d)) {
-      for (int k = 1; k < 8; ++k)
+    if (y == 0 && mine) {
+      for (int i = 1; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += s[k][lane][j];
-      emb_finish<VEC>(grad, ldg, word, c, d, acc, scale, add);
+        for (int j = 0; j < 8; ++j) acc[j] += s[i][lane][j];
+      emb_finish<VEC>(grad, ldg, key[(unsigned long long)(from + 1) * len], c, d, acc, scale, add);
     }
     __syncthreads();
   }
@@ -731,7 +744,7 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
     embed_sum_kernel<VEC, T, G><<<sums + (unsigned)(groups < 148 * 8 ? groups : 148 * 8), block, 0, st>>>(
         a, (const T*)dy, (G*)grad, ldg, part, p.len, d, p.d8, scale, add, grid.x > 0 ? grid.x : 1, sums);
     if (p.pieces > 1)
-      embed_join_kernel<VEC, G><<<dim3((p.pieces + JOIN_PIECES - 1) / JOIN_PIECES, (d + 255) / 256), dim3(32, 8), 0, st>>>(
+      embed_join_kernel<VEC, G><<<dim3((p.pieces + 7) / 8, (d + 255) / 256), dim3(32, 8), 0, st>>>(
           key, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
   };
   auto typed = [&](auto t, auto g) { vec ? run(t, g, std::true_type()) : run(t, g, std::false_type()); };
