@@ -16,6 +16,8 @@ import torch.nn as tnn
 
 from ..nn.modules import Embedding, Linear, Module, RMSNorm
 from ..ops import functional as ops
+from ..ops.act8 import glu_8bit
+from ..ops.token_loss import linear_token_loss
 from .config import ModelConfig, config_from_name
 
 
@@ -56,8 +58,11 @@ class LlamaMLP(Module):
         self.down_proj = Linear(d_ff, cfg.hidden_size, bias=False, dtype=dtype, device=device,
                                 init_std=cfg.initializer_range)
 
+    held_bits = 16      # what backward needs of gate and up is held in 16 bits or, with 8, in 8 (training.extras.enable_8bit_activations)
+
     def forward(self, x):
-        return self.down_proj(ops.glu(self.gate_up_proj(x), self.act))
+        gu = self.gate_up_proj(x)
+        return self.down_proj(glu_8bit(gu, self.act) if self.held_bits == 8 and self.training else ops.glu(gu, self.act))
 
 
 class LlamaBlock(Module):
@@ -110,6 +115,7 @@ class LlamaForCausalLM(Module):
                                   init_std=cfg.initializer_range)
         self._rope = None
         self.activation_checkpointing = False
+        self.checkpoint_bits = 16      # of what activation checkpointing keeps: 16, or 8 with a power of two for 32 values
 
     # ------------------------------------------------------------------ helpers
     def rope(self, device, need):
@@ -140,8 +146,8 @@ class LlamaForCausalLM(Module):
         for i, layer in enumerate(self.layers):
             cache = past_key_values[i] if past_key_values else None
             if self.activation_checkpointing and self.training and cache is None:
-                from torch.utils.checkpoint import checkpoint
-                delta, resid = checkpoint(layer, delta, resid, rope, position_ids, None, use_reentrant=False)
+                from ..training.extras import checkpoint
+                delta, resid = checkpoint(layer, delta, resid, rope, position_ids, None, bits=self.checkpoint_bits)
             else:
                 delta, resid = layer(delta, resid, rope, position_ids, cache)
         if resid is None:
@@ -166,6 +172,16 @@ class LlamaForCausalLM(Module):
         else:
             out["logits"] = ops.linear(h, self.head_weight())
         return out
+
+    def next_token_logprobs(self, input_ids):
+        """log p(next token) [B, S - 1], fp32. On the GPU (bf16) the logits exist in tiles only, in the backward pass too."""
+        h, w = self.hidden_states(input_ids), self.head_weight()
+        if h.is_cuda and h.dtype == w.dtype == torch.bfloat16:
+            target = torch.full_like(input_ids, -100, dtype=torch.int64)
+            target[:, :-1] = input_ids[:, 1:]
+            return -linear_token_loss(h, w, target)[0][:, :-1]
+        lp = torch.log_softmax(ops.linear(h, w).float()[:, :-1], -1)
+        return lp.gather(-1, input_ids[:, 1:].long().unsqueeze(-1)).squeeze(-1)
 
     # ------------------------------------------------------------------ checkpoint name mapping
     def to_reference_state_dict(self):

@@ -10,9 +10,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .functional import GLU_ACT
+from .functional import GLU_ACT, glu_reference
 
 BLOCK = 32
+_NAMES = {v: k for k, v in GLU_ACT.items()}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -138,7 +139,7 @@ class _Glu8Fn(torch.autograd.Function):
             gate, up = g2[:, :f], g2[:, f:]
             parts = [pack_8bit_reference(t) for t in (gate, up)]
             ctx.save_for_backward(torch.cat([c for c, _ in parts], 1), torch.cat([e for _, e in parts], 1))
-            return (_gate(gate.float(), act)[0] * up.float()).to(gu.dtype).view(*gu.shape[:-1], f)
+            return glu_reference(gu, _NAMES[act])
         h = gu.new_empty((*gu.shape[:-1], f))
         held = gu.new_empty(rows * 2 * nb * (BLOCK + 1), dtype=torch.uint8)           # codes of gate and up for each row, then their exponents
         with _lib.on_device(gu):

@@ -14,17 +14,43 @@ import torch
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as _ckpt
 
+from ..ops.act8 import checkpoint_8bit
+
 
 # ---- activation checkpointing
-def checkpoint(fn, *args, **kw):
+def checkpoint(fn, *args, bits: int = 16, **kw):
+    """``fn(*args)`` whose inner activations are recomputed in backward; with ``bits=8`` from arguments that are held in 8 bits
+    (``ops.checkpoint_8bit``, half of the memory; gradients are then those at the restored arguments)."""
+    if bits == 8:
+        if kw:
+            raise TypeError(f"checkpoint(bits=8) takes no further options, got {sorted(kw)}")
+        return checkpoint_8bit(fn, *args)
+    if bits != 16:
+        raise ValueError(f"checkpoint: bits must be 16 or 8, not {bits}")
     return _ckpt(fn, *args, use_reentrant=False, **kw)
 
 
-def enable_activation_checkpointing(model, every: int = 1):
-    """Recompute every ``every``-th repeated layer in backward (models expose ``activation_checkpointing``)."""
+def enable_activation_checkpointing(model, every: int = 1, bits: int = 16):
+    """Recompute every ``every``-th repeated layer in backward (models expose ``activation_checkpointing``). ``bits=8`` holds the layers' inputs in
+    8 bits meanwhile (models expose ``checkpoint_bits``)."""
+    if bits not in (8, 16):
+        raise ValueError(f"enable_activation_checkpointing: bits must be 16 or 8, not {bits}")
+    if bits == 8 and not hasattr(model, "checkpoint_bits"):
+        raise ValueError(f"{type(model).__name__} holds the inputs of its layers in 16 bits only")
     if hasattr(model, "activation_checkpointing"):
         model.activation_checkpointing = True
+    if hasattr(model, "checkpoint_bits"):
+        model.checkpoint_bits = bits
     return model
+
+
+def enable_8bit_activations(model, on: bool = True):
+    """The gated feed-forward blocks of ``model`` hold gate and up in 8 bits between forward and backward (``ops.glu_8bit``) instead of 16. Returns
+    how many do."""
+    blocks = [m for m in model.modules() if hasattr(m, "held_bits")]
+    for m in blocks:
+        m.held_bits = 8 if on else 16
+    return len(blocks)
 
 
 # ---- differential privacy

@@ -95,9 +95,13 @@ def apply_lora(model, r=8, alpha=16.0, targets=("qkv_proj", "o_proj", "gate_up_p
 
 
 def sequence_logprob(model, ids, mask=None):
-    """Sum of next-token log-probabilities of ``ids`` [B, S] under the model."""
-    logits = model(ids)["logits"].float()
-    lp = torch.log_softmax(logits[:, :-1], -1).gather(-1, ids[:, 1:].unsqueeze(-1)).squeeze(-1)
+    """Sum of next-token log-probabilities of ``ids`` [B, S] under the model. Models that give them without their logits
+    (``next_token_logprobs``) do so on the GPU: a batch's logits in 32 bits are the largest tensor of a preference step."""
+    if ids.is_cuda and hasattr(model, "next_token_logprobs"):
+        lp = model.next_token_logprobs(ids)
+    else:
+        logits = model(ids)["logits"].float()
+        lp = torch.log_softmax(logits[:, :-1], -1).gather(-1, ids[:, 1:].unsqueeze(-1)).squeeze(-1)
     if mask is not None:
         lp = lp * mask[:, 1:]
     return lp.sum(-1)
