@@ -37,10 +37,6 @@ def _lookup(ids, table, scale, padding_idx=None, sort=False):
 def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
     """grad [V, d] = scale * (sums of the rows of dy [.., d] by their word), or, with ``add``, grad += that (rows of other words are not touched
     then). Sums are in 32 bits and in the order of the tokens, so they are the same each time. grad has dy's type or is fp32."""
-    return _backward(grad, ids, dy, scale, padding_idx, add, None)
-
-
-def _backward(grad, ids, dy, scale, padding_idx, add, order):
     V, d = grad.shape
     if dy.dtype not in _TYPES or grad.dtype not in (dy.dtype, torch.float32) or grad.stride(1) != 1 or (V > 1 and grad.stride(0) < d):
         raise ValueError(f"embedding_backward_: gradients {dy.dtype} into {grad.dtype} with strides {grad.stride()}")
@@ -50,14 +46,23 @@ def _backward(grad, ids, dy, scale, padding_idx, add, order):
         raise TypeError(f"embedding_backward_: ids of {ids.dtype}")
     if not (grad.is_cuda and grad.get_device() == dy.get_device() == ids.get_device()):
         raise ValueError(f"embedding_backward_: tensors on {grad.device}, {dy.device} and {ids.device}")
-    ids, dy = ids.contiguous(), dy.contiguous()
+    if V == 0:
+        raise ValueError("embedding_backward_: a table of no rows")
+    if padding_idx is not None and not 0 <= padding_idx < V:
+        raise ValueError(f"embedding_backward_: padding_idx {padding_idx} outside a table of {V} rows")
+    return _backward(grad, ids.contiguous(), dy.contiguous(), float(scale), padding_idx, bool(add), None)
+
+
+def _backward(grad, ids, dy, scale, padding_idx, add, order):
+    """ids and dy contiguous, all on one device; order: what the forward pass left, or None."""
+    V, d = grad.shape
     n = ids.numel()
     size = _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)
     with _lib.on_device(grad):
         _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")(
             ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, -1 if padding_idx is None else padding_idx,
-            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], order.data_ptr() if order is not None else 0, work.data_ptr(), size,
+            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], 0 if order is None else order.data_ptr(), work.data_ptr(), size,
             _lib.status_ptr(grad), _lib.here(grad))
     return grad
 
@@ -76,6 +81,7 @@ class _EmbeddingFn(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         table, (scale, padding_idx, order) = ctx.table, ctx.meta
         mg = getattr(table, "main_grad", None)
+        dy = dy.contiguous()
         if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:
             _backward(mg, ids, dy, scale, padding_idx, getattr(table, "_main_grad_written", False), order)
             table._main_grad_written = True
