@@ -116,7 +116,8 @@ __device__ __forceinline__ uint32_t exponent_of(uint32_t top) { return top >= 0x
 __device__ __forceinline__ float per_step(uint32_t byte) { return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23); }
 __device__ __forceinline__ uint32_t code_of(float f, float inv) { return __float_as_uint(fmaf(f, inv, 12582912.f)); }
 __device__ __forceinline__ uint32_t finite_mask(uint32_t byte) { return byte == 255u ? 0u : 0xffffffffu; }
-__device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23); }
+// 2^(byte - 127); packing makes no byte below 1
+__device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23); }
 // PAIR: word j of four codes of a thread in its block, by vectors of 8 values (16-bit types) or 4.
 template <typename T>
 __device__ __forceinline__ int word_at(int j, int side) { return sizeof(T) == 2 ? (j >> 1) * 4 + side * 2 + (j & 1) : j * 2 + side; }

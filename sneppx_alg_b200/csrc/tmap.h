@@ -33,10 +33,12 @@ inline int make_tmap(CUtensorMap* out, CUtensorMapDataType dt, int rank, const v
   EncodeTiledFn fn = get_encode_tiled();
   if (!fn) return -1;
   // The driver call needs a current context; a thread that has only been handed a device by
-  // cudaSetDevice (e.g. an autograd worker) may not have bound the primary context yet.
+  // cudaSetDevice (e.g. an autograd worker) may not have bound the primary context yet. Setting the device once more binds it, and may be done while
+  // a stream is being captured, which cudaFree(0) may not.
   static thread_local bool ctx_bound = false;
   if (!ctx_bound) {
-    cudaFree(0);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return -1;
     ctx_bound = true;
   }
   cuuint64_t d[5];

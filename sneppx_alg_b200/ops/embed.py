@@ -108,6 +108,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {table.shape[0]} rows")
         padding_idx %= table.shape[0]
+    if table.shape[0] == 0 and ids.numel():
+        raise IndexError("embedding: ids for a table of no rows")
     if not (table.is_cuda and table.dtype in _TYPES and table.shape[0] > 0 and _lib.available()):
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:

@@ -19,6 +19,14 @@ def linear_token_loss_reference(h, w, target, ignore_index=-100, softcap=0.0):
         z = softcap * torch.tanh(z / softcap)
     lse = torch.logsumexp(z, -1)
     valid = target != ignore_index
+    bad = valid & ((target < 0) | (target >= w.shape[0]))
+    if not target.is_cuda:
+        if bool(bad.any()):
+            raise IndexError(f"linear_token_loss: a target outside a vocabulary of {w.shape[0]}")
+    else:                                          # as the kernels do: ignored, and told by the status word
+        word = _lib.status_word(target.device)[:1]
+        word.copy_(torch.where(bad.any() & (word == 0), 5, word))
+        valid = valid & ~bad
     zt = z.gather(-1, torch.where(valid, target, 0).unsqueeze(-1)).squeeze(-1)
     return torch.where(valid, lse - zt, 0.0), lse
 
@@ -113,7 +121,8 @@ def linear_token_loss(h, w, target, ignore_index=-100, softcap=0.0, piece=0):
     Backward holds dz for about ``piece`` columns of the vocabulary at a time (0: as many as fit 256 MiB) and computes the logits again: it trades a
     fourth product of h and w for logits that ``linear_cross_entropy`` holds a chunk of, and need not know the tokens' weights beforehand.
     Where w carries ``main_grad`` its gradient is written or added there and ``.grad`` stays empty. On the GPU a target outside [0, V) counts as
-    ignored and sets the status word (``check_status`` raises); on the CPU it raises at once."""
+    ignored and sets the status word (``check_status`` raises); on the CPU it raises at once. Ignored tokens take part in the products with weight 0:
+    their hidden states have to be finite. Scratch of the forward pass: 8 bytes for a token and 256 words."""
     if w.dim() != 2 or h.dim() == 0 or h.shape[-1] != w.shape[1]:
         raise ValueError(f"linear_token_loss: hidden states {tuple(h.shape)} and weights {tuple(w.shape)} do not fit")
     if target.shape != h.shape[:-1]:

@@ -44,3 +44,6 @@ def test_refusals():
         ops.embedding(torch.tensor([1]), w, padding_idx=9)
     with pytest.raises(IndexError):
         ops.embedding(torch.tensor([9]), w)
+    with pytest.raises(IndexError):
+        ops.embedding(torch.tensor([0]), torch.randn(0, 4))
+    assert ops.embedding(torch.zeros(0, dtype=torch.int64), torch.randn(0, 4)).shape == (0, 4)

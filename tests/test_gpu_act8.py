@@ -37,6 +37,16 @@ def test_strided_rows_odd_bases_and_overflows(dtype):
         assert torch.equal(ops.unpack_8bit(ops.pack_8bit(z)), z)
 
 
+def test_every_exponent_byte():
+    """2^(byte - 127) from the smallest on; 255 is NaN."""
+    codes = torch.arange(-128, 128, dtype=torch.int16).to(torch.int8).repeat(256, 1).contiguous()
+    exps = torch.arange(256, dtype=torch.int16).to(torch.uint8)[:, None].repeat(1, 8).contiguous()
+    p = ops.Packed8bit(codes, exps, torch.Size((256, 256)), torch.float32)
+    q = ops.Packed8bit(codes.cuda(), exps.cuda(), p.shape, p.dtype)
+    want, got = ops.unpack_8bit(p), ops.unpack_8bit(q).cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[:255], want[:255])
+
+
 def test_refusals():
     with pytest.raises(TypeError):
         ops.pack_8bit(torch.zeros(4, 64, dtype=torch.float64, device="cuda"))

@@ -157,6 +157,35 @@ def test_refusals():
         ops.embedding_backward_(torch.zeros(50, 64, device="cuda"), torch.tensor([1], device="cuda"), torch.zeros(2, 64, device="cuda"))
 
 
+def test_backward_twice_and_changed_ids():
+    """A graph that is kept may be gone through again, into main_grad too; ids changed in between are an error, as for any saved tensor."""
+    torch.manual_seed(0)
+    w = torch.randn(300, 64, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 300, (500,), device="cuda")
+    y = ops.embedding(ids, w)
+    dy = torch.randn_like(y)
+    a, = torch.autograd.grad(y, w, dy, retain_graph=True)
+    b, = torch.autograd.grad(y, w, dy, retain_graph=True)
+    assert torch.equal(a, b)
+    w.main_grad, w._main_grad_written = torch.empty_like(w), False
+    y.backward(dy, retain_graph=True)
+    y.backward(dy, retain_graph=True)
+    assert torch.equal(w.main_grad, a + a)
+    ids.add_(0)
+    with pytest.raises(RuntimeError):
+        y.backward(dy)
+
+
+def test_expanded_gradient_and_no_grad():
+    w = torch.randn(40, 24, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    ids = torch.randint(0, 40, (17,), device="cuda")
+    ops.embedding(ids, w).sum().backward()                       # a gradient of stride 0
+    assert torch.equal(w.grad.float(), torch.bincount(ids, minlength=40)[:, None].float().expand(40, 24))
+    with torch.no_grad():
+        assert not ops.embedding(ids, w).requires_grad
+    assert not ops.embedding(ids, w.detach()).requires_grad
+
+
 def test_other_stream_and_captured_graph():
     torch.manual_seed(0)
     w = torch.randn(1000, 256, device="cuda")

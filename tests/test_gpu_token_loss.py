@@ -188,6 +188,20 @@ def test_targets_out_of_range_count_as_ignored_and_are_reported():
     assert not nll[(t <= 0)].any()
 
 
+def test_other_types_on_the_gpu():
+    """fp32 takes the PyTorch form: the same values, the same answer to targets out of range."""
+    h, w, t, gn, gz = _inputs(30, 300, 64, 11)
+    nll, lse = ops.linear_token_loss(h.float(), w.float(), t)
+    want, tol = _want(h, w, t, gn, gz, 0.0)
+    _check(dict(nll=nll, lse=lse), want, tol)
+    ops.check_status()
+    t[3] = 300
+    nll, _ = ops.linear_token_loss(h.float(), w.float(), t)
+    with pytest.raises(KernelTimeout):
+        ops.check_status()
+    assert nll[3] == 0 and torch.isfinite(nll).all()
+
+
 def test_large_logits_and_infinities():
     h, w, t, _, _ = _inputs(50, 400, 64, 8)
     h = h * 300                                             # logits up to some thousands: exponentials of differences only

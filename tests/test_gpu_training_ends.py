@@ -164,3 +164,29 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
     ops.check_status()
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first product, forward and backward, is captured into a graph: nothing on the way is a call that a capture does not allow."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from sneppx_alg_b200 import ops
+w = torch.randn(3000, 256, device="cuda").to(torch.bfloat16).requires_grad_()
+h = torch.randn(500, 256, device="cuda").to(torch.bfloat16).requires_grad_()
+ids = torch.randint(0, 3000, (500,), device="cuda")
+def step():
+    nll, lse = ops.linear_token_loss(h, w, ids)
+    return torch.autograd.grad((ops.embedding(ids, w), nll), (w, h), (h.detach(), torch.ones_like(nll)))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
