@@ -432,17 +432,23 @@ struct VocabLossPlan {
 };
 constexpr long long PIECE_BYTES = 256ll << 20;       // of dz, where the caller does not say how wide a piece is
 // dh has T d results only, and for few tokens or narrow models these are too few tiles for the machine: the product is then split over the words into sums of
-// their own (4095 tokens of 768: 48 tiles on 74 pairs of SMs; 3 x 48 fill two rounds, and 50280 words take 255 us instead of 321; 64 tokens of 4096: 16
-// tiles on 148 SMs, 128256 words 693 us). Parts of 2048 words at least: shorter ones are bound by the sums' own traffic.
-static int dh_splits(long long T, int d, long long words) {
+// their own (4095 tokens of 768: 48 tiles on 74 pairs of SMs; 3 x 48 fill two rounds, and 50280 words take 225 us instead of 321; 64 tokens of 4096: 16
+// tiles on 148 SMs, 128256 words 152 us in nine parts, 693 in one). The split that takes least: the product at 1.4 PFLOP/s where every place has a
+// tile, and the sums written, and read for each further piece and once more at the end, at 6 TB/s.
+static int dh_splits(long long T, int d, long long words, long long pieces) {
   const int places = T < 256 ? 148 : 74;             // the GEMM takes pairs of SMs from 256 rows on
   const long long tiles = (T < 256 ? (T + 127) / 128 : (T + 255) / 256) * ((d + 255) / 256);
-  auto use = [&](int s) { return (double)(tiles * s) / (double)(places * ((tiles * s + places - 1) / places)); };
+  const long long rows = T < 256 ? (T + 127) / 128 * 128 : (T + 255) / 256 * 256;
   int best = 1;
-  for (int s = 1; s <= 16; ++s) {
-    if (s > 1 && words / s < 2048) break;
-    if (use(s) >= 0.9) return s;
-    if (use(s) > use(best)) best = s;
+  double least = 0;
+  for (int s = 1; s <= 16 && (s == 1 || words / s >= 1024); ++s) {
+    const double use = (double)(tiles * s) / (double)(places * ((tiles * s + places - 1) / places));
+    const double sums = s > 1 || pieces > 1 ? 4.0 * s * (double)T * d * (2 * pieces) : 0;
+    const double cost = 2.0 * (double)rows * d * (double)(words * pieces) / use / 1.4e15 + sums / 6e12;
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
   }
   return best;
 }
@@ -455,7 +461,7 @@ static VocabLossPlan vocab_loss_plan(const SxVocabLossArgs* a) {
   if (piece > a->V) piece = a->V;
   p.splits = 1;
   if (a->dh) {
-    const int s = dh_splits(a->T, a->d, piece);
+    const int s = dh_splits(a->T, a->d, piece, (a->V + piece - 1) / piece);
     p.splits = (int)((piece + k_part(piece, s) - 1) / k_part(piece, s));
   }
   p.piece = piece;
