@@ -90,9 +90,12 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* sP = reinterpret_cast<float*>(smem);                         // [BT][128] fp32 partial tile, over the drained stages
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.stages * STAGE_BYTES);
-  uint64_t* full = bars;
-  uint64_t* empty = bars + DQ_MAX_STAGES;                             // four converter warps and one MMA warp a k-block
-  uint64_t* a_full = bars + 2 * DQ_MAX_STAGES;                        // [NA] four converter warps
+  // Two barriers a stage, for the ring's even and odd turns: with six stages and four groups of converters (fp8, 64 rows) two groups take a stage in turn,
+  // and the parity of one barrier would say nothing to a group that has not seen the phase before (loads of a ring need not arrive in order). So each barrier
+  // has the same groups every time.
+  uint64_t* full = bars;                                              // [2][DQ_MAX_STAGES]
+  uint64_t* empty = bars + 2 * DQ_MAX_STAGES;                         // four converter warps and one MMA warp a k-block
+  uint64_t* a_full = bars + 3 * DQ_MAX_STAGES;                        // [NA] four converter warps
   uint64_t* a_empty = a_full + Cfg::NA;                               // [NA] MMA
   uint64_t* d_full = a_empty + Cfg::NA;                               // [2] MMA
   uint64_t* d_empty = d_full + 2;                                     // [2] promotion warps
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&full[i], 1);
+      mbar_init(&full[DQ_MAX_STAGES + i], 1);
       mbar_init(&empty[i], 5 * KPS);
     }
     for (int i = 0; i < Cfg::NA; ++i) {
@@ -137,15 +141,16 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
   if (warp == Cfg::MMA_WARP + 2) {
     // ------------------------------------------------------------ TMA
     if (elect_one()) {
+      auto bar_of = [&](int i, int s) { return &full[(i / p.stages & 1) * DQ_MAX_STAGES + s]; };
       auto load_w = [&](int i, int s) {
-        mbar_expect_tx(&full[s], STAGE_BYTES);
-        tma_load_2d(smem + s * STAGE_BYTES, &p.tmW, &full[s], (st0 + i) * 128, n0);
+        mbar_expect_tx(bar_of(i, s), STAGE_BYTES);
+        tma_load_2d(smem + s * STAGE_BYTES, &p.tmW, bar_of(i, s), (st0 + i) * 128, n0);
       };
       auto load_x = [&](int i, int s) {
         // an odd last int4 k-block: the second half of the stage lies past K and arrives as zeros
 #pragma unroll
         for (int c = 0; c < 2 * KPS; ++c)
-          tma_load_2d(smem + s * STAGE_BYTES + DQ_W_BYTES + c * (Cfg::X_BYTES / 2), &p.tmX, &full[s],
+          tma_load_2d(smem + s * STAGE_BYTES + DQ_W_BYTES + c * (Cfg::X_BYTES / 2), &p.tmX, bar_of(i, s),
                       (st0 + i) * KPS * DQ_BK + c * 64, m0);
       };
       const int pre = p.early_weights ? min(nst, p.stages) : 0;
@@ -166,14 +171,14 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
       const int buf = warp - Cfg::MMA_WARP;
       const uint32_t tD = tmem_base + Cfg::TM_D + buf * BT;
       const uint32_t sm0 = smem_u32(smem);
-      int s = INT4 ? 0 : buf;                                          // stage and its phase, followed without a division
-      uint32_t sph = 0, dph = 1, aph = 0;
+      int s = INT4 ? 0 : buf;                                          // stage and turn of the ring, followed without a division
+      uint32_t turn = 0, dph = 1, aph = 0;
       int g = buf;                                                     // A buffer and its phase
       for (int i = buf; i < nk; i += 2) {
         if (g >= Cfg::NA) { g -= Cfg::NA; aph ^= 1; }
-        if (s >= p.stages) { s -= p.stages; sph ^= 1; }
+        if (s >= p.stages) { s -= p.stages; ++turn; }
         // a_full follows full of the stage (the converters read it), but the X tile arrived through the async proxy: wait for it here too
-        if (!mbar_wait(&full[s], sph, s_abort, p.status, ST_TIMEOUT_MMA)) break;
+        if (!mbar_wait(&full[(turn & 1) * DQ_MAX_STAGES + s], turn >> 1 & 1, s_abort, p.status, ST_TIMEOUT_MMA)) break;
         if (!mbar_wait(&d_empty[buf], dph, s_abort, p.status, ST_TIMEOUT_MMA)) break;
         const uint64_t x0 = umma_desc_sw128(sm0 + s * STAGE_BYTES + DQ_W_BYTES + (INT4 ? buf : 0) * Cfg::X_BYTES, 16, 1024);
         if (!mbar_wait(&a_full[g], aph, s_abort, p.status, ST_TIMEOUT_MMA)) break;
@@ -194,12 +199,12 @@ __global__ void __launch_bounds__(DqCfg<BT>::THREADS, DqCfg<BT>::CTAS) gemm_dq_k
     const int g = (warp - Cfg::PW) >> 2, q = warp & 3;                // q: TMEM lane quadrant of this warp (PW is a multiple of 4)
     const int row = q * 32 + lane;
     int s = g / KPS, ab = g;
-    uint32_t sph = 0, aph = 1;
+    uint32_t turn = 0, aph = 1;
     for (int i = g; i < nk; i += Cfg::NG, s += Cfg::NG / KPS, ab += Cfg::NG) {
       if (ab >= Cfg::NA) { ab -= Cfg::NA; aph ^= 1; }
       const uint32_t tA = tmem_base + ab * 64 + (static_cast<uint32_t>(q * 32) << 16);
-      while (s >= p.stages) { s -= p.stages; sph ^= 1; }
-      if (!mbar_wait_warp(&full[s], sph, s_abort, p.status, ST_TIMEOUT_CONVERT)) break;
+      while (s >= p.stages) { s -= p.stages; ++turn; }
+      if (!mbar_wait_warp(&full[(turn & 1) * DQ_MAX_STAGES + s], turn >> 1 & 1, s_abort, p.status, ST_TIMEOUT_CONVERT)) break;
       const uint8_t* src = smem + s * STAGE_BYTES + row * 128;
       bool ok = true;
 #pragma unroll
@@ -344,12 +349,12 @@ template <int BT, bool INT4>
 static int dq_launch(DqParams& p, int sms, cudaStream_t st) {
   using Cfg = DqCfg<BT>;
   constexpr int STAGE_BYTES = DQ_W_BYTES + (INT4 ? 2 : 1) * Cfg::X_BYTES;
-  // A stage belongs to the same groups of converters each time it is filled: the parity of a barrier says nothing to a group that has not seen the phase
-  // before (a ring's loads need not arrive in order). With six stages and four groups, fp8 at 64 rows, a group could take a stage that was still empty.
-  constexpr int KPS = INT4 ? 2 : 1, ROOM = Cfg::BUDGET / STAGE_BYTES < DQ_MAX_STAGES ? Cfg::BUDGET / STAGE_BYTES : DQ_MAX_STAGES;
-  constexpr int TURN = Cfg::NG > KPS ? Cfg::NG / KPS : 1;
-  p.stages = ROOM / TURN * TURN;
-  static_assert(ROOM / TURN * TURN >= 2, "at least two stages");
+  constexpr int KPS = INT4 ? 2 : 1;
+  p.stages = Cfg::BUDGET / STAGE_BYTES < DQ_MAX_STAGES ? Cfg::BUDGET / STAGE_BYTES : DQ_MAX_STAGES;
+  // k-block i of turn u of the ring is i = stages KPS u + ...: the same group after two turns (the barriers' comment in the kernel)
+  static_assert(2 * (Cfg::BUDGET / STAGE_BYTES < DQ_MAX_STAGES ? Cfg::BUDGET / STAGE_BYTES : DQ_MAX_STAGES) * KPS % Cfg::NG == 0, "groups of a barrier");
+  static_assert(Cfg::BUDGET / STAGE_BYTES >= 2, "at least two stages");
+  static_assert((3 * DQ_MAX_STAGES + 2 * Cfg::NA + 4) * 8 + 8 <= 256, "barriers");
   static_assert(2 * STAGE_BYTES >= BT * DQ_BM * 4, "the partial tile lies over the stages");
   const int smem = p.stages * STAGE_BYTES + 1024 + 256;
   static int set = 0;
