@@ -221,10 +221,16 @@ __global__ void unpack8_kernel(const signed char* __restrict__ codes, const unsi
 }
 
 // Value and derivative of the gate's function: 0 silu, 1 gelu by tanh, 2 relu. Both smooth ones by a logistic function s: gelu's (1 + tanh y) / 2 is
-// s(2 y), which loses nothing for negative g. 16-bit results need 2^-9 of it: the approximate exponential and quotient (a few 2^-22) do; 32-bit ones
-// take the exact functions.
+// s(2 y), which loses nothing for negative g. 16-bit results need 2^-9 of it: e^-x = 2^(-x log2 e) and a reciprocal by the approximate instructions (a few
+// 2^-22) do, whose results below 2^-126 are 0 (forward at 8192 x 14336 150.5 us; 156 by __expf and __fdividef); 32-bit ones take the exact functions.
 template <bool FAST>
-__device__ __forceinline__ float logistic(float x) { return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float logistic(float x) {
+  if (!FAST) return 1.f / (1.f + expf(-x));
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
+}
 template <bool FAST>
 __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
   if (act == 0) {
@@ -243,9 +249,9 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
 }
 
 // gu [rows, 2 width] (gate | up): h = act(gate) * up, and gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb].
-// Blocks of up to 256 threads; 16-bit types in 48 registers: 8192 x 14336 bf16 forward 155 us and backward 153, 168 and 195 with the registers that the
-// compiler would take (56 and 64), 180 and 164 in blocks of 448 threads besides. 32-bit types have more on their way and keep theirs (41 and 37 us at 4096
-// x 4096; 41 and 42 with fewer).
+// Blocks of up to 256 threads; 16-bit types forward in 48 registers and backward in 64: 8192 x 14336 bf16 forward 150.5 us, 158 in 64, and backward 147 us,
+// 161 in 48 (both move 947 MB; 180 and 164 in blocks of 448 threads). 32-bit types have more on their way and keep the registers that the compiler takes (39
+// and 38 us at 4096 x 4096; 41 and 42 with fewer).
 template <int MODE, typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 1) glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps,
                                 unsigned rows, int width, long long ld, int nb, int act) {
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 1) glu8_fwd_kernel(c
 }
 // dgu = (dh * up * act'(gate) | dh * act(gate)) with gate and up as their 8 bits say.
 template <int MODE, typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 1) glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1) glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
                                 T* __restrict__ dgu, unsigned rows, int width, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
