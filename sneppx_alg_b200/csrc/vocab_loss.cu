@@ -11,8 +11,9 @@
 // Sixteen epilogue warps (four TMEM quadrants, four groups of 64 columns): the exponentials of a tile are behind the products from widths of 256 on only
 // if four warps of each scheduler take turns.
 // The tensor cores cut what they add to an accumulator: over 4096 products a logit of 14 loses 1e-4. The forward pass, whose losses are differences of
-// logits, therefore takes the accumulator out after 1024 products and adds in registers, rounded: lse of 4088 tokens over [128256, 4096] is off by 1.4e-6
-// without that, by 3.7e-7 with it in the same time, by 2.2e-7 after 512 products, which cost 3% more. dz is rounded to bf16 anyway.
+// logits, therefore takes the accumulator out after 1024 products at most and adds in registers, rounded: lse of 4088 tokens over [128256, 4096] is off by
+// 1.4e-6 without that, by 3.7e-7 with it in the same time, by 2.2e-7 after 512 products, which cost 3% more (20% over 768 columns). dz is rounded to bf16
+// anyway.
 // Takes the place of the reference's softmax / cross-entropy kernels (kernel/cuda/autodiff_cuda.cu:519-608).
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -30,7 +31,7 @@ constexpr int VL_GROUPS = 4;                         // epilogue warps of a TMEM
 constexpr int VL_COLS = 256 / VL_GROUPS;             // columns of an epilogue warp
 constexpr int VL_EPI_WARPS = 4 * VL_GROUPS;
 constexpr int VL_THREADS = 64 + 32 * VL_EPI_WARPS;
-constexpr int VL_CHUNK = 1024 / VL_BK;               // forward: k-blocks that stay in one accumulator
+constexpr int VL_CHUNK = 1024 / VL_BK;               // forward: k-blocks that stay in one accumulator at most
 constexpr int VL_SLOTS = 4;                          // tiles whose pairs may wait to be joined (below)
 constexpr int VL_OFF_PAIRS = VL_STAGES * VL_STAGE_BYTES;
 constexpr int VL_PAIR_BYTES = VL_SLOTS * (VL_GROUPS - 1) * 128 * 8;
@@ -131,7 +132,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = p.m_blks * p.n_blks;
   const int num_kb = (p.d + VL_BK - 1) / VL_BK;
-  const int chunk = GRAD ? num_kb : VL_CHUNK;
+  const int parts = (num_kb + VL_CHUNK - 1) / VL_CHUNK;
+  const int chunk = GRAD ? num_kb : (num_kb + parts - 1) / parts;      // equal ones: what is cut grows with the longest
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
