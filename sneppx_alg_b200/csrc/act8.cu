@@ -318,7 +318,9 @@ static int row_mode(int width, long long ld, const void* p, const void* q, int s
   if (width % PER == 0 && ld * size % 32 == 0 && at % 32 == 0) return WIDE;
   return width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0 ? PAIR : SINGLE;
 }
-static bool act8_args_ok(long long rows, int width, int dtype) { return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2; }
+static bool act8_args_ok(const void* codes, long long rows, int width, int dtype) {
+  return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+}
 
 // dtype 0 bf16, 1 fp16, 2 fp32
 template <typename F>
@@ -334,7 +336,7 @@ using namespace sx;
 
 extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(rows, width, dtype)) return -1;
+  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -347,7 +349,7 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(rows, width, dtype)) return -1;
+  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -360,7 +362,7 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(rows, width, dtype)) return -1;
+  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -376,7 +378,7 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
                            cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(rows, width, dtype)) return -1;
+  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);

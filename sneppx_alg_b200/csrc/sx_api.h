@@ -508,7 +508,8 @@ int sx_win_decode(const SxWinAttnArgs* args, cudaStream_t stream);        // dec
 int sx_win_merge(const SxWinAttnArgs* args, cudaStream_t stream);         // key slices -> y
 
 // ------------------------------------------------------------------ L2 activations in 8 bits (act8.cu)
-// dtype: 0 bf16, 1 fp16, 2 fp32. Per 32 values of a row a power of two and signed codes: codes [rows, 32 nb], exps [rows, nb], nb = ceil(width / 32).
+// dtype: 0 bf16, 1 fp16, 2 fp32. Per 32 values of a row a power of two and signed codes: codes [rows, 32 nb] (16-byte aligned), exps [rows, nb], nb =
+// ceil(width / 32).
 int sx_pack8(const void* x, void* codes, void* exps, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
 int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
 // gu [rows, 2 width] (gate | up, pitch ld) -> h [rows, width], gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb]; and back with dh.

@@ -32,7 +32,7 @@ class Packed8bit:
     __slots__ = ("codes", "exponents", "shape", "dtype")
 
     def __init__(self, codes, exponents, shape, dtype):
-        self.codes, self.exponents, self.shape, self.dtype = codes, exponents, shape, dtype
+        self.codes, self.exponents, self.shape, self.dtype = codes, exponents, torch.Size(shape), dtype
 
     @property
     def nbytes(self) -> int:
@@ -102,6 +102,8 @@ def unpack_8bit(p: Packed8bit, dtype=None):
     if dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
     codes, exps = p.codes.contiguous(), p.exponents.contiguous()
+    if codes.data_ptr() % 16:                  # a view into something larger: the kernels read four words at once
+        codes = codes.clone()
     x = codes.new_empty(p.shape, dtype=dtype)
     with _lib.on_device(x):
         _lib.entry("sx_unpack8", "ppplilip")(codes.data_ptr(), exps.data_ptr(), x.data_ptr(), rows, w, w, _TYPES[dtype], _lib.here(x))

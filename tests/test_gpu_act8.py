@@ -4,6 +4,7 @@ import torch
 
 from act8_common import TYPES, gate, held, inputs
 from sneppx_alg_b200 import ops
+from sneppx_alg_b200.ops import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +126,18 @@ def test_checkpoint_of_a_block():
     b = ops.unpack_8bit(ops.pack_8bit(a.detach())).requires_grad_()
     ga, gw = torch.autograd.grad(ops.glu(ops.linear(b, w).repeat(1, 2)).float().sum(), (b, w))
     assert torch.equal(a.grad, ga) and torch.equal(w.grad, gw)
+
+
+@pytest.mark.parametrize("width", [64, 72, 77])
+@pytest.mark.parametrize("offset", [1, 4, 8, 16])
+def test_codes_inside_a_larger_buffer(width, offset):
+    """Held values may be views of any alignment; the entry point itself takes none that its loads could not."""
+    x = torch.randn(5, width, device="cuda").bfloat16()
+    p = ops.pack_8bit(x)
+    buf = torch.zeros(offset + p.codes.numel(), device="cuda", dtype=torch.int8)
+    view = buf[offset:].view(p.codes.shape)
+    view.copy_(p.codes)
+    assert torch.equal(ops.unpack_8bit(ops.Packed8bit(view, p.exponents, tuple(x.shape), x.dtype)), ops.unpack_8bit(p))
+    if offset < 16:
+        with pytest.raises(RuntimeError, match="code -1"):
+            _lib.entry("sx_unpack8", "ppplilip")(view.data_ptr(), p.exponents.data_ptr(), x.data_ptr(), 5, width, width, 0, _lib.here(x))
