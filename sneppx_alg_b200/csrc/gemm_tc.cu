@@ -26,6 +26,7 @@ namespace sx {
 
 constexpr int BM = 128;
 constexpr int BK = 64;
+constexpr int MN_GROUP_BYTES = 64 * BK * 2;   // 64 columns of an MN-major operand's stage
 constexpr int GEMM_THREADS = 192;
 
 // Collective fused into the GEMM (template parameter COMM):
@@ -82,6 +83,7 @@ struct GemmKernelParams {
   int M, N, K, batch;
   int k_step;             // > 0: batch b reduces over [b k_step, (b + 1) k_step) of K; operands have no batches
   int a_batched, b_batched;
+  int a_ragged, b_ragged; // MN-major operands whose extent is no multiple of 64
   int out_fp32, c_fp32, act;
   float alpha, beta, act_a, act_b;
   int m_blks, n_blks;
@@ -475,10 +477,20 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
           uint8_t* sb = sa + Cfg::A_BYTES;
           mbar_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
           const int kc = k0 + kb * BK;
-          if (A_MN) tma_load_4d(sa, &p.tmA, &full_bar[stage], 0, kc, m_blk * (BM / 64), ab);
-          else      tma_load_3d(sa, &p.tmA, &full_bar[stage], kc, m_blk * BM, ab);
-          if (B_MN) tma_load_4d(sb, &p.tmB, &full_bar[stage], 0, kc, n_blk * (BN / 64), bb);
-          else      tma_load_3d(sb, &p.tmB, &full_bar[stage], kc, n_blk * BN, bb);
+          if (A_MN && p.a_ragged) {
+            for (int g = 0; g < BM / 64; ++g) tma_load_3d(sa + g * MN_GROUP_BYTES, &p.tmA, &full_bar[stage], m_blk * BM + g * 64, kc, ab);
+          } else if (A_MN) {
+            tma_load_4d(sa, &p.tmA, &full_bar[stage], 0, kc, m_blk * (BM / 64), ab);
+          } else {
+            tma_load_3d(sa, &p.tmA, &full_bar[stage], kc, m_blk * BM, ab);
+          }
+          if (B_MN && p.b_ragged) {
+            for (int g = 0; g < BN / 64; ++g) tma_load_3d(sb + g * MN_GROUP_BYTES, &p.tmB, &full_bar[stage], n_blk * BN + g * 64, kc, bb);
+          } else if (B_MN) {
+            tma_load_4d(sb, &p.tmB, &full_bar[stage], 0, kc, n_blk * (BN / 64), bb);
+          } else {
+            tma_load_3d(sb, &p.tmB, &full_bar[stage], kc, n_blk * BN, bb);
+          }
           if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -739,8 +751,12 @@ static int launch_cfg(const GemmKernelParams& kp, int grid, cudaStream_t st) {
 
 static int make_operand_map(CUtensorMap* tm, const void* ptr, int mn, int K, long long ld, int batched, int batch,
                             long long stride, bool mn_major, int tile_mn) {
-  if (mn_major) {
-    if (mn % 64 != 0) return -20;
+  if (mn_major && mn % 64) {      // the last 64 columns of a row would go on into the next one: loaded 64 at a time, what is behind the row as zeros
+    uint64_t dims[3] = {(uint64_t)mn, (uint64_t)K, (uint64_t)(batched ? batch : 1)};
+    uint64_t strides[2] = {(uint64_t)ld * 2, (uint64_t)(batched ? stride : (long long)K * ld) * 2};
+    uint32_t box[3] = {64, (uint32_t)BK, 1};
+    return make_tmap(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides, box);
+  } else if (mn_major) {
     uint64_t dims[4] = {64, (uint64_t)K, (uint64_t)(mn / 64), (uint64_t)(batched ? batch : 1)};
     uint64_t strides[3] = {(uint64_t)ld * 2, 128, (uint64_t)(batched ? stride : (long long)K * ld) * 2};
     uint32_t box[4] = {64, (uint32_t)BK, (uint32_t)(tile_mn / 64), 1};
@@ -844,10 +860,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
           if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * G2_STAGE_BYTES);
           const uint32_t fb = smem_u32(&full_bar[stage]) & PEER_MASK;
           const int kc = k0 + kb * BK;
-          if (A_MN) tma2_load_4d(sa, &p.tmA, fb, 0, kc, arow / 64, ab);
-          else      tma2_load_3d(sa, &p.tmA, fb, kc, arow, ab);
-          if (B_MN) tma2_load_4d(sb, &p.tmB, fb, 0, kc, brow / 64, bb);
-          else      tma2_load_3d(sb, &p.tmB, fb, kc, brow, bb);
+          if (A_MN && p.a_ragged) {
+            for (int g = 0; g < 128 / 64; ++g) tma2_load_3d(sa + g * MN_GROUP_BYTES, &p.tmA, fb, arow + g * 64, kc, ab);
+          } else if (A_MN) {
+            tma2_load_4d(sa, &p.tmA, fb, 0, kc, arow / 64, ab);
+          } else {
+            tma2_load_3d(sa, &p.tmA, fb, kc, arow, ab);
+          }
+          if (B_MN && p.b_ragged) {
+            for (int g = 0; g < BN2 / 2 / 64; ++g) tma2_load_3d(sb + g * MN_GROUP_BYTES, &p.tmB, fb, brow + g * 64, kc, bb);
+          } else if (B_MN) {
+            tma2_load_4d(sb, &p.tmB, fb, 0, kc, brow / 64, bb);
+          } else {
+            tma2_load_3d(sb, &p.tmB, fb, kc, brow, bb);
+          }
           if (++stage == G2_STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
@@ -1022,10 +1048,10 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
       (reinterpret_cast<uintptr_t>(a->B) & 15))
     return -1;
   // Tensor maps take any K (what is behind it is read as zero); callers that ask for it by flag have seen to the pitches.
-  const bool any_size = (a->flags & 2) != 0;
-  if (a->K % 8 && !any_size) return -2;
-  const int a_mn_rows = any_size && a->a_mn && (a->M + 63) / 64 * 64 <= a->lda ? (a->M + 63) / 64 * 64 : a->M;   // extent of an MN-major A
+  if (a->K % 8 && !(a->flags & 2)) return -2;
   GemmKernelParams kp;
+  kp.a_ragged = a->a_mn && a->M % 64;
+  kp.b_ragged = a->b_mn && a->N % 64;
   int BN = (a->N > 128 || a->force_bn == 256) && a->force_bn != 128 ? 256 : 128;
   if (cm && cm->mode == 2 && (cm->sub_rows % 256) != 0) BN = 128;
   if (a->k_step && (a->k_step < 0 || a->k_step % BK || a->strideA || a->strideB || a->tile_group || a->k_ranges || cm ||
@@ -1043,7 +1069,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     use_pair = e ? atoi(e) : 1;
   }
   if (use_pair && !cm && !a->tile_group && !a->k_ranges && a->M >= 256 && a->N >= 256 && a->force_bn == 0 &&
-      a->sm_limit == 0 && (!a->a_mn || a_mn_rows % 64 == 0) && (!a->b_mn || a->N % 64 == 0)) {
+      a->sm_limit == 0) {
     const int bb2 = a->strideB != 0 && a->batch > 1;
     int dev2 = 0, sms2 = 148;
     cudaGetDevice(&dev2);
@@ -1056,7 +1082,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
       pair_bn = (e && atoi(e) == 128) ? 128 : 256;
     }
     const int bn2 = pair_bn;
-    int rc2 = make_operand_map(&kp.tmA, a->A, a_mn_rows, a->K, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, 128);
+    int rc2 = make_operand_map(&kp.tmA, a->A, a->M, a->K, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, 128);
     if (rc2) return rc2;
     rc2 = make_operand_map(&kp.tmB, a->B, a->N, a->K, a->ldb, bb2, a->batch, a->strideB, a->b_mn != 0, bn2 / 2);
     if (rc2) return rc2;
@@ -1070,7 +1096,7 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     const int am2 = a->a_mn != 0, bm2 = a->b_mn != 0;
     return bn2 == 256 ? launch_cfg2_any<256>(kp, am2, bm2, sms2, st) : launch_cfg2_any<128>(kp, am2, bm2, sms2, st);
   }
-  int rc = make_operand_map(&kp.tmA, a->A, a_mn_rows, Kfull, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, BM);
+  int rc = make_operand_map(&kp.tmA, a->A, a->M, Kfull, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, BM);
   if (rc) return rc;
   rc = make_operand_map(&kp.tmB, a->B, a->N, Kfull, a->ldb, b_batched, b_nbatch, a->strideB, a->b_mn != 0, BN);
   if (rc) return rc;

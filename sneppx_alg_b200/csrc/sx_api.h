@@ -34,7 +34,7 @@ typedef struct SxGemmArgs {
   int force_bn;  // 0 auto, 128 or 256
   int flags;     // bit 0: B is not written by any kernel launched before this one on the stream (a weight at
                  // inference time), so a kernel may start fetching it before its predecessor has finished;
-                 // bit 1: K need not be a multiple of 8, nor M one of 64 with a_mn: lda covers whole groups of 64 then
+                 // bit 1: K need not be a multiple of 8 (pitches still are)
   float act_a, act_b;
   int k_step;    // > 0 (a multiple of 64): one product split over K; batch b sums [b k_step, (b + 1) k_step) into D[b], operands without batches
 } SxGemmArgs;
@@ -537,7 +537,7 @@ int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long
 // part: scratch of ceil(V / 256) T pairs of floats; zt: scratch of T floats.
 int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                       long long ignore_index, float cap, void* part, float* zt, float* nll, float* lse, int* status, cudaStream_t stream);
-// Backward: dh [T, d] bf16 and dw [V, d] (bf16, or fp32 with dw_fp32; written, or added to with dw_add), either may be null; d a multiple of 64. g_nll and
+// Backward: dh [T, d] bf16 and dw [V, d] (bf16, or fp32 with dw_fp32; written, or added to with dw_add), either may be null. g_nll and
 // g_lse (either may be null): gradients of nll and lse. dz, the gradient of the logits, exists for `piece` words at a time (0: as many as fit 256 MiB).
 typedef struct SxVocabLossArgs {
   const void* h; const void* w; long long ldh, ldw;

@@ -481,7 +481,7 @@ static VocabLossPlan vocab_loss_plan(const SxVocabLossArgs* a) {
   return p;
 }
 static bool vocab_loss_args_ok(const SxVocabLossArgs* a) {
-  return a->T > 0 && a->T <= (1 << 30) && a->V > 0 && a->V <= (1 << 30) && a->d > 0 && a->d % 64 == 0 && a->piece >= 0;
+  return a->T > 0 && a->T <= (1 << 30) && a->V > 0 && a->V <= (1 << 30) && a->d > 0 && a->d % 8 == 0 && a->piece >= 0;
 }
 
 }  // namespace sx

@@ -77,7 +77,7 @@ class _TokenLossFn(torch.autograd.Function):
         ignore_index, softcap, piece = ctx.meta
         need_h, need_w = ctx.needs_input_grad[:2]
         T, V, d0 = tgt.numel(), w.shape[0], w.shape[1]
-        d = (d0 + 63) // 64 * 64                       # what the products' layouts take
+        d = (d0 + 7) // 8 * 8                          # what the products' pitches take
         (h2, ldh), (w2, ldw) = _rows16(h.reshape(-1, d0), d), _rows16(w, d)
         gn, gz = (None if g is None else g.reshape(-1).float().contiguous() for g in (g_nll, g_lse))
         dh = h2.new_empty((T, d)) if need_h else None

@@ -6,12 +6,14 @@ exponentials (each a few 2^-23, at most 300 additions one after another: 300 x 2
 relative error of ez + elsa from its exponential and half a step of bf16, 2^-8; dh and dw add up its errors times the other factor, one rounding of
 2^-24 for each addition, and half a step of their own.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
 from sneppx_alg_b200 import ops
+from sneppx_alg_b200.ops import _lib
 from sneppx_alg_b200.ops._lib import KernelTimeout
 
 pytestmark = pytest.mark.gpu
@@ -235,3 +237,42 @@ def test_other_stream_and_captured_graph():
         want = ops.linear_token_loss(x, w, t)
         assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
     ops.check_status()
+
+
+@pytest.mark.parametrize("T,V,d", [(700, 1318, 328), (40, 5000, 1000), (2000, 700, 744), (257, 513, 3848), (5, 300, 24), (300, 4000, 136), (64, 9000, 264)])
+def test_widths_between_multiples_of_64(T, V, d):
+    x = _inputs(T, V, d, 21)
+    got = _run(*x, 0.0)
+    want, tol = _want(*x, 0.0)
+    _check(got, want, tol)
+
+
+@pytest.mark.parametrize("into", [torch.float32, torch.bfloat16])
+def test_main_grad_of_a_width_between_multiples_of_64(into):
+    h, w, t, gn, gz = _inputs(300, 1001, 328, 22)
+    want, tol = _want(h, w, t, gn, gz, 0.0)
+    w = w.detach().requires_grad_()
+    w.main_grad = torch.full((1001, 328), math.nan, device="cuda", dtype=into)
+    nll, lse = ops.linear_token_loss(h, w, t)
+    assert torch.autograd.grad((nll, lse), w, (gn, gz), allow_unused=True)[0] is None
+    _check(dict(dw=w.main_grad.float()), want, tol)
+
+
+@pytest.mark.parametrize("M,N,K", [(72, 40, 64), (300, 200, 136), (1000, 328, 700), (264, 3848, 77), (520, 8, 300)])
+@pytest.mark.parametrize("a_mn,b_mn", [(False, True), (True, False), (True, True)])
+def test_products_of_ragged_operands(M, N, K, a_mn, b_mn):
+    """Operands with K along their rows, whose rows are no whole groups of 64; behind each row of the storage stands NaN."""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    full = [torch.full((r, c + 8 - c % 8 + 8), math.nan, device="cuda", dtype=torch.bfloat16) for r, c in ((K, M) if a_mn else (M, K), (K, N) if b_mn else (N, K))]
+    a, b = (f[:, :c] for f, c in zip(full, (M if a_mn else K, N if b_mn else K)))
+    for x in (a, b):
+        x.copy_(torch.randn(x.shape, device="cuda", generator=g))
+    d = torch.full((M, N), math.nan, device="cuda")
+    p = _lib.SxGemmArgs()
+    p.A, p.B, p.D, p.M, p.N, p.K, p.batch = a.data_ptr(), b.data_ptr(), d.data_ptr(), M, N, K, 1
+    p.lda, p.ldb, p.ldd, p.a_mn, p.b_mn, p.out_fp32 = a.stride(0), b.stride(0), N, a_mn, b_mn, 1
+    p.alpha, p.flags, p.status = 1.0, 2, _lib.status_ptr(d)
+    _lib.call("sx_gemm_bf16", ctypes.byref(p), _lib.stream())
+    ops.check_status()
+    A, B = (a.T if a_mn else a).double(), (b if b_mn else b.T).double()
+    assert ((d.double() - A @ B).abs() <= K * 2.0 ** -23 * (A.abs() @ B.abs())).all()       # K additions, each cut by at most 2^-23 of what is added up
