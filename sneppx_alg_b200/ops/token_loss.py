@@ -32,9 +32,14 @@ def linear_token_loss_reference(h, w, target, ignore_index=-100, softcap=0.0):
 
 
 def _rows16(t, d):
-    """(t, pitch): t [n, <= d] as the tensor maps take it: d columns, a multiple of 8 (padded with zeros), rows 16-byte aligned."""
-    if t.shape[1] != d:
-        t = F.pad(t, (0, d - t.shape[1]))
+    """(t, pitch): t [..., <= d] as the tensor maps take it: rows of d columns, a multiple of 8 (padded with zeros), 16-byte aligned."""
+    w = t.shape[-1]
+    if w == d and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, d
+    if t.dim() != 2:
+        t = t.reshape(-1, w)
+    if w != d:
+        t = F.pad(t, (0, d - w))
     one = t.shape[0] == 1                      # its pitch may be anything and means nothing
     if t.stride(1) != 1 or (not one and (t.stride(0) % 8 or t.stride(0) < d)) or t.data_ptr() % 16:
         t = t.contiguous()
@@ -44,24 +49,23 @@ def _rows16(t, d):
 
 
 def _forward(h, w, target, ignore_index, softcap):
-    """(nll, lse) in target's shape."""
+    """(nll, lse) in target's shape, and the targets as they were read."""
     T, V, d = target.numel(), w.shape[0], (w.shape[1] + 7) // 8 * 8
-    (h2, ldh), (w2, ldw) = _rows16(h.reshape(-1, h.shape[-1]), d), _rows16(w, d)
+    (h2, ldh), (w2, ldw) = _rows16(h, d), _rows16(w, d)
     tgt = target.contiguous()
-    nll, lse = (h2.new_empty(target.shape, dtype=torch.float32) for _ in range(2))
+    nll, lse = h2.new_empty(target.shape, dtype=torch.float32), h2.new_empty(target.shape, dtype=torch.float32)
     scratch = h2.new_empty(T * (2 * -(-V // 256) + 1), dtype=torch.float32)          # pairs of a row's maximum and sum, and its target's logit
     with _lib.on_device(h):
         _lib.entry("sx_vocab_loss_fwd", "plplpllilfpppppp")(
             h2.data_ptr(), ldh, w2.data_ptr(), ldw, tgt.data_ptr(), T, V, d, ignore_index, softcap, scratch.data_ptr(),
             scratch.data_ptr() + 8 * T * -(-V // 256), nll.data_ptr(), lse.data_ptr(), _lib.status_ptr(h), _lib.here(h))
-    return nll, lse
+    return nll, lse, tgt
 
 
 class _TokenLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, target, ignore_index, softcap, piece):
-        nll, lse = _forward(h, w, target, ignore_index, softcap)
-        tgt = target.reshape(-1).contiguous()
+        nll, lse, tgt = _forward(h, w, target, ignore_index, softcap)
         ctx.save_for_backward(h, w, tgt, lse)
         ctx.meta = ignore_index, softcap, piece
         ctx.set_materialize_grads(False)
@@ -78,9 +82,9 @@ class _TokenLossFn(torch.autograd.Function):
         need_h, need_w = ctx.needs_input_grad[:2]
         T, V, d0 = tgt.numel(), w.shape[0], w.shape[1]
         d = (d0 + 7) // 8 * 8                          # what the products' pitches take
-        (h2, ldh), (w2, ldw) = _rows16(h.reshape(-1, d0), d), _rows16(w, d)
-        gn, gz = (None if g is None else g.reshape(-1).float().contiguous() for g in (g_nll, g_lse))
-        dh = h2.new_empty((T, d)) if need_h else None
+        (h2, ldh), (w2, ldw) = _rows16(h, d), _rows16(w, d)
+        gn, gz = (g if g is None or g.is_contiguous() else g.contiguous() for g in (g_nll, g_lse))       # fp32, as the results are
+        dh = h2.new_empty(h.shape if d == d0 else (T, d)) if need_h else None
         mg = getattr(w, "main_grad", None) if need_w and d == d0 else None
         if mg is not None and (mg.dtype not in (torch.bfloat16, torch.float32) or mg.stride(1) != 1):
             mg = None
@@ -108,8 +112,8 @@ class _TokenLossFn(torch.autograd.Function):
             dw = None
         elif need_w and d != d0:
             dw = dw[:, :d0].contiguous()
-        if need_h:
-            dh = (dh if d == d0 else dh[:, :d0]).reshape(h.shape)
+        if need_h and d != d0:
+            dh = dh[:, :d0].reshape(h.shape)
         return dh, dw, None, None, None, None
 
 
@@ -141,5 +145,5 @@ def linear_token_loss(h, w, target, ignore_index=-100, softcap=0.0, piece=0):
     if _dbg.ENABLED:
         _dbg.check_indices(target, 0, w.shape[0], _dbg.SITE_CE_TARGET, also_ok=ignore_index)
     if not (torch.is_grad_enabled() and (h.requires_grad or w.requires_grad)):
-        return _forward(h, w, target, int(ignore_index), float(softcap))
+        return _forward(h, w, target, int(ignore_index), float(softcap))[:2]
     return _TokenLossFn.apply(h, w, target, int(ignore_index), float(softcap), int(piece))
