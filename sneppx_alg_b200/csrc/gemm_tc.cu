@@ -780,7 +780,7 @@ static int make_operand_map(CUtensorMap* tm, const void* ptr, int mn, int K, lon
 //   full[s]   even CTA only: its producer arms 64 KB, the TMA loads of BOTH CTAs complete on it
 //   empty[s]  both CTAs: released by the even CTA's tcgen05.commit, multicast to the pair
 //   tfull[a]  both CTAs: accumulator a complete, multicast commit
-//   tempty[a] even CTA only, 8 arrivals: the four epilogue warps of each CTA arrive on it (the odd CTA remotely)
+//   tempty[a] even CTA only: the epilogue warps of both CTAs arrive on it (the odd CTA's remotely)
 // Dense, non-grouped, non-fused calls only; everything else stays on gemm_tc_kernel.
 // Pair tile 256 x BN2 (BN2 = 256, or 128 when the wider tile would leave the last wave of pairs mostly idle).
 template <int BN2>
@@ -791,8 +791,11 @@ struct G2Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 };
-template <int BN2, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+// EPI epilogue warps. One on each scheduler takes 3 us for a tile, which the products of about 700 hide; behind fewer, two on each do it in 2.5 ([128256,
+// 4096] from 64 products in bf16 317 -> 270 us, added to a gradient in fp32 1373 -> 1033; [4095, 50304] from 512 217 -> 197). Behind 1024 and more they take
+// the products' power (3 to 10 % slower), so long sums keep four.
+template <int BN2, int EPI, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EPI, 1)
     gemm2_kernel(const __grid_constant__ GemmKernelParams p) {
   constexpr int G2_STAGES = G2Cfg<BN2>::STAGES;
   constexpr int G2_A_BYTES = G2Cfg<BN2>::A_BYTES;
@@ -820,7 +823,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull_bar[i], 1);
-      mbar_init(&tempty_bar[i], 8);
+      mbar_init(&tempty_bar[i], 2 * EPI);
     }
     *s_abort = 0;
     mbar_fence_init();
@@ -917,8 +920,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue (4 warps per CTA, this CTA's 128 rows)
-    const int q = warp & 3;
+    // ------------------------------------------------------------ epilogue (this CTA's 128 rows; four warps a part of the columns)
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    constexpr int CHUNKS = BN2 / 32 / (EPI / 4);
     int it = 0;
     for (int t = cluster_id; t < total_tiles; t += n_clusters) {
       int b, m_blk, n_blk;
@@ -932,7 +936,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
       const long long drow = (long long)b * p.strideD + (long long)row * p.ldd;
       const long long crow = (long long)b * p.strideC + (long long)row * p.ldc;
 #pragma unroll 1
-      for (int c = 0; c < BN2 / 32; ++c) {
+      for (int c = part * CHUNKS; c < (part + 1) * CHUNKS; ++c) {
         const int col0 = n_blk * BN2 + c * 32;
         if (col0 >= p.N) break;  // uniform across the warp
         uint32_t r[32];
@@ -1000,17 +1004,18 @@ static int g2_max_clusters(int sms) {
   return sms / 2;
 }
 
-template <int BN2, bool A_MN, bool B_MN>
+template <int BN2, int EPI, bool A_MN, bool B_MN>
 static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
   static bool attr_set = false;
   static int max_clusters = 0;
-  auto kern = gemm2_kernel<BN2, A_MN, B_MN>;
+  auto kern = gemm2_kernel<BN2, EPI, A_MN, B_MN>;
+  constexpr int THREADS = 64 + 32 * EPI;
   constexpr int SMEM = G2Cfg<BN2>::SMEM_BYTES;
   if (!attr_set) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -10;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms & ~1, 1, 1);
-    cfg.blockDim = dim3(GEMM_THREADS, 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = SMEM;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1025,16 +1030,16 @@ static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
   const long long tiles = (long long)kp.batch * kp.m_blks * kp.n_blks;
   int clusters = (int)(tiles < max_clusters ? tiles : max_clusters);
   if (clusters > sms / 2) clusters = sms / 2;
-  kern<<<2 * clusters, GEMM_THREADS, SMEM, st>>>(kp);
+  kern<<<2 * clusters, THREADS, SMEM, st>>>(kp);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
-template <int BN2>
+template <int BN2, int EPI>
 static int launch_cfg2_any(const GemmKernelParams& kp, int am, int bm, int sms, cudaStream_t st) {
-  if (!am && !bm) return launch_cfg2<BN2, false, false>(kp, sms, st);
-  if (!am && bm) return launch_cfg2<BN2, false, true>(kp, sms, st);
-  if (am && !bm) return launch_cfg2<BN2, true, false>(kp, sms, st);
-  return launch_cfg2<BN2, true, true>(kp, sms, st);
+  if (!am && !bm) return launch_cfg2<BN2, EPI, false, false>(kp, sms, st);
+  if (!am && bm) return launch_cfg2<BN2, EPI, false, true>(kp, sms, st);
+  if (am && !bm) return launch_cfg2<BN2, EPI, true, false>(kp, sms, st);
+  return launch_cfg2<BN2, EPI, true, true>(kp, sms, st);
 }
 
 }  // namespace sx
@@ -1094,7 +1099,8 @@ static int gemm_launch(const SxGemmArgs* a, const SxGemmCommArgs* cm, cudaStream
     kp.act_a = a->act_a; kp.act_b = a->act_b;
     kp.m_blks = (a->M + 255) / 256; kp.n_blks = (a->N + bn2 - 1) / bn2;
     const int am2 = a->a_mn != 0, bm2 = a->b_mn != 0;
-    return bn2 == 256 ? launch_cfg2_any<256>(kp, am2, bm2, sms2, st) : launch_cfg2_any<128>(kp, am2, bm2, sms2, st);
+    if (bn2 == 128) return launch_cfg2_any<128, 4>(kp, am2, bm2, sms2, st);
+    return (a->k_step ? a->k_step : a->K) <= 512 ? launch_cfg2_any<256, 8>(kp, am2, bm2, sms2, st) : launch_cfg2_any<256, 4>(kp, am2, bm2, sms2, st);
   }
   int rc = make_operand_map(&kp.tmA, a->A, a->M, Kfull, a->lda, a_batched, a->batch, a->strideA, a->a_mn != 0, BM);
   if (rc) return rc;
