@@ -35,13 +35,14 @@ template <> struct Act8<float> {
 constexpr int PER = 16;      // values of a thread
 
 // How rows are read and written: 32-byte accesses where base, pitch and width are whole multiples of a thread's values (16 of them: WIDE), 16-byte ones
-// where they are multiples of 8 (PAIR; the block's two threads take its vectors in turn, so that they fill sectors together). Else one value at a time
-// (SINGLE), and a warp then shares 512 values so that neighbouring threads touch
-// neighbouring ones: value j of a thread is 32 j behind its first, in the j-th block of the warp's (4101 columns: packed and restored in 222 us with 16
-// neighbouring values a thread, 74 so).
-enum { SINGLE = 0, PAIR = 1, WIDE = 2 };
+// where they are multiples of 8 (PAIR; the block's two threads take its vectors in turn, so that they fill sectors together). Rows that begin anywhere (ODD)
+// are read and written by a warp as whole aligned words, 32 next to each other, and turned into 16 neighbouring values a thread and back through shared
+// memory; a word that two rows or two warps share is read and written by halves. (8192 x 4101 in bf16: packed and restored in 57 us, gated with
+// its gradient 167; 78 and 226 with values one by one, 32 apart, which is no slower up to some 80 columns; 222 packed and restored with a thread's 16
+// neighbours one by one.)
+enum { ODD = 0, PAIR = 1, WIDE = 2 };
 template <int MODE>
-__host__ __device__ __forceinline__ int threads_of(int nb) { return MODE == SINGLE ? (nb + 15) / 16 * 32 : nb * 2; }   // of a row of nb blocks
+__host__ __device__ __forceinline__ int threads_of(int nb) { return MODE == ODD ? (nb + 15) / 16 * 32 : nb * 2; }   // of a row of nb blocks
 
 __device__ __forceinline__ void ld32(const void* p, uint32_t (&r)[8]) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -58,9 +59,19 @@ template <typename T> union Row16 {
   uint4 q[sizeof(T)];
   T t[PER];
 };
-// c: 16 times the thread's place in the row
+// A warp's part of a row in shared memory: a thread's 32 or 64 bytes and 16 more, so that neither access meets a bank twice.
+template <typename T> constexpr int STAGED = 4 * (int)sizeof(T) + 4;                          // words of a thread
+template <typename T>
+__device__ __forceinline__ int staged(int k) { return sizeof(T) == 2 ? (k >> 3) * 12 + (k & 7) : (k >> 4) * 20 + (k & 15); }
 template <int MODE, typename T>
-__device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>& v) {
+__device__ __forceinline__ uint32_t* stage_of_warp() {
+  __shared__ __align__(16) uint32_t stage[MODE == ODD ? 8 * 32 * STAGED<T> : 4];
+  return stage + (MODE == ODD ? ((threadIdx.y * blockDim.x + threadIdx.x) >> 5) * 32 * STAGED<T> : 0);
+}
+__device__ __forceinline__ uint32_t bits16(const void* p) { return *reinterpret_cast<const uint16_t*>(p); }
+// c: 16 times the thread's place in the row. ODD: words as they lie, to be settled; `tail` the last thread's word behind the warp's.
+template <int MODE, typename T>
+__device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>& v, uint32_t& tail) {
   if (MODE == WIDE) {
     if (c < width) {
 #pragma unroll
@@ -76,13 +87,43 @@ __device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>&
       v.q[i] = at < width ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
     }
   } else {
-    const int first = (c & ~511) + ((c >> 4) & 31);
+    const int lane = c >> 4 & 31, first = c & ~511, n = width - first;
+    const T* p = row + first;
+    if (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) v.t[j] = first + 32 * j < width ? row[first + 32 * j] : Act8<T>::out(0.f);
+      for (int j = 0; j < 16; ++j) v.w[j >> 3 & (sizeof(T) / 2 - 1)][j & 7] = lane + 32 * j < n ? reinterpret_cast<const uint32_t*>(p)[lane + 32 * j] : 0u;
+    } else {
+      const int s = (int)(reinterpret_cast<uintptr_t>(p) >> 1 & 1);      // the first value is a word's second half
+      auto word = [&](int k) {                                           // values 2 k - s and the next
+        const int lo = 2 * k - s, hi = lo + 1;
+        if (lo >= 0 && hi < n) return *reinterpret_cast<const uint32_t*>(p + lo);
+        return (lo >= 0 && lo < n ? bits16(p + lo) : 0u) | (hi < n ? bits16(p + hi) << 16 : 0u);
+      };
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v.w[0][j] = word(lane + 32 * j);
+      tail = s && lane == 31 ? word(256) : 0u;
+    }
   }
 }
 template <int MODE, typename T>
-__device__ __forceinline__ void store16(T* row, int c, int width, const float (&f)[PER]) {
+__device__ __forceinline__ void settle16(const T* row, int c, Row16<T>& v, uint32_t tail, uint32_t* stage) {
+  if (MODE != ODD) return;
+  const int lane = c >> 4 & 31;
+#pragma unroll
+  for (int j = 0; j < 4 * (int)sizeof(T); ++j) stage[staged<T>(lane + 32 * j)] = v.w[j >> 3][j & 7];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) v.q[i] = *reinterpret_cast<const uint4*>(stage + lane * STAGED<T> + 4 * i);
+  __syncwarp();
+  if (sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(row) & 2)) {
+    uint32_t next = __shfl_down_sync(0xffffffffu, v.w[0][0], 1);
+    if (lane == 31) next = tail;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.w[0][j] = __funnelshift_r(v.w[0][j], j < 7 ? v.w[0][j + 1] : next, 16);
+  }
+}
+template <int MODE, typename T>
+__device__ __forceinline__ void store16(T* row, int c, int width, const float (&f)[PER], uint32_t* stage) {
   Row16<T> v;
 #pragma unroll
   for (int j = 0; j < PER; ++j) v.t[j] = Act8<T>::out(f[j]);
@@ -98,10 +139,35 @@ __device__ __forceinline__ void store16(T* row, int c, int width, const float (&
       if (at < width) *reinterpret_cast<uint4*>(row + at) = v.q[i];
     }
   } else {
-    const int first = (c & ~511) + ((c >> 4) & 31);
+    const int lane = c >> 4 & 31, first = c & ~511, n = width - first;
+    T* p = row + first;
+    const int s = sizeof(T) == 2 ? (int)(reinterpret_cast<uintptr_t>(p) >> 1 & 1) : 0;
+    if (s) {
+      if (lane == 31 && 511 < n) p[511] = v.t[15];
+      const uint32_t before = __shfl_up_sync(0xffffffffu, v.w[0][7], 1);
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (first + 32 * j < width) row[first + 32 * j] = v.t[j];
+      for (int j = 7; j >= 0; --j) v.w[0][j] = __funnelshift_l(j > 0 ? v.w[0][j - 1] : before, v.w[0][j], 16);
+    }
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) *reinterpret_cast<uint4*>(stage + lane * STAGED<T> + 4 * i) = v.q[i];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4 * (int)sizeof(T); ++j) {
+      const int k = lane + 32 * j;
+      const uint32_t x = stage[staged<T>(k)];
+      if (sizeof(T) == 4) {
+        if (k < n) reinterpret_cast<uint32_t*>(p)[k] = x;
+      } else {
+        const int lo = 2 * k - s, hi = lo + 1;
+        if (lo >= 0 && hi < n) {
+          *reinterpret_cast<uint32_t*>(p + lo) = x;
+        } else {
+          if (lo >= 0 && lo < n) *reinterpret_cast<uint16_t*>(p + lo) = (uint16_t)x;
+          if (hi < n) *reinterpret_cast<uint16_t*>(p + hi) = (uint16_t)(x >> 16);
+        }
+      }
+    }
+    __syncwarp();
   }
 }
 template <typename T>
@@ -121,22 +187,9 @@ __device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float
 // PAIR: word j of four codes of a thread in its block, by vectors of 8 values (16-bit types) or 4.
 template <typename T>
 __device__ __forceinline__ int word_at(int j, int side) { return sizeof(T) == 2 ? (j >> 1) * 4 + side * 2 + (j & 1) : j * 2 + side; }
-// Blocks of a row of nb, from the threads of whole warps (SINGLE) or pairs that hold them: codes and exponents of the row.
+// Blocks of a row of nb, from the pairs of threads that hold them: codes and exponents of the row.
 template <int MODE, typename T>
 __device__ __forceinline__ void encode16(const float (&f)[PER], int place, int nb, signed char* codes, unsigned char* exps) {
-  if (MODE == SINGLE) {
-    const int lane = place & 31, first = (place >> 5) * 16;      // the warp's first block
-    uint32_t mine = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (first + j >= nb) break;                                // uniform across the warp
-      const uint32_t byte = exponent_of(__reduce_max_sync(0xffffffffu, __float_as_uint(f[j]) & 0x7fffffffu));
-      codes[(first + j) * 32 + lane] = (signed char)(code_of(f[j], per_step(byte)) & finite_mask(byte));
-      if (lane == j) mine = byte;
-    }
-    if (lane < PER && first + lane < nb) exps[first + lane] = (unsigned char)mine;
-    return;
-  }
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
@@ -150,7 +203,8 @@ __device__ __forceinline__ void encode16(const float (&f)[PER], int place, int n
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     r[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040), __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410) & mask;
-  if (MODE == WIDE) {
+  if (MODE == ODD && place >= 2 * nb) return;          // the last warp of a row may have threads to spare
+  if (MODE != PAIR) {
     reinterpret_cast<uint4*>(codes)[place] = make_uint4(r[0], r[1], r[2], r[3]);
   } else {
     uint32_t* at = reinterpret_cast<uint32_t*>(codes) + (place >> 1) * 8;
@@ -163,30 +217,20 @@ template <int MODE, typename T>
 struct Held16 {                                                  // read first, restored when the other operands are there
   uint4 k;
   uint32_t byte;
-  signed char c[MODE == SINGLE ? PER : 1];
   __device__ __forceinline__ void load(int place, int nb, const signed char* codes, const unsigned char* exps) {
-    if (MODE == SINGLE) {
-      const int lane = place & 31, first = (place >> 5) * 16;
-      byte = lane < PER && first + lane < nb ? exps[first + lane] : 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) c[MODE == SINGLE ? j : 0] = first + j < nb ? codes[(first + j) * 32 + lane] : 0;
+    k = make_uint4(0, 0, 0, 0);
+    byte = 1;
+    if (MODE == ODD && place >= 2 * nb) return;
+    if (MODE != PAIR) {
+      k = reinterpret_cast<const uint4*>(codes)[place];
     } else {
-      if (MODE == WIDE) {
-        k = reinterpret_cast<const uint4*>(codes)[place];
-      } else {
-        const uint32_t* at = reinterpret_cast<const uint32_t*>(codes) + (place >> 1) * 8;
-        const int side = place & 1;
-        k = make_uint4(at[word_at<T>(0, side)], at[word_at<T>(1, side)], at[word_at<T>(2, side)], at[word_at<T>(3, side)]);
-      }
-      byte = exps[place >> 1];
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(codes) + (place >> 1) * 8;
+      const int side = place & 1;
+      k = make_uint4(at[word_at<T>(0, side)], at[word_at<T>(1, side)], at[word_at<T>(2, side)], at[word_at<T>(3, side)]);
     }
+    byte = exps[place >> 1];
   }
   __device__ __forceinline__ void restore(float (&f)[PER]) const {
-    if (MODE == SINGLE) {
-#pragma unroll
-      for (int j = 0; j < PER; ++j) f[j] = (float)c[MODE == SINGLE ? j : 0] * step_of(__shfl_sync(0xffffffffu, byte, j));
-      return;
-    }
     const float step = step_of(byte);
     const uint32_t r[4] = {k.x ^ 0x80808080u, k.y ^ 0x80808080u, k.z ^ 0x80808080u, k.w ^ 0x80808080u};
 #pragma unroll
@@ -202,7 +246,9 @@ __global__ void pack8_kernel(const T* __restrict__ x, signed char* __restrict__ 
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
   if (row >= rows || piece >= threads_of<MODE>(nb)) return;     // by twos, or by whole warps, as the block's size is
   Row16<T> v;
-  load16<MODE>(x + row * ld, piece * PER, width, v);
+  uint32_t tail;
+  load16<MODE>(x + row * ld, piece * PER, width, v, tail);
+  settle16<MODE>(x + row * ld, piece * PER, v, tail, stage_of_warp<MODE, T>());
   float f[PER];
   widen(v, f);
   encode16<MODE, T>(f, piece, nb, codes + (long long)row * (nb * 32), exps + (long long)row * nb);
@@ -217,7 +263,7 @@ __global__ void unpack8_kernel(const signed char* __restrict__ codes, const unsi
   Held16<MODE, T> x8;
   x8.load(piece, nb, codes + (long long)row * (nb * 32), exps + (long long)row * nb);
   x8.restore(f);
-  store16<MODE>(x + row * ld, piece * PER, width, f);
+  store16<MODE>(x + row * ld, piece * PER, width, f, stage_of_warp<MODE, T>());
 }
 
 // Value and derivative of the gate's function: 0 silu, 1 gelu by tanh, 2 relu. Both smooth ones by a logistic function s: gelu's (1 + tanh y) / 2 is
@@ -249,18 +295,21 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
 }
 
 // gu [rows, 2 width] (gate | up): h = act(gate) * up, and gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb].
-// Blocks of up to 256 threads; 16-bit types forward in 48 registers and backward in 64: 8192 x 14336 bf16 forward 150.5 us, 158 in 64, and backward 147 us,
+// Blocks of up to 256 threads; 16-bit types forward in 48 registers (ODD 64: 84 us at 8192 x 4101, 87 in 48) and backward in 64: 8192 x 14336 bf16 forward 150.5 us, 158 in 64, and backward 147 us,
 // 161 in 48 (both move 947 MB; 180 and 164 in blocks of 448 threads). 32-bit types have more on their way and keep the registers that the compiler takes (39
 // and 38 us at 4096 x 4096; 41 and 42 with fewer).
 template <int MODE, typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 1) glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps,
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 1) glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps,
                                 unsigned rows, int width, long long ld, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
   if (row >= rows || piece >= threads_of<MODE>(nb)) return;
   Row16<T> gv, uv;
-  load16<MODE>(gu + row * ld, piece * PER, width, gv);
-  load16<MODE>(gu + row * ld + width, piece * PER, width, uv);
+  uint32_t gt, ut, *stage = stage_of_warp<MODE, T>();
+  load16<MODE>(gu + row * ld, piece * PER, width, gv, gt);
+  load16<MODE>(gu + row * ld + width, piece * PER, width, uv, ut);
+  settle16<MODE>(gu + row * ld, piece * PER, gv, gt, stage);
+  settle16<MODE>(gu + row * ld + width, piece * PER, uv, ut, stage);
   float g[PER], u[PER];
   widen(gv, g);
   widen(uv, u);
@@ -274,7 +323,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 5 : 1) glu8_fwd_kernel(c
     gate8<sizeof(T) == 2>(g[j], act, a, da);
     g[j] = a * u[j];
   }
-  store16<MODE>(h + (long long)row * width, piece * PER, width, g);
+  store16<MODE>(h + (long long)row * width, piece * PER, width, g, stage);
 }
 // dgu = (dh * up * act'(gate) | dh * act(gate)) with gate and up as their 8 bits say.
 template <int MODE, typename T>
@@ -286,10 +335,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1) glu8_bwd_kernel(c
   const signed char* kr = codes + (long long)row * (nb * 64);
   const unsigned char* er = exps + (long long)row * (2 * nb);
   Row16<T> dv;
-  load16<MODE>(dh + (long long)row * width, piece * PER, width, dv);
+  uint32_t tail, *stage = stage_of_warp<MODE, T>();
+  load16<MODE>(dh + (long long)row * width, piece * PER, width, dv, tail);
   Held16<MODE, T> g8, u8;
   g8.load(piece, nb, kr, er);
   u8.load(piece, nb, kr + nb * 32, er + nb);
+  settle16<MODE>(dh + (long long)row * width, piece * PER, dv, tail, stage);
   float g[PER], u[PER], d[PER];
   g8.restore(g);
   u8.restore(u);
@@ -302,8 +353,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1) glu8_bwd_kernel(c
     d[j] *= a;
   }
   T* o = dgu + (long long)row * (2 * (long long)width);
-  store16<MODE>(o, piece * PER, width, g);
-  store16<MODE>(o + width, piece * PER, width, d);
+  store16<MODE>(o, piece * PER, width, g, stage);
+  store16<MODE>(o + width, piece * PER, width, d, stage);
 }
 
 // As token_grid, but rows of 128 threads and more in blocks of 128 at most: a block's registers are what limits how many run.
@@ -316,7 +367,7 @@ static void rows_grid(long long rows, int threads, dim3* grid, dim3* block) {
 static int row_mode(int width, long long ld, const void* p, const void* q, int size) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
   if (width % PER == 0 && ld * size % 32 == 0 && at % 32 == 0) return WIDE;
-  return width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0 ? PAIR : SINGLE;
+  return width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0 ? PAIR : ODD;
 }
 static bool act8_args_ok(const void* codes, long long rows, int width, int dtype) {
   return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
@@ -343,8 +394,8 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
     auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
-    rows_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : run(pack8_kernel<SINGLE, T>, grid, block);
+    rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : run(pack8_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
@@ -356,8 +407,8 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
     auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
-    rows_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : run(unpack8_kernel<SINGLE, T>, grid, block);
+    rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : run(unpack8_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
@@ -371,8 +422,8 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
     };
     const int mode = row_mode(width, ld, gu, h, sizeof(T));
     dim3 grid, block;
-    rows_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : run(glu8_fwd_kernel<SINGLE, T>, grid, block);
+    rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : run(glu8_fwd_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
@@ -387,7 +438,7 @@ extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, 
     };
     const int mode = row_mode(width, width, dh, dgu, sizeof(T));
     dim3 grid, block;
-    rows_grid(rows, mode == SINGLE ? threads_of<SINGLE>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : run(glu8_bwd_kernel<SINGLE, T>, grid, block);
+    rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
+    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : run(glu8_bwd_kernel<ODD, T>, grid, block);
   });
 }
