@@ -3,6 +3,8 @@
 module (interface_bindings/nn.py, ``Embedding``)."""
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
@@ -17,6 +19,16 @@ def embedding_reference(ids, table, scale=1.0, padding_idx=None):
     return y if scale == 1.0 else (y.float() * scale).to(y.dtype) if y.dtype != torch.float64 else y * scale
 
 
+@functools.lru_cache(1024)
+def _sorted_bytes(n, V):
+    return _lib.entry("sx_embed_sorted_bytes", "ll", _lib.c_ll)(n, V)
+
+
+@functools.lru_cache(1024)
+def _workspace(n, V, d, presorted):
+    return _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, presorted)
+
+
 def _lookup(ids, table, scale, padding_idx=None, sort=False):
     """(rows, ids as they were read, those in the order of their words or None)."""
     if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
@@ -25,7 +37,7 @@ def _lookup(ids, table, scale, padding_idx=None, sort=False):
     V, d = table.shape
     n = ids.numel()
     y = table.new_empty((*ids.shape, d))
-    size = _lib.entry("sx_embed_sorted_bytes", "ll", _lib.c_ll)(n, V) if sort and d else 0
+    size = _sorted_bytes(n, V) if sort and d else 0
     order = table.new_empty(size, dtype=torch.uint8) if size else None
     with _lib.on_device(table):
         _lib.entry("sx_embed_fwd", "piplplilfilppp")(
@@ -57,7 +69,7 @@ def _backward(grad, ids, dy, scale, padding_idx, add, order):
     """ids and dy contiguous, all on one device; order: what the forward pass left, or None."""
     V, d = grad.shape
     n = ids.numel()
-    size = _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, order is not None)
+    size = _workspace(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)
     with _lib.on_device(grad):
         _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")(
