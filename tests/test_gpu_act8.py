@@ -141,3 +141,40 @@ def test_codes_inside_a_larger_buffer(width, offset):
     if offset < 16:
         with pytest.raises(RuntimeError, match="code -1"):
             _lib.entry("sx_unpack8", "ppplilip")(view.data_ptr(), p.exponents.data_ptr(), x.data_ptr(), 5, width, width, 0, _lib.here(x))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("width", [1, 2, 15, 17, 33, 479, 511, 513, 1023, 1025, 1537])
+def test_rows_that_begin_anywhere(width, dtype):
+    """Every place of a row's first and last value in a word, and one and several warps a row; what stands before, between and behind the rows is not
+    read (NaN) nor written."""
+    rows = 10
+    x = inputs(rows, width, dtype, 6)
+    want = held(x)
+    for before, pitch in ((0, width), (1, width), (0, width + 3), (3, width + 2)):
+        big = torch.full((before + rows * pitch + 8,), float("nan"), dtype=x.dtype, device="cuda")
+        v = big[before:before + rows * pitch].view(rows, pitch)[:, :width]
+        v.copy_(x)
+        p = ops.pack_8bit(v)
+        assert torch.equal(ops.unpack_8bit(p, torch.float32).double().cpu(), want), (before, pitch)
+        out = torch.full((rows * width + before + 8,), 7.0, dtype=x.dtype, device="cuda")
+        y = out[before:before + rows * width].view(rows, width)
+        _lib.entry("sx_unpack8", "ppplilip")(p.codes.data_ptr(), p.exponents.data_ptr(), y.data_ptr(), rows, width, width,
+                                            {"bf16": 0, "fp16": 1, "fp32": 2}[dtype], _lib.here(y))
+        assert torch.equal(y.cpu(), want.to(x.dtype)), (before, pitch)
+        assert (out[:before] == 7).all() and (out[before + rows * width:] == 7).all()
+
+
+@pytest.mark.parametrize("f", [1, 15, 257, 511, 513, 1025])
+def test_glu_of_rows_that_begin_anywhere(f):
+    gu, dh = inputs(9, 2 * f, "bf16", 7, edge=False).clamp(-8, 8).cuda(), inputs(9, f, "bf16", 8, edge=False).cuda()
+    wide = -(-f // 32) * 32                        # the same values in rows of whole blocks take the other way through the kernels
+    pad = lambda t: torch.nn.functional.pad(t, (0, wide - f))  # noqa: E731
+    y = torch.cat([pad(gu[:, :f]), pad(gu[:, f:])], 1).requires_grad_()
+    h2 = ops.glu_8bit(y)
+    h2.backward(pad(dh))
+    for before in (0, 1):
+        x = torch.empty(9 * 2 * f + 1, dtype=torch.bfloat16, device="cuda")[before:before + 18 * f].view(9, 2 * f).copy_(gu).requires_grad_()
+        h = ops.glu_8bit(x)
+        h.backward(dh)
+        assert torch.equal(h, h2[:, :f]) and torch.equal(x.grad, torch.cat([y.grad[:, :f], y.grad[:, wide:wide + f]], 1))
