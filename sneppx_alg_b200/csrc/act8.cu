@@ -37,10 +37,11 @@ constexpr int PER = 16;      // values of a thread
 // How rows are read and written: 32-byte accesses where base, pitch and width are whole multiples of a thread's values (16 of them: WIDE), 16-byte ones
 // where they are multiples of 8 (PAIR; the block's two threads take its vectors in turn, so that they fill sectors together). Rows that begin anywhere (ODD)
 // are read and written by a warp as whole aligned words, 32 next to each other, and turned into 16 neighbouring values a thread and back through shared
-// memory; a word that two rows or two warps share is read and written by halves. (8192 x 4101 in bf16: packed and restored in 57 us, gated with
-// its gradient 167; 78 and 226 with values one by one, 32 apart, which is no slower up to some 80 columns; 222 packed and restored with a thread's 16
-// neighbours one by one.)
-enum { ODD = 0, PAIR = 1, WIDE = 2 };
+// memory; a word that two rows or two warps share is read and written by halves (8192 x 4101 in bf16: packed and restored in 57 us, gated with its gradient
+// 167; 78 and 226 with values one by one, 32 apart). Where a row has two blocks at most, of which a warp would be empty otherwise, threads take their 16
+// neighbours one by one, and a warp several rows (NEAR: 22222 x 45 packed and restored 11.8 us, 17.5 as ODD; gated 30 and 45; at 77 columns 11.4 and 11.9,
+// 30 and 28).
+enum { ODD = 0, PAIR = 1, WIDE = 2, NEAR = 3 };
 template <int MODE>
 __host__ __device__ __forceinline__ int threads_of(int nb) { return MODE == ODD ? (nb + 15) / 16 * 32 : nb * 2; }   // of a row of nb blocks
 
@@ -86,6 +87,9 @@ __device__ __forceinline__ void load16(const T* row, int c, int width, Row16<T>&
       const int at = (c & ~31) + (2 * i + (c >> 4 & 1)) * (16 / (int)sizeof(T));
       v.q[i] = at < width ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
     }
+  } else if (MODE == NEAR) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v.t[j] = c + j < width ? row[c + j] : Act8<T>::out(0.f);
   } else {
     const int lane = c >> 4 & 31, first = c & ~511, n = width - first;
     const T* p = row + first;
@@ -138,6 +142,10 @@ __device__ __forceinline__ void store16(T* row, int c, int width, const float (&
       const int at = (c & ~31) + (2 * i + (c >> 4 & 1)) * (16 / (int)sizeof(T));
       if (at < width) *reinterpret_cast<uint4*>(row + at) = v.q[i];
     }
+  } else if (MODE == NEAR) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (c + j < width) row[c + j] = v.t[j];
   } else {
     const int lane = c >> 4 & 31, first = c & ~511, n = width - first;
     T* p = row + first;
@@ -367,7 +375,8 @@ static void rows_grid(long long rows, int threads, dim3* grid, dim3* block) {
 static int row_mode(int width, long long ld, const void* p, const void* q, int size) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
   if (width % PER == 0 && ld * size % 32 == 0 && at % 32 == 0) return WIDE;
-  return width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0 ? PAIR : ODD;
+  if (width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0) return PAIR;
+  return width <= 64 ? NEAR : ODD;
 }
 static bool act8_args_ok(const void* codes, long long rows, int width, int dtype) {
   return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
@@ -395,7 +404,7 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : run(pack8_kernel<ODD, T>, grid, block);
+    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(pack8_kernel<NEAR, T>, grid, block) : run(pack8_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
@@ -408,7 +417,7 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : run(unpack8_kernel<ODD, T>, grid, block);
+    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(unpack8_kernel<NEAR, T>, grid, block) : run(unpack8_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
@@ -423,7 +432,7 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
     const int mode = row_mode(width, ld, gu, h, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : run(glu8_fwd_kernel<ODD, T>, grid, block);
+    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(glu8_fwd_kernel<NEAR, T>, grid, block) : run(glu8_fwd_kernel<ODD, T>, grid, block);
   });
 }
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
@@ -439,6 +448,6 @@ extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, 
     const int mode = row_mode(width, width, dh, dgu, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : run(glu8_bwd_kernel<ODD, T>, grid, block);
+    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(glu8_bwd_kernel<NEAR, T>, grid, block) : run(glu8_bwd_kernel<ODD, T>, grid, block);
   });
 }
