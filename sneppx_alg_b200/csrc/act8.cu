@@ -13,6 +13,7 @@
 // instructions run at an eighth of the rate. Sums and functions are in 32 bits; this file is compiled without fast math, so that 32-bit inputs keep
 // their small values.
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "common.cuh"
 #include "sx_api.h"
 
@@ -303,12 +304,13 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
 }
 
 // gu [rows, 2 width] (gate | up): h = act(gate) * up, and gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb].
-// Blocks of up to 256 threads; 16-bit types forward in 48 registers (ODD 64: 84 us at 8192 x 4101, 87 in 48) and backward in 64: 8192 x 14336 bf16 forward 150.5 us, 158 in 64, and backward 147 us,
-// 161 in 48 (both move 947 MB; 180 and 164 in blocks of 448 threads). 32-bit types have more on their way and keep the registers that the compiler takes (39
-// and 38 us at 4096 x 4096; 41 and 42 with fewer).
+// Blocks of up to 256 threads; 16-bit types forward in 48 registers (ODD 64: 84 us at 8192 x 4101, 87 in 48) and backward in 64: 8192 x 14336 bf16 forward
+// 150.5 us, 158 in 64, and backward 147 us, 161 in 48 (both move 947 MB; 180 and 164 in blocks of 448 threads). 32-bit types have more on their way and keep
+// the registers that the compiler takes (39 and 38 us at 4096 x 4096; 41 and 42 with fewer).
 template <int MODE, typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 1) glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps,
-                                unsigned rows, int width, long long ld, int nb, int act) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 1)
+    glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps, unsigned rows, int width,
+                    long long ld, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
   if (row >= rows || piece >= threads_of<MODE>(nb)) return;
@@ -335,8 +337,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 
 }
 // dgu = (dh * up * act'(gate) | dh * act(gate)) with gate and up as their 8 bits say.
 template <int MODE, typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1) glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
-                                T* __restrict__ dgu, unsigned rows, int width, int nb, int act) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 1)
+    glu8_bwd_kernel(const T* __restrict__ dh, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps, T* __restrict__ dgu,
+                    unsigned rows, int width, int nb, int act) {
   const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
   const int piece = blockIdx.y * blockDim.x + threadIdx.x;
   if (row >= rows || piece >= threads_of<MODE>(nb)) return;
@@ -391,6 +394,14 @@ static int by_type(int dtype, F f) {
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
+template <typename F>
+static void by_mode(int mode, F f) {
+  if (mode == WIDE) f(std::integral_constant<int, WIDE>());
+  else if (mode == PAIR) f(std::integral_constant<int, PAIR>());
+  else if (mode == NEAR) f(std::integral_constant<int, NEAR>());
+  else f(std::integral_constant<int, ODD>());
+}
+
 }  // namespace sx
 using namespace sx;
 
@@ -400,11 +411,12 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(pack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(pack8_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(pack8_kernel<NEAR, T>, grid, block) : run(pack8_kernel<ODD, T>, grid, block);
+    by_mode(mode, [&](auto m) {
+      pack8_kernel<decltype(m)::value, T><<<grid, block, 0, st>>>((const T*)x, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb);
+    });
   });
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
@@ -413,11 +425,13 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern, dim3 grid, dim3 block) { kern<<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld, nb); };
     const int mode = row_mode(width, ld, x, nullptr, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(unpack8_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(unpack8_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(unpack8_kernel<NEAR, T>, grid, block) : run(unpack8_kernel<ODD, T>, grid, block);
+    by_mode(mode, [&](auto m) {
+      unpack8_kernel<decltype(m)::value, T><<<grid, block, 0, st>>>((const signed char*)codes, (const unsigned char*)exps, (T*)x, (unsigned)rows, width, ld,
+                                                                    nb);
+    });
   });
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
@@ -426,13 +440,13 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern, dim3 grid, dim3 block) {
-      kern<<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb, act);
-    };
     const int mode = row_mode(width, ld, gu, h, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_fwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_fwd_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(glu8_fwd_kernel<NEAR, T>, grid, block) : run(glu8_fwd_kernel<ODD, T>, grid, block);
+    by_mode(mode, [&](auto m) {
+      glu8_fwd_kernel<decltype(m)::value, T><<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width,
+                                                                     ld, nb, act);
+    });
   });
 }
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
@@ -442,12 +456,12 @@ extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, 
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto kern, dim3 grid, dim3 block) {
-      kern<<<grid, block, 0, st>>>((const T*)dh, (const signed char*)codes, (const unsigned char*)exps, (T*)dgu, (unsigned)rows, width, nb, act);
-    };
     const int mode = row_mode(width, width, dh, dgu, sizeof(T));
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
-    mode == WIDE ? run(glu8_bwd_kernel<WIDE, T>, grid, block) : mode == PAIR ? run(glu8_bwd_kernel<PAIR, T>, grid, block) : mode == NEAR ? run(glu8_bwd_kernel<NEAR, T>, grid, block) : run(glu8_bwd_kernel<ODD, T>, grid, block);
+    by_mode(mode, [&](auto m) {
+      glu8_bwd_kernel<decltype(m)::value, T><<<grid, block, 0, st>>>((const T*)dh, (const signed char*)codes, (const unsigned char*)exps, (T*)dgu,
+                                                                     (unsigned)rows, width, nb, act);
+    });
   });
 }

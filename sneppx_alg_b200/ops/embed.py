@@ -79,6 +79,14 @@ def _backward(grad, ids, dy, scale, padding_idx, add, order):
     return grad
 
 
+def _differentiable_backward(ids, dy, V, scale, padding_idx):
+    counts = (ids >= 0) & (ids < V)
+    if padding_idx is not None:
+        counts &= ids != padding_idx
+    rows = torch.where(counts[..., None], dy.float() * scale, 0.0).reshape(-1, dy.shape[-1])
+    return rows.new_zeros(V, dy.shape[-1]).index_add(0, torch.where(counts, ids, 0).reshape(-1), rows).to(dy.dtype)
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
@@ -88,10 +96,11 @@ class _EmbeddingFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_lib.once
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         table, (scale, padding_idx, order) = ctx.table, ctx.meta
+        if torch.is_grad_enabled():                # a graph of this pass is wanted: the same sums by operations that have one
+            return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding_idx), None, None
         mg = getattr(table, "main_grad", None)
         dy = dy.contiguous()
         if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:

@@ -224,3 +224,17 @@ def test_embedding_layer_in_a_model():
     want, mag = _sums(ids.reshape(-1), dy.reshape(-1, 128), 300, 1.0)
     assert torch.equal(y, e.weight[ids])
     _close(e.weight.grad, want, mag, torch.bfloat16, 800)
+
+
+@pytest.mark.parametrize("padding_idx", [None, 2])
+def test_second_derivatives(padding_idx):
+    w = torch.randn(11, 24, device="cuda")
+    ids = torch.randint(0, 11, (3, 7), device="cuda")
+    got = []
+    for f in (lambda t: ops.embedding(ids, t, scale=1.5, padding_idx=padding_idx), lambda t: 1.5 * torch.nn.functional.embedding(ids, t, padding_idx)):
+        t = w.clone().requires_grad_()
+        (g,) = torch.autograd.grad((f(t) ** 3).sum(), t, create_graph=True)
+        got += [g.detach(), torch.autograd.grad((g ** 2).sum(), t)[0]]
+    # sums of at most 21 values in another order: 21 roundings of 2^-24, and a few of the products, of what is added up
+    for a, b in zip(got[:2], got[2:]):
+        assert ((a - b).abs() <= 32 * 2.0 ** -24 * 21 * b.abs().amax()).all()
