@@ -735,15 +735,23 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
   }
 }
 
+// A kernel's attributes hold for one device: bit of the current one in what a launcher has set up.
+static unsigned long long device_bit() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return 1ull << (dev & 63);
+}
+
 template <int BN, bool A_MN, bool B_MN, int COMM = 0>
 static int launch_cfg(const GemmKernelParams& kp, int grid, cudaStream_t st) {
   using Cfg = GemmCfg<BN, COMM>;
-  static bool attr_set = false;
+  static unsigned long long set = 0;
   auto kern = gemm_tc_kernel<BN, A_MN, B_MN, COMM>;
-  if (!attr_set) {
+  const unsigned long long dev = device_bit();
+  if (!(__atomic_load_n(&set, __ATOMIC_ACQUIRE) & dev)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess)
       return -10;
-    attr_set = true;
+    __atomic_fetch_or(&set, dev, __ATOMIC_RELEASE);
   }
   kern<<<grid, GEMM_THREADS, Cfg::SMEM_BYTES, st>>>(kp);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
@@ -1006,12 +1014,13 @@ static int g2_max_clusters(int sms) {
 
 template <int BN2, int EPI, bool A_MN, bool B_MN>
 static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
-  static bool attr_set = false;
+  static unsigned long long set = 0;
   static int max_clusters = 0;
   auto kern = gemm2_kernel<BN2, EPI, A_MN, B_MN>;
   constexpr int THREADS = 64 + 32 * EPI;
   constexpr int SMEM = G2Cfg<BN2>::SMEM_BYTES;
-  if (!attr_set) {
+  const unsigned long long dev = device_bit();
+  if (!(__atomic_load_n(&set, __ATOMIC_ACQUIRE) & dev)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -10;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms & ~1, 1, 1);
@@ -1025,7 +1034,7 @@ static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
       cudaGetLastError();
       max_clusters = g2_max_clusters(sms);
     }
-    attr_set = true;
+    __atomic_fetch_or(&set, dev, __ATOMIC_RELEASE);
   }
   const long long tiles = (long long)kp.batch * kp.m_blks * kp.n_blks;
   int clusters = (int)(tiles < max_clusters ? tiles : max_clusters);
