@@ -4,16 +4,16 @@
 //   dz_v = ((g_nll + g_lse) e^{z_v - lse} - g_nll [v = target]) (1 - (z_v / c)^2)
 //
 // One kernel, two epilogues, on the CTA-pair GEMM (256 x 256 tiles, accumulators double-buffered in TMEM, operands by TMA):
-//   forward  each row's maximum and sum of exponentials over a tile's columns leave the SM as one pair of numbers, the target's logit by itself; a second
-//            kernel joins the pairs of a row. 8 bytes leave for 256 logits.
+//   forward  each row's maximum and sum of exponentials over a tile's columns but the target leave the SM as one pair of numbers, the target's logit by
+//            itself; a second kernel joins the pairs of a row. 8 bytes leave for 256 logits.
 //   backward the tile is computed again and leaves as dz in bf16 (half a step, 2^-9, of each value: what the products that follow take), for one piece of the
 //            vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
 // Sixteen epilogue warps (four TMEM quadrants, four groups of 64 columns): the exponentials of a tile are behind the products from widths of 256 on only
 // if four warps of each scheduler take turns.
 // The tensor cores cut what they add to an accumulator: over 4096 products a logit of 14 loses 1e-4. The forward pass, whose losses are differences of
-// logits, therefore takes the accumulator out after 1024 products at most and adds in registers, rounded: lse of 4088 tokens over [128256, 4096] is off by
-// 1.4e-6 without that, by 3.7e-7 with it in the same time, by 2.2e-7 after 512 products, which cost 3% more (20% over 768 columns). dz is rounded to bf16
-// anyway.
+// logits, therefore takes the accumulator out after 768 products at most, in equal parts, and adds in registers, rounded: lse of 4088 tokens over [128256,
+// 4096] is off by 1.4e-6 without that, by 3.7e-7 in parts of 1024 and by 2.3e-7 in these, in the same time; parts of 512 cost 3% more there and 20% over 768
+// columns. dz is rounded to bf16 anyway.
 // Takes the place of the reference's softmax / cross-entropy kernels (kernel/cuda/autodiff_cuda.cu:519-608).
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -31,7 +31,7 @@ constexpr int VL_GROUPS = 4;                         // epilogue warps of a TMEM
 constexpr int VL_COLS = 256 / VL_GROUPS;             // columns of an epilogue warp
 constexpr int VL_EPI_WARPS = 4 * VL_GROUPS;
 constexpr int VL_THREADS = 64 + 32 * VL_EPI_WARPS;
-constexpr int VL_CHUNK = 1024 / VL_BK;               // forward: k-blocks that stay in one accumulator at most
+constexpr int VL_CHUNK = 768 / VL_BK;                // forward: k-blocks that stay in one accumulator at most
 constexpr int VL_SLOTS = 4;                          // tiles whose pairs may wait to be joined (below)
 constexpr int VL_OFF_PAIRS = VL_STAGES * VL_STAGE_BYTES;
 constexpr int VL_PAIR_BYTES = VL_SLOTS * (VL_GROUPS - 1) * 128 * 8;
@@ -100,8 +100,8 @@ __device__ __forceinline__ void softcap_row(float (&v)[N], float cap, float inv)
   }
 }
 __device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
-  const float top = fmaxf(a.x, b.x), at = top == -INFINITY ? 0.f : top * LOG2E;
-  return make_float2(top, a.y * exp2f(fmaf(a.x, LOG2E, -at)) + b.y * exp2f(fmaf(b.x, LOG2E, -at)));
+  const float top = fmaxf(a.x, b.x), at = top == -INFINITY ? 0.f : top;
+  return make_float2(top, a.y * exp2f((a.x - at) * LOG2E) + b.y * exp2f((b.x - at) * LOG2E));      // the larger one's factor is 1, whatever it is
 }
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&r)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
@@ -257,8 +257,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
         if (__any_sync(0xffffffffu, tgt >= 0)) {
           float zt = 0.f;
 #pragma unroll
-          for (int j = 0; j < VL_COLS; ++j)
-            if (tgt == j) zt = v[j];
+          for (int j = 0; j < VL_COLS; ++j) {
+            if (tgt == j) {
+              zt = v[j];
+              v[j] = -INFINITY;          // the pairs are of the other words
+            }
+          }
           if (tgt >= 0) p.zt[row] = zt;
         }
         float top = fmaxf(v[0], v[1]);
@@ -271,7 +275,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
           sum[j & 3] += exp2f(fmaf(v[j], LOG2E, -at));
           sum[(j & 3) + 1] += exp2f(fmaf(v[j + 1], LOG2E, -at));
         }
-        float2 pair = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // top log2 e was rounded, by `off`: the exponentials are 2^off too large
+        const float off = top == -INFINITY ? 0.f : fmaf(top, LOG2E, -at);
+        float2 pair = make_float2(top, fmaf(total, off * -0.6931471805599453f, total));
         // The first warp of a quadrant joins the four. The others may be two tiles ahead of it at most: an accumulator is filled again when all
         // sixteen have read it. Four slots, each with a barrier that they arrive on, are enough.
         const int slot = tile % VL_SLOTS;
@@ -356,7 +363,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
   }
 }
 
-// Joins the pairs of eight rows a block, 64 threads a row. The last logarithm is taken in 64 bits: one a row.
+// Joins the pairs of eight rows a block, 64 threads a row. With d the logarithm of the other words' sum over the target's exponential, nll = log(1 + e^d),
+// which is right to a few 2^-20 of itself also where the model is sure and nll small; lse - z would be right to as much of z. In 64 bits: one a row.
 __global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
                                                               const long long* __restrict__ target, float* __restrict__ nll, float* __restrict__ lse, int T,
                                                               int V, int parts, long long ignore_index, int* status) {
@@ -373,12 +381,18 @@ __global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __re
     if (threadIdx.y < n) s[threadIdx.y][threadIdx.x] = pair = join_pairs(pair, s[threadIdx.y + n][threadIdx.x]);
   }
   if (threadIdx.y != 0 || row >= T) return;
-  const float l = (float)((double)pair.x + log((double)pair.y));
+  const double others = (double)pair.x + log((double)pair.y);          // -infinity where there are none
   const long long t = target[row];
   const bool valid = t != ignore_index && t >= 0 && t < V;
   if (t != ignore_index && !valid && status) atomicCAS(status, 0, (int)ST_BAD_ARGUMENT);
-  lse[row] = l;
-  nll[row] = valid ? l - zt[row] : 0.f;
+  if (valid) {
+    const double z = zt[row], d = others - z, more = log1p(exp(d <= 0 ? d : -d));
+    nll[row] = (float)(d <= 0 ? more : d + more);
+    lse[row] = (float)((d <= 0 ? z : others) + more);
+  } else {
+    nll[row] = 0.f;
+    lse[row] = (float)others;
+  }
 }
 
 // dh of several sums over parts of the vocabulary (parts [n, count] fp32): their sum, rounded once. Eight values a thread; count is a multiple of 8.

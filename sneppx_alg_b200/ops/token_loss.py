@@ -120,7 +120,7 @@ class _TokenLossFn(torch.autograd.Function):
 def linear_token_loss(h, w, target, ignore_index=-100, softcap=0.0, piece=0):
     """(nll, lse) of every token, fp32: logits z = h @ w^T, with ``softcap`` c > 0 c * tanh(z / c); lse = log sum exp z over the vocabulary, nll = lse
     - z[target], 0 where target is ``ignore_index``. h [..., d], w [V, d], target [...] int64. Both results are differentiable (a z-loss is a function of
-    lse), with any weight for each token; the logits exist in tiles only.
+    lse), with any weight for each token; the logits exist in tiles only. On the GPU nll is right to a part of itself also where it is small.
 
     Backward holds dz for about ``piece`` columns of the vocabulary at a time (0: as many as fit 256 MiB) and computes the logits again: it trades a
     fourth product of h and w for logits that ``linear_cross_entropy`` holds a chunk of, and need not know the tokens' weights beforehand.

@@ -276,3 +276,19 @@ def test_products_of_ragged_operands(M, N, K, a_mn, b_mn):
     ops.check_status()
     A, B = (a.T if a_mn else a).double(), (b if b_mn else b.T).double()
     assert ((d.double() - A @ B).abs() <= K * 2.0 ** -23 * (A.abs() @ B.abs())).all()       # K additions, each cut by at most 2^-23 of what is added up
+
+
+@pytest.mark.parametrize("T,V,d", [(2, 1244, 72), (3, 1517, 656), (40, 5000, 1000), (300, 700, 64)])
+def test_losses_of_tokens_that_the_model_is_sure_of(T, V, d):
+    """nll down to 1e-9 is right to a part of itself, not of the logits: it is a sum of the other words' exponentials over the target's, each off by e^(2 ez)."""
+    h, w, t, _, _ = _inputs(T, V, d, 23, ignored=0.0)
+    h = (h + torch.linspace(6, 28, T, device="cuda")[:, None] * w[t].float() / (w[t].float() ** 2).sum(1, keepdim=True)).to(torch.bfloat16)
+    nll, lse = ops.linear_token_loss(h, w, t)
+    z = h.double() @ w.double().t()
+    own = z.gather(1, t[:, None])
+    want = torch.log1p(torch.exp(z - own).scatter(1, t[:, None], 0.0).sum(1))
+    ez = d * 2.0 ** -23 * (h.double().abs() @ w.double().abs().t()).amax(1)
+    # 2^-18: exponentials and their sums, a few 2^-23 each, and at most 30 additions one after another
+    assert ((nll.double() - want).abs() <= want * (torch.expm1(2 * ez) + 2.0 ** -18)).all()
+    assert ((lse.double() - torch.logsumexp(z, 1)).abs() <= ez + 2.0 ** -18 + 2.0 ** -23 * lse.abs()).all()
+    assert want.min() < 1e-3
