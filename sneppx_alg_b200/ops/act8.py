@@ -194,6 +194,7 @@ def checkpoint_8bit(fn, *args):
     """``fn(*args)``, whose inner activations are recomputed in backward from arguments that are held in 8 bits: of ``args``, the floating CUDA / CPU
     tensors that autograd reaches (those that require a gradient and are no leaves) are packed, the others are kept as they are. The first pass runs
     on the arguments themselves; gradients are those of ``fn`` at the restored ones. Random state and autocast are as in torch.utils.checkpoint."""
+    from torch.utils._pytree import tree_leaves
     from torch.utils.checkpoint import checkpoint
 
     held, kept = list(args), list(args)
@@ -203,7 +204,10 @@ def checkpoint_8bit(fn, *args):
         if torch.is_tensor(a) and a.is_floating_point() and a.requires_grad and not a.is_leaf and (a.dtype in _TYPES):
             kept[i] = pack_8bit(a)
 
-    def run():
+    # generators are saved and set back for the devices of what checkpoint is handed: nothing of each device, as the arguments themselves go past it
+    places = [torch.empty(0, device=d) for d in {t.device for t in tree_leaves(args) if torch.is_tensor(t)}]
+
+    def run(*_):
         if held:                       # forward
             now = list(held)
             held.clear()
@@ -211,4 +215,4 @@ def checkpoint_8bit(fn, *args):
             now = [unpack_8bit(a).requires_grad_() if isinstance(a, Packed8bit) else a for a in kept]
         return fn(*now)
 
-    return checkpoint(run, use_reentrant=False)
+    return checkpoint(run, *places, use_reentrant=False)

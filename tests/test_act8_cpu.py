@@ -120,3 +120,32 @@ def test_checkpoint_without_gradients_and_with_leaves():
     ops.checkpoint_8bit(lambda t: lin(t).square().sum(), leaf).backward()      # a leaf is kept as it is: the gradient is the function's own
     want, = torch.autograd.grad(lin(leaf).square().sum(), leaf)
     assert torch.equal(leaf.grad, want)
+
+
+def test_checkpoint_is_told_the_devices_of_the_arguments(monkeypatch):
+    """torch.utils.checkpoint saves and restores the generators of the devices of the tensors that it is handed, nested ones included."""
+    import torch.utils.checkpoint as tc
+    plain, seen = tc.checkpoint, []
+
+    def spy(fn, *args, **kw):
+        seen.append({t.device.type for t in args if torch.is_tensor(t)})
+        assert not any(t.numel() for t in args)          # which are not kept through it
+        return plain(fn, *args, **kw)
+
+    monkeypatch.setattr(tc, "checkpoint", spy)
+    x = torch.randn(3, 8, requires_grad=True) * 1
+    ops.checkpoint_8bit(lambda t, k: t * 2, x, (torch.zeros(2, device="meta"), None))
+    assert seen == [{"cpu", "meta"}]
+
+
+def test_checkpoint_draws_the_same_random_numbers_again():
+    a = (torch.randint(-100, 100, (9, 40)) / 32.0).requires_grad_()          # 8 bits hold whole multiples of a power of two
+    a.data[:, ::32] = 127 / 32.0
+    torch.manual_seed(3)
+    y = ops.checkpoint_8bit(lambda t: torch.nn.functional.dropout(t, 0.5).square(), a * 1)
+    state = torch.get_rng_state()
+    y.sum().backward()
+    assert torch.equal(torch.get_rng_state(), state)
+    torch.manual_seed(3)
+    want, = torch.autograd.grad(torch.nn.functional.dropout(a * 1, 0.5).square().sum(), a)
+    assert torch.equal(a.grad, want)

@@ -178,3 +178,25 @@ def test_glu_of_rows_that_begin_anywhere(f):
         h = ops.glu_8bit(x)
         h.backward(dh)
         assert torch.equal(h, h2[:, :f]) and torch.equal(x.grad, torch.cat([y.grad[:, :f], y.grad[:, wide:wide + f]], 1))
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_checkpoint_draws_the_same_random_numbers_again(bits):
+    """Gradients are those of the mask that the forward pass drew, and the generator is where the forward pass left it."""
+    from sneppx_alg_b200.training.extras import checkpoint
+    w = torch.randn(40, 40, device="cuda").requires_grad_()
+    a = (torch.randint(-100, 100, (9, 40), device="cuda") / 32.0)          # 8 bits hold whole multiples of a power of two
+    a[:, ::32] = 127 / 32.0
+    a.requires_grad_()
+
+    def fn(t, rope):
+        return torch.nn.functional.dropout(t, 0.5) @ w
+
+    torch.manual_seed(3)
+    y = checkpoint(fn, a * 1, (None, torch.zeros(1, device="cuda")), bits=bits)
+    state = torch.cuda.get_rng_state()
+    got = torch.autograd.grad(y.square().sum(), (a, w))
+    assert torch.equal(torch.cuda.get_rng_state(), state)
+    torch.manual_seed(3)
+    want = torch.autograd.grad(fn(a * 1, None).square().sum(), (a, w))
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
