@@ -8,6 +8,8 @@ serves CPU tensors. The reference recomputes layers from inputs kept in full (gr
 from __future__ import annotations
 
 import torch
+import torch.nn.functional as F
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 from .functional import GLU_ACT, glu_reference
@@ -18,7 +20,7 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _native(x) -> bool:
-    if not x.is_cuda:
+    if not x.is_cuda or has_torch_function_variadic(x):      # a trace sees the kernels' allocations only: it records the PyTorch form
         return False
     if x.dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {x.dtype} is not one of bfloat16, float16, float32")
@@ -56,9 +58,7 @@ def pack_8bit_reference(x2):
     """[rows, width] -> (codes, exponents)."""
     rows, w = x2.shape
     nb = -(-w // BLOCK)
-    b = torch.zeros(rows, nb * BLOCK, dtype=torch.float32, device=x2.device)
-    b[:, :w] = x2.float()
-    b = b.view(rows, nb, BLOCK)
+    b = F.pad(x2.float(), (0, nb * BLOCK - w)).view(rows, nb, BLOCK)
     top = b.abs().amax(-1) if nb else b.new_zeros(rows, 0)
     finite = torch.isfinite(top)
     m, e = torch.frexp(torch.where(finite, top, 1.0))                        # top = m 2^e with m in [1/2, 1)
@@ -97,7 +97,7 @@ def unpack_8bit(p: Packed8bit, dtype=None):
     if tuple(p.codes.shape) != (rows, nb * BLOCK) or nb != -(-w // BLOCK) or rows * w != p.shape.numel() or p.codes.dtype != torch.int8 \
             or p.exponents.dtype != torch.uint8 or p.codes.device != p.exponents.device:
         raise ValueError(f"unpack_8bit: codes {tuple(p.codes.shape)} and exponents {tuple(p.exponents.shape)} do not hold {tuple(p.shape)}")
-    if not (p.codes.is_cuda and _lib.available()):
+    if not (p.codes.is_cuda and _lib.available()) or has_torch_function_variadic(p.codes, p.exponents):
         return unpack_8bit_reference(p.codes, p.exponents, w, dtype).view(p.shape)
     if dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
@@ -176,6 +176,8 @@ class _Glu8Fn(torch.autograd.Function):
 def glu_8bit(gu, act="silu"):
     """act(gate) * up with gu = [..., 2F] laid out (gate | up), as ``glu``; what backward needs of gu is held in 8 bits (2.06 bytes instead of
     4 for a gate and an up value of 16 bits), so the gradient is that of the restored gate and up. The result is computed from gu itself."""
+    if has_torch_function_variadic(gu):
+        return handle_torch_function(glu_8bit, (gu,), gu, act)
     if act not in GLU_ACT:
         raise ValueError(f"glu_8bit: act {act!r} is not one of {sorted(GLU_ACT)}")
     if gu.dim() == 0 or gu.shape[-1] % 2:

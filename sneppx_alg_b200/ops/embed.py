@@ -7,6 +7,7 @@ import functools
 
 import torch
 import torch.nn.functional as F
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 from . import debug as _dbg
@@ -49,6 +50,8 @@ def _lookup(ids, table, scale, padding_idx=None, sort=False):
 def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
     """grad [V, d] = scale * (sums of the rows of dy [.., d] by their word), or, with ``add``, grad += that (rows of other words are not touched
     then). Sums are in 32 bits and in the order of the tokens, so they are the same each time. grad has dy's type or is fp32."""
+    if has_torch_function_variadic(grad, ids, dy):
+        return handle_torch_function(embedding_backward_, (grad, ids, dy), grad, ids, dy, scale, padding_idx, add)
     V, d = grad.shape
     if dy.dtype not in _TYPES or grad.dtype not in (dy.dtype, torch.float32) or grad.stride(1) != 1 or (V > 1 and grad.stride(0) < d):
         raise ValueError(f"embedding_backward_: gradients {dy.dtype} into {grad.dtype} with strides {grad.stride()}")
@@ -117,6 +120,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     there, or added to what is there already (a tied output projection's), and ``.grad`` stays empty. ``padding_idx`` (negative counts from the
     end): tokens of this word give no gradient. On the GPU an id outside [0, V) gives a row of zeros and sets the status word
     (``check_status`` raises); on the CPU it raises at once."""
+    if has_torch_function_variadic(ids, table):      # a trace records this call: of the kernel's it would see the allocation of the result only
+        return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
     if table.dim() != 2:
         raise ValueError(f"embedding: table of shape {tuple(table.shape)} is no matrix")
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:

@@ -7,6 +7,7 @@ import ctypes as C
 
 import torch
 import torch.nn.functional as F
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 from . import debug as _dbg
@@ -127,6 +128,8 @@ def linear_token_loss(h, w, target, ignore_index=-100, softcap=0.0, piece=0):
     Where w carries ``main_grad`` its gradient is written or added there and ``.grad`` stays empty. On the GPU a target outside [0, V) counts as
     ignored and sets the status word (``check_status`` raises); on the CPU it raises at once. Ignored tokens take part in the products with weight 0:
     their hidden states have to be finite. Scratch of the forward pass: 8 bytes for a token and 256 words."""
+    if has_torch_function_variadic(h, w, target):      # a trace records this call: of the kernels' it would see their allocations only
+        return handle_torch_function(linear_token_loss, (h, w, target), h, w, target, ignore_index, softcap, piece)
     if w.dim() != 2 or h.dim() == 0 or h.shape[-1] != w.shape[1]:
         raise ValueError(f"linear_token_loss: hidden states {tuple(h.shape)} and weights {tuple(w.shape)} do not fit")
     if target.shape != h.shape[:-1]:
