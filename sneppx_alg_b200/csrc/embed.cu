@@ -459,8 +459,8 @@ __global__ void __launch_bounds__(256, 5) embed_sum_kernel(const SortArgs a, con
         const bool none = word >= V;
         word = __shfl_sync(0xffffffffu, kl, j);
         open = none && word == before;
-        // the row that the sum will be added to is on its way while the tokens are (68 -> 65 us)
-        if (add && mine) asm volatile("prefetch.global.L2 [%0];" ::"l"(grad + (long long)word * ldg + emb_first<VEC>(c)));
+        // the row that the sum will be added to is on its way while the tokens are (68 -> 65 us); a thread whose values lie all behind the row asks for none
+        if (add && emb_first<VEC>(c) < d) asm volatile("prefetch.global.L2 [%0];" ::"l"(grad + (long long)word * ldg + emb_first<VEC>(c)));
 #pragma unroll
         for (int k = 0; k < 8; ++k) acc[k] = 0.f;
       }

@@ -238,3 +238,21 @@ def test_second_derivatives(padding_idx):
     # sums of at most 21 values in another order: 21 roundings of 2^-24, and a few of the products, of what is added up
     for a, b in zip(got[:2], got[2:]):
         assert ((a - b).abs() <= 32 * 2.0 ** -24 * 21 * b.abs().amax()).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [1, 7, 31, 33, 250, 257, 2049])
+def test_sums_added_to_rows_that_end_a_buffer(d, dtype):
+    """The last word's row is the last of an allocation of its own: no thread asks for what is behind it, and nothing there changes."""
+    V, n = 9, 200
+    buf = torch.full((V * d + 64,), 3.0, device="cuda")
+    grad = buf[:V * d].view(V, d)
+    grad.copy_(torch.randn(V, d, device="cuda"))
+    start = grad.clone()
+    ids = torch.randint(0, V, (n,), device="cuda")
+    ids[:5] = V - 1
+    dy = torch.randn(n, d, device="cuda").to(TYPES[dtype])
+    ops.embedding_backward_(grad, ids, dy, add=True)
+    want, mag = _sums(ids, dy, V, 1.0)
+    _close(grad, want + start.double(), mag + start.double().abs(), torch.float32, int(torch.bincount(ids).max()) + 1)
+    assert (buf[V * d:] == 3).all()
