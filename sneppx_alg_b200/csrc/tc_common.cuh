@@ -325,9 +325,12 @@ __device__ __forceinline__ float squared_relu(float z) {
   const float r = fmaxf(z, 0.f);
   return r * r;
 }
-// cap * tanh(z / cap) with inv = 1 / cap; tanh x = 1 - 2 / (e^2x + 1) keeps an absolute error of a few 2^-24 everywhere
+// cap * tanh(z / cap) with inv = 1 / cap; tanh x = 1 - 2 / (e^2x + 1) keeps an absolute error of a few 2^-24 everywhere. The minimum lets NaN through, which
+// fminf would turn into the cap.
 __device__ __forceinline__ float softcap(float z, float cap, float inv) {
-  return cap * (1.f - __fdividef(2.f, __expf(fminf(2.f * z * inv, 80.f)) + 1.f));
+  float x;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(2.f * z * inv), "f"(80.f));
+  return cap * (1.f - __fdividef(2.f, __expf(x) + 1.f));
 }
 
 }  // namespace sx

@@ -292,3 +292,37 @@ def test_losses_of_tokens_that_the_model_is_sure_of(T, V, d):
     assert ((nll.double() - want).abs() <= want * (torch.expm1(2 * ez) + 2.0 ** -18)).all()
     assert ((lse.double() - torch.logsumexp(z, 1)).abs() <= ez + 2.0 ** -18 + 2.0 ** -23 * lse.abs()).all()
     assert want.min() < 1e-3
+
+
+@pytest.mark.parametrize("d", [64, 1000])
+def test_soft_cap_keeps_nan(d):
+    """A word whose weights are NaN, beside logits on both sides of 0.6 of the cap; a hidden state that holds NaN, and one with infinities of both signs."""
+    h, w, t, gn, gz = _inputs(40, 400, d, 31, ignored=0.0)
+    clean = _run(h, w, t, gn, gz, 3.0)
+    bad = w.clone()
+    bad[77] = math.nan
+    got = _run(h, bad, t, gn, gz, 3.0)
+    assert torch.isnan(got["lse"]).all() and torch.isnan(got["nll"]).all() and torch.isnan(got["dh"]).all()
+    for k in (0, 1):
+        x = h.clone()
+        x[7, :2] = torch.tensor([math.nan, 1.0] if k else [math.inf, -math.inf])
+        wz = w.clone()
+        wz[:, :2] = 0.5
+        base, got = _run(h, wz, t, gn, gz, 3.0), _run(x, wz, t, gn, gz, 3.0)
+        rest = torch.arange(40, device="cuda") != 7
+        assert torch.isnan(got["lse"][7]) and torch.isnan(got["nll"][7])
+        assert torch.isnan(got["dh"][7]).all()
+        assert all(torch.equal(got[i][rest], base[i][rest]) for i in ("nll", "lse", "dh"))
+    assert torch.isfinite(clean["lse"]).all()
+
+
+@pytest.mark.parametrize("M", [4, 300])
+def test_soft_capped_product_keeps_nan(M):
+    """The same cap in the epilogues of the products."""
+    from sneppx_alg_b200.ops.gemm import SoftCap
+    x, w = (4 * torch.randn(M, 256, device="cuda")).to(torch.bfloat16), torch.randn(512, 256, device="cuda").to(torch.bfloat16)
+    want = ops.gemm(x, w, act=SoftCap(30.0))
+    w[5] = math.nan
+    got = ops.gemm(x, w, act=SoftCap(30.0))
+    rest = torch.arange(512, device="cuda") != 5
+    assert torch.isnan(got[:, 5]).all() and torch.equal(got[:, rest], want[:, rest])
