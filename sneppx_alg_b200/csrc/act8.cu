@@ -2,9 +2,11 @@
 //
 // Per 32 consecutive values of a row one exponent byte b and 32 signed codes: x ~ code * 2^(b - 127), with the smallest power of two of which
 // round(amax / 2^e) <= 127 steps reach the block's largest magnitude, ties to even. amax = m 2^x with m in [1, 2): e = x - 6, one more from m =
-// 255/128 on (127.5 would round to 128). Everything but the rounding to whole steps is exact: amax and e come from the bits, x / 2^e is a product
-// with a power of two, code * 2^e has 7 bits and fits every type that x may have. b = 255 marks a block that holds an infinity or a NaN: all of it is
-// restored as NaN, so that an overflow is not hidden. e is at least -126, which holds blocks below 2^-120 more coarsely.
+// 255/128 on (127.5 would round to 128), but not where 64 of those steps would be the type's infinity: at the top of its range (65280 on in fp16, from
+// 255/256 of 2^128 on in the others) e stays and codes end at 127, which is off by less than a step, half of the step that e + 1 would have.
+// Everything but the rounding to whole steps is exact: amax and e come from the bits, x / 2^e is a product with a power of two, code * 2^e has 7 bits and
+// fits the type of x. b = 255 marks a block that holds an infinity or a NaN: all of it is restored as NaN, so that an overflow is not hidden. e is at least
+// -126, which holds blocks below 2^-120 more coarsely.
 // 33 bytes for 32 values. A power of two for 32 values costs what a 32-bit scale for 128 costs and is as near on normal values
 // (the block's maximum is smaller by what the step is rounded up), nearer where single values stand out.
 //
@@ -187,7 +189,11 @@ __device__ __forceinline__ void widen(const Row16<T>& v, float (&f)[PER]) {
 
 // A block's exponent byte from the bits of its largest magnitude, the factor that turns a value into steps, and the sum whose low byte is the code (to be
 // masked out in a block that is not finite: infinity times 0 is a NaN whose low byte may be anything).
-__device__ __forceinline__ uint32_t exponent_of(uint32_t top) { return top >= 0x7f800000u ? 255u : max((int)((top + 0x10000u) >> 23) - 6, 1); }
+template <typename T> constexpr int TOP_BYTE = std::is_same<T, __half>::value ? 15 - 6 + 127 : 127 - 6 + 127;      // of the type's largest values
+template <typename T>
+__device__ __forceinline__ uint32_t exponent_of(uint32_t top) {
+  return top >= 0x7f800000u ? 255u : min(max((int)((top + 0x10000u) >> 23) - 6, 1), TOP_BYTE<T>);
+}
 __device__ __forceinline__ float per_step(uint32_t byte) { return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23); }
 __device__ __forceinline__ uint32_t code_of(float f, float inv) { return __float_as_uint(fmaf(f, inv, 12582912.f)); }
 __device__ __forceinline__ uint32_t finite_mask(uint32_t byte) { return byte == 255u ? 0u : 0xffffffffu; }
@@ -203,12 +209,16 @@ __device__ __forceinline__ void encode16(const float (&f)[PER], int place, int n
 #pragma unroll
   for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
   top = max(top, __shfl_xor_sync(3u << ((threadIdx.y * blockDim.x + threadIdx.x) & 30u), top, 1));
-  const uint32_t byte = exponent_of(top);
+  const uint32_t byte = exponent_of<T>(top);
   const float inv = per_step(byte);
   const uint32_t mask = finite_mask(byte);
   uint32_t k[PER], r[4];
 #pragma unroll
   for (int j = 0; j < PER; ++j) k[j] = code_of(f[j], inv);
+  if (byte == TOP_BYTE<T>) {             // rare: 128 steps are 127 here
+#pragma unroll
+    for (int j = 0; j < PER; ++j) k[j] = code_of(fminf(fmaxf(f[j] * inv, -127.f), 127.f), 1.f);
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     r[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040), __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410) & mask;

@@ -62,8 +62,8 @@ def pack_8bit_reference(x2):
     top = b.abs().amax(-1) if nb else b.new_zeros(rows, 0)
     finite = torch.isfinite(top)
     m, e = torch.frexp(torch.where(finite, top, 1.0))                        # top = m 2^e with m in [1/2, 1)
-    e = torch.where(top > 0, e - 7 + (m >= 127.5 / 128).int(), -126).clamp(min=-126)
-    codes = torch.where(finite[..., None], torch.round(torch.ldexp(b, -e[..., None])), 0.0)
+    e = torch.where(top > 0, e - 7 + (m >= 127.5 / 128).int(), -126).clamp(-126, 9 if x2.dtype == torch.float16 else 121)      # 121: of values from 2^127 on
+    codes = torch.where(finite[..., None], torch.round(torch.ldexp(b, -e[..., None])).clamp(-127, 127), 0.0)
     return codes.to(torch.int8).view(rows, nb * BLOCK), torch.where(finite, e + 127, 255).to(torch.uint8)
 
 
@@ -75,7 +75,8 @@ def unpack_8bit_reference(codes, exponents, width, dtype):
 
 
 def pack_8bit(x) -> Packed8bit:
-    """x (any shape, blocks along its last dimension; float types) in 8 bits. Not differentiable: what backward reads."""
+    """x (any shape, blocks along its last dimension; float types) in 8 bits. Finite values come back finite: steps are never so wide that whole ones leave
+    the type. Not differentiable: what backward reads."""
     if not x.is_floating_point():
         raise TypeError(f"pack_8bit: {x.dtype} is not a floating type")
     x2 = _rows(x.detach())

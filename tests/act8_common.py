@@ -53,3 +53,25 @@ def inputs(rows, width, dtype, seed, edge=True, device="cpu"):
         x[6, width // 2] = 60000.0
         x[7] = -1.9921875
     return x.to(TYPES[dtype]).to(device)
+
+
+def largest(dtype):
+    """Blocks whose largest magnitude is at the top of a type's range, and what 8 bits hold of them, fp64: 64 steps of the exponent that the border between
+    127 and 128 steps asks for would be the type's infinity, so the steps are 2^-6 of the largest power of two and end at 127."""
+    t = TYPES[dtype]
+    top = torch.finfo(t).max
+    power = 2.0 ** math.floor(math.log2(top / 1.5))
+    eps = torch.finfo(t).eps
+    x = torch.zeros(9, 32, dtype=torch.float64)
+    x[0] = top
+    x[1, 0] = -top
+    x[2, 3], x[2, 4:] = top, torch.arange(28.0, dtype=torch.float64) * power / 64
+    x[3, 31], x[3, 30] = power * (255 / 128), power * (255 / 128 - eps)        # the border and what is below it
+    x[4, 0] = power * (255 / 128 - eps)                                        # just below: 127 steps, as ever
+    x[5, 0] = power
+    x[6, 0], x[6, 1] = -power * 1.5, top
+    x[7, 0], x[7, 1] = top, 1.0
+    x[8, 7] = -power * (255 / 128)
+    x = x.to(t)
+    step = power / 64
+    return x, torch.round(x.double() / step).clamp(-127, 127) * step, step

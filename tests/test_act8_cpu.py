@@ -149,3 +149,16 @@ def test_checkpoint_draws_the_same_random_numbers_again():
     torch.manual_seed(3)
     want, = torch.autograd.grad(torch.nn.functional.dropout(a * 1, 0.5).square().sum(), a)
     assert torch.equal(a.grad, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_the_largest_values_come_back_finite(dtype):
+    from act8_common import largest
+    x, want, step = largest(dtype)
+    p = ops.pack_8bit(x)
+    y = ops.unpack_8bit(p)
+    assert torch.equal(y.double(), want) and torch.equal(ops.unpack_8bit(p, torch.float32).double(), want) and int(p.codes.abs().max()) <= 127
+    assert ((y.double() - x.double()).abs() < step).all()
+    gu = torch.cat([x, torch.full_like(x, 2.0 ** -20)], 1).requires_grad_()
+    ops.glu_8bit(gu, "relu").sum().backward()
+    assert torch.equal(gu.grad[:, 32:].double(), want.clamp(min=0))

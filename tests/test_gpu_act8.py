@@ -200,3 +200,24 @@ def test_checkpoint_draws_the_same_random_numbers_again(bits):
     torch.manual_seed(3)
     want = torch.autograd.grad(fn(a * 1, None).square().sum(), (a, w))
     assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("width", [32, 1000, 1001, 1008])
+def test_the_largest_values_come_back_finite(width, dtype):
+    """In every place of a row, through each way of reading rows."""
+    from act8_common import largest
+    block, want, _ = largest(dtype)
+    x, y = (torch.cat([t.repeat(1, width // 32), t[:, :width % 32]], 1) for t in (block, want))
+    if width % 32:                                # what is left of a block may have lost its largest value
+        cut = width // 32 * 32
+        y[:, cut:] = ops.unpack_8bit(ops.pack_8bit(x[:, cut:]), torch.float32).double()
+    p = ops.pack_8bit(x.cuda())
+    assert torch.equal(ops.unpack_8bit(p).cpu().double(), y)
+    ref = ops.pack_8bit(x)
+    assert torch.equal(p.codes.cpu(), ref.codes) and torch.equal(p.exponents.cpu(), ref.exponents)
+    gu = torch.cat([x, torch.full_like(x, 2.0 ** -20)], 1).cuda().requires_grad_()
+    h = ops.glu_8bit(gu, "relu")
+    assert torch.isfinite(h).all()
+    h.backward(torch.ones_like(h))
+    assert torch.equal(gu.grad[:, width:].double().cpu(), y.clamp(min=0))
