@@ -308,8 +308,8 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
     a = g * s;
     da = fmaf(2.f * a * (1.f - s), k0 * fmaf(3.f * k1 * g, g, 1.f), s);
   } else {
-    a = fmaxf(g, 0.f);
-    da = g > 0.f ? 1.f : 0.f;
+    a = g < 0.f ? 0.f : g;                     // NaN stays: it stands for an overflow
+    da = g > 0.f ? 1.f : g <= 0.f ? 0.f : g;
   }
 }
 

@@ -121,7 +121,7 @@ def _gate(g, act):
         k0, k1 = 0.7978845608028654, 0.044715
         t = torch.tanh(k0 * (g + k1 * g ** 3))
         return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * k0 * (1 + 3 * k1 * g * g)
-    return torch.relu(g), (g > 0).to(g.dtype)
+    return torch.relu(g), torch.where(torch.isnan(g), g, (g > 0).to(g.dtype))
 
 
 def glu_8bit_backward_reference(dh, gate, up, act):

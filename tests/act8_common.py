@@ -75,3 +75,24 @@ def largest(dtype):
     x = x.to(t)
     step = power / 64
     return x, torch.round(x.double() / step).clamp(-127, 127) * step, step
+
+
+def check_glu_of_overflows(glu, act, dtype, device, f):
+    """An infinite and a NaN gate, and an infinite up: the result is NaN where the definition's is, and the gradients of a whole block are NaN where one of its
+    gates or ups overflowed, as the block is held as NaN. Nothing else is."""
+    x = inputs(9, 2 * f, dtype, 9, edge=False, device=device).clamp(-8, 8)
+    x[1, 3], x[2, 5], x[3, f + 7], x[4, 0] = math.inf, math.nan, math.inf, -math.inf
+    x = x.requires_grad_()
+    h = glu(x, act)
+    h.backward(torch.ones_like(h))
+    g, u = x.detach().double()[:, :f], x.detach().double()[:, f:]
+    a = torch.relu(g) if act == "relu" else gate(g, act)[0]
+    nan = torch.isnan(a * u)
+    assert not math.isfinite(h[3, 7])               # an infinite up times a gate that 32 bits may hold as 0 and 64 do not: infinite or NaN
+    nan[3, 7] = torch.isnan(h[3, 7])
+    assert torch.equal(torch.isnan(h), nan)
+    block = lambda r, c: (torch.arange(9)[:, None] == r) & (torch.arange(f)[None] // 32 == c // 32)  # noqa: E731
+    gates, ups = block(1, 3) | block(2, 5) | block(4, 0), block(3, 7)
+    bad = torch.isnan(x.grad).cpu()                 # dgate = d up act'(gate), dup = d act(gate); 0 times NaN is NaN
+    assert torch.equal(bad[:, f:], gates)
+    assert torch.equal(bad[:, :f], gates | ups)

@@ -162,3 +162,11 @@ def test_the_largest_values_come_back_finite(dtype):
     gu = torch.cat([x, torch.full_like(x, 2.0 ** -20)], 1).requires_grad_()
     ops.glu_8bit(gu, "relu").sum().backward()
     assert torch.equal(gu.grad[:, 32:].double(), want.clamp(min=0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("f", [32, 70, 96])
+def test_glu_of_overflows(f, act, dtype):
+    from act8_common import check_glu_of_overflows
+    check_glu_of_overflows(ops.glu_8bit, act, dtype, "cpu", f)

@@ -221,3 +221,11 @@ def test_the_largest_values_come_back_finite(width, dtype):
     assert torch.isfinite(h).all()
     h.backward(torch.ones_like(h))
     assert torch.equal(gu.grad[:, width:].double().cpu(), y.clamp(min=0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("f", [32, 1001, 96])
+def test_glu_of_overflows(f, act, dtype):
+    from act8_common import check_glu_of_overflows
+    check_glu_of_overflows(ops.glu_8bit, act, dtype, "cuda", f)
