@@ -534,14 +534,14 @@ int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void* grad, long
 // ------------------------------------------------------------------ L4 per-token losses of a vocabulary projection (vocab_loss.cu)
 // h [T, d], w [V, d] bf16 (pitches ldh, ldw; d and pitches multiples of 8, 16-byte aligned); z = h w^T, cap tanh(z / cap) with cap > 0.
 // lse [T] = log sum exp z; nll [T] = lse - z[target], 0 for ignore_index (and for targets outside [0, V), which set ST_BAD_ARGUMENT).
-// part: scratch of ceil(V / 256) T pairs of floats; zt: scratch of T floats.
+// part: scratch of ceil(V / 256) T pairs of floats; zt: T floats, nll again of tokens that have a target, for sx_vocab_loss_bwd.
 int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                       long long ignore_index, float cap, void* part, float* zt, float* nll, float* lse, int* status, cudaStream_t stream);
 // Backward: dh [T, d] bf16 and dw [V, d] (bf16, or fp32 with dw_fp32; written, or added to with dw_add), either may be null. g_nll and
 // g_lse (either may be null): gradients of nll and lse. dz, the gradient of the logits, exists for `piece` words at a time (0: as many as fit 256 MiB).
 typedef struct SxVocabLossArgs {
   const void* h; const void* w; long long ldh, ldw;
-  const long long* target; const float* lse; const float* g_nll; const float* g_lse;
+  const long long* target; const float* lse; const float* nll; const float* g_nll; const float* g_lse;
   void* dh; void* dw; long long lddw;
   long long T, V, ignore_index, piece;
   void* work; long long work_bytes;                      // sx_vocab_loss_bwd_workspace bytes, 256-byte aligned

@@ -1,19 +1,24 @@
 // L4: per-token losses of a vocabulary projection, in tiles of the vocabulary, without the logits ever being held.
 //
 //   z = h w^T, soft-capped: c tanh(z / c);   lse = log sum_v e^{z_v};   nll = lse - z_target
-//   dz_v = ((g_nll + g_lse) e^{z_v - lse} - g_nll [v = target]) (1 - (z_v / c)^2)
+//   dz_v = ((g_nll + g_lse) e^{z_v - lse} - g_nll [v = target]) (1 - (z_v / c)^2),
+//   and of the target, without a difference of near-equal numbers, (g_nll (e^{-nll} - 1) + g_lse e^{-nll}) (1 - (z / c)^2)
 //
 // One kernel, two epilogues, on the CTA-pair GEMM (256 x 256 tiles, accumulators double-buffered in TMEM, operands by TMA):
 //   forward  each row's maximum and sum of exponentials over a tile's columns but the target leave the SM as one pair of numbers, the target's logit by
 //            itself; a second kernel joins the pairs of a row. 8 bytes leave for 256 logits.
-//   backward the tile is computed again and leaves as dz in bf16 (half a step, 2^-9, of each value: what the products that follow take), for one piece of the
-//            vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
+//   backward the tile is computed again and leaves as dz in bf16 (half a step, 2^-9, of each value: the products that follow take no other type at this
+//            rate, and the logits of linear_cross_entropy's gradient are held so too; dh and dw are off by 2.3e-3 with it, 1.7e-3 by their own rounding
+//            alone), for one piece of the vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
 // Sixteen epilogue warps (four TMEM quadrants, four groups of 64 columns): the exponentials of a tile are behind the products from widths of 256 on only
 // if four warps of each scheduler take turns.
 // The tensor cores cut what they add to an accumulator: over 4096 products a logit of 14 loses 1e-4. The forward pass, whose losses are differences of
 // logits, therefore takes the accumulator out after 768 products at most, in equal parts, and adds in registers, rounded: lse of 4088 tokens over [128256,
 // 4096] is off by 1.4e-6 without that, by 3.7e-7 in parts of 1024 and by 2.3e-7 in these, in the same time; parts of 512 cost 3% more there and 20% over 768
-// columns. dz is rounded to bf16 anyway.
+// columns. Backward leaves a logit in one accumulator: an error of 1e-4 in it is one of 1e-4 of its e^{z - lse}, a twentieth of what the rounding of dz to bf16
+// takes. The target's value alone would lose it against 1 - e^{z - lse}, which may be smaller, so that is computed from the forward pass's nll
+// (64 tokens over [32000, 4096]: dw of a target that the model gives an nll of 1e-3 is off by 1.9e-3 of itself, 6.8e-2 by the difference; of 2.5e-5
+// by 2.5e-3, 0.46 by the difference).
 // Takes the place of the reference's softmax / cross-entropy kernels (kernel/cuda/autodiff_cuda.cu:519-608).
 #include "tc_common.cuh"
 #include "tc_pair.cuh"
@@ -44,8 +49,9 @@ struct VocabLossParams {
   const long long* target;
   long long ignore_index;
   float2* part;               // forward: [n_blks, T] maximum and sum
-  float* zt;                  // forward: [T] the target's logit
+  float* zt;                  // forward: [T] the target's logit, in the place of which the joining kernel leaves nll
   const float* lse;           // backward
+  const float* nll;           // backward: of tokens that have a target
   const float* g_nll;         // backward: [T] or null
   const float* g_lse;
   __nv_bfloat16* dz;          // backward: [rows, ld]
@@ -218,14 +224,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
       const int left = p.v1 - first;                              // columns that the vocabulary has from there on
       // the target as a column of this warp's, or none
       int tgt = -1;
-      float a = 0.f, gn = 0.f, off = 0.f;
+      float a = 0.f, gn = 0.f, off = 0.f, at_target = 0.f;
       if (row < p.T) {
         const long long tv = p.target[row];
         if (tv != p.ignore_index && tv >= first && tv < first + VL_COLS && tv < p.v1) tgt = (int)(tv - first);
         if (GRAD) {
+          const float gz = p.g_lse ? p.g_lse[row] : 0.f;
           if (p.g_nll && tv != p.ignore_index && tv >= 0 && tv < p.V) gn = p.g_nll[row];
-          a = gn + (p.g_lse ? p.g_lse[row] : 0.f);
+          a = gn + gz;
           off = -p.lse[row] * LOG2E;
+          if (tgt >= 0) {
+            const float nll = p.nll[row];
+            at_target = fmaf(gn, expm1f(-nll), gz * __expf(-nll));
+          }
         }
       }
       if (!GRAD) {
@@ -324,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
           if (__any_sync(0xffffffffu, (tgt >> 5) == c)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (tgt == c * 32 + j) g[j] -= gn;
+              if (tgt == c * 32 + j) g[j] = at_target;
           }
           if (CAP) {
 #pragma unroll
@@ -365,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
 
 // Joins the pairs of eight rows a block, 64 threads a row. With d the logarithm of the other words' sum over the target's exponential, nll = log(1 + e^d),
 // which is right to a few 2^-20 of itself also where the model is sure and nll small; lse - z would be right to as much of z. In 64 bits: one a row.
-__global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
+__global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __restrict__ part, float* __restrict__ zt,
                                                               const long long* __restrict__ target, float* __restrict__ nll, float* __restrict__ lse, int T,
                                                               int V, int parts, long long ignore_index, int* status) {
   __shared__ float2 s[64][8];
@@ -387,7 +398,7 @@ __global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __re
   if (t != ignore_index && !valid && status) atomicCAS(status, 0, (int)ST_BAD_ARGUMENT);
   if (valid) {
     const double z = zt[row], d = others - z, more = log1p(exp(d <= 0 ? d : -d));
-    nll[row] = (float)(d <= 0 ? more : d + more);
+    nll[row] = zt[row] = (float)(d <= 0 ? more : d + more);
     lse[row] = (float)((d <= 0 ? z : others) + more);
   } else {
     nll[row] = 0.f;
@@ -539,7 +550,7 @@ extern "C" int sx_vocab_loss_bwd(const SxVocabLossArgs* a, cudaStream_t st) {
   __nv_bfloat16* dz = (__nv_bfloat16*)(work + plan.o_dz);
   float* acc = (float*)(work + plan.o_acc);
   p.target = a->target; p.ignore_index = a->ignore_index; p.status = a->status;
-  p.lse = a->lse; p.g_nll = a->g_nll; p.g_lse = a->g_lse; p.dz = dz; p.rows = (int)a->T;
+  p.lse = a->lse; p.nll = a->nll; p.g_nll = a->g_nll; p.g_lse = a->g_lse; p.dz = dz; p.rows = (int)a->T;
   p.m_blks = (int)((a->T + 255) / 256);
   for (long long v0 = 0; v0 < a->V; v0 += plan.piece) {
     const long long v1 = v0 + plan.piece < a->V ? v0 + plan.piece : a->V, n = v1 - v0;

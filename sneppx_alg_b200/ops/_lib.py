@@ -174,7 +174,7 @@ class SxWinAttnArgs(C.Structure):
 
 class SxVocabLossArgs(C.Structure):
     _fields_ = [
-        ("h", c_void_p), ("w", c_void_p), ("ldh", c_ll), ("ldw", c_ll), ("target", c_void_p), ("lse", c_void_p), ("g_nll", c_void_p),
+        ("h", c_void_p), ("w", c_void_p), ("ldh", c_ll), ("ldw", c_ll), ("target", c_void_p), ("lse", c_void_p), ("nll", c_void_p), ("g_nll", c_void_p),
         ("g_lse", c_void_p), ("dh", c_void_p), ("dw", c_void_p), ("lddw", c_ll), ("T", c_ll), ("V", c_ll), ("ignore_index", c_ll), ("piece", c_ll),
         ("work", c_void_p), ("work_bytes", c_ll), ("status", c_void_p), ("d", c_int), ("dw_fp32", c_int), ("dw_add", c_int), ("cap", c_float),
     ]

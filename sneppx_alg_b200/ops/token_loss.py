@@ -49,25 +49,27 @@ def _rows16(t, d):
     return t, d if one else t.stride(0)
 
 
-def _forward(h, w, target, ignore_index, softcap):
-    """(nll, lse) in target's shape, and the targets as they were read."""
+def _forward(h, w, target, ignore_index, softcap, keep=False):
+    """(nll, lse) in target's shape, the targets as they were read, and with ``keep`` nll once more for backward (the caller's may be written over)."""
     T, V, d = target.numel(), w.shape[0], (w.shape[1] + 7) // 8 * 8
     (h2, ldh), (w2, ldw) = _rows16(h, d), _rows16(w, d)
     tgt = target.contiguous()
     nll, lse = h2.new_empty(target.shape, dtype=torch.float32), h2.new_empty(target.shape, dtype=torch.float32)
-    scratch = h2.new_empty(T * (2 * -(-V // 256) + 1), dtype=torch.float32)          # pairs of a row's maximum and sum, and its target's logit
+    pairs = 2 * T * -(-V // 256)                          # of a row's maximum and sum, and behind them its target's logit
+    scratch = h2.new_empty(pairs if keep else pairs + T, dtype=torch.float32)
+    own = h2.new_empty(T, dtype=torch.float32) if keep else None
     with _lib.on_device(h):
         _lib.entry("sx_vocab_loss_fwd", "plplpllilfpppppp")(
             h2.data_ptr(), ldh, w2.data_ptr(), ldw, tgt.data_ptr(), T, V, d, ignore_index, softcap, scratch.data_ptr(),
-            scratch.data_ptr() + 8 * T * -(-V // 256), nll.data_ptr(), lse.data_ptr(), _lib.status_ptr(h), _lib.here(h))
-    return nll, lse, tgt
+            own.data_ptr() if keep else scratch.data_ptr() + 4 * pairs, nll.data_ptr(), lse.data_ptr(), _lib.status_ptr(h), _lib.here(h))
+    return nll, lse, tgt, own
 
 
 class _TokenLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, target, ignore_index, softcap, piece):
-        nll, lse, tgt = _forward(h, w, target, ignore_index, softcap)
-        ctx.save_for_backward(h, w, tgt, lse)
+        nll, lse, tgt, own = _forward(h, w, target, ignore_index, softcap, True)
+        ctx.save_for_backward(h, w, tgt, lse, own)
         ctx.meta = ignore_index, softcap, piece
         ctx.set_materialize_grads(False)
         return nll, lse
@@ -78,7 +80,7 @@ class _TokenLossFn(torch.autograd.Function):
         none = (None,) * 6
         if g_nll is None and g_lse is None:
             return none
-        h, w, tgt, lse = ctx.saved_tensors
+        h, w, tgt, lse, own = ctx.saved_tensors
         ignore_index, softcap, piece = ctx.meta
         need_h, need_w = ctx.needs_input_grad[:2]
         T, V, d0 = tgt.numel(), w.shape[0], w.shape[1]
@@ -92,7 +94,7 @@ class _TokenLossFn(torch.autograd.Function):
         dw = (mg if mg is not None else w2.new_empty((V, d))) if need_w else None
         a = _lib.SxVocabLossArgs()
         a.h, a.w, a.ldh, a.ldw = h2.data_ptr(), w2.data_ptr(), ldh, ldw
-        a.target, a.lse, a.status = tgt.data_ptr(), lse.data_ptr(), _lib.status_ptr(h)
+        a.target, a.lse, a.nll, a.status = tgt.data_ptr(), lse.data_ptr(), own.data_ptr(), _lib.status_ptr(h)
         a.T, a.V, a.d, a.ignore_index, a.cap, a.piece = T, V, d, ignore_index, softcap, piece
         if gn is not None:
             a.g_nll = gn.data_ptr()

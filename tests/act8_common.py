@@ -88,7 +88,7 @@ def check_glu_of_overflows(glu, act, dtype, device, f):
     g, u = x.detach().double()[:, :f], x.detach().double()[:, f:]
     a = torch.relu(g) if act == "relu" else gate(g, act)[0]
     nan = torch.isnan(a * u)
-    assert not math.isfinite(h[3, 7])               # an infinite up times a gate that 32 bits may hold as 0 and 64 do not: infinite or NaN
+    assert not torch.isfinite(h[3, 7])               # an infinite up times a gate that 32 bits may hold as 0 and 64 do not: infinite or NaN
     nan[3, 7] = torch.isnan(h[3, 7])
     assert torch.equal(torch.isnan(h), nan)
     block = lambda r, c: (torch.arange(9)[:, None] == r) & (torch.arange(f)[None] // 32 == c // 32)  # noqa: E731

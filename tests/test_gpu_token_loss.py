@@ -326,3 +326,50 @@ def test_soft_capped_product_keeps_nan(M):
     got = ops.gemm(x, w, act=SoftCap(30.0))
     rest = torch.arange(512, device="cuda") != 5
     assert torch.isnan(got[:, 5]).all() and torch.equal(got[:, rest], want[:, rest])
+
+
+@pytest.mark.parametrize("cap", [0.0, 40.0])
+@pytest.mark.parametrize("T,V,d", [(2, 1244, 72), (40, 5000, 1000), (300, 700, 64), (70, 3000, 4096)])
+def test_gradients_of_tokens_that_the_model_is_sure_of(T, V, d, cap):
+    """A target's dz is g_nll (p - 1) + g_lse p times the cap's slope, right to a part of itself where p is next to 1. Each token in its own direction: dw of a
+    word that is one token's target and nobody else's is that token's dz times h."""
+    g = torch.Generator(device="cuda").manual_seed(29)
+    w = (torch.randn(V, d, generator=g, device="cuda") / math.sqrt(d)).to(torch.bfloat16)
+    t = torch.randperm(V, generator=g, device="cuda")[:T]
+    own = w[t].float()
+    up = torch.linspace(8, 20, T, device="cuda")[:, None]
+    h = (torch.randn(T, d, generator=g, device="cuda") * 0.1 + up * own / (own ** 2).sum(1, keepdim=True)).to(torch.bfloat16)
+    gn, gz = torch.rand(T, generator=g, device="cuda") + 0.5, 1e-3 * torch.rand(T, generator=g, device="cuda")
+    for zl in (torch.zeros_like(gz), gz):
+        got = _run(h, w, t, gn, zl, cap)
+        h64, w64 = h.double(), w.double()
+        raw = h64 @ w64.t()
+        z = cap * torch.tanh(raw / cap) if cap else raw
+        others = torch.logsumexp(z.scatter(1, t[:, None], -math.inf), 1)
+        zt = z.gather(1, t[:, None]).squeeze(1)
+        nll = torch.nn.functional.softplus(others - zt, threshold=1e9)
+        assert nll.min() < 1e-3
+        slope = 1 - (z / cap) ** 2 if cap else torch.ones_like(z)
+        p = torch.exp(z - (zt + nll)[:, None])
+        rest = ((gn + zl).double()[:, None] * p)
+        dz = rest.scatter(1, t[:, None], (gn.double() * torch.expm1(-nll) + zl.double() * torch.exp(-nll))[:, None]) * slope
+        ez = d * 2.0 ** -23 * (h64.abs() @ w64.abs().t()).amax(1) + 2.0 ** -21 * cap
+        # of dz itself: exponentials of logits off by ez, in the soft cap's slope 2 |z / cap| ez / cap and 2^-20, half a step of bf16; of the target's two
+        # parts each, which may cancel. 2^-17: sums and functions, a few 2^-23 each and at most 30 additions one after another
+        part = torch.expm1(3 * ez)[:, None] + 2.0 ** -17 + ((4 * ez[:, None] / cap + 2.0 ** -20) / slope.clamp(min=1e-9) if cap else 0.0)
+        mag = rest.scatter(1, t[:, None], (gn.double() * -torch.expm1(-nll) + zl.double() * torch.exp(-nll))[:, None]) * slope
+        edz = mag * part + 2.0 ** -8 * dz.abs()
+        tol = dict(dh=edz @ w64.abs() + V * 2.0 ** -23 * (dz.abs() @ w64.abs()), dw=edz.t() @ h64.abs() + T * 2.0 ** -23 * (dz.abs().t() @ h64.abs()))
+        want = dict(dh=dz @ w64, dw=dz.t() @ h64)
+        _check({k: got[k] for k in tol}, want, {k: tol[k] + 2.0 ** -8 * want[k].abs() for k in tol})
+
+
+def test_losses_may_be_written_over():
+    """What backward needs of nll is its own."""
+    h, w, t, gn, gz = _inputs(50, 400, 64, 30)
+    want = _run(h, w, t, gn, torch.zeros_like(gz), 0.0)
+    hg, wg = h.detach().requires_grad_(), w.detach().requires_grad_()
+    nll, _ = ops.linear_token_loss(hg, wg, t)
+    nll.mul_(2.0)
+    dh, dw = torch.autograd.grad(nll, (hg, wg), gn / 2)
+    assert torch.equal(dh, want["dh"]) and torch.equal(dw, want["dw"])
