@@ -10,6 +10,7 @@ import ctypes as C
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _build
 
@@ -227,6 +228,12 @@ def on_device(t):
 def here(t) -> int:
     """Handle of the current stream of t's device (a CUDA tensor)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def elementary() -> bool:
+    """Whether torch has to see elementary operations, of which kernels that are launched past it are none: inside a function transform (torch.func, also
+    offered by ``jit``), in forward-mode differentiation and under a dispatch mode."""
+    return torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
 
 
 _status_ptr = {}

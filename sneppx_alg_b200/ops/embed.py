@@ -16,7 +16,14 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def embedding_reference(ids, table, scale=1.0, padding_idx=None):
-    y = F.embedding(ids, table, padding_idx)
+    if not table.is_cuda:
+        y = F.embedding(ids, table, padding_idx)
+    else:                                          # ids out of range as the kernels have them: rows of zeros, told by the status word
+        ok = (ids >= 0) & (ids < table.shape[0])
+        y = torch.where(ok.unsqueeze(-1), F.embedding(torch.where(ok, ids, 0), table, padding_idx), 0.0)
+        if not _lib.elementary():                  # which nobody may write to there
+            word = _lib.status_word(table.device)[:1]
+            word.copy_(torch.where((~ok).any() & (word == 0), 5, word))
     return y if scale == 1.0 else (y.float() * scale).to(y.dtype) if y.dtype != torch.float64 else y * scale
 
 
@@ -119,7 +126,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     The gradient of the table is dense; where the table carries ``main_grad`` (a view into a flat gradient buffer, of its type or fp32) it is written
     there, or added to what is there already (a tied output projection's), and ``.grad`` stays empty. ``padding_idx`` (negative counts from the
     end): tokens of this word give no gradient. On the GPU an id outside [0, V) gives a row of zeros and sets the status word
-    (``check_status`` raises); on the CPU it raises at once."""
+    (``check_status`` raises); on the CPU it raises at once. Inside function transforms (``jit.grad``, ``vmap``, ``jvp``, ``hessian``) and in forward-mode
+    differentiation the PyTorch form is taken; the status word is left alone there."""
     if has_torch_function_variadic(ids, table):      # a trace records this call: of the kernel's it would see the allocation of the result only
         return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
     if table.dim() != 2:
@@ -136,7 +144,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         padding_idx %= table.shape[0]
     if table.shape[0] == 0 and ids.numel():
         raise IndexError("embedding: ids for a table of no rows")
-    if not (table.is_cuda and table.dtype in _TYPES and table.shape[0] > 0 and _lib.available()):
+    if not (table.is_cuda and table.dtype in _TYPES and table.shape[0] > 0 and _lib.available()) or _lib.elementary():
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:
         _dbg.check_indices(ids, 0, table.shape[0], _dbg.SITE_USER)

@@ -66,3 +66,61 @@ def test_a_default_device_does_not_change_the_lookup():
     ids = torch.randint(0, 50, (9,), device="cuda")
     with torch.device("cuda"):                           # a function mode, too
         assert torch.equal(ops.embedding(ids, w, math.sqrt(16)), w[ids] * 4)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32", "fp64"])
+def test_function_transforms_through_a_lookup(dtype):
+    """Each against the same transform of the library's lookup."""
+    torch.manual_seed(0)
+    t = dict(TYPES, fp64=torch.float64)[dtype]
+    e = Embedding(40, 8, dtype=t, device="cuda")
+    w, v = e.weight.detach(), torch.randn(40, 8, device="cuda").to(t)
+    ids = torch.randint(0, 40, (5, 6), device="cuda")
+
+    def loss(look):
+        return lambda i, x: (look(i, x).float() ** 2).sum()
+
+    def own(i, x):
+        return torch.func.functional_call(e, {"weight": x}, (i,))
+
+    def plain(i, x):
+        return torch.nn.functional.embedding(i, x)
+
+    for f in (lambda look: jit.grad(loss(look), 1)(ids, w), lambda look: jit.vmap(look, (0, None))(ids, w), lambda look: jit.vmap(look, (None, 0))(ids, torch.stack([w, v])),
+              lambda look: jit.jvp(lambda x: look(ids, x), (w,), (v,)), lambda look: jit.vmap(jit.grad(loss(look), 1), (0, None))(ids, w),
+              lambda look: jit.hessian(lambda x: loss(look)(ids[0, :2], x))(w[:, :2].float()) if look is plain else
+              jit.hessian(lambda x: loss(lambda i, y: ops.embedding(i, y))(ids[0, :2], x))(w[:, :2].float())):
+        got, want = f(own), f(plain)
+        for a, b in zip(*([x] if torch.is_tensor(x) else x for x in (got, want))):
+            assert a.dtype == b.dtype and torch.equal(a, b)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        y = ops.embedding(ids, fwd.make_dual(w, v), scale=2.0)
+        assert torch.equal(fwd.unpack_dual(y).tangent, v[ids] * 2)
+
+
+def test_lookups_under_a_dispatch_mode():
+    from torch.utils.flop_counter import FlopCounterMode
+    w = torch.randn(40, 8, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 40, (7,), device="cuda")
+    with FlopCounterMode(display=False):
+        y = ops.embedding(ids, w)
+        y.sum().backward()
+    assert torch.equal(y, w[ids]) and torch.equal(w.grad, torch.bincount(ids, minlength=40)[:, None].float().expand(40, 8))
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32])
+def test_ids_out_of_range_in_the_pytorch_form(dtype):
+    """fp64 tables, and any table inside a transform: rows of zeros and no gradient, as from the kernels."""
+    w = torch.randn(20, 8, device="cuda", dtype=dtype)
+    ids = torch.tensor([3, -1, 20, 2 ** 40, 19], device="cuda")
+    ok = torch.tensor([1, 0, 0, 0, 1], device="cuda", dtype=torch.bool)
+    g, y = jit.value_and_grad(lambda x: ops.embedding(ids, x, scale=2.0).sum())(w)
+    want = torch.zeros_like(w)
+    want[3], want[19] = 2, 2
+    assert torch.equal(g, want)
+    ops.check_status()
+    y = ops.embedding(ids, w)
+    with pytest.raises(ops.KernelTimeout):
+        ops.check_status()
+    assert torch.equal(y[ok], w[ids[ok]]) and not y[~ok].any()
