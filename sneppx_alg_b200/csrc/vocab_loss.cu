@@ -43,6 +43,9 @@ constexpr int VL_PAIR_BYTES = VL_SLOTS * (VL_GROUPS - 1) * 128 * 8;
 constexpr int VL_OFF_BAR = VL_OFF_PAIRS + VL_PAIR_BYTES;
 constexpr int VL_SMEM = VL_OFF_BAR + 1024 + 512;
 constexpr float LOG2E = 1.4426950408889634f;
+// Up to this magnitude of a row's maximum (or lse) exponentials of differences are 2^(z log2 e - top log2 e) by one multiply-add, off by the rounding of top
+// log2 e, 2^-13 of its exponent at most; beyond, the difference is taken first, or finite logits of 1e7 and more would overflow.
+constexpr float VL_NEAR = 2048.f;
 
 struct VocabLossParams {
   CUtensorMap tmA, tmB;       // h [T, d], w [V, d]
@@ -105,8 +108,9 @@ __device__ __forceinline__ void softcap_row(float (&v)[N], float cap, float inv)
     for (int j = 0; j < N; ++j) v[j] = softcap(v[j], cap, inv);
   }
 }
+// Infinite maxima are not subtracted: a logit of infinity makes the sum infinite, as the definition has it, and not a NaN.
 __device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
-  const float top = fmaxf(a.x, b.x), at = top == -INFINITY ? 0.f : top;
+  const float top = fmaxf(a.x, b.x), at = isinf(top) ? 0.f : top;
   return make_float2(top, a.y * exp2f((a.x - at) * LOG2E) + b.y * exp2f((b.x - at) * LOG2E));      // the larger one's factor is 1, whatever it is
 }
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&r)[8]) {
@@ -279,7 +283,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
         float top = fmaxf(v[0], v[1]);
 #pragma unroll
         for (int j = 2; j < VL_COLS; j += 2) top = fmax3(top, v[j], v[j + 1]);
-        const float at = top == -INFINITY ? 0.f : top * LOG2E;
+        float at = top * LOG2E, off = fmaf(top, LOG2E, -at);         // top log2 e was rounded, by `off`: the exponentials are 2^off too large
+        if (fabsf(top) > VL_NEAR) {                                  // rare: too far out for that
+          const float from = isinf(top) ? 0.f : top;
+#pragma unroll
+          for (int j = 0; j < VL_COLS; ++j) v[j] -= from;
+          at = off = 0.f;
+        }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < VL_COLS; j += 2) {
@@ -287,9 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
           sum[(j & 3) + 1] += exp2f(fmaf(v[j + 1], LOG2E, -at));
         }
         const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        // top log2 e was rounded, by `off`: the exponentials are 2^off too large
-        const float off = top == -INFINITY ? 0.f : fmaf(top, LOG2E, -at);
-        float2 pair = make_float2(top, fmaf(total, off * -0.6931471805599453f, total));
+        float2 pair = make_float2(top, off == 0.f ? total : fmaf(total, off * -0.6931471805599453f, total));
         // The first warp of a quadrant joins the four. The others may be two tiles ahead of it at most: an accumulator is filled again when all
         // sixteen have read it. Four slots, each with a barrier that they arrive on, are enough.
         const int slot = tile % VL_SLOTS;
@@ -326,23 +334,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
           if (CAP) softcap_row(v, p.cap, p.inv_cap);
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x, y;
-            apart(fma2(two(v[j], v[j + 1]), two(LOG2E, LOG2E), two(off, off)), x, y);
-            apart(mul2(two(a, a), two(exp2f(x), exp2f(y))), g[j], g[j + 1]);
-          }
-          if (__any_sync(0xffffffffu, (tgt >> 5) == c)) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (tgt == c * 32 + j) g[j] = at_target;
-          }
-          if (CAP) {
+          if (CAP) {                                               // the slope, before v may be moved
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               const uint64_t u = mul2(two(v[j], v[j + 1]), two(p.inv_cap, p.inv_cap)), w = mul2(u, two(-1.f, -1.f));
-              apart(mul2(two(g[j], g[j + 1]), fma2(w, u, two(1.f, 1.f))), g[j], g[j + 1]);
+              apart(fma2(w, u, two(1.f, 1.f)), g[j], g[j + 1]);
             }
+          }
+          const bool hot = __any_sync(0xffffffffu, (tgt >> 5) == c);
+          float own = at_target;
+          if (CAP && hot) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (tgt == c * 32 + j) own *= g[j];
+          }
+          float at = off;
+          if (fabsf(off) > VL_NEAR * LOG2E) {
+            const float lse = p.lse[row];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] -= lse;
+            at = 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float x, y;
+            apart(fma2(two(v[j], v[j + 1]), two(LOG2E, LOG2E), two(at, at)), x, y);
+            const uint64_t e = mul2(two(a, a), two(exp2f(x), exp2f(y)));
+            apart(CAP ? mul2(two(g[j], g[j + 1]), e) : e, g[j], g[j + 1]);
+          }
+          if (hot) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (tgt == c * 32 + j) g[j] = own;
           }
           if (left < (c + 1) * 32) {
 #pragma unroll
@@ -398,8 +421,9 @@ __global__ void __launch_bounds__(512) vocab_loss_join_kernel(const float2* __re
   if (t != ignore_index && !valid && status) atomicCAS(status, 0, (int)ST_BAD_ARGUMENT);
   if (valid) {
     const double z = zt[row], d = others - z, more = log1p(exp(d <= 0 ? d : -d));
-    nll[row] = zt[row] = (float)(d <= 0 ? more : d + more);
-    lse[row] = (float)((d <= 0 ? z : others) + more);
+    const bool over = z == INFINITY;           // lse and z infinite: no difference
+    nll[row] = zt[row] = over ? NAN : (float)(d <= 0 ? more : d + more);
+    lse[row] = over && others == others ? INFINITY : (float)((d <= 0 ? z : others) + more);
   } else {
     nll[row] = 0.f;
     lse[row] = (float)others;

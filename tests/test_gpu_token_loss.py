@@ -373,3 +373,57 @@ def test_losses_may_be_written_over():
     nll.mul_(2.0)
     dh, dw = torch.autograd.grad(nll, (hg, wg), gn / 2)
     assert torch.equal(dh, want["dh"]) and torch.equal(dw, want["dw"])
+
+
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_infinite_logits(cap):
+    """A hidden state that overflowed, and products that do: lse, nll and gradients are infinite and NaN where the definition's are."""
+    h, w, t, gn, gz = _inputs(60, 700, 64, 32, ignored=0.0)
+    w[:, 3] = torch.where(w[:, 3] == 0, 0.25, w[:, 3])
+    h[5, 3], h[6, 3], h[7] = math.inf, -math.inf, 0.0
+    big = torch.finfo(torch.bfloat16).max
+    w[100, :2] = big
+    h[:, :2] = 0.0                                          # the word's logit is 0 but for one token, where it overflows
+    h[9, 0], h[10, 0] = big, -big
+    t[5], t[9] = 300, 100
+    got = _run(h, w, t, gn, gz, cap)
+    hg, wg = h.double().requires_grad_(), w.double().requires_grad_()
+    z = (hg @ wg.t()).float().double()                       # where 32 bits overflow
+    z = cap * torch.tanh(z / cap) if cap else z
+    lse = torch.logsumexp(z, 1)
+    nll = lse - z.gather(1, t[:, None]).squeeze(1)
+    for k, v in dict(nll=nll, lse=lse).items():
+        assert torch.equal(torch.isnan(got[k]), torch.isnan(v)), k
+        assert torch.equal(torch.isposinf(got[k]), torch.isposinf(v)), k
+    sure = torch.isfinite(nll)
+    if not cap:
+        assert torch.isposinf(lse[[5, 6]]).all() and torch.isnan(nll[9])
+    # tokens whose lse is finite have finite gradients, the others none
+    finite = torch.isfinite(lse) & torch.isfinite(hg).all(1)
+    assert torch.isfinite(got["dh"][finite & sure][:, 2:]).all()
+    if not cap:
+        assert not torch.isfinite(got["dh"][~finite]).all(1).any()
+
+
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e8, 1e20, 1e36])
+def test_logits_of_any_finite_size(size):
+    """Losses of logits up to the type's range: right to what 32 bits hold of a logit, finite, and dz that of the word that stands out."""
+    h, w, t, _, _ = _inputs(50, 700, 64, 33, ignored=0.0)
+    h = (h.float() * size).to(torch.bfloat16)
+    gn, gz = torch.ones(50, device="cuda"), torch.zeros(50, device="cuda")
+    got = _run(h, w, t, gn, gz, 0.0)
+    h64, w64 = h.double(), w.double()
+    z = h64 @ w64.t()
+    ez = 64 * 2.0 ** -23 * (h64.abs() @ w64.abs().t()).amax(1)
+    lse = torch.logsumexp(z, 1)
+    nll = lse - z.gather(1, t[:, None]).squeeze(1)
+    assert ((got["lse"].double() - lse).abs() <= ez + 2e-5 + 2.0 ** -23 * lse.abs()).all()
+    assert ((got["nll"].double() - nll).abs() <= 2 * ez + 2e-5 + 2.0 ** -23 * nll.abs()).all()
+    # where one word stands out by more than the errors of two logits, dz is 1 for it and -1 for the target, or nothing
+    top = z.topk(2, 1).values
+    clear = top[:, 0] - top[:, 1] > 2 * ez + 120
+    right = z.argmax(1) == t
+    dh = torch.where(right[:, None], 0.0, w64[z.argmax(1)] - w64[t])
+    assert clear.float().mean() > (0.5 if size > 2e3 else 0.1) and torch.isfinite(got["dh"]).all()
+    off = (got["dh"].double() - dh).abs()[clear]
+    assert (off <= 2.0 ** -7 * (w64[z.argmax(1)].abs() + w64[t].abs())[clear]).all()
