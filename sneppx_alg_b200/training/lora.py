@@ -94,10 +94,23 @@ def apply_lora(model, r=8, alpha=16.0, targets=("qkv_proj", "o_proj", "gate_up_p
     return params
 
 
+def _answers_with_its_logits(model) -> bool:
+    """Whether calling the model gives the logits that its ``next_token_logprobs`` stands for: ``forward`` is that of the class which has the method (no
+    subclass's, no wrapper's, none set on the model itself) and no hook sees the call."""
+    cls = type(model)
+    owner = next((c for c in cls.__mro__ if "next_token_logprobs" in vars(c)), None)
+    if owner is None or cls.forward is not owner.forward or cls.__call__ is not tnn.Module.__call__ or "forward" in vars(model):
+        return False
+    every = tnn.modules.module
+    return not (model._forward_hooks or model._forward_pre_hooks or model._backward_hooks or model._backward_pre_hooks or every._global_forward_hooks or
+                every._global_forward_pre_hooks or every._global_backward_hooks or every._global_backward_pre_hooks)
+
+
 def sequence_logprob(model, ids, mask=None):
     """Sum of next-token log-probabilities of ``ids`` [B, S] under the model. Models that give them without their logits
-    (``next_token_logprobs``) do so on the GPU: a batch's logits in 32 bits are the largest tensor of a preference step."""
-    if ids.is_cuda and hasattr(model, "next_token_logprobs"):
+    (``next_token_logprobs``) do so on the GPU: a batch's logits in 32 bits are the largest tensor of a preference step. A model whose call is somebody
+    else's (hooks, another ``forward``) is called."""
+    if ids.is_cuda and _answers_with_its_logits(model):
         lp = model.next_token_logprobs(ids)
     else:
         logits = model(ids)["logits"].float()

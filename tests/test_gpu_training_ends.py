@@ -190,3 +190,56 @@ print("captured")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=180)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_sequence_logprob_calls_models_that_answer_otherwise():
+    """A hook, a subclass's forward, a forward set on the model and a wrapper all change the logits, and with them the log-probabilities."""
+    model = _model(False, vocab=203, layers=1)
+    ids = torch.randint(0, 203, (2, 20), device="cuda")
+    mask = torch.ones(2, 20, device="cuda")
+
+    def of(logits):
+        lp = torch.log_softmax(logits.float()[:, :-1], -1).gather(-1, ids[:, 1:, None]).squeeze(-1)
+        return lp.sum(-1)
+
+    def halved(out):
+        return dict(out, logits=out["logits"] / 2)
+
+    class Tempered(type(model)):
+        def forward(self, *args, **kw):
+            return halved(super().forward(*args, **kw))
+
+    class Wrapper(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                return getattr(self.inner, name)
+
+        def forward(self, ids):
+            return halved(self.inner(ids))
+
+    with torch.no_grad():
+        plain, want = sequence_logprob(model, ids, mask), of(model(ids)["logits"] / 2)
+        assert not torch.allclose(plain, want, rtol=1e-3)
+        assert torch.equal(sequence_logprob(Wrapper(model), ids, mask), want)
+        handle, seen = model.register_forward_hook(lambda m, a, out: halved(out)), []
+        assert torch.equal(sequence_logprob(model, ids, mask), want)
+        handle.remove()
+        handle = model.register_forward_pre_hook(lambda m, a: seen.append(len(a)))
+        sequence_logprob(model, ids, mask)
+        assert seen == [1]
+        handle.remove()
+        first = model.forward
+        model.forward = lambda *a, **k: halved(first(*a, **k))
+        assert torch.equal(sequence_logprob(model, ids, mask), want)
+        del model.forward
+        model.__class__ = Tempered
+        assert torch.equal(sequence_logprob(model, ids, mask), want)
+        model.__class__ = Tempered.__mro__[1]
+        assert torch.equal(sequence_logprob(model, ids, mask), plain)
+    ops.check_status()

@@ -64,3 +64,19 @@ def test_next_token_logprobs_are_those_of_the_logits():
     mask = torch.ones(3, 11)
     mask[0, 5:] = 0
     assert torch.equal(sequence_logprob(model, ids, mask), (lp * mask[:, 1:]).sum(-1))
+
+
+def test_models_that_answer_with_their_logits():
+    from sneppx_alg_b200.models.llama import MistralForCausalLM
+    from sneppx_alg_b200.training.lora import _answers_with_its_logits, apply_lora
+    model = _model()
+    assert _answers_with_its_logits(model) and _answers_with_its_logits(copy.deepcopy(model))
+    apply_lora(model)
+    assert _answers_with_its_logits(model)
+    model.__class__ = MistralForCausalLM
+    assert _answers_with_its_logits(model)
+    assert not _answers_with_its_logits(torch.nn.Linear(2, 2)) and not _answers_with_its_logits(torch.nn.DataParallel(model))
+    handle = model.register_full_backward_hook(lambda *a: None)
+    assert not _answers_with_its_logits(model)
+    handle.remove()
+    assert _answers_with_its_logits(model)
