@@ -33,7 +33,9 @@ template <> __device__ __forceinline__ float emb_out<float>(float v) { return v;
 // A thread's place c, a multiple of 8, in a row of d values. VEC (whole 16-byte accesses: d, pitch and base allow them): the values c to c + 7. Else the 32
 // threads of a warp share 256 values so that neighbours touch neighbouring ones: value j of a thread is 32 j behind its first (2049 columns: 385 us
 // with eight neighbouring values a thread, 97 so).
-template <typename T> union Emb8 { uint4 q[sizeof(T) / 2]; T t[8]; };
+template <typename T> union Emb8 { uint4 q[sizeof(T) / 2]; uint32_t w[2 * sizeof(T)]; T t[8]; };
+// Eight fp32 values are a sector: with accesses of 16 bytes each sector is touched twice (rows of zeros of [32000, 4096] fp32 128 -> 98 us, of [128256, 4096] 446 -> 338).
+__device__ __forceinline__ bool emb_sector(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 template <bool VEC>
 __host__ __device__ __forceinline__ int emb_places(int d) { return VEC ? (d + 7) / 8 : (d + 255) / 256 * 32; }   // threads of a row
 template <bool VEC>
@@ -42,7 +44,12 @@ template <bool VEC>
 __device__ __forceinline__ int emb_first(int c) { return VEC ? c : (c & ~255) + ((c >> 3) & 31); }
 template <bool VEC, typename T>
 __device__ __forceinline__ void emb_load(const T* row, int c, int d, Emb8<T>& v) {
-  if (VEC) {
+  if (VEC && sizeof(T) == 4 && emb_sector(row + c)) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4 % (2 * sizeof(T))]), "=r"(v.w[5 % (2 * sizeof(T))]),
+                   "=r"(v.w[6 % (2 * sizeof(T))]), "=r"(v.w[7 % (2 * sizeof(T))])
+                 : "l"(row + c));
+  } else if (VEC) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v.q[i] = reinterpret_cast<const uint4*>(row + c)[i];
   } else {
@@ -53,7 +60,11 @@ __device__ __forceinline__ void emb_load(const T* row, int c, int d, Emb8<T>& v)
 }
 template <bool VEC, typename T>
 __device__ __forceinline__ void emb_store(T* row, int c, int d, const Emb8<T>& v) {
-  if (VEC) {
+  if (VEC && sizeof(T) == 4 && emb_sector(row + c)) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]),
+                 "r"(v.w[4 % (2 * sizeof(T))]), "r"(v.w[5 % (2 * sizeof(T))]), "r"(v.w[6 % (2 * sizeof(T))]), "r"(v.w[7 % (2 * sizeof(T))])
+                 : "memory");
+  } else if (VEC) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = v.q[i];
   } else {

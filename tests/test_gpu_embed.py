@@ -256,3 +256,25 @@ def test_sums_added_to_rows_that_end_a_buffer(d, dtype):
     want, mag = _sums(ids, dy, V, 1.0)
     _close(grad, want + start.double(), mag + start.double().abs(), torch.float32, int(torch.bincount(ids).max()) + 1)
     assert (buf[V * d:] == 3).all()
+
+
+@pytest.mark.parametrize("offset", [0, 4, 8, 12])
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_fp32_rows_at_any_16_byte_address(dtype, add, offset):
+    """Rows of fp32 values that begin at a sector or in the middle of one: tables, gradients and what is looked up."""
+    torch.manual_seed(0)
+    V, d, n = 300, 40, 500
+    t = TYPES[dtype]
+    buf = torch.full((offset + V * d + 16,), 5.0, device="cuda")
+    grad = buf[offset:offset + V * d].view(V, d)
+    grad.copy_(torch.randn(V, d, device="cuda"))
+    ids = _ids(n, V, "skew", 4).cuda()
+    dy = torch.randn(n, d, device="cuda").to(t)
+    start = grad.double() if add else torch.zeros(V, d, device="cuda", dtype=torch.float64)
+    if dtype == "fp32":
+        assert torch.equal(ops.embedding(ids, grad, 2.0), grad[ids] * 2)
+    ops.embedding_backward_(grad, ids, dy, add=add)
+    want, mag = _sums(ids, dy, V, 1.0)
+    _close(grad, want + start, mag + start.abs(), torch.float32, int(torch.bincount(ids).max()) + 1)
+    assert (buf[:offset] == 5).all() and (buf[offset + V * d:] == 5).all()
