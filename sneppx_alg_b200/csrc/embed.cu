@@ -9,6 +9,7 @@
 // Words that do not occur are known without a table of flags that would have to be cleared: mark[v] holds the position of one token of word v, or
 // whatever was there, and only counts if that token exists and is v's.
 // Ids outside [0, V) give rows of zeros and no gradient, and ST_BAD_ARGUMENT in the status word.
+// This file is compiled without fast math, so that fp32 tables and gradients keep their values below 2^-126.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -379,16 +380,7 @@ template <bool VEC, typename G>
 __device__ __forceinline__ void emb_finish(G* grad, long long ldg, unsigned word, int c, int d, const float (&acc)[8], float scale, int add) {
   G* row = grad + (long long)word * ldg;
   Emb8<G> o;
-  if (VEC && sizeof(G) == 4 && add) {
-    // nobody else writes this row in this launch: the addition at the cache has the load and addition's result, and nothing waits for it
-#pragma unroll
-    for (int j = 0; j < 8; j += 4)
-      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + c + j), "f"(acc[j] * scale), "f"(acc[j + 1] * scale), "f"(acc[j + 2] * scale),
-                   "f"(acc[j + 3] * scale)
-                   : "memory");
-    return;
-  }
-  if (add) {
+  if (add) {       // nobody else writes this row in this launch. By whole sectors as fast as vector reductions at the cache, which make small sums 0
     emb_load<VEC>(row, c, d, o);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o.t[j] = emb_out<G>(emb_in(o.t[j]) + acc[j] * scale);
@@ -436,9 +428,10 @@ __device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long 
 }
 // Keys and positions of 32 tokens are read by the lanes at once and passed round; a warp goes from run to run and asks for four rows of a run at a time.
 // Most words occur a few times only: what keeps memory busy is many warps, not long loads (eight rows of several runs in registers: 103 of them, a quarter
-// of the warps, 93 us instead of 65 for 32768 tokens of 2048).
+// of the warps, 93 us instead of 65 for 32768 tokens of 2048). Four rows of eight fp32 values do not fit the 48 registers that five blocks leave (added to
+// [32000, 1024] fp32: four blocks 43 us, five 57).
 template <bool VEC, typename T, typename G>
-__global__ void __launch_bounds__(256, 5) embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part,
+__global__ void __launch_bounds__(256, VEC && sizeof(T) == 4 ? 4 : 5) embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part,
                                                            unsigned len, int d, int d8, float scale, int add, unsigned blocks_x, unsigned blocks) {
   if (blockIdx.x >= blocks) {          // the gradient is written whole: rows that have no sum, beside those that have
     zero_rows<VEC>(a, grad, ldg, d, blockIdx.x - blocks, gridDim.x - blocks);

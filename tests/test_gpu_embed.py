@@ -278,3 +278,22 @@ def test_fp32_rows_at_any_16_byte_address(dtype, add, offset):
     want, mag = _sums(ids, dy, V, 1.0)
     _close(grad, want + start, mag + start.abs(), torch.float32, int(torch.bincount(ids).max()) + 1)
     assert (buf[:offset] == 5).all() and (buf[offset + V * d:] == 5).all()
+
+
+@pytest.mark.parametrize("d", [8, 33])
+def test_small_values_of_fp32_tables(d):
+    """Values and sums below 2^-126, the smallest normal number, are kept, scaled and not, as the library's lookup keeps them."""
+    torch.manual_seed(0)
+    w = (torch.randint(-100, 100, (20, d), device="cuda").double() * 2.0 ** -140).float().requires_grad_()
+    ids = torch.randint(0, 20, (50,), device="cuda")
+    dy = (torch.randint(-100, 100, (50, d), device="cuda").double() * 2.0 ** -145).float()
+    assert w.abs().max() > 0 and w.abs().max() < torch.finfo(torch.float32).tiny
+    for scale in (1.0, 4.0):
+        y = ops.embedding(ids, w, scale)
+        assert torch.equal(y.double(), w.double()[ids] * scale)
+        (g,) = torch.autograd.grad(y, w, dy)
+        want, _ = _sums(ids, dy, 20, scale)                    # whole multiples of 2^-145: exact
+        assert torch.equal(g.double(), want)
+        base = (torch.randint(-100, 100, (20, d), device="cuda").double() * 2.0 ** -143).float()
+        start = base.double()
+        assert torch.equal(ops.embedding_backward_(base, ids, dy, scale, add=True).double(), start + want)
