@@ -217,7 +217,7 @@ __device__ __forceinline__ void encode16(const float (&f)[PER], int place, int n
   for (int j = 0; j < PER; ++j) k[j] = code_of(f[j], inv);
   if (byte == TOP_BYTE<T>) {             // rare: 128 steps are 127 here
 #pragma unroll
-    for (int j = 0; j < PER; ++j) k[j] = code_of(fminf(fmaxf(f[j] * inv, -127.f), 127.f), 1.f);
+    for (int j = 0; j < PER; ++j) k[j] = min(max((int)k[j], 0x4b400000 - 127), 0x4b400000 + 127);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
