@@ -333,10 +333,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 
   float g[PER], u[PER];
   widen(gv, g);
   widen(uv, u);
-  signed char* kr = codes + (long long)row * (nb * 64);
-  unsigned char* er = exps + (long long)row * (2 * nb);
-  encode16<MODE, T>(g, piece, nb, kr, er);
-  encode16<MODE, T>(u, piece, nb, kr + nb * 32, er + nb);
+  if (codes) {                           // null: nothing is kept
+    signed char* kr = codes + (long long)row * (nb * 64);
+    unsigned char* er = exps + (long long)row * (2 * nb);
+    encode16<MODE, T>(g, piece, nb, kr, er);
+    encode16<MODE, T>(u, piece, nb, kr + nb * 32, er + nb);
+  }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     float a, da;

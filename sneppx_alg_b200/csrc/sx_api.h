@@ -512,7 +512,8 @@ int sx_win_merge(const SxWinAttnArgs* args, cudaStream_t stream);         // key
 // ceil(width / 32).
 int sx_pack8(const void* x, void* codes, void* exps, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
 int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t stream);
-// gu [rows, 2 width] (gate | up, pitch ld) -> h [rows, width], gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb]; and back with dh.
+// gu [rows, 2 width] (gate | up, pitch ld) -> h [rows, width], gate and up in 8 bits: codes [rows, 2, 32 nb], exps [rows, 2, nb] (both null: not held);
+// and back with dh.
 int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t stream);
 int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype, cudaStream_t stream);
 

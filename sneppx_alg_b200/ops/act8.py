@@ -12,7 +12,7 @@ import torch.nn.functional as F
 from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
-from .functional import GLU_ACT, glu_reference
+from .functional import GLU_ACT, glu, glu_reference
 
 BLOCK = 32
 _NAMES = {v: k for k, v in GLU_ACT.items()}
@@ -131,26 +131,31 @@ def glu_8bit_backward_reference(dh, gate, up, act):
     return torch.cat([d * up.float() * da, d * a], -1).to(dh.dtype)
 
 
+def _glu_forward(gu, act, held=None):
+    """The kernel's value of gu; with ``held`` (a buffer for the codes of gate and up for each row and then their exponents) packed there, too."""
+    f = gu.shape[-1] // 2
+    g2 = _rows(gu)
+    h = gu.new_empty((*gu.shape[:-1], f))
+    at = 0 if held is None else held.data_ptr()
+    with _lib.on_device(gu):
+        _lib.entry("sx_glu8_fwd", "ppppliliip")(g2.data_ptr(), h.data_ptr(), at, at and at + g2.shape[0] * 2 * -(-f // BLOCK) * BLOCK, g2.shape[0], f,
+                                               g2.stride(0), act, _TYPES[gu.dtype], _lib.here(gu))
+    return h
+
+
 class _Glu8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gu, act):
         f = gu.shape[-1] // 2
-        g2 = _rows(gu)
-        rows, nb = g2.shape[0], -(-f // BLOCK)
         ctx.meta = act, gu.shape
         if not _native(gu):
-            gate, up = g2[:, :f], g2[:, f:]
-            parts = [pack_8bit_reference(t) for t in (gate, up)]
+            g2 = _rows(gu)
+            parts = [pack_8bit_reference(t) for t in (g2[:, :f], g2[:, f:])]
             ctx.save_for_backward(torch.cat([c for c, _ in parts], 1), torch.cat([e for _, e in parts], 1))
             return glu_reference(gu, _NAMES[act])
-        h = gu.new_empty((*gu.shape[:-1], f))
-        held = gu.new_empty(rows * 2 * nb * (BLOCK + 1), dtype=torch.uint8)           # codes of gate and up for each row, then their exponents
-        with _lib.on_device(gu):
-            at = held.data_ptr()
-            _lib.entry("sx_glu8_fwd", "ppppliliip")(g2.data_ptr(), h.data_ptr(), at, at + rows * 2 * nb * BLOCK, rows, f, g2.stride(0), act,
-                                                   _TYPES[gu.dtype], _lib.here(gu))
+        held = gu.new_empty(gu.shape[:-1].numel() * 2 * -(-f // BLOCK) * (BLOCK + 1), dtype=torch.uint8)
         ctx.save_for_backward(held)
-        return h
+        return _glu_forward(gu, act, held)
 
     @staticmethod
     @_lib.once
@@ -186,9 +191,9 @@ def glu_8bit(gu, act="silu"):
     if not gu.is_floating_point():
         raise TypeError(f"glu_8bit: {gu.dtype} is not a floating type")
     if not (torch.is_grad_enabled() and gu.requires_grad):      # nothing is kept
-        from .functional import glu
         if gu.is_cuda and gu.dtype == torch.bfloat16:
             return glu(gu, act)
+        return _glu_forward(gu, GLU_ACT[act]) if _native(gu) else glu_reference(gu, act)
     return _Glu8Fn.apply(gu, GLU_ACT[act])
 
 

@@ -229,3 +229,22 @@ def test_the_largest_values_come_back_finite(width, dtype):
 def test_glu_of_overflows(f, act, dtype):
     from act8_common import check_glu_of_overflows
     check_glu_of_overflows(ops.glu_8bit, act, dtype, "cuda", f)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+@pytest.mark.parametrize("f", [31, 64, 1000, 1001])
+def test_glu_without_a_gradient_keeps_nothing(f, dtype):
+    x = inputs(77, 2 * f, dtype, 10, edge=False).clamp(-8, 8).cuda()
+    want = ops.glu_8bit(x.clone().requires_grad_()).detach()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = ops.glu_8bit(x)
+    used = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(got, want)
+    # the result, in the allocator's blocks of 512 bytes, and no codes
+    assert used <= (got.numel() * got.element_size() + 511) // 512 * 512
+    with torch.no_grad():
+        assert torch.equal(ops.glu_8bit(x.requires_grad_()), want)
+    e = torch.zeros(0, 64, device="cuda", dtype=TYPES[dtype])
+    assert ops.glu_8bit(e).shape == (0, 32)
