@@ -29,6 +29,7 @@
 #include "tc_common.cuh"
 #include "common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -617,13 +618,8 @@ extern "C" int sx_attn_bwd(const SxAttnArgs* a, cudaStream_t st) {
   p.B = a->B; p.Sq = a->Sq; p.Skv = a->Skv; p.Hq = a->Hq; p.Hk = a->Hk;
   p.causal = a->causal; p.window = a->window;
   p.scale = a->scale; p.scale_log2 = a->scale * 1.4426950408889634f;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BwdCfg::SMEM_BYTES) !=
-        cudaSuccess)
-      return -10;
-    set = true;
-  }
+  static SharedMemory smem;
+  if (smem.allow(BwdCfg::SMEM_BYTES, attn_bwd_kernel)) return -10;
   dim3 grid(((a->Skv + BWD_KV - 1) / BWD_KV) * a->Hk, 1, a->B);
   attn_bwd_kernel<<<grid, BWD_THREADS, BwdCfg::SMEM_BYTES, st>>>(p);
   attn_dq_convert_kernel<<<(unsigned)(acc_floats / (32 * BWD_D)), 256, 0, st>>>(a->dq_accum, (__nv_bfloat16*)a->dQ, a->Sq, a->Hq,

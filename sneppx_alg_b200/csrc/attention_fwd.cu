@@ -25,6 +25,7 @@
 #include <limits.h>
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -419,14 +420,14 @@ static int make_attn_map(CUtensorMap* tm, const void* base, int B, int S, int H,
 
 template <int D, bool MASK>
 static int attn_fwd_launch(const AttnFwdParams& p, dim3 grid, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
+  static SharedMemory smem;
+  static PerDevice regs;
+  if (smem.allow(AttnCfg<D>::SMEM_BYTES, attn_fwd_kernel<D, MASK>)) return -10;
+  const int has = regs.get([](int) {
     cudaFuncAttributes fa;
-    if (cudaFuncSetAttribute(attn_fwd_kernel<D, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnCfg<D>::SMEM_BYTES) != cudaSuccess ||
-        cudaFuncGetAttributes(&fa, attn_fwd_kernel<D, MASK>) != cudaSuccess) return -10;
-    if (fa.numRegs < ATT_REGS) return -12;
-    set = true;
-  }
+    return cudaFuncGetAttributes(&fa, attn_fwd_kernel<D, MASK>) == cudaSuccess ? fa.numRegs : -10;
+  });
+  if (has < ATT_REGS) return has < 0 ? -10 : -12;
   attn_fwd_kernel<D, MASK><<<grid, ATT_THREADS, AttnCfg<D>::SMEM_BYTES, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

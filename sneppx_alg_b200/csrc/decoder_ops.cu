@@ -6,6 +6,7 @@
 // throughout; only what is stored as an activation is rounded to A.
 #include "common.cuh"
 #include "ragged.cuh"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -475,12 +476,9 @@ template <typename A, int NT, int MT>
 static int launch_qkv(const QkvParams& p, int ctas, cudaStream_t st) {
   const int grp = p.H / p.G;
   const int smem = (NT * p.rot + NT * (grp + 1) * p.d + p.H * grp) * 4;
-  static int set = 48 * 1024;
+  static SharedMemory allowed;
   if (smem > 227 * 1024) return -2;
-  if (smem > set) {
-    if (cudaFuncSetAttribute(qkv_prep_kernel<A, NT, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -10;
-    set = smem;
-  }
+  if (smem > 48 * 1024 && allowed.allow(smem, qkv_prep_kernel<A, NT, MT>)) return -10;
   qkv_prep_kernel<A, NT, MT><<<dim3(ctas, p.G), 256, smem, st>>>(p);
   return last_rc();
 }

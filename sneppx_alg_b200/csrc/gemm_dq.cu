@@ -23,6 +23,7 @@
 #include "dq_convert.cuh"
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -357,11 +358,8 @@ static int dq_launch(DqParams& p, int sms, cudaStream_t st) {
   static_assert((3 * DQ_MAX_STAGES + 2 * Cfg::NA + 4) * 8 + 8 <= 256, "barriers");
   static_assert(2 * STAGE_BYTES >= BT * DQ_BM * 4, "the partial tile lies over the stages");
   const int smem = p.stages * STAGE_BYTES + 1024 + 256;
-  static int set = 0;
-  if (set < smem) {
-    if (cudaFuncSetAttribute(gemm_dq_kernel<BT, INT4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -10;
-    set = smem;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(smem, gemm_dq_kernel<BT, INT4>)) return -10;
   const int tiles = (p.N + DQ_BM - 1) / DQ_BM, mt = (p.M + BT - 1) / BT;
   const int kblks = p.K / DQ_BK;
   const int S = dq_splits(tiles * mt, INT4 ? (kblks + 1) / 2 : kblks, Cfg::CTAS * sms);

@@ -20,6 +20,7 @@
 #include "tc_common.cuh"
 #include "common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -222,13 +223,8 @@ __global__ void f8_finish_kernel(const float* __restrict__ work, const float* __
 
 template <int BT>
 static int f8_launch(const F8Params& p, dim3 grid, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(gemm_f8_kernel<BT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F8Cfg<BT>::SMEM_BYTES) !=
-        cudaSuccess)
-      return -10;
-    set = true;
-  }
+  static SharedMemory smem;
+  if (smem.allow(F8Cfg<BT>::SMEM_BYTES, gemm_f8_kernel<BT>)) return -10;
   gemm_f8_kernel<BT><<<grid, F8_THREADS, F8Cfg<BT>::SMEM_BYTES, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

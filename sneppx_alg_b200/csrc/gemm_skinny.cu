@@ -16,6 +16,7 @@
 #include <stdlib.h>
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -310,18 +311,9 @@ extern "C" int sx_gemm_skinny(const SxGemmArgs* a, cudaStream_t st) {
   p.ldc = a->ldc; p.beta = a->beta; p.act_a = a->act_a; p.act_b = a->act_b;
   p.flags = a->flags;
   const int smem = stages * stage_bytes + 1024 + 1024;
-  static int smem_set = 0;
-  if (smem_set < smem) {
-    if (cudaFuncSetAttribute(gemm_skinny_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 101376) != cudaSuccess)
-      return -10;
-    smem_set = 101376;
-  }
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(101376, gemm_skinny_kernel)) return -10;
+  const int sms = multiprocessors();
   const int S = sx_gemm_skinny_splits(a->N, a->K, sms);
   const int tiles = (a->N + SK_BM - 1) / SK_BM;
   cudaLaunchConfig_t cfg = {};

@@ -20,6 +20,7 @@
 #include "comm_common.cuh"
 #include "common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -735,24 +736,12 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_tc_kernel(const __grid_c
   }
 }
 
-// A kernel's attributes hold for one device: bit of the current one in what a launcher has set up.
-static unsigned long long device_bit() {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  return 1ull << (dev & 63);
-}
-
 template <int BN, bool A_MN, bool B_MN, int COMM = 0>
 static int launch_cfg(const GemmKernelParams& kp, int grid, cudaStream_t st) {
   using Cfg = GemmCfg<BN, COMM>;
-  static unsigned long long set = 0;
+  static SharedMemory smem;
   auto kern = gemm_tc_kernel<BN, A_MN, B_MN, COMM>;
-  const unsigned long long dev = device_bit();
-  if (!(__atomic_load_n(&set, __ATOMIC_ACQUIRE) & dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES) != cudaSuccess)
-      return -10;
-    __atomic_fetch_or(&set, dev, __ATOMIC_RELEASE);
-  }
+  if (smem.allow(Cfg::SMEM_BYTES, kern)) return -10;
   kern<<<grid, GEMM_THREADS, Cfg::SMEM_BYTES, st>>>(kp);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
@@ -1014,14 +1003,13 @@ static int g2_max_clusters(int sms) {
 
 template <int BN2, int EPI, bool A_MN, bool B_MN>
 static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
-  static unsigned long long set = 0;
-  static int max_clusters = 0;
+  static SharedMemory smem;
+  static PerDevice clusters_at_once;
   auto kern = gemm2_kernel<BN2, EPI, A_MN, B_MN>;
   constexpr int THREADS = 64 + 32 * EPI;
   constexpr int SMEM = G2Cfg<BN2>::SMEM_BYTES;
-  const unsigned long long dev = device_bit();
-  if (!(__atomic_load_n(&set, __ATOMIC_ACQUIRE) & dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return -10;
+  if (smem.allow(SMEM, kern)) return -10;
+  const int max_clusters = clusters_at_once.get([&](int) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms & ~1, 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
@@ -1030,12 +1018,14 @@ static int launch_cfg2(const GemmKernelParams& kp, int sms, cudaStream_t st) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&max_clusters, kern, &cfg) != cudaSuccess || max_clusters <= 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
-      max_clusters = g2_max_clusters(sms);
+      n = g2_max_clusters(sms);
     }
-    __atomic_fetch_or(&set, dev, __ATOMIC_RELEASE);
-  }
+    return n;
+  });
+  if (max_clusters <= 0) return -10;
   const long long tiles = (long long)kp.batch * kp.m_blks * kp.n_blks;
   int clusters = (int)(tiles < max_clusters ? tiles : max_clusters);
   if (clusters > sms / 2) clusters = sms / 2;

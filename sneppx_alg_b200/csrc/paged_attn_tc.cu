@@ -14,6 +14,7 @@
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -433,19 +434,9 @@ extern "C" int sx_paged_decode_tc(const void* q, long long q_row_stride, const v
   p.status = status;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.nsplit = nsplit;
   p.scale_log2 = scale * 1.4426950408889634f;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(paged_decode_tc_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(paged_decode_tc_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM) != cudaSuccess)
-      return -10;
-    set = true;
-  }
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
-  }
+  static SharedMemory smem;
+  if (smem.allow(PT_SMEM, paged_decode_tc_kernel<true>, paged_decode_tc_kernel<false>)) return -10;
+  const int sms = multiprocessors();
   const long long items = (long long)B * Hkv * nsplit;
   auto run = [&](auto kern) { launch_dependent(kern, (unsigned)(items < sms ? items : sms), PT_THREADS, PT_SMEM, st, p); };
   items <= (long long)PT_FEW_ITEMS * sms ? run(paged_decode_tc_kernel<true>) : run(paged_decode_tc_kernel<false>);

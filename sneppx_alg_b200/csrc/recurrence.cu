@@ -9,6 +9,7 @@
 #include "common.cuh"
 #include "ragged.cuh"
 #include "tc_common.cuh"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -1005,19 +1006,13 @@ extern "C" int sx_recur_record(int d, int delta) {
 }
 
 template <typename K>
-static int allow_smem(K kern, int bytes, bool* done) {
-  if (!*done && bytes > 48 * 1024) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -10;
-    *done = true;
-  }
-  return 0;
-}
+static int allow_smem(K kern, int bytes, SharedMemory& allowed) { return bytes > 48 * 1024 ? allowed.allow(bytes, kern) : 0; }
 
 template <typename A, int DP>
 static int launch_gate_chunks(const SxGateArgs* a, cudaStream_t st) {
-  static bool set = false;
+  static SharedMemory allowed;
   const int smem = 3 * RC * DP * 4;
-  if (int rc = allow_smem(gate_chunk_kernel<A, DP>, smem, &set)) return rc;
+  if (int rc = allow_smem(gate_chunk_kernel<A, DP>, smem, allowed)) return rc;
   gate_chunk_kernel<A, DP><<<dim3(a->chunks.n, a->H), 256, smem, st>>>((const A*)a->q, (const A*)a->f, a->ld, a->bias, a->lower, a->rec,
                                                                        view(&a->ragged), chunks(&a->chunks), a->H, a->d);
   return last_rc();
@@ -1040,9 +1035,9 @@ extern "C" int sx_gate_chunks(const SxGateArgs* a, cudaStream_t st) {
 
 template <typename A, int DP>
 static int launch_ssd_chunks(const SxSsdArgs* a, float* rec, cudaStream_t st) {
-  static bool set = false;
+  static SharedMemory allowed;
   const int smem = 3 * RC * DP * 4;
-  if (int rc = allow_smem(ssd_chunk_kernel<A, DP>, smem, &set)) return rc;
+  if (int rc = allow_smem(ssd_chunk_kernel<A, DP>, smem, allowed)) return rc;
   ssd_chunk_kernel<A, DP><<<dim3(a->chunks.n, a->H), 256, smem, st>>>((const A*)a->b, (const A*)a->c, a->dt, a->la, rec, view(&a->ragged),
                                                                       chunks(&a->chunks), a->H, a->G, a->N, a->np);
   return last_rc();
@@ -1065,9 +1060,9 @@ extern "C" int sx_ssd_chunks(const SxSsdArgs* a, float* rec, cudaStream_t st) {
 
 template <typename A, int DP, int MT>
 static int launch_delta_chunks(const DeltaParams& p, float* rec, const ChunkView& cv, cudaStream_t st) {
-  static bool set = false;
+  static SharedMemory allowed;
   const int smem = (3 * RC * DP + RC * RC + RC) * 4;
-  if (int rc = allow_smem(delta_chunk_kernel<A, DP, MT>, smem, &set)) return rc;
+  if (int rc = allow_smem(delta_chunk_kernel<A, DP, MT>, smem, allowed)) return rc;
   delta_chunk_kernel<A, DP, MT><<<dim3(cv.n_chunks, p.H), 256, smem, st>>>(p, rec, cv);
   return last_rc();
 }
@@ -1097,8 +1092,8 @@ extern "C" int sx_delta_chunks(const SxDeltaArgs* a, const SxChunks* c, float* r
 template <typename A, bool DELTA, int LANES, int CN>
 static int launch_scan(const ScanParams& p, cudaStream_t st) {
   using Cfg = ScanCfg<A, DELTA, LANES, CN>;
-  static bool set = false;
-  if (int rc = allow_smem(recur_scan_kernel<A, DELTA, LANES, CN>, Cfg::SMEM, &set)) return rc;
+  static SharedMemory allowed;
+  if (int rc = allow_smem(recur_scan_kernel<A, DELTA, LANES, CN>, Cfg::SMEM, allowed)) return rc;
   dim3 grid((p.dv + Cfg::CT - 1) / Cfg::CT, p.H, p.rv.n);
   recur_scan_kernel<A, DELTA, LANES, CN><<<grid, 128, Cfg::SMEM, st>>>(p);
   return last_rc();
@@ -1121,8 +1116,8 @@ static int pick_scan(const ScanParams& p, cudaStream_t st) {
 template <typename A, bool DELTA, int DP, bool SPLITD>
 static int launch_scan_tc(const ScanParams& p, cudaStream_t st) {
   using Cfg = TcScanCfg<DELTA, DP, SPLITD>;
-  static bool set = false;
-  if (int rc = allow_smem(recur_scan_tc_kernel<A, DELTA, DP, SPLITD>, Cfg::SMEM, &set)) return rc;
+  static SharedMemory allowed;
+  if (int rc = allow_smem(recur_scan_tc_kernel<A, DELTA, DP, SPLITD>, Cfg::SMEM, allowed)) return rc;
   dim3 grid((p.dv + Cfg::COLS - 1) / Cfg::COLS, p.H, p.rv.n);
   recur_scan_tc_kernel<A, DELTA, DP, SPLITD><<<grid, 128, Cfg::SMEM, st>>>(p);
   return last_rc();

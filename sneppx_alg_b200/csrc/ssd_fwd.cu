@@ -20,6 +20,7 @@
 // (algorithms/hss/cuda/hss_cuda_extended.cu:27-77) and its Mamba-2 block is a stub (kernel/arch/mamba2.c:36-133).
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -312,12 +313,8 @@ extern "C" int sx_ssd_chunk_fwd(const void* C, long long c_ld, const void* B, lo
   const int want = ctas >= 148 ? 1 : (int)(148 / ctas < most ? 148 / ctas : most);
   p.per = (rep + want - 1) / want;
   p.splits = (rep + p.per - 1) / p.per;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(ssd_chunk_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             SsdFwdCfg::SMEM_BYTES) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory smem;
+  if (smem.allow(SsdFwdCfg::SMEM_BYTES, ssd_chunk_fwd_kernel)) return -10;
   ssd_chunk_fwd_kernel<<<dim3((unsigned)(G * p.splits), (unsigned)BC), SF_THREADS, SsdFwdCfg::SMEM_BYTES, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }

@@ -17,6 +17,7 @@
 // state in front of every segment, and the full pass starts from there.
 #include "tc_common.cuh"
 #include "ragged.cuh"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -424,11 +425,8 @@ __global__ void __launch_bounds__(256) ssd_chain_kernel(const SsdScanParams P) {
 
 template <int KN, bool STATE>
 static int launch_ssd_scan(const SsdScanParams& p, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(ssd_scan_kernel<KN, STATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SsdScanCfg<KN>::SMEM) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory smem;
+  if (smem.allow(SsdScanCfg<KN>::SMEM, ssd_scan_kernel<KN, STATE>)) return -10;
   ssd_scan_kernel<KN, STATE><<<dim3((p.a.P + 63) / 64, p.a.H, p.a.n_seg ? p.a.n_seg : p.rv.n), 256, SsdScanCfg<KN>::SMEM, st>>>(p);
   return last_rc();
 }

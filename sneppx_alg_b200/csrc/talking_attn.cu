@@ -7,6 +7,7 @@
 // different CTAs whose partial results a second kernel merges.
 #include "common.cuh"
 #include "ragged.cuh"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -147,13 +148,8 @@ static int launch_talk(const TalkParams& P, cudaStream_t st) {
   const SxTalkArgs& a = P.a;
   const int smem = (a.H * a.d + a.H * a.H + 2 * a.H * TA_KT + a.H * a.dv + 3 * a.H) * 4;
   if (smem > 227 * 1024) return -2;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(talk_attn_kernel<A, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
-        cudaFuncSetAttribute(talk_attn_kernel<A, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
-      return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(227 * 1024, talk_attn_kernel<A, false>, talk_attn_kernel<A, true>)) return -10;
   const dim3 grid(a.T, a.splits);
   if (a.block_table) talk_attn_kernel<A, true><<<grid, 256, smem, st>>>(P);
   else talk_attn_kernel<A, false><<<grid, 256, smem, st>>>(P);

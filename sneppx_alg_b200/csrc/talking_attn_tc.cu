@@ -17,6 +17,7 @@
 #include "ragged.cuh"
 #include "tc_common.cuh"
 #include "tmap.h"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -353,11 +354,8 @@ extern "C" int sx_talk_attn_tc(const SxTalkTcArgs* a, cudaStream_t st) {
   p.stages = room / stage;
   if (p.stages > TT_MAX_STAGES) p.stages = TT_MAX_STAGES;
   const int smem = held + p.stages * stage + 1024 + 256;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(talk_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(227 * 1024, talk_tc_kernel)) return -10;
   if (smem > 227 * 1024) return -4;
   talk_tc_kernel<<<dim3(a->H, a->n_tiles), TT_THREADS, smem, st>>>(p);
   return last_rc();

@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "ragged.cuh"
 #include "tc_common.cuh"
+#include "per_device.h"
 #include "sx_api.h"
 
 namespace sx {
@@ -384,11 +385,8 @@ extern "C" int sx_talk_decode_ok(int H, int G, int d, int dv) { return dec_plan(
 
 template <int KT, int MAXI, bool QREG>
 static int launch_dec(const TalkDecParams& p, int n, int smem, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(talk_decode_kernel<KT, MAXI, QREG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(227 * 1024, talk_decode_kernel<KT, MAXI, QREG>)) return -10;
   talk_decode_kernel<KT, MAXI, QREG><<<dim3(n, p.splits), DT, smem, st>>>(p);
   return last_rc();
 }

@@ -5,6 +5,7 @@
 // Values are rotated by their position before they are cached, outputs turned back by the query's position, so the weight of a
 // value depends on its distance.
 #include "window_attn.cuh"
+#include "per_device.h"
 
 namespace sx {
 
@@ -410,13 +411,8 @@ static int launch_win(const WinParams& p, cudaStream_t st) {
   const SxWinAttnArgs& a = p.a;
   const int grp = a.H / a.G, smem = grp * (a.d + WA_KT + a.dv + 3) * 4;
   if (smem > 227 * 1024) return -2;
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(win_attn_kernel<A, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
-        cudaFuncSetAttribute(win_attn_kernel<A, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
-      return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(227 * 1024, win_attn_kernel<A, false>, win_attn_kernel<A, true>)) return -10;
   const dim3 grid(a.T, a.G, a.splits);
   if (a.block_table) win_attn_kernel<A, true><<<grid, 128, smem, st>>>(p);
   else win_attn_kernel<A, false><<<grid, 128, smem, st>>>(p);

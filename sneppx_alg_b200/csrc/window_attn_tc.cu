@@ -14,6 +14,7 @@
 #include "tc_common.cuh"
 #include "tmap.h"
 #include "window_attn.cuh"
+#include "per_device.h"
 
 namespace sx {
 
@@ -405,11 +406,8 @@ static int win_rows_map(CUtensorMap* tm, const void* base, long long width, long
 
 template <bool INTER, bool PAIR, int NQ>
 static int launch_win_tc(const WinTcParams& p, int smem, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(win_tc_kernel<INTER, PAIR, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(227 * 1024, win_tc_kernel<INTER, PAIR, NQ>)) return -10;
   win_tc_kernel<INTER, PAIR, NQ><<<dim3(PAIR ? p.a.H / 2 : p.a.H, p.a.n_tiles), WT_THREADS, smem, st>>>(p);
   return last_rc();
 }

@@ -8,6 +8,7 @@
 // it). The warps are merged at the end, the slices by sx_win_merge.
 #include "tc_common.cuh"
 #include "window_attn.cuh"
+#include "per_device.h"
 
 namespace sx {
 
@@ -214,11 +215,8 @@ __global__ void __launch_bounds__(WD_T) win_decode_kernel(const WinParams P, int
 
 template <int KD, int NV>
 static int launch_win_decode(const WinParams& p, cudaStream_t st) {
-  static bool set = false;
-  if (!set) {
-    if (cudaFuncSetAttribute(win_decode_kernel<KD, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, WinDecCfg<KD, NV>::SMEM) != cudaSuccess) return -10;
-    set = true;
-  }
+  static SharedMemory allowed;
+  if (allowed.allow(WinDecCfg<KD, NV>::SMEM, win_decode_kernel<KD, NV>)) return -10;
   const int parts = (p.a.H / p.a.G + 15) / 16;
   win_decode_kernel<KD, NV><<<dim3(p.a.T, p.a.G * parts, p.a.splits), WD_T, WinDecCfg<KD, NV>::SMEM, st>>>(p, parts);
   return last_rc();
