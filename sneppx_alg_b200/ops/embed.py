@@ -37,20 +37,31 @@ def _workspace(n, V, d, presorted):
     return _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, presorted)
 
 
-def _lookup(ids, table, scale, padding_idx=None, sort=False):
-    """(rows, ids as they were read, those in the order of their words or None)."""
-    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
-        table = table.contiguous()
-    ids = ids.contiguous()
+# Both launches are a call's whole cost for few tokens (the library's lookup of one row: 5.5 us): numbers are read once, nothing is wrapped.
+def _lookup(ids, table, scale, padding=-1, sort=False):
+    """(rows, ids as they were read, those in the order of their words or None). padding: a word, or -1."""
     V, d = table.shape
+    ldw, step = table.stride()
+    if step != 1 or ldw < d:
+        table, ldw = table.contiguous(), d
+    ids = ids.contiguous()
     n = ids.numel()
     y = table.new_empty((*ids.shape, d))
-    size = _sorted_bytes(n, V) if sort and d else 0
-    order = table.new_empty(size, dtype=torch.uint8) if size else None
-    with _lib.on_device(table):
-        _lib.entry("sx_embed_fwd", "piplplilfilppp")(
-            ids.data_ptr(), ids.dtype is torch.int64, table.data_ptr(), table.stride(0), y.data_ptr(), n, d, V, scale, _TYPES[table.dtype],
-            -1 if padding_idx is None else padding_idx, order.data_ptr() if size else 0, _lib.status_ptr(table), _lib.here(table))
+    order, at = None, 0
+    if sort and d:
+        size = _sorted_bytes(n, V)
+        if size:
+            order = table.new_empty(size, dtype=torch.uint8)
+            at = order.data_ptr()
+    dev = table.get_device()
+    launch = _lib.entry("sx_embed_fwd", "piplplilfilppp")
+    args = (ids.data_ptr(), ids.dtype is torch.int64, table.data_ptr(), ldw, y.data_ptr(), n, d, V, scale, _TYPES[table.dtype], padding, at,
+            _lib.status_ptr(table), torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        launch(*args)
+    else:
+        with torch.cuda.device(dev):
+            launch(*args)
     return y, ids, order
 
 
@@ -72,52 +83,55 @@ def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
         raise ValueError("embedding_backward_: a table of no rows")
     if padding_idx is not None and not 0 <= padding_idx < V:
         raise ValueError(f"embedding_backward_: padding_idx {padding_idx} outside a table of {V} rows")
-    return _backward(grad, ids.contiguous(), dy.contiguous(), float(scale), padding_idx, bool(add), None)
+    return _backward(grad, ids.contiguous(), dy.contiguous(), float(scale), -1 if padding_idx is None else padding_idx, bool(add), None)
 
 
-def _backward(grad, ids, dy, scale, padding_idx, add, order):
+def _backward(grad, ids, dy, scale, padding, add, order):
     """ids and dy contiguous, all on one device; order: what the forward pass left, or None."""
     V, d = grad.shape
     n = ids.numel()
     size = _workspace(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)
-    with _lib.on_device(grad):
-        _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")(
-            ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, -1 if padding_idx is None else padding_idx,
-            scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], 0 if order is None else order.data_ptr(), work.data_ptr(), size,
-            _lib.status_ptr(grad), _lib.here(grad))
+    dev = grad.get_device()
+    launch = _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")
+    args = (ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, padding, scale, add, _TYPES[dy.dtype],
+            _TYPES[grad.dtype], 0 if order is None else order.data_ptr(), work.data_ptr(), size, _lib.status_ptr(grad),
+            torch._C._cuda_getCurrentRawStream(dev))
+    if dev == torch._C._cuda_getDevice():
+        launch(*args)
+    else:
+        with torch.cuda.device(dev):
+            launch(*args)
     return grad
 
 
-def _differentiable_backward(ids, dy, V, scale, padding_idx):
-    counts = (ids >= 0) & (ids < V)
-    if padding_idx is not None:
-        counts &= ids != padding_idx
+def _differentiable_backward(ids, dy, V, scale, padding):
+    counts = (ids >= 0) & (ids < V) & (ids != padding)
     rows = torch.where(counts[..., None], dy.float() * scale, 0.0).reshape(-1, dy.shape[-1])
     return rows.new_zeros(V, dy.shape[-1]).index_add(0, torch.where(counts, ids, 0).reshape(-1), rows).to(dy.dtype)
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, padding_idx):
-        y, ids, order = _lookup(ids, table, scale, padding_idx, sort=True)
+    def forward(ctx, ids, table, scale, padding):
+        y, ids, order = _lookup(ids, table, scale, padding, True)
         ctx.save_for_backward(ids)
-        ctx.table, ctx.meta = table, (scale, padding_idx, order)
+        ctx.meta = table, scale, padding, order
         return y
 
     @staticmethod
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
-        table, (scale, padding_idx, order) = ctx.table, ctx.meta
+        table, scale, padding, order = ctx.meta
         if torch.is_grad_enabled():                # a graph of this pass is wanted: the same sums by operations that have one
-            return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding_idx), None, None
+            return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding), None, None
         mg = getattr(table, "main_grad", None)
         dy = dy.contiguous()
-        if mg is not None and mg.dtype in (dy.dtype, torch.float32) and mg.stride(1) == 1:
-            _backward(mg, ids, dy, scale, padding_idx, getattr(table, "_main_grad_written", False), order)
-            table._main_grad_written = True
-            return None, None, None, None
-        return None, _backward(dy.new_empty(table.shape), ids, dy, scale, padding_idx, False, order), None, None
+        if mg is None or mg.dtype not in (dy.dtype, torch.float32) or mg.stride(1) != 1:
+            return None, _backward(dy.new_empty(table.shape), ids, dy, scale, padding, False, order), None, None
+        _backward(mg, ids, dy, scale, padding, getattr(table, "_main_grad_written", False), order)
+        table._main_grad_written = True
+        return None, None, None, None
 
 
 def embedding(ids, table, scale=1.0, padding_idx=None):
@@ -132,6 +146,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
     if table.dim() != 2:
         raise ValueError(f"embedding: table of shape {tuple(table.shape)} is no matrix")
+    V = table.shape[0]
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
             raise TypeError(f"embedding: ids of {ids.dtype}")
@@ -139,15 +154,15 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     if ids.get_device() != table.get_device():
         raise ValueError(f"embedding: ids on {ids.device}, table on {table.device}")
     if padding_idx is not None:
-        if not -table.shape[0] <= padding_idx < table.shape[0]:
-            raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {table.shape[0]} rows")
-        padding_idx %= table.shape[0]
-    if table.shape[0] == 0 and ids.numel():
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {V} rows")
+        padding_idx %= V
+    if V == 0 and ids.numel():
         raise IndexError("embedding: ids for a table of no rows")
-    if not (table.is_cuda and table.dtype in _TYPES and table.shape[0] > 0 and _lib.available()) or _lib.elementary():
+    if not table.is_cuda or table.dtype not in _TYPES or V == 0 or not _lib.available() or _lib.elementary():
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:
-        _dbg.check_indices(ids, 0, table.shape[0], _dbg.SITE_USER)
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _EmbeddingFn.apply(ids, table, float(scale), padding_idx)
+        _dbg.check_indices(ids, 0, V, _dbg.SITE_USER)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(ids, table, float(scale), -1 if padding_idx is None else padding_idx)
     return _lookup(ids, table, scale)[0]
