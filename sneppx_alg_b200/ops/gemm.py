@@ -144,8 +144,9 @@ def gemm(a, b, *, a_mn=False, b_mn=False, out=None, out_dtype=None, c=None, beta
     if (a_mn and a.dim() == 2 and a.shape[-1] % 64 != 0 and a.shape[-1] > 256 and tile_group is None
             and k_ranges is None and a.stride(-1) == 1 and (out is None or out.dim() == 2)
             and (c is None or c.dim() == 2)):
-        # MN-major operands are tiled in 64-element atoms: run the aligned part in place and only the ragged
-        # tail (< 64 rows of the result) through a transposed copy
+        # rows that are no whole groups of 64: the aligned part runs in place and only the tail (< 64 rows of the result) through a transposed copy. The
+        # kernel also takes such operands whole, by maps of 64 columns (the gradients of ops.linear_token_loss do so); for these calls the two have not
+        # been measured against each other
         m0 = a.shape[-1] // 64 * 64
         if out is None:
             n_out = b.shape[-1] if b_mn else b.shape[-2]

@@ -297,3 +297,13 @@ def test_small_values_of_fp32_tables(d):
         base = (torch.randint(-100, 100, (20, d), device="cuda").double() * 2.0 ** -143).float()
         start = base.double()
         assert torch.equal(ops.embedding_backward_(base, ids, dy, scale, add=True).double(), start + want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint8, torch.bool, torch.complex64, torch.float8_e4m3fn])
+def test_tables_of_other_types(dtype):
+    """They take the library's lookup, as they are."""
+    w = torch.randint(0, 2, (30, 8), device="cuda").to(dtype)
+    ids = torch.tensor([[3, 29], [0, 3]], device="cuda")
+    y = ops.embedding(ids, w)
+    assert y.dtype == dtype and torch.equal(y.to(torch.complex64), torch.nn.functional.embedding(ids, w).to(torch.complex64))
+    ops.check_status()
