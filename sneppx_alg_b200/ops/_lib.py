@@ -231,9 +231,9 @@ def here(t) -> int:
 
 
 def elementary() -> bool:
-    """Whether torch has to see elementary operations, of which kernels that are launched past it are none: inside a function transform (torch.func, also
-    offered by ``jit``), in forward-mode differentiation and under a dispatch mode."""
-    return torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
+    """Whether torch has to see elementary operations, of which kernels that are launched past it are none: while torch.compile reads a function, inside a
+    function transform (torch.func, also offered by ``jit``), in forward-mode differentiation and under a dispatch mode."""
+    return torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
 
 
 _status_ptr = {}

@@ -140,8 +140,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     The gradient of the table is dense; where the table carries ``main_grad`` (a view into a flat gradient buffer, of its type or fp32) it is written
     there, or added to what is there already (a tied output projection's), and ``.grad`` stays empty. ``padding_idx`` (negative counts from the
     end): tokens of this word give no gradient. On the GPU an id outside [0, V) gives a row of zeros and sets the status word
-    (``check_status`` raises); on the CPU it raises at once. Inside function transforms (``jit.grad``, ``vmap``, ``jvp``, ``hessian``) and in forward-mode
-    differentiation the PyTorch form is taken; the status word is left alone there."""
+    (``check_status`` raises); on the CPU it raises at once. Inside function transforms (``jit.grad``, ``vmap``, ``jvp``, ``hessian``), in forward-mode
+    differentiation and under torch.compile the PyTorch form is taken; the status word is left alone there."""
     if has_torch_function_variadic(ids, table):      # a trace records this call: of the kernel's it would see the allocation of the result only
         return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
     if table.dim() != 2:
@@ -159,7 +159,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         padding_idx %= V
     if V == 0 and ids.numel():
         raise IndexError("embedding: ids for a table of no rows")
-    if not table.is_cuda or table.dtype not in _TYPES or V == 0 or not _lib.available() or _lib.elementary():
+    if not table.is_cuda or table.dtype not in _TYPES or V == 0 or _lib.elementary() or not _lib.available():
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:
         _dbg.check_indices(ids, 0, V, _dbg.SITE_USER)

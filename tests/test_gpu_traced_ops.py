@@ -124,3 +124,14 @@ def test_ids_out_of_range_in_the_pytorch_form(dtype):
     with pytest.raises(ops.KernelTimeout):
         ops.check_status()
     assert torch.equal(y[ok], w[ids[ok]]) and not y[~ok].any()
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_a_lookup_that_torch_compile_reads(backend):
+    """In one graph, as it was when the layer called the library's lookup."""
+    e = Embedding(50, 8, device="cuda")
+    ids = torch.randint(0, 50, (7,), device="cuda")
+    y = torch.compile(lambda i: e(i) * 2, fullgraph=True, backend=backend)(ids)
+    y.sum().backward()
+    assert torch.equal(y, e.weight[ids] * 2)
+    assert torch.equal(e.weight.grad, 2 * torch.bincount(ids, minlength=50)[:, None].float().expand(50, 8))
