@@ -393,8 +393,8 @@ static int row_mode(int width, long long ld, const void* p, const void* q, int s
   if (width % 8 == 0 && ld * size % 16 == 0 && at % 16 == 0) return PAIR;
   return width <= 64 ? NEAR : ODD;
 }
-static bool act8_args_ok(const void* codes, long long rows, int width, int dtype) {
-  return rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+static bool act8_args_ok(const void* values, const void* codes, const void* exps, long long rows, int width, int dtype) {
+  return values && !codes == !exps && rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
 }
 
 // dtype 0 bf16, 1 fp16, 2 fp32
@@ -419,7 +419,7 @@ using namespace sx;
 
 extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
+  if (!codes || !act8_args_ok(x, codes, exps, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -433,7 +433,7 @@ extern "C" int sx_pack8(const void* x, void* codes, void* exps, long long rows, 
 }
 extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long long rows, int width, long long ld, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
+  if (!codes || !act8_args_ok(x, codes, exps, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -448,7 +448,7 @@ extern "C" int sx_unpack8(const void* codes, const void* exps, void* x, long lon
 }
 extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, long long rows, int width, long long ld, int act, int dtype, cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
+  if (!h || !act8_args_ok(gu, codes, exps, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -464,7 +464,7 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
 extern "C" int sx_glu8_bwd(const void* dh, const void* codes, const void* exps, void* dgu, long long rows, int width, int act, int dtype,
                            cudaStream_t st) {
   if (rows == 0 || width == 0) return 0;
-  if (!act8_args_ok(codes, rows, width, dtype)) return -1;
+  if (!codes || !dgu || !act8_args_ok(dh, codes, exps, rows, width, dtype)) return -1;
   const int nb = (width + 31) / 32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);

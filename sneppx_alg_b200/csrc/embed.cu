@@ -681,7 +681,7 @@ extern "C" long long sx_embed_sorted_bytes(long long tokens, long long V) { retu
 extern "C" int sx_embed_fwd(const void* ids, int ids_wide, const void* w, long long ldw, void* y, long long tokens, int d, long long V, float scale, int dtype,
                             long long padding, void* sorted, int* status, cudaStream_t st) {
   if (tokens == 0 || d == 0) return 0;
-  if (!emb_args_ok(tokens, d, V, dtype) || (sorted && (tokens > ONE_CLUSTER || (reinterpret_cast<uintptr_t>(sorted) & 255)))) return -1;
+  if (!emb_args_ok(tokens, d, V, dtype) || !ids || !w || !y || (sorted && (tokens > ONE_CLUSTER || (reinterpret_cast<uintptr_t>(sorted) & 255)))) return -1;
   const bool vec = d % 8 == 0 && ldw % 8 == 0 && emb_aligned(w) && emb_aligned(y);
   auto run = [&](auto t, auto v) {
     using T = decltype(t);
@@ -711,7 +711,7 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
                             float scale, int add, int dtype, int grad_dtype, const void* sorted, void* work, long long work_bytes, int* status,
                             cudaStream_t st) {
   if (d == 0 || (tokens == 0 && add)) return 0;
-  if (!emb_args_ok(tokens, d, V, dtype)) return -1;
+  if (!emb_args_ok(tokens, d, V, dtype) || !grad || (tokens > 0 && (!ids || !dy || !work))) return -1;
   if (grad_dtype != dtype && grad_dtype != 2) return -2;
   const EmbSorted s(tokens, V);
   const EmbWork p(tokens, V, d, sorted != nullptr);

@@ -487,6 +487,7 @@ using namespace sx;
 
 extern "C" int sx_vocab_loss_fwd(const void* h, long long ldh, const void* w, long long ldw, const long long* target, long long T, long long V, int d,
                                  long long ignore_index, float cap, void* part, float* zt, float* nll, float* lse, int* status, cudaStream_t st) {
+  if (!h || !w || !target || !part || !zt || !nll || !lse) return -1;
   VocabLossParams p = {};
   int rc = vocab_loss_setup(&p, h, ldh, w, ldw, T, V, d, cap);
   if (rc) return rc;
@@ -565,7 +566,7 @@ static bool vocab_loss_args_ok(const SxVocabLossArgs* a) {
 extern "C" long long sx_vocab_loss_bwd_workspace(const SxVocabLossArgs* a) { return vocab_loss_args_ok(a) ? vocab_loss_plan(a).bytes : -1; }
 
 extern "C" int sx_vocab_loss_bwd(const SxVocabLossArgs* a, cudaStream_t st) {
-  if (!vocab_loss_args_ok(a)) return -1;
+  if (!vocab_loss_args_ok(a) || !a->h || !a->w || !a->target || !a->lse || !a->nll || !a->work) return -1;
   const VocabLossPlan plan = vocab_loss_plan(a);
   if (a->work_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a->work) & 255)) return -3;
   VocabLossParams p = {};

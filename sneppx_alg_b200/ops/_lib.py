@@ -230,10 +230,19 @@ def here(t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def elementary() -> bool:
-    """Whether torch has to see elementary operations, of which kernels that are launched past it are none: while torch.compile reads a function, inside a
-    function transform (torch.func, also offered by ``jit``), in forward-mode differentiation and under a dispatch mode."""
-    return torch.compiler.is_compiling() or torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
+_NO_DISPATCH = torch._C._disabled_torch_dispatch_impl
+
+
+def elementary(*tensors) -> bool:
+    """Whether torch has to see elementary operations on the tensors, of which kernels that are launched past it are none: while torch.compile or
+    torch.jit.trace reads a function, inside a function transform (torch.func, also offered by ``jit``), in forward-mode differentiation, under a dispatch
+    mode, and for tensors of a class with a dispatch of its own, whose address says nothing."""
+    for t in tensors:
+        c = type(t)
+        if c is not torch.Tensor and c is not torch.nn.Parameter and c.__torch_dispatch__ is not _NO_DISPATCH:
+            return True
+    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None or
+            forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0)
 
 
 _status_ptr = {}

@@ -20,7 +20,7 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _native(x) -> bool:
-    if not x.is_cuda or has_torch_function_variadic(x):      # a trace sees the kernels' allocations only: it records the PyTorch form
+    if not x.is_cuda or has_torch_function_variadic(x) or _lib.elementary(x):      # a trace would see the kernels' allocations only
         return False
     if x.dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {x.dtype} is not one of bfloat16, float16, float32")
@@ -98,7 +98,7 @@ def unpack_8bit(p: Packed8bit, dtype=None):
     if tuple(p.codes.shape) != (rows, nb * BLOCK) or nb != -(-w // BLOCK) or rows * w != p.shape.numel() or p.codes.dtype != torch.int8 \
             or p.exponents.dtype != torch.uint8 or p.codes.device != p.exponents.device:
         raise ValueError(f"unpack_8bit: codes {tuple(p.codes.shape)} and exponents {tuple(p.exponents.shape)} do not hold {tuple(p.shape)}")
-    if not (p.codes.is_cuda and _lib.available()) or has_torch_function_variadic(p.codes, p.exponents):
+    if not (p.codes.is_cuda and _lib.available()) or has_torch_function_variadic(p.codes, p.exponents) or _lib.elementary(p.codes, p.exponents):
         return unpack_8bit_reference(p.codes, p.exponents, w, dtype).view(p.shape)
     if dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
@@ -147,8 +147,9 @@ class _Glu8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gu, act):
         f = gu.shape[-1] // 2
-        ctx.meta = act, gu.shape
-        if not _native(gu):
+        native = _native(gu)
+        ctx.meta = act, gu.shape, native
+        if not native:
             g2 = _rows(gu)
             parts = [pack_8bit_reference(t) for t in (g2[:, :f], g2[:, f:])]
             ctx.save_for_backward(torch.cat([c for c, _ in parts], 1), torch.cat([e for _, e in parts], 1))
@@ -160,9 +161,9 @@ class _Glu8Fn(torch.autograd.Function):
     @staticmethod
     @_lib.once
     def backward(ctx, dh):
-        act, shape = ctx.meta
+        act, shape, native = ctx.meta
         f = shape[-1] // 2
-        if not _native(dh):
+        if not native:
             codes, exps = ctx.saved_tensors
             rows = codes.shape[0]
             gate, up = (unpack_8bit_reference(c, e, f, torch.float32) for c, e in zip(codes.chunk(2, 1), exps.chunk(2, 1)))

@@ -21,7 +21,7 @@ def embedding_reference(ids, table, scale=1.0, padding_idx=None):
     else:                                          # ids out of range as the kernels have them: rows of zeros, told by the status word
         ok = (ids >= 0) & (ids < table.shape[0])
         y = torch.where(ok.unsqueeze(-1), F.embedding(torch.where(ok, ids, 0), table, padding_idx), 0.0)
-        if not _lib.elementary():                  # which nobody may write to there
+        if not _lib.elementary(ids, table):        # which nobody may write to there
             word = _lib.status_word(table.device)[:1]
             word.copy_(torch.where((~ok).any() & (word == 0), 5, word))
     return y if scale == 1.0 else (y.float() * scale).to(y.dtype) if y.dtype != torch.float64 else y * scale
@@ -83,6 +83,9 @@ def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
         raise ValueError("embedding_backward_: a table of no rows")
     if padding_idx is not None and not 0 <= padding_idx < V:
         raise ValueError(f"embedding_backward_: padding_idx {padding_idx} outside a table of {V} rows")
+    if _lib.elementary(grad, ids, dy):
+        sums = _differentiable_backward(ids, dy, V, scale, -1 if padding_idx is None else padding_idx, torch.float32)
+        return grad.add_(sums) if add else grad.copy_(sums)
     return _backward(grad, ids.contiguous(), dy.contiguous(), float(scale), -1 if padding_idx is None else padding_idx, bool(add), None)
 
 
@@ -105,10 +108,10 @@ def _backward(grad, ids, dy, scale, padding, add, order):
     return grad
 
 
-def _differentiable_backward(ids, dy, V, scale, padding):
+def _differentiable_backward(ids, dy, V, scale, padding, dtype):
     counts = (ids >= 0) & (ids < V) & (ids != padding)
     rows = torch.where(counts[..., None], dy.float() * scale, 0.0).reshape(-1, dy.shape[-1])
-    return rows.new_zeros(V, dy.shape[-1]).index_add(0, torch.where(counts, ids, 0).reshape(-1), rows).to(dy.dtype)
+    return rows.new_zeros(V, dy.shape[-1]).index_add(0, torch.where(counts, ids, 0).reshape(-1), rows).to(dtype)
 
 
 class _EmbeddingFn(torch.autograd.Function):
@@ -123,8 +126,8 @@ class _EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         table, scale, padding, order = ctx.meta
-        if torch.is_grad_enabled():                # a graph of this pass is wanted: the same sums by operations that have one
-            return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding), None, None
+        if torch.is_grad_enabled() or type(dy) is not torch.Tensor:      # a graph of this pass is wanted: the same sums by operations that have one
+            return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding, dy.dtype), None, None
         mg = getattr(table, "main_grad", None)
         dy = dy.contiguous()
         if mg is None or mg.dtype not in (dy.dtype, torch.float32) or mg.stride(1) != 1:
@@ -141,7 +144,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     there, or added to what is there already (a tied output projection's), and ``.grad`` stays empty. ``padding_idx`` (negative counts from the
     end): tokens of this word give no gradient. On the GPU an id outside [0, V) gives a row of zeros and sets the status word
     (``check_status`` raises); on the CPU it raises at once. Inside function transforms (``jit.grad``, ``vmap``, ``jvp``, ``hessian``), in forward-mode
-    differentiation and under torch.compile the PyTorch form is taken; the status word is left alone there."""
+    differentiation, under torch.compile and torch.jit.trace and for tensor classes with a dispatch of their own the PyTorch form is taken; the status word
+    is left alone there."""
     if has_torch_function_variadic(ids, table):      # a trace records this call: of the kernel's it would see the allocation of the result only
         return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
     if table.dim() != 2:
@@ -159,7 +163,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         padding_idx %= V
     if V == 0 and ids.numel():
         raise IndexError("embedding: ids for a table of no rows")
-    if not table.is_cuda or table.dtype not in _TYPES or V == 0 or _lib.elementary() or not _lib.available():
+    if not table.is_cuda or table.dtype not in _TYPES or V == 0 or _lib.elementary(ids, table) or not _lib.available():
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:
         _dbg.check_indices(ids, 0, V, _dbg.SITE_USER)

@@ -25,8 +25,9 @@ def linear_token_loss_reference(h, w, target, ignore_index=-100, softcap=0.0):
         if bool(bad.any()):
             raise IndexError(f"linear_token_loss: a target outside a vocabulary of {w.shape[0]}")
     else:                                          # as the kernels do: ignored, and told by the status word
-        word = _lib.status_word(target.device)[:1]
-        word.copy_(torch.where(bad.any() & (word == 0), 5, word))
+        if not _lib.elementary(h, w, target):
+            word = _lib.status_word(target.device)[:1]
+            word.copy_(torch.where(bad.any() & (word == 0), 5, word))
         valid = valid & ~bad
     zt = z.gather(-1, torch.where(valid, target, 0).unsqueeze(-1)).squeeze(-1)
     return torch.where(valid, lse - zt, 0.0), lse
@@ -142,7 +143,7 @@ def linear_token_loss(h, w, target, ignore_index=-100, softcap=0.0, piece=0):
         raise ValueError(f"linear_token_loss: tensors on {h.device}, {w.device} and {target.device}")
     if w.shape[0] == 0 or softcap < 0 or piece < 0:
         raise ValueError(f"linear_token_loss: vocabulary of {w.shape[0]}, softcap {softcap}, piece {piece}")
-    if not (h.is_cuda and h.dtype == w.dtype == torch.bfloat16 and w.shape[1] > 0 and _lib.available()):
+    if not (h.is_cuda and h.dtype == w.dtype == torch.bfloat16 and w.shape[1] > 0 and not _lib.elementary(h, w, target) and _lib.available()):
         return linear_token_loss_reference(h, w, target, ignore_index, softcap)
     if target.numel() == 0:                    # nothing to compute, but results that backward can be called on
         z = h.sum(-1).float() + 0.0 * w[0, 0].float()

@@ -135,3 +135,85 @@ def test_a_lookup_that_torch_compile_reads(backend):
     y.sum().backward()
     assert torch.equal(y, e.weight[ids] * 2)
     assert torch.equal(e.weight.grad, 2 * torch.bincount(ids, minlength=50)[:, None].float().expand(50, 8))
+
+
+class _Held(torch.Tensor):
+    """A tensor class whose values are another tensor's and that has no address of its own, as sharded and lazily loaded weights are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    __torch_function__ = torch._C._disabled_torch_function_impl
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        from torch.utils._pytree import tree_map
+        args, kwargs = tree_map(lambda t: t.inner if isinstance(t, _Held) else t, (args, kwargs or {}))
+        return func(*args, **kwargs)
+
+
+def test_tensor_classes_without_an_address():
+    w, h = torch.randn(40, 16, device="cuda"), torch.randn(7, 64, device="cuda").to(torch.bfloat16)
+    v = (torch.randn(50, 64, device="cuda") / 8).to(torch.bfloat16)
+    ids = torch.randint(0, 40, (7,), device="cuda")
+    assert _Held(w).data_ptr() == 0
+    for table, i in ((_Held(w), ids), (w, _Held(ids)), (_Held(w), _Held(ids))):
+        assert torch.equal(ops.embedding(i, table, 2.0), w[ids] * 2)
+    dy = torch.randn(7, 16, device="cuda")
+    want = ops.embedding_backward_(torch.empty_like(w), ids, dy)
+    for add in (False, True):
+        got = ops.embedding_backward_(torch.zeros_like(w), _Held(ids), _Held(dy), add=add)
+        assert torch.allclose(got, want, rtol=1e-6, atol=1e-6)
+    # the PyTorch form's products in 32 bits against sums that the tensor cores cut: 64 additions, each off by 2^-23 of at most 64 x 4 x 0.6
+    for args in ((_Held(h), v), (h, _Held(v))):
+        for a, b in zip(ops.linear_token_loss(*args, ids), ops.linear_token_loss(h, v, ids)):
+            assert torch.allclose(a, b, rtol=0, atol=64 * 2.0 ** -23 * 154)
+    held = ops.pack_8bit(_Held(h))
+    want = ops.pack_8bit(h)
+    assert torch.equal(held.codes, want.codes) and torch.equal(held.exponents, want.exponents)
+    assert torch.equal(ops.unpack_8bit(ops.Packed8bit(_Held(want.codes), want.exponents, want.shape, want.dtype)), ops.unpack_8bit(want))
+    assert torch.allclose(ops.glu_8bit(_Held(h)).float(), ops.glu_8bit(h).float(), rtol=2.0 ** -7, atol=0)
+    ops.check_status()
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning", "ignore::torch.jit.TracerWarning")
+def test_torch_jit_trace():
+    e = Embedding(40, 64, dtype=torch.bfloat16, device="cuda").requires_grad_(False)          # torch.jit.trace takes no other constants
+    w = (torch.randn(50, 64, device="cuda") / 8).to(torch.bfloat16)
+    first, second = (torch.randint(0, 40, (7,), device="cuda") for _ in range(2))
+    with torch.no_grad():
+        f = torch.jit.trace(lambda i: e(i) * 2, (first,), check_trace=False)
+        g = torch.jit.trace(lambda i: ops.linear_token_loss(e.weight[i], w, i)[0], (first,), check_trace=False)
+        k = torch.jit.trace(lambda i: ops.unpack_8bit(ops.pack_8bit(e.weight[i])) + ops.glu_8bit(e.weight[i]).repeat(1, 2), (first,), check_trace=False)
+        for ids in (first, second):
+            x = e.weight[ids]
+            assert torch.equal(f(ids), x * 2)
+            assert torch.allclose(g(ids), ops.linear_token_loss(x, w, ids)[0], rtol=0, atol=1e-3)
+            with torch.jit.optimized_execution(False):          # the tape as it was recorded: TorchScript's fuser drops the conversion to int8
+                got = k(ids).float()
+            # restored values are exact in both; the gated one may be a step of bf16 off, 2^-7 of it, and the sum is rounded
+            a, b = ops.unpack_8bit(ops.pack_8bit(x)).float(), ops.glu_8bit(x).repeat(1, 2).float()
+            assert ((got - (a + b)).abs() <= 2.0 ** -7 * (b.abs() + (a + b).abs())).all()
+
+
+def test_backward_under_a_mode_that_forward_was_not_in():
+    from torch.utils.flop_counter import FlopCounterMode
+    w, x = torch.randn(40, 16, device="cuda", requires_grad=True), torch.randn(7, 64, device="cuda", requires_grad=True)
+    h, v = torch.randn(7, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(50, 64, device="cuda").bfloat16().requires_grad_()
+    ids = torch.randint(0, 40, (7,), device="cuda")
+
+    def forward():
+        return ops.embedding(ids, w).sum() + ops.glu_8bit(x).sum() + ops.linear_token_loss(h, v, ids)[0].sum()
+
+    want = torch.autograd.grad(forward(), (w, x, h, v))
+    loss = forward()
+    with FlopCounterMode(display=False):
+        got = torch.autograd.grad(loss, (w, x, h, v), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.device("cuda"):
+        got = torch.autograd.grad(loss, (w, x, h, v))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
