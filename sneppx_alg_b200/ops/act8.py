@@ -47,6 +47,7 @@ class Packed8bit:
 
 def _rows(x):
     """x as [rows, width] whose rows are contiguous (a view where x allows one)."""
+    x = x.resolve_neg()                        # the imaginary part of a conjugate is a view whose sign is still to be turned
     if x.dim() > 1 and x.is_contiguous() and x.numel():
         return x.view(-1, x.shape[-1])
     w = x.shape[-1] if x.dim() else 1
@@ -102,7 +103,7 @@ def unpack_8bit(p: Packed8bit, dtype=None):
         return unpack_8bit_reference(p.codes, p.exponents, w, dtype).view(p.shape)
     if dtype not in _TYPES:
         raise TypeError(f"8-bit activations: {dtype} is not one of bfloat16, float16, float32")
-    codes, exps = p.codes.contiguous(), p.exponents.contiguous()
+    codes, exps = p.codes.contiguous(), p.exponents.contiguous()               # whole numbers: no sign is left to be turned
     if codes.data_ptr() % 16:                  # a view into something larger: the kernels read four words at once
         codes = codes.clone()
     x = codes.new_empty(p.shape, dtype=dtype)
@@ -171,7 +172,7 @@ class _Glu8Fn(torch.autograd.Function):
         (held,) = ctx.saved_tensors
         nb = -(-f // BLOCK)
         rows = held.numel() // (2 * nb * (BLOCK + 1)) if nb else 0
-        dh = dh.contiguous()
+        dh = dh.contiguous().resolve_neg()
         dgu = dh.new_empty(shape)
         with _lib.on_device(dh):
             at = held.data_ptr()

@@ -41,6 +41,7 @@ def _workspace(n, V, d, presorted):
 def _lookup(ids, table, scale, padding=-1, sort=False):
     """(rows, ids as they were read, those in the order of their words or None). padding: a word, or -1."""
     V, d = table.shape
+    table = table.resolve_neg()                # the imaginary part of a conjugate is a view whose sign is still to be turned
     ldw, step = table.stride()
     if step != 1 or ldw < d:
         table, ldw = table.contiguous(), d
@@ -83,7 +84,7 @@ def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
         raise ValueError("embedding_backward_: a table of no rows")
     if padding_idx is not None and not 0 <= padding_idx < V:
         raise ValueError(f"embedding_backward_: padding_idx {padding_idx} outside a table of {V} rows")
-    if _lib.elementary(grad, ids, dy):
+    if _lib.elementary(grad, ids, dy) or grad.is_neg():
         sums = _differentiable_backward(ids, dy, V, scale, -1 if padding_idx is None else padding_idx, torch.float32)
         return grad.add_(sums) if add else grad.copy_(sums)
     return _backward(grad, ids.contiguous(), dy.contiguous(), float(scale), -1 if padding_idx is None else padding_idx, bool(add), None)
@@ -92,6 +93,7 @@ def embedding_backward_(grad, ids, dy, scale=1.0, padding_idx=None, add=False):
 def _backward(grad, ids, dy, scale, padding, add, order):
     """ids and dy contiguous, all on one device; order: what the forward pass left, or None."""
     V, d = grad.shape
+    dy = dy.resolve_neg()
     n = ids.numel()
     size = _workspace(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)

@@ -36,6 +36,7 @@ def linear_token_loss_reference(h, w, target, ignore_index=-100, softcap=0.0):
 def _rows16(t, d):
     """(t, pitch): t [..., <= d] as the tensor maps take it: rows of d columns, a multiple of 8 (padded with zeros), 16-byte aligned."""
     w = t.shape[-1]
+    t = t.resolve_neg()                        # the imaginary part of a conjugate is a view whose sign is still to be turned
     if w == d and t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t, d
     if t.dim() != 2:
@@ -87,7 +88,7 @@ class _TokenLossFn(torch.autograd.Function):
         T, V, d0 = tgt.numel(), w.shape[0], w.shape[1]
         d = (d0 + 7) // 8 * 8                          # what the products' pitches take
         (h2, ldh), (w2, ldw) = _rows16(h, d), _rows16(w, d)
-        gn, gz = (g if g is None or g.is_contiguous() else g.contiguous() for g in (g_nll, g_lse))       # fp32, as the results are
+        gn, gz = (g if g is None else g.contiguous().resolve_neg() for g in (g_nll, g_lse))       # fp32, as the results are
         dh = h2.new_empty(h.shape if d == d0 else (T, d)) if need_h else None
         mg = getattr(w, "main_grad", None) if need_w and d == d0 else None
         if mg is not None and (mg.dtype not in (torch.bfloat16, torch.float32) or mg.stride(1) != 1):

@@ -307,3 +307,36 @@ def test_tables_of_other_types(dtype):
     y = ops.embedding(ids, w)
     assert y.dtype == dtype and torch.equal(y.to(torch.complex64), torch.nn.functional.embedding(ids, w).to(torch.complex64))
     ops.check_status()
+
+
+def test_views_whose_sign_is_still_to_be_turned():
+    """The imaginary part of a conjugate, as a table, as activations and as incoming gradients."""
+    def turned(*shape):
+        z = torch.randn(shape, dtype=torch.complex64, device="cuda").conj().imag
+        assert z.is_neg()
+        return z, z.clone()
+
+    def plain(t):
+        return torch.empty_like(t).copy_(t)
+
+    table, t2 = turned(40, 16)
+    dy, d2 = turned(7, 16)
+    ids = torch.randint(0, 40, (7,), device="cuda")
+    assert torch.equal(ops.embedding(ids, table, 2.0), table[ids] * 2)
+    w = torch.randn(40, 16, device="cuda", requires_grad=True)
+    want = torch.zeros(40, 16, device="cuda").index_add_(0, ids, plain(dy))
+    assert torch.allclose(torch.autograd.grad(ops.embedding(ids, w), w, dy)[0], want, atol=1e-5)
+    assert torch.allclose(ops.embedding_backward_(torch.empty_like(w), ids, dy), want, atol=1e-5)
+    for shape in ((9, 64), (9, 1), (1,), ()):
+        x, _ = turned(*shape)
+        assert torch.equal(ops.unpack_8bit(ops.pack_8bit(x)), ops.unpack_8bit(ops.pack_8bit(plain(x))))
+    x, _ = turned(9, 64)
+    g, h = x.detach().requires_grad_(), plain(x).requires_grad_()
+    dh, _ = turned(9, 32)
+    a, b = ops.glu_8bit(g), ops.glu_8bit(h)
+    assert torch.equal(a, b) and torch.equal(torch.autograd.grad(a, g, dh)[0], torch.autograd.grad(b, h, plain(dh))[0])
+    hb, wb = (torch.randn(7, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    gn, _ = turned(7)
+    t = torch.arange(7, device="cuda")
+    got, want = (torch.autograd.grad(ops.linear_token_loss(hb, wb, t)[0], (hb, wb), v) for v in (gn, plain(gn)))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
