@@ -1,12 +1,14 @@
 """Builds and loads the native libraries of the framework, in-tree.
 
-Two shared objects are produced under ``sneppx_alg_b200/lib``:
+Three shared objects are produced under ``sneppx_alg_b200/lib``:
 
 * ``libsneppx_b200.so``  - every CUDA kernel (``csrc/*.cu``), compiled by ``nvcc`` for sm_100a only
   (``-gencode arch=compute_100a,code=sm_100a``); exported through a C ABI (``csrc/sx_api.h``) and
   called from Python with ``ctypes``.
 * ``libsneppx_host.so``  - the host-side C++ runtime (``csrc/host/*.cpp``): checkpoint container,
   TCP ring all-reduce, heartbeat, model factory, serving batch core, tokenizer, edge runtime.
+* ``libsneppx_torch.so`` - nodes of torch's graph in C++ (``ops/native/*.cpp``) for operators whose calls are short: the only one that includes torch's
+  headers and belongs to one version of it. Operators work without it, at more host time.
 
 A content hash of the sources is stored beside each library; ``load_*`` rebuilds when the hash no
 longer matches and a compiler is available, and fails loudly otherwise.
@@ -49,6 +51,7 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-fun
 _lock = threading.Lock()
 _cuda_lib = None
 _host_lib = None
+_torch_mod = None
 
 
 def _nvcc() -> str | None:
@@ -168,6 +171,32 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
     return lib
 
 
+def build_torch(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the graph nodes (``ops/native/*.cpp``) into ``libsneppx_torch.so``, for the installed versions of torch and Python."""
+    import sysconfig
+
+    import torch
+    LIBDIR.mkdir(parents=True, exist_ok=True)
+    lib, stamp = LIBDIR / "libsneppx_torch.so", LIBDIR / "libsneppx_torch.hash"
+    srcs = sorted((PKG / "ops" / "native").glob("*.cpp"))
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    want = _hash_files(srcs, [*flags, torch.__version__, sys.version])
+    if not force and _current(lib, stamp, want):
+        return lib
+    cxx, nvcc = shutil.which("g++") or shutil.which("c++"), _nvcc()
+    if cxx is None or nvcc is None:
+        raise RuntimeError("g++ and the CUDA headers beside nvcc are needed to build libsneppx_torch.so")
+    home = Path(torch.__file__).parent
+    use = ["-isystem", str(home / "include"), "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(Path(nvcc).resolve().parents[1] / "include")]
+    out = _run([cxx, *flags, *use, "-shared", *map(str, srcs), "-o", str(lib), "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+                "-ltorch_python"])
+    stamp.write_text(want)
+    if verbose and out.strip():
+        print(out, file=sys.stderr)
+    return lib
+
+
 SANITIZE_FLAGS = ["-O1", "-g", "-std=c++17", "-fPIC", "-pthread", "-fsanitize=address,undefined", "-fno-omit-frame-pointer"]
 
 
@@ -191,7 +220,7 @@ def build_host_sanitized(verbose: bool = False, kind: str = "address") -> Path:
 
 
 def build_all(force: bool = False, verbose: bool = False):
-    return build_cuda(force, verbose), build_host(force, verbose)
+    return build_cuda(force, verbose), build_host(force, verbose), build_torch(force, verbose)
 
 
 def load_cuda(subset: str | None = None) -> ctypes.CDLL:
@@ -230,6 +259,23 @@ def load_host() -> ctypes.CDLL:
                     raise
             _host_lib = ctypes.CDLL(str(lib))
         return _host_lib
+
+
+def load_torch():
+    """The module of graph nodes, built first where it is missing or made for another version; RuntimeError where it cannot be."""
+    global _torch_mod
+    with _lock:
+        if _torch_mod is None:
+            from importlib import machinery, util
+            path = str(build_torch())
+            spec = util.spec_from_loader("libsneppx_torch", machinery.ExtensionFileLoader("libsneppx_torch", path))
+            try:
+                mod = util.module_from_spec(spec)
+                spec.loader.exec_module(mod)
+            except ImportError as e:
+                raise RuntimeError(f"{path} cannot be loaded: {e}") from e
+            _torch_mod = mod
+        return _torch_mod
 
 
 if __name__ == "__main__":

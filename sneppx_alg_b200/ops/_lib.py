@@ -230,7 +230,9 @@ def here(t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-_NO_DISPATCH = torch._C._disabled_torch_dispatch_impl
+_TENSOR, _PARAMETER, _NO_DISPATCH = torch.Tensor, torch.nn.Parameter, torch._C._disabled_torch_dispatch_impl
+_compiling, _tracing = torch.compiler.is_compiling, torch._C._get_tracing_state
+_transform, _modes = torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
 
 
 def elementary(*tensors) -> bool:
@@ -239,10 +241,9 @@ def elementary(*tensors) -> bool:
     mode, and for tensors of a class with a dispatch of its own, whose address says nothing."""
     for t in tensors:
         c = type(t)
-        if c is not torch.Tensor and c is not torch.nn.Parameter and c.__torch_dispatch__ is not _NO_DISPATCH:
+        if c is not _TENSOR and c is not _PARAMETER and c.__torch_dispatch__ is not _NO_DISPATCH:
             return True
-    return (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None or torch._C._functorch.peek_interpreter_stack() is not None or
-            forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0)
+    return _compiling() or _tracing() is not None or _transform() is not None or forward_ad._current_level >= 0 or _modes() > 0
 
 
 _status_ptr = {}

@@ -3,7 +3,9 @@
 module (interface_bindings/nn.py, ``Embedding``)."""
 from __future__ import annotations
 
+import ctypes
 import functools
+import warnings
 
 import torch
 import torch.nn.functional as F
@@ -11,6 +13,7 @@ from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 from . import debug as _dbg
+from .. import _build
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -37,7 +40,25 @@ def _workspace(n, V, d, presorted):
     return _lib.entry("sx_embed_bwd_workspace", "llii", _lib.c_ll)(n, V, d, presorted)
 
 
-# Both launches are a call's whole cost for few tokens (the library's lookup of one row: 5.5 us): numbers are read once, nothing is wrapped.
+_nodes = None        # the graph node in C++, False where it cannot be built
+
+
+def _load_nodes():
+    """ops/native/embed_node.cpp, which the calls take where it is there: the same kernels at less host time than the Python function below."""
+    global _nodes
+    try:
+        nodes = _build.load_torch()
+        L = _lib.lib()
+        nodes.bind(_lib, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in
+                           ("sx_embed_sorted_bytes", "sx_embed_bwd_workspace", "sx_embed_fwd", "sx_embed_bwd")))
+        _nodes = nodes
+    except RuntimeError as e:
+        warnings.warn(f"sneppx_alg_b200: embeddings take more host time without libsneppx_torch.so: {e}", RuntimeWarning, stacklevel=3)
+        _nodes = False
+    return _nodes
+
+
+# Numbers are read once and nothing is wrapped: for few tokens the host's time is all that the calls take.
 def _lookup(ids, table, scale, padding=-1, sort=False):
     """(rows, ids as they were read, those in the order of their words or None). padding: a word, or -1."""
     V, d = table.shape
@@ -117,6 +138,8 @@ def _differentiable_backward(ids, dy, V, scale, padding, dtype):
 
 
 class _EmbeddingFn(torch.autograd.Function):
+    """What ops/native/embed_node.cpp does, where that cannot be built."""
+
     @staticmethod
     def forward(ctx, ids, table, scale, padding):
         y, ids, order = _lookup(ids, table, scale, padding, True)
@@ -128,7 +151,8 @@ class _EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         table, scale, padding, order = ctx.meta
-        if torch.is_grad_enabled() or type(dy) is not torch.Tensor:      # a graph of this pass is wanted: the same sums by operations that have one
+        if torch.is_grad_enabled() or type(dy) is not torch.Tensor or torch._C._functorch.is_legacy_batchedtensor(dy):
+            # a graph of this pass, or of a batch of them, is wanted: the same sums by operations that have one
             return None, _differentiable_backward(ids, dy, table.shape[0], scale, padding, dy.dtype), None, None
         mg = getattr(table, "main_grad", None)
         dy = dy.contiguous()
@@ -169,6 +193,10 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
         return embedding_reference(ids, table, scale, padding_idx)
     if _dbg.ENABLED:
         _dbg.check_indices(ids, 0, V, _dbg.SITE_USER)
+    padding = -1 if padding_idx is None else padding_idx
+    nodes = _nodes if _nodes is not None else _load_nodes()
+    if nodes:
+        return nodes.lookup(ids, table, scale, padding, _lib.status_ptr(table))
     if table.requires_grad and torch.is_grad_enabled():
-        return _EmbeddingFn.apply(ids, table, float(scale), -1 if padding_idx is None else padding_idx)
+        return _EmbeddingFn.apply(ids, table, float(scale), padding)
     return _lookup(ids, table, scale)[0]
