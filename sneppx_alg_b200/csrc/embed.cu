@@ -395,20 +395,20 @@ __device__ __forceinline__ void part_store(float* part, unsigned piece, int side
   p[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   p[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
 }
-// Rows of words that do not occur, 32 words at a time a block, their marks read together; narrow rows several at once.
+// Rows of words that do not occur, `words` of up to 32 at a time a block, their marks read together; narrow rows several at once.
 template <bool VEC, typename G>
-__device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long ldg, int d, unsigned block, unsigned blocks) {
+__device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long ldg, int d, unsigned words, unsigned block, unsigned blocks) {
   __shared__ unsigned row_of[32], rows;
   const unsigned threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
   const unsigned vecs = emb_places<VEC>(d), side = max(threads / vecs, 1u), mine = tid / vecs, c0 = (tid - mine * vecs) * 8;
   Emb8<G> z;
 #pragma unroll
   for (int j = 0; j < 8; ++j) z.t[j] = emb_out<G>(0.f);
-  for (unsigned long long v0 = (unsigned long long)block * 32; v0 < (unsigned long long)a.V; v0 += (unsigned long long)blocks * 32) {
+  for (unsigned long long v0 = (unsigned long long)block * words; v0 < (unsigned long long)a.V; v0 += (unsigned long long)blocks * words) {
     __syncthreads();
     if (tid < 32) {
       const unsigned long long v = v0 + tid;
-      bool zero = v < (unsigned long long)a.V;
+      bool zero = tid < words && v < (unsigned long long)a.V;
       if (zero && (long long)v != a.padding) {
         const unsigned m = a.mark[v];
         zero = m >= a.n || emb_id(a.ids, a.wide, m) != (long long)v;
@@ -432,9 +432,10 @@ __device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long 
 // [32000, 1024] fp32: four blocks 43 us, five 57).
 template <bool VEC, typename T, typename G>
 __global__ void __launch_bounds__(256, VEC && sizeof(T) == 4 ? 4 : 5) embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part,
-                                                           unsigned len, int d, int d8, float scale, int add, unsigned blocks_x, unsigned blocks) {
+                                                           unsigned len, int d, int d8, float scale, int add, unsigned blocks_x, unsigned blocks,
+                                                           unsigned words) {
   if (blockIdx.x >= blocks) {          // the gradient is written whole: rows that have no sum, beside those that have
-    zero_rows<VEC>(a, grad, ldg, d, blockIdx.x - blocks, gridDim.x - blocks);
+    zero_rows<VEC>(a, grad, ldg, d, words, blockIdx.x - blocks, gridDim.x - blocks);
     return;
   }
   const unsigned *key = a.key_out, *pos = a.pos_out, n = a.n, V = (unsigned)a.V;
@@ -751,10 +752,13 @@ extern "C" int sx_embed_bwd(const void* ids, int ids_wide, const void* dy, void*
     using G = decltype(g);
     constexpr bool VEC = decltype(v)::value;
     const unsigned sums = grid.x * grid.y;
-    // rows of zeros: many short blocks, which fill up what the sums leave (a [128256, 4096] gradient in 169 us; 185 by eight blocks an SM, 212 by four)
-    const long long groups = add ? 0 : (V + 31) / 32;
-    embed_sum_kernel<VEC, T, G><<<sums + (unsigned)(groups < 148 * 32 ? groups : 148 * 32), block, 0, st>>>(
-        a, (const T*)dy, (G*)grad, ldg, part, p.len, d, p.d8, scale, add, grid.x > 0 ? grid.x : 1, sums);
+    // rows of zeros: many short blocks, which fill up what the sums leave, of about 64 KB each ([32000, 4096] fp32 87 us, 96 by 32 words a block; bf16 53 and
+    // 64, [128256, 4096] 185 and 196; rows of 128 bytes want all 32: a million of them 74 us, 105 by 16)
+    const long long row = (long long)d * sizeof(G);
+    const unsigned words = (unsigned)(row >= 16384 ? 4 : row <= 2048 ? 32 : 65536 / row);
+    const long long groups = add ? 0 : (V + words - 1) / words;
+    embed_sum_kernel<VEC, T, G><<<sums + (unsigned)(groups < 148 * 128 ? groups : 148 * 128), block, 0, st>>>(
+        a, (const T*)dy, (G*)grad, ldg, part, p.len, d, p.d8, scale, add, grid.x > 0 ? grid.x : 1, sums, words);
     if (p.pieces > 1)
       embed_join_kernel<VEC, G><<<dim3((p.pieces + 7) / 8, (d + 255) / 256), dim3(32, 8), 0, st>>>(
           key, (G*)grad, ldg, part, (unsigned)tokens, p.len, d, p.d8, (unsigned)V, scale, add);
