@@ -5,7 +5,6 @@ unloadable library is an error: there is no silent fallback to PyTorch kernels f
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import threading
 
@@ -216,15 +215,6 @@ def stream() -> c_void_p:
     return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
-_here = contextlib.nullcontext()
-
-
-def on_device(t):
-    """Context in which the device of t (a CUDA tensor) is the current one, as launches on its streams need (nothing to do where it is already)."""
-    i = t.get_device()
-    return _here if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
-
-
 def here(t) -> int:
     """Handle of the current stream of t's device (a CUDA tensor)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
@@ -244,6 +234,16 @@ def elementary(*tensors) -> bool:
         if c is not _TENSOR and c is not _PARAMETER and c.__torch_dispatch__ is not _NO_DISPATCH:
             return True
     return _compiling() or _tracing() is not None or _transform() is not None or forward_ad._current_level >= 0 or _modes() > 0
+
+
+def launch(t, name: str, sig: str, *args):
+    """``entry(name, sig)`` with the arguments and the current stream of t's device (a CUDA tensor), on that device."""
+    i = t.get_device()
+    fn = _entries.get(name) or entry(name, sig)
+    if i == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    with torch.cuda.device(i):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
 
 
 _status_ptr = {}

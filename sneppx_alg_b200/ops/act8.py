@@ -86,8 +86,7 @@ def pack_8bit(x) -> Packed8bit:
     if not _native(x):
         return Packed8bit(*pack_8bit_reference(x2), x.shape, x.dtype)
     codes, exps = x2.new_empty((rows, nb * BLOCK), dtype=torch.int8), x2.new_empty((rows, nb), dtype=torch.uint8)
-    with _lib.on_device(x):
-        _lib.entry("sx_pack8", "ppplilip")(x2.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, w, x2.stride(0), _TYPES[x.dtype], _lib.here(x))
+    _lib.launch(x, "sx_pack8", "ppplilip", x2.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, w, x2.stride(0), _TYPES[x.dtype])
     return Packed8bit(codes, exps, x.shape, x.dtype)
 
 
@@ -96,7 +95,7 @@ def unpack_8bit(p: Packed8bit, dtype=None):
     dtype = dtype or p.dtype
     w = p.shape[-1] if len(p.shape) else 1
     rows, nb = p.exponents.shape
-    if tuple(p.codes.shape) != (rows, nb * BLOCK) or nb != -(-w // BLOCK) or rows * w != p.shape.numel() or p.codes.dtype != torch.int8 \
+    if p.codes.shape != (rows, nb * BLOCK) or nb != -(-w // BLOCK) or rows * w != p.shape.numel() or p.codes.dtype != torch.int8 \
             or p.exponents.dtype != torch.uint8 or p.codes.device != p.exponents.device:
         raise ValueError(f"unpack_8bit: codes {tuple(p.codes.shape)} and exponents {tuple(p.exponents.shape)} do not hold {tuple(p.shape)}")
     if not (p.codes.is_cuda and _lib.available()) or has_torch_function_variadic(p.codes, p.exponents) or _lib.elementary(p.codes, p.exponents):
@@ -107,8 +106,7 @@ def unpack_8bit(p: Packed8bit, dtype=None):
     if codes.data_ptr() % 16:                  # a view into something larger: the kernels read four words at once
         codes = codes.clone()
     x = codes.new_empty(p.shape, dtype=dtype)
-    with _lib.on_device(x):
-        _lib.entry("sx_unpack8", "ppplilip")(codes.data_ptr(), exps.data_ptr(), x.data_ptr(), rows, w, w, _TYPES[dtype], _lib.here(x))
+    _lib.launch(x, "sx_unpack8", "ppplilip", codes.data_ptr(), exps.data_ptr(), x.data_ptr(), rows, w, w, _TYPES[dtype])
     return x
 
 
@@ -138,9 +136,8 @@ def _glu_forward(gu, act, held=None):
     g2 = _rows(gu)
     h = gu.new_empty((*gu.shape[:-1], f))
     at = 0 if held is None else held.data_ptr()
-    with _lib.on_device(gu):
-        _lib.entry("sx_glu8_fwd", "ppppliliip")(g2.data_ptr(), h.data_ptr(), at, at and at + g2.shape[0] * 2 * -(-f // BLOCK) * BLOCK, g2.shape[0], f,
-                                               g2.stride(0), act, _TYPES[gu.dtype], _lib.here(gu))
+    _lib.launch(gu, "sx_glu8_fwd", "ppppliliip", g2.data_ptr(), h.data_ptr(), at, at and at + g2.shape[0] * 2 * -(-f // BLOCK) * BLOCK, g2.shape[0], f,
+                g2.stride(0), act, _TYPES[gu.dtype])
     return h
 
 
@@ -174,10 +171,8 @@ class _Glu8Fn(torch.autograd.Function):
         rows = held.numel() // (2 * nb * (BLOCK + 1)) if nb else 0
         dh = dh.contiguous().resolve_neg()
         dgu = dh.new_empty(shape)
-        with _lib.on_device(dh):
-            at = held.data_ptr()
-            _lib.entry("sx_glu8_bwd", "ppppliiip")(dh.data_ptr(), at, at + rows * 2 * nb * BLOCK, dgu.data_ptr(), rows, f, act, _TYPES[dh.dtype],
-                                                  _lib.here(dh))
+        at = held.data_ptr()
+        _lib.launch(dh, "sx_glu8_bwd", "ppppliiip", dh.data_ptr(), at, at + rows * 2 * nb * BLOCK, dgu.data_ptr(), rows, f, act, _TYPES[dh.dtype])
         return dgu, None
 
 

@@ -75,15 +75,8 @@ def _lookup(ids, table, scale, padding=-1, sort=False):
         if size:
             order = table.new_empty(size, dtype=torch.uint8)
             at = order.data_ptr()
-    dev = table.get_device()
-    launch = _lib.entry("sx_embed_fwd", "piplplilfilppp")
-    args = (ids.data_ptr(), ids.dtype is torch.int64, table.data_ptr(), ldw, y.data_ptr(), n, d, V, scale, _TYPES[table.dtype], padding, at,
-            _lib.status_ptr(table), torch._C._cuda_getCurrentRawStream(dev))
-    if dev == torch._C._cuda_getDevice():
-        launch(*args)
-    else:
-        with torch.cuda.device(dev):
-            launch(*args)
+    _lib.launch(table, "sx_embed_fwd", "piplplilfilppp", ids.data_ptr(), ids.dtype is torch.int64, table.data_ptr(), ldw, y.data_ptr(), n, d, V, scale,
+                _TYPES[table.dtype], padding, at, _lib.status_ptr(table))
     return y, ids, order
 
 
@@ -118,16 +111,9 @@ def _backward(grad, ids, dy, scale, padding, add, order):
     n = ids.numel()
     size = _workspace(n, V, d, order is not None)
     work = grad.new_empty(size, dtype=torch.uint8)
-    dev = grad.get_device()
-    launch = _lib.entry("sx_embed_bwd", "pippllillfiiipplpp")
-    args = (ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V, padding, scale, add, _TYPES[dy.dtype],
-            _TYPES[grad.dtype], 0 if order is None else order.data_ptr(), work.data_ptr(), size, _lib.status_ptr(grad),
-            torch._C._cuda_getCurrentRawStream(dev))
-    if dev == torch._C._cuda_getDevice():
-        launch(*args)
-    else:
-        with torch.cuda.device(dev):
-            launch(*args)
+    _lib.launch(grad, "sx_embed_bwd", "pippllillfiiipplpp", ids.data_ptr(), ids.dtype is torch.int64, dy.data_ptr(), grad.data_ptr(), grad.stride(0), n, d, V,
+                padding, scale, add, _TYPES[dy.dtype], _TYPES[grad.dtype], 0 if order is None else order.data_ptr(), work.data_ptr(), size,
+                _lib.status_ptr(grad))
     return grad
 
 

@@ -60,10 +60,8 @@ def _forward(h, w, target, ignore_index, softcap, keep=False):
     pairs = 2 * T * -(-V // 256)                          # of a row's maximum and sum, and behind them its target's logit
     scratch = h2.new_empty(pairs if keep else pairs + T, dtype=torch.float32)
     own = h2.new_empty(T, dtype=torch.float32) if keep else None
-    with _lib.on_device(h):
-        _lib.entry("sx_vocab_loss_fwd", "plplpllilfpppppp")(
-            h2.data_ptr(), ldh, w2.data_ptr(), ldw, tgt.data_ptr(), T, V, d, ignore_index, softcap, scratch.data_ptr(),
-            own.data_ptr() if keep else scratch.data_ptr() + 4 * pairs, nll.data_ptr(), lse.data_ptr(), _lib.status_ptr(h), _lib.here(h))
+    _lib.launch(h, "sx_vocab_loss_fwd", "plplpllilfpppppp", h2.data_ptr(), ldh, w2.data_ptr(), ldw, tgt.data_ptr(), T, V, d, ignore_index, softcap,
+                scratch.data_ptr(), own.data_ptr() if keep else scratch.data_ptr() + 4 * pairs, nll.data_ptr(), lse.data_ptr(), _lib.status_ptr(h))
     return nll, lse, tgt, own
 
 
@@ -110,8 +108,7 @@ class _TokenLossFn(torch.autograd.Function):
         a.work_bytes = _lib.entry("sx_vocab_loss_bwd_workspace", "p", _lib.c_ll)(C.addressof(a))
         work = h2.new_empty(a.work_bytes, dtype=torch.uint8)
         a.work = work.data_ptr()
-        with _lib.on_device(h):
-            _lib.entry("sx_vocab_loss_bwd", "pp")(C.addressof(a), _lib.here(h))
+        _lib.launch(h, "sx_vocab_loss_bwd", "pp", C.addressof(a))
         if mg is not None:
             w._main_grad_written = True
             dw = None
