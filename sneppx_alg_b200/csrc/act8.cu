@@ -41,7 +41,8 @@ constexpr int PER = 16;      // values of a thread
 // where they are multiples of 8 (PAIR; the block's two threads take its vectors in turn, so that they fill sectors together). Rows that begin anywhere (ODD)
 // are read and written by a warp as whole aligned words, 32 next to each other, and turned into 16 neighbouring values a thread and back through shared
 // memory; a word that two rows or two warps share is read and written by halves (8192 x 4101 in bf16: packed and restored in 57 us, gated with its gradient
-// 167; 78 and 226 with values one by one, 32 apart). Where a row has two blocks at most, of which a warp would be empty otherwise, threads take their 16
+// 167; 78 and 226 with values one by one, 32 apart; 33 and 89 for whole vectors). What bounds them is the issue of instructions, 70 % of the SMs' rate with
+// a third of DRAM's: each value goes through shared memory and a shift. Where a row has two blocks at most, of which a warp would be empty otherwise, threads take their 16
 // neighbours one by one, and a warp several rows (NEAR: 22222 x 45 packed and restored 11.8 us, 17.5 as ODD; gated 30 and 45; at 77 columns 11.4 and 11.9,
 // 30 and 28).
 enum { ODD = 0, PAIR = 1, WIDE = 2, NEAR = 3 };
@@ -394,7 +395,8 @@ static int row_mode(int width, long long ld, const void* p, const void* q, int s
   return width <= 64 ? NEAR : ODD;
 }
 static bool act8_args_ok(const void* values, const void* codes, const void* exps, long long rows, int width, int dtype) {
-  return values && !codes == !exps && rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+  return values && !codes == !exps && rows > 0 && rows <= 0x7fffffffll && width > 0 && width <= (1 << 26) && dtype >= 0 && dtype <= 2 &&
+         (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
 }
 
 // dtype 0 bf16, 1 fp16, 2 fp32

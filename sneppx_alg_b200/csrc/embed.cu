@@ -33,9 +33,11 @@ template <> __device__ __forceinline__ float emb_out<float>(float v) { return v;
 
 // A thread's place c, a multiple of 8, in a row of d values. VEC (whole 16-byte accesses: d, pitch and base allow them): the values c to c + 7. Else the 32
 // threads of a warp share 256 values so that neighbours touch neighbouring ones: value j of a thread is 32 j behind its first (2049 columns: 385 us
-// with eight neighbouring values a thread, 97 so).
+// with eight neighbouring values a thread, 97 so). Such rows wait for their loads, of which two-byte ones bring little each: a lookup of 8192 rows of 2049
+// in bf16 20.5 us with half of the warps that an SM holds (52 registers), 12.4 at 2048.
 template <typename T> union Emb8 { uint4 q[sizeof(T) / 2]; uint32_t w[2 * sizeof(T)]; T t[8]; };
-// Eight fp32 values are a sector: with accesses of 16 bytes each sector is touched twice (rows of zeros of [32000, 4096] fp32 128 -> 98 us, of [128256, 4096] 446 -> 338).
+// Eight fp32 values are a sector: with accesses of 16 bytes each sector is touched twice (rows of zeros of [32000, 4096] fp32 128 -> 98 us, of [128256,
+// 4096] 446 -> 338).
 __device__ __forceinline__ bool emb_sector(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 template <bool VEC>
 __host__ __device__ __forceinline__ int emb_places(int d) { return VEC ? (d + 7) / 8 : (d + 255) / 256 * 32; }   // threads of a row
@@ -431,9 +433,9 @@ __device__ __forceinline__ void zero_rows(const SortArgs& a, G* grad, long long 
 // of the warps, 93 us instead of 65 for 32768 tokens of 2048). Four rows of eight fp32 values do not fit the 48 registers that five blocks leave (added to
 // [32000, 1024] fp32: four blocks 43 us, five 57).
 template <bool VEC, typename T, typename G>
-__global__ void __launch_bounds__(256, VEC && sizeof(T) == 4 ? 4 : 5) embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part,
-                                                           unsigned len, int d, int d8, float scale, int add, unsigned blocks_x, unsigned blocks,
-                                                           unsigned words) {
+__global__ void __launch_bounds__(256, VEC && sizeof(T) == 4 ? 4 : 5)
+    embed_sum_kernel(const SortArgs a, const T* __restrict__ dy, G* grad, long long ldg, float* __restrict__ part, unsigned len, int d, int d8, float scale,
+                     int add, unsigned blocks_x, unsigned blocks, unsigned words) {
   if (blockIdx.x >= blocks) {          // the gradient is written whole: rows that have no sum, beside those that have
     zero_rows<VEC>(a, grad, ldg, d, words, blockIdx.x - blocks, gridDim.x - blocks);
     return;

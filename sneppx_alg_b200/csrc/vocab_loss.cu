@@ -16,10 +16,11 @@
 // logits, therefore takes the accumulator out after 768 products at most, in equal parts, and adds in registers, rounded: lse of 4088 tokens over [128256,
 // 4096] is off by 1.4e-6 without that, by 3.7e-7 in parts of 1024 and by 2.3e-7 in these, in the same time; parts of 512 cost 3% more there and 20% over 768
 // columns. Widths just above one part pay little for their second: 4095 tokens over [50280, 1024] 276 us in two, 275 in one, with the soft cap 299 and 281,
-// at half the error (lse 2.3e-7 and 4.5e-7). Backward leaves a logit in one accumulator: an error of 1e-4 in it is one of 1e-4 of its e^{z - lse}, a twentieth of what the rounding of dz to bf16
-// takes. The target's value alone would lose it against 1 - e^{z - lse}, which may be smaller, so that is computed from the forward pass's nll
-// (64 tokens over [32000, 4096]: dw of a target that the model gives an nll of 1e-3 is off by 1.9e-3 of itself, 6.8e-2 by the difference; of 2.5e-5
-// by 2.5e-3, 0.46 by the difference).
+// at half the error (lse 2.3e-7 and 4.5e-7).
+// Backward leaves a logit in one accumulator: an error of 1e-4 in it is one of 1e-4 of its e^{z - lse}, a twentieth of what the rounding of dz to bf16 takes.
+// The target's value alone would lose it against 1 - e^{z - lse}, which may be smaller, so that is computed from the forward pass's nll (64 tokens over
+// [32000, 4096]: dw of a target that the model gives an nll of 1e-3 is off by 1.9e-3 of itself, 6.8e-2 by the difference; of 2.5e-5 by 2.5e-3, 0.46 by the
+// difference).
 // Takes the place of the reference's softmax / cross-entropy kernels (kernel/cuda/autodiff_cuda.cu:519-608).
 #include "tc_common.cuh"
 #include "tc_pair.cuh"

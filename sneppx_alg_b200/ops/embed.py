@@ -160,6 +160,10 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     is left alone there."""
     if has_torch_function_variadic(ids, table):      # a trace records this call: of the kernel's it would see the allocation of the result only
         return handle_torch_function(embedding, (ids, table), ids, table, scale, padding_idx)
+    if _nodes and padding_idx is None and not _dbg.ENABLED and not torch.compiler.is_compiling():
+        y = _nodes.ordinary(ids, table, scale)
+        if y is not None:
+            return y
     if table.dim() != 2:
         raise ValueError(f"embedding: table of shape {tuple(table.shape)} is no matrix")
     V = table.shape[0]

@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -32,6 +33,8 @@ SortedBytes sorted_bytes;
 Workspace workspace;
 Forward embed_fwd;
 Backward embed_bwd;
+constexpr int MOST_DEVICES = 64;
+int* status_of[MOST_DEVICES];        // status words, of devices that have been used
 PyObject *counter, *name_count, *name_main_grad, *name_written;      // counter: the module whose launch_count counts launches
 
 int code_of(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : 2; }
@@ -86,7 +89,8 @@ struct EmbeddingBackward : public torch::autograd::Node {
     }
     if (!dy.defined()) return {Tensor()};
     const int64_t V = table.size(0), d = table.size(1);
-    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(dy)) {      // a graph of this pass, or of a batch of them: the same sums by operations that have one
+    if (at::GradMode::is_enabled() || at::isTensorSubclassLike(dy)) {
+      // a graph of this pass, or of a batch of them, is wanted: the same sums by operations that have one
       const Tensor counts = i.ge(0).logical_and(i.lt(V)).logical_and(i.ne(padding));
       const Tensor rows = at::where(counts.unsqueeze(-1), dy.to(at::kFloat) * scale, 0.0).reshape({-1, d});
       return {at::zeros({V, d}, table.options().dtype(at::kFloat)).index_add(0, at::where(counts, i, 0).reshape(-1), rows).to(table.scalar_type())};
@@ -141,8 +145,8 @@ Tensor looked_up(const Tensor& given, const Tensor& source, double scale, int64_
     y = at::empty(shape, table.options());
     const long long bytes = train && d ? sorted_bytes(n, V) : 0;
     if (bytes) order = at::empty({bytes}, table.options().dtype(at::kByte));
-    const int rc = embed_fwd(ids.const_data_ptr(), ids.scalar_type() == at::kLong, table.const_data_ptr(), ldw, y.mutable_data_ptr(), n, (int)d, V, (float)scale,
-                             code_of(table.scalar_type()), padding, bytes ? order.mutable_data_ptr() : nullptr, status, stream_of(table));
+    const int rc = embed_fwd(ids.const_data_ptr(), ids.scalar_type() == at::kLong, table.const_data_ptr(), ldw, y.mutable_data_ptr(), n, (int)d, V,
+                             (float)scale, code_of(table.scalar_type()), padding, bytes ? order.mutable_data_ptr() : nullptr, status, stream_of(table));
     TORCH_CHECK(rc == 0, "sx_embed_fwd failed with code ", rc);
   }
   if (train) {
@@ -159,6 +163,38 @@ Tensor looked_up(const Tensor& given, const Tensor& source, double scale, int64_
   return y;
 }
 
+// Whether torch has to see no elementary operations on a tensor here (ops/_lib.py: elementary), torch.compile aside.
+bool plain(const Tensor& t) { return !at::isTensorSubclassLike(t) && !t._fw_grad(0).defined(); }
+bool in_a_transform() {
+  return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer);
+}
+
+// (ids, table, scale) -> rows where that is an ordinary call, which is most of them; else None: ops/embed.py looks closer.
+PyObject* ordinary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n == 3 && THPVariable_Check(args[0]) && THPVariable_Check(args[1]) && PyFloat_CheckExact(args[2])) {
+    const Tensor& ids = THPVariable_Unpack(args[0]);
+    const Tensor& table = THPVariable_Unpack(args[1]);
+    const auto type = table.scalar_type(), kind = ids.scalar_type();
+    const int dev = table.is_cuda() ? table.get_device() : -1;
+    if (dev >= 0 && dev < MOST_DEVICES && status_of[dev] && ids.is_cuda() && ids.get_device() == dev && plain(ids) && plain(table) && !in_a_transform() &&
+        table.dim() == 2 && table.size(0) > 0 && (type == at::kBFloat16 || type == at::kHalf || type == at::kFloat) && (kind == at::kLong || kind == at::kInt) &&
+        table.layout() == at::kStrided && ids.layout() == at::kStrided) {
+      const double scale = PyFloat_AS_DOUBLE(args[2]);
+      count_launch();
+      Tensor y;
+      {
+        const pybind11::gil_scoped_release release;
+        y = looked_up(ids, table, scale, -1, status_of[dev]);
+      }
+      return THPVariable_Wrap(std::move(y));
+    }
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // (ids, table, scale, padding, address of the status word) -> rows. ids and table have been checked.
 PyObject* lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -167,6 +203,8 @@ PyObject* lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t padding = PyLong_AsLongLong(args[3]);
   int* status = static_cast<int*>(PyLong_AsVoidPtr(args[4]));
   if (PyErr_Occurred()) return nullptr;
+  const int dev = THPVariable_Unpack(args[1]).get_device();
+  if (dev >= 0 && dev < MOST_DEVICES) status_of[dev] = status;
   count_launch();
   Tensor y;
   {
@@ -193,6 +231,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
+    {"ordinary", (PyCFunction)(void (*)())ordinary, METH_FASTCALL, nullptr},
     {"lookup", (PyCFunction)(void (*)())lookup, METH_FASTCALL, nullptr},
     {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -46,7 +46,7 @@ def enable_activation_checkpointing(model, every: int = 1, bits: int = 16):
 
 def enable_8bit_activations(model, on: bool = True):
     """The gated feed-forward blocks of ``model`` hold gate and up in 8 bits between forward and backward (``ops.glu_8bit``) instead of 16. Returns
-    how many do."""
+    how many do: those of the Llama models; 0 says that a model has no such blocks and keeps what it kept."""
     blocks = [m for m in model.modules() if hasattr(m, "held_bits")]
     for m in blocks:
         m.held_bits = 8 if on else 16
