@@ -101,6 +101,8 @@ class KVCache:
 
 
 class LlamaForCausalLM(Module):
+    checkpoint_bits = 16      # of what activation checkpointing keeps: 16, or 8 with a power of two for 32 values; models saved before have none of their own
+
     def __init__(self, cfg: ModelConfig, dtype=None, device=None, with_head: bool = True):
         super().__init__()
         self.config = cfg
@@ -115,7 +117,6 @@ class LlamaForCausalLM(Module):
                                   init_std=cfg.initializer_range)
         self._rope = None
         self.activation_checkpointing = False
-        self.checkpoint_bits = 16      # of what activation checkpointing keeps: 16, or 8 with a power of two for 32 values
 
     # ------------------------------------------------------------------ helpers
     def rope(self, device, need):

@@ -80,3 +80,13 @@ def test_models_that_answer_with_their_logits():
     assert not _answers_with_its_logits(model)
     handle.remove()
     assert _answers_with_its_logits(model)
+
+
+def test_models_saved_before_there_was_a_choice_of_bits():
+    model, ids = _model(), torch.randint(0, 50, (2, 30), generator=torch.Generator().manual_seed(1))
+    _, want = _grads(model, ids)
+    model.activation_checkpointing = True
+    vars(model).pop("checkpoint_bits", None)                   # what an object pickled earlier comes back without
+    _, got = _grads(model, ids)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    assert extras.enable_activation_checkpointing(model, bits=8).checkpoint_bits == 8 and type(model).checkpoint_bits == 16
