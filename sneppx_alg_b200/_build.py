@@ -189,8 +189,13 @@ def build_torch(force: bool = False, verbose: bool = False) -> Path:
     home = Path(torch.__file__).parent
     use = ["-isystem", str(home / "include"), "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(Path(nvcc).resolve().parents[1] / "include")]
-    out = _run([cxx, *flags, *use, "-shared", *map(str, srcs), "-o", str(lib), "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
-                "-ltorch_python"])
+    new = lib.with_suffix(f".{os.getpid()}.so")             # put in place whole: several ranks may build at once
+    try:
+        out = _run([cxx, *flags, *use, "-shared", *map(str, srcs), "-o", str(new), "-L", str(home / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+                    "-ltorch_python"])
+        os.replace(new, lib)
+    finally:
+        new.unlink(missing_ok=True)
     stamp.write_text(want)
     if verbose and out.strip():
         print(out, file=sys.stderr)

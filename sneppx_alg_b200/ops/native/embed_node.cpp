@@ -199,10 +199,12 @@ PyObject* ordinary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(n == 5 && THPVariable_Check(args[0]) && THPVariable_Check(args[1]), "lookup: two tensors and three numbers");
+  TORCH_CHECK(embed_fwd && THPVariable_Unpack(args[0]).is_cuda() && THPVariable_Unpack(args[1]).is_cuda(), "lookup: not bound, or tensors on the CPU");
   const double scale = PyFloat_AsDouble(args[2]);
   const int64_t padding = PyLong_AsLongLong(args[3]);
   int* status = static_cast<int*>(PyLong_AsVoidPtr(args[4]));
   if (PyErr_Occurred()) return nullptr;
+  TORCH_CHECK(status, "lookup: no status word");
   const int dev = THPVariable_Unpack(args[1]).get_device();
   if (dev >= 0 && dev < MOST_DEVICES) status_of[dev] = status;
   count_launch();

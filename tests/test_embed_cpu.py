@@ -47,3 +47,18 @@ def test_refusals():
     with pytest.raises(IndexError):
         ops.embedding(torch.tensor([0]), torch.randn(0, 4))
     assert ops.embedding(torch.zeros(0, dtype=torch.int64), torch.randn(0, 4)).shape == (0, 4)
+
+
+def test_graph_node_without_a_gpu():
+    """The module in C++ can be built and loaded; it takes no tensors of the CPU, and says so."""
+    from sneppx_alg_b200 import _build
+    nodes = _build.load_torch()
+    assert _build.load_torch() is nodes
+    ids, w = torch.tensor([1, 2]), torch.randn(9, 4)
+    for args in ((ids, w, 1.0), (ids, w, 1), (ids, w), (1, w, 1.0), (ids, None, 1.0), (w, ids, 1.0)):
+        assert nodes.ordinary(*args) is None
+    for args in ((ids, w, 1.0, -1, 0), (ids, w, 1.0, -1), (ids, "w", 1.0, -1, 0), ()):
+        with pytest.raises(RuntimeError, match="lookup"):
+            nodes.lookup(*args)
+    with pytest.raises(RuntimeError, match="bind"):
+        nodes.bind(1, 2)
