@@ -96,18 +96,18 @@ struct EmbeddingBackward : public torch::autograd::Node {
       return {at::zeros({V, d}, table.options().dtype(at::kFloat)).index_add(0, at::where(counts, i, 0).reshape(-1), rows).to(table.scalar_type())};
     }
     dy = dy.contiguous().resolve_neg();
+    Tensor main;
+    bool written = false;
     {
-      pybind11::gil_scoped_acquire gil;
+      const pybind11::gil_scoped_acquire gil;        // for the table's attributes only: the launches below may have to wait for room
       count_launch();
       PyObject* t = THPVariable_Wrap(table);
       PyObject* g = t ? attribute(t, name_main_grad) : nullptr;
-      Tensor grad;
       if (g && THPVariable_Check(g)) {
-        grad = THPVariable_Unpack(g);
-        if ((grad.scalar_type() != dy.scalar_type() && grad.scalar_type() != at::kFloat) || grad.stride(1) != 1) grad = Tensor();
+        main = THPVariable_Unpack(g);
+        if ((main.scalar_type() != dy.scalar_type() && main.scalar_type() != at::kFloat) || main.stride(1) != 1) main = Tensor();
       }
-      bool written = false;
-      if (grad.defined()) {
+      if (main.defined()) {
         PyObject* w = attribute(t, name_written);
         written = w && PyObject_IsTrue(w) == 1;
         Py_XDECREF(w);
@@ -115,10 +115,10 @@ struct EmbeddingBackward : public torch::autograd::Node {
       }
       Py_XDECREF(g);
       Py_XDECREF(t);
-      if (grad.defined()) {
-        sums(grad, i, dy, scale, padding, written, sorted, status);
-        return {Tensor()};
-      }
+    }
+    if (main.defined()) {
+      sums(main, i, dy, scale, padding, written, sorted, status);
+      return {Tensor()};
     }
     const Tensor grad = at::empty({V, d}, dy.options());
     sums(grad, i, dy, scale, padding, false, sorted, status);
