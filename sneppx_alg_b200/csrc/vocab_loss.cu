@@ -16,7 +16,9 @@
 // logits, therefore takes the accumulator out after 768 products at most, in equal parts, and adds in registers, rounded: lse of 4088 tokens over [128256,
 // 4096] is off by 1.4e-6 without that, by 3.7e-7 in parts of 1024 and by 2.3e-7 in these, in the same time; parts of 512 cost 3% more there and 20% over 768
 // columns. Widths just above one part pay little for their second: 4095 tokens over [50280, 1024] 276 us in two, 275 in one, with the soft cap 299 and 281,
-// at half the error (lse 2.3e-7 and 4.5e-7).
+// at half the error (lse 2.3e-7 and 4.5e-7). Up to 256 tokens, one row of tiles, wait for the weights more than for their epilogue and take parts of 384: half
+// the error (nll of 4 tokens over [16377, 640] with a soft cap 6.1e-7 -> 3.1e-7, of 64 over [128256, 4096] 6.1e-7 -> 3.1e-7) in 18.6 us as before and 203
+// instead of 200.
 // Backward leaves a logit in one accumulator: an error of 1e-4 in it is one of 1e-4 of its e^{z - lse}, a twentieth of what the rounding of dz to bf16 takes.
 // The target's value alone would lose it against 1 - e^{z - lse}, which may be smaller, so that is computed from the forward pass's nll (64 tokens over
 // [32000, 4096]: dw of a target that the model gives an nll of 1e-3 is off by 1.9e-3 of itself, 6.8e-2 by the difference; of 2.5e-5 by 2.5e-3, 0.46 by the
@@ -39,6 +41,7 @@ constexpr int VL_COLS = 256 / VL_GROUPS;             // columns of an epilogue w
 constexpr int VL_EPI_WARPS = 4 * VL_GROUPS;
 constexpr int VL_THREADS = 64 + 32 * VL_EPI_WARPS;
 constexpr int VL_CHUNK = 768 / VL_BK;                // forward: k-blocks that stay in one accumulator at most
+constexpr int VL_FEW_CHUNK = 384 / VL_BK;            // and of up to 256 tokens
 constexpr int VL_SLOTS = 4;                          // tiles whose pairs may wait to be joined (below)
 constexpr int VL_OFF_PAIRS = VL_STAGES * VL_STAGE_BYTES;
 constexpr int VL_PAIR_BYTES = VL_SLOTS * (VL_GROUPS - 1) * 128 * 8;
@@ -163,7 +166,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VL_THREADS, 1) vocab
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = p.m_blks * p.n_blks;
   const int num_kb = (p.d + VL_BK - 1) / VL_BK;
-  const int parts = (num_kb + VL_CHUNK - 1) / VL_CHUNK;
+  const int most = p.m_blks == 1 ? VL_FEW_CHUNK : VL_CHUNK;
+  const int parts = (num_kb + most - 1) / most;
   const int chunk = GRAD ? num_kb : (num_kb + parts - 1) / parts;      // equal ones: what is cut grows with the longest
 
   if (warp == 0) {

@@ -427,3 +427,20 @@ def test_logits_of_any_finite_size(size):
     assert clear.float().mean() > (0.5 if size > 2e3 else 0.1) and torch.isfinite(got["dh"]).all()
     off = (got["dh"].double() - dh).abs()[clear]
     assert (off <= 2.0 ** -7 * (w64[z.argmax(1)].abs() + w64[t].abs())[clear]).all()
+
+
+@pytest.mark.parametrize("T,V,d", [(4, 16377, 640), (64, 3000, 4096), (256, 4000, 768), (200, 5000, 2304)])
+def test_few_tokens_lose_little(T, V, d):
+    """The tensor cores cut what they add to an accumulator, by as much as there are products in a part of the sum: of up to 256 tokens a part has half as many
+    as of more, so that the same tokens' lse is off by about half of what it is among 600 (by less than three quarters, which leaves room for the rounding of
+    lse itself, 2^-24 of it, on both sides)."""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    few = many = 0.0
+    for _ in range(8):
+        w = (torch.randn(V, d, generator=g, device="cuda") / math.sqrt(d)).to(torch.bfloat16)
+        t = torch.randint(0, V, (600,), generator=g, device="cuda")
+        h = (torch.randn(600, d, generator=g, device="cuda") + 14 * torch.rand(600, 1, generator=g, device="cuda") * w[t].float()).to(torch.bfloat16)
+        want = torch.logsumexp(h[:T].double() @ w.double().t(), 1)
+        few += float((ops.linear_token_loss(h[:T], w, t[:T])[1].double() - want).square().sum())
+        many += float((ops.linear_token_loss(h, w, t)[1][:T].double() - want).square().sum())
+    assert math.sqrt(few) < 0.75 * math.sqrt(many)
