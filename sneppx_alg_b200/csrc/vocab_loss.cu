@@ -8,8 +8,8 @@
 //   forward  each row's maximum and sum of exponentials over a tile's columns but the target leave the SM as one pair of numbers, the target's logit by
 //            itself; a second kernel joins the pairs of a row. 8 bytes leave for 256 logits.
 //   backward the tile is computed again and leaves as dz in bf16 (half a step, 2^-9, of each value: the products that follow take no other type at this
-//            rate, and the logits of linear_cross_entropy's gradient are held so too; dh and dw are off by 2.3e-3 with it, 1.7e-3 by their own rounding
-//            alone), for one piece of the vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
+//            rate, and the logits of linear_cross_entropy's gradient are held so too; dh and dw are off by 2.4e-3 with it, 1.7e-3 by their own rounding
+//            alone; up to 2.7e-3 where tokens are few and one value, the target's, makes most of a row), for one piece of the vocabulary at a time; the products dh += dz w and dw = dz^T h run on the GEMM kernel.
 // Sixteen epilogue warps (four TMEM quadrants, four groups of 64 columns): the exponentials of a tile are behind the products from widths of 256 on only
 // if four warps of each scheduler take turns.
 // The tensor cores cut what they add to an accumulator: over 4096 products a logit of 14 loses 1e-4. The forward pass, whose losses are differences of
