@@ -213,16 +213,21 @@ __device__ __forceinline__ void encode16(const float (&f)[PER], int place, int n
   const uint32_t byte = exponent_of<T>(top);
   const float inv = per_step(byte);
   const uint32_t mask = finite_mask(byte);
-  uint32_t k[PER], r[4];
+  uint32_t r[4];
+  auto codes_of = [&](auto limited) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) k[j] = code_of(f[j], inv);
-  if (byte == TOP_BYTE<T>) {             // rare: 128 steps are 127 here
+    for (int j = 0; j < 4; ++j) {
+      uint32_t k[4];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) k[j] = min(max((int)k[j], 0x4b400000 - 127), 0x4b400000 + 127);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    r[j] = __byte_perm(__byte_perm(k[4 * j], k[4 * j + 1], 0x0040), __byte_perm(k[4 * j + 2], k[4 * j + 3], 0x0040), 0x5410) & mask;
+      for (int i = 0; i < 4; ++i) {
+        k[i] = code_of(f[4 * j + i], inv);
+        if (limited) k[i] = min(max((int)k[i], 0x4b400000 - 127), 0x4b400000 + 127);
+      }
+      r[j] = __byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410) & mask;
+    }
+  };
+  if (byte == TOP_BYTE<T>) codes_of(std::true_type());      // rare: 128 steps are 127 here. Apart, so that neither holds sixteen codes in registers at once
+  else codes_of(std::false_type());
   if (MODE == ODD && place >= 2 * nb) return;          // the last warp of a row may have threads to spare
   if (MODE != PAIR) {
     reinterpret_cast<uint4*>(codes)[place] = make_uint4(r[0], r[1], r[2], r[3]);
@@ -318,7 +323,8 @@ __device__ __forceinline__ void gate8(float g, int act, float& a, float& da) {
 // Blocks of up to 256 threads; 16-bit types forward in 48 registers (ODD 64: 84 us at 8192 x 4101, 87 in 48) and backward in 64: 8192 x 14336 bf16 forward
 // 150.5 us, 158 in 64, and backward 147 us, 161 in 48 (both move 947 MB; 180 and 164 in blocks of 448 threads). 32-bit types have more on their way and keep
 // the registers that the compiler takes (39 and 38 us at 4096 x 4096; 41 and 42 with fewer).
-template <int MODE, typename T>
+// HOLD: gate and up are packed; without a gradient to come nothing is (a template argument: a branch takes registers that these blocks do not have).
+template <int MODE, bool HOLD, typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 1)
     glu8_fwd_kernel(const T* __restrict__ gu, T* __restrict__ h, signed char* __restrict__ codes, unsigned char* __restrict__ exps, unsigned rows, int width,
                     long long ld, int nb, int act) {
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (MODE == ODD ? 4 : 5) : 
   float g[PER], u[PER];
   widen(gv, g);
   widen(uv, u);
-  if (codes) {                           // null: nothing is kept
+  if (HOLD) {
     signed char* kr = codes + (long long)row * (nb * 64);
     unsigned char* er = exps + (long long)row * (2 * nb);
     encode16<MODE, T>(g, piece, nb, kr, er);
@@ -458,8 +464,8 @@ extern "C" int sx_glu8_fwd(const void* gu, void* h, void* codes, void* exps, lon
     dim3 grid, block;
     rows_grid(rows, mode == ODD ? threads_of<ODD>(nb) : threads_of<WIDE>(nb), &grid, &block);
     by_mode(mode, [&](auto m) {
-      glu8_fwd_kernel<decltype(m)::value, T><<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width,
-                                                                     ld, nb, act);
+      auto kernel = codes ? glu8_fwd_kernel<decltype(m)::value, true, T> : glu8_fwd_kernel<decltype(m)::value, false, T>;
+      kernel<<<grid, block, 0, st>>>((const T*)gu, (T*)h, (signed char*)codes, (unsigned char*)exps, (unsigned)rows, width, ld, nb, act);
     });
   });
 }
